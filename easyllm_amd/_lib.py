@@ -27,7 +27,14 @@ class LayerGrad(ctypes.Structure):
     _fields_ = [("f32", _vp), ("bf16", _vp), ("accumulate", _i32)]
 
 
+class Dropout(ctypes.Structure):
+    """struct ezl_dropout"""
+    _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint32), ("drop_of_65536", ctypes.c_int32), ("step", _vp)]
+
+
 _layerp = ctypes.POINTER(Layer)
+_dropp = ctypes.POINTER(Dropout)
+_gradp = ctypes.POINTER(LayerGrad)
 
 # name -> argtypes; the single source of truth for the symbol table on the Python side
 SIGNATURES = {
@@ -36,6 +43,10 @@ SIGNATURES = {
     "ezl_rmsnorm_bwd_noalloc": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp],
     "ezl_rmsnorm_fwd_swapped": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _vp],
     "ezl_rmsnorm_bwd_swapped": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp],
+    "ezl_dropout_add_fwd": [_vp, _vp, _vp, _dropp, _vp, _i64, _i64, _vp],
+    "ezl_dropout_add_bwd": [_vp, _dropp, _vp, _gradp, _vp, _i64, _i64, _i64, _vp],
+    "ezl_norm_fwd": [_i32, _vp, _vp, _vp, _dropp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp],
+    "ezl_norm_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _dropp, _vp, _vp, _gradp, _gradp, _gradp, _vp, _i64, _i64, _i64, _vp],
     "ezl_swiglu_fwd": [_vp, _vp, _vp, _i64, _vp],
     "ezl_swiglu_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "ezl_rope_table": [_vp, _vp, _vp, _i64, _i64, _f32, _vp],
@@ -86,6 +97,8 @@ _SPECIAL = {
     "ezl_last_error": ([], ctypes.c_char_p),
     "ezl_rmsnorm_bwd_workspace_bytes": ([_i64, _i64], _i64),
     "ezl_rmsnorm_bwd_noalloc_max_h": ([], _i64),
+    "ezl_column_sum_workspace_bytes": ([_i64, _i64], _i64),
+    "ezl_norm_bwd_workspace_bytes": ([_i64, _i64], _i64),
     "ezl_bias_grad_workspace_bytes": ([_i64, _i64], _i64),
     "ezl_embed_scatter_add_workspace_bytes": ([_i64, _i64], _i64),
     "ezl_attn_bwd_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
@@ -144,6 +157,14 @@ def call(name, *args):
 
 def rmsnorm_bwd_workspace_bytes(rows, h):
     return load().ezl_rmsnorm_bwd_workspace_bytes(rows, h)
+
+
+def column_sum_workspace_bytes(rows, n):
+    return load().ezl_column_sum_workspace_bytes(rows, n)
+
+
+def norm_bwd_workspace_bytes(rows, h):
+    return load().ezl_norm_bwd_workspace_bytes(rows, h)
 
 
 def bias_grad_workspace_bytes(rows, n):

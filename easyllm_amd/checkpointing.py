@@ -3,10 +3,12 @@ forward re-run inside backward.
 
 Stands in for `deepspeed.checkpointing.checkpoint` as bound by the reference (llm/utils/env/gene_env.py:45-47)
 for what this step needs from it: "re-run the chunk's forward in backward and backprop through it; same numbers".
-Dropout is 0 everywhere in this path, so there is no RNG state to restore; partitioned / CPU / contiguous
+Dropout's numbers are recorded in the forward and replayed (dropout.py); partitioned / CPU / contiguous
 checkpoint variants of DeepSpeed are not reproduced.
 """
 import torch
+
+from . import dropout
 
 
 class _CheckpointFunction(torch.autograd.Function):
@@ -16,7 +18,7 @@ class _CheckpointFunction(torch.autograd.Function):
         ctx.tensor_idx = [i for i, a in enumerate(args) if torch.is_tensor(a)]
         ctx.others = [None if torch.is_tensor(a) else a for a in args]
         ctx.save_for_backward(*[args[i] for i in ctx.tensor_idx])
-        with torch.no_grad():
+        with torch.no_grad(), dropout.recording() as ctx.draws:
             outputs = run_function(*args)
         return outputs
 
@@ -29,7 +31,7 @@ class _CheckpointFunction(torch.autograd.Function):
             d.requires_grad_(t.requires_grad and t.is_floating_point())
             args[i] = d
             detached.append(d)
-        with torch.enable_grad():
+        with torch.enable_grad(), dropout.replaying(ctx.draws):
             outputs = ctx.run_function(*args)  # the recompute-forward
         if torch.is_tensor(outputs):
             outputs = (outputs,)

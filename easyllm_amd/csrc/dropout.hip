@@ -1,0 +1,170 @@
+// Dropout with bias and residual sum, and the column sums of its backward pass (HBM-bound).
+#include "activation.h"
+#include "column_sums.h"
+#include "dropout.h"
+
+namespace {
+
+struct DropAdd {
+    const bf16_t *x, *bias, *res;
+    bf16_t* out;
+    int64_t groups;  // of 8 elements
+    int cols8;       // groups of a row
+    DropArgs drop;
+};
+
+// A thread takes every gridDim.x * 256-th group of 8 elements; its column advances with it.
+template <bool DROP, bool BIAS>
+__global__ __launch_bounds__(256) void dropout_add_kernel(const DropAdd a) {
+    const int64_t stride = (int64_t)gridDim.x * 256;
+    int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int col = 0, col_step = 0;
+    if constexpr (BIAS) {
+        col = (int)(g % a.cols8);
+        col_step = (int)(stride % a.cols8);
+    }
+    uint32_t step = 0;
+    if constexpr (DROP) step = drop_step(a.drop);
+    for (; g < a.groups; g += stride) {
+        float v[8];
+        unpack8(ld_bf16x8(a.x + g * 8), v);
+        float r[8];
+        if (a.res) unpack8(ld_bf16x8(a.res + g * 8), r);
+        if constexpr (BIAS) {
+            float b[8];
+            unpack8(ld_bf16x8(a.bias + col * 8), b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += b[i];
+            col += col_step;
+            if (col >= a.cols8) col -= a.cols8;
+        }
+        if constexpr (DROP) drop8(v, g, a.drop, step);
+        if (a.res)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += r[i];
+        st_bf16x8(a.out + g * 8, pack8(v));
+    }
+}
+
+// dx = f(dy) with the column sums of f(dy) before rounding: a block owns 512 columns (64 lanes of 8) and every gridDim.y * 4-th row from its four
+// waves' on, and leaves one partial row of them.
+constexpr int kSumBlocks = 256;  // partial rows at most
+struct DropSum {
+    const bf16_t* dy;
+    bf16_t* dx;
+    float* partial;
+    int rows, n;
+    DropArgs drop;
+};
+template <class F>
+__device__ __forceinline__ void rows_with_column_sums(int rows, int n, float* partial, F&& f) {
+    __shared__ float fold[4][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = (blockIdx.x * 64 + lane) * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (col < n)
+        for (int row = blockIdx.y * 4 + wave; row < rows; row += gridDim.y * 4) {
+            float v[8];
+            f((int64_t)row * n + col, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += v[i];
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fold[wave][lane * 8 + i] = acc[i];
+    __syncthreads();
+    for (int j = threadIdx.x; j < 512; j += 256)
+        if (blockIdx.x * 512 + j < n) partial[(int64_t)blockIdx.y * n + blockIdx.x * 512 + j] = fold[0][j] + fold[1][j] + fold[2][j] + fold[3][j];
+}
+__global__ __launch_bounds__(256) void dropout_sum_kernel(const DropSum a) {
+    const uint32_t step = drop_step(a.drop);
+    rows_with_column_sums(a.rows, a.n, a.partial, [&](int64_t at, float (&v)[8]) {
+        unpack8(ld_bf16x8(a.dy + at), v);
+        drop8(v, at >> 3, a.drop, step);
+        st_bf16x8(a.dx + at, pack8(v));
+    });
+}
+
+struct SumsArgs {
+    ColumnSum s[kColumnSums];
+};
+__global__ __launch_bounds__(kColsumThreads) void column_sums_kernel(const SumsArgs a, int blocks, int n) {
+    const ColumnSum s = a.s[blockIdx.y];
+    ezl_colsum(s.partials, blocks, n, (bf16_t*)s.bf16, (float*)s.f32, s.accumulate);
+}
+
+dim3 sum_grid(int64_t rows, int64_t n) {
+    const int64_t slabs = (n + 511) / 512;
+    int64_t segs = (2048 + slabs - 1) / slabs;
+    const int64_t most = (rows + 3) / 4;
+    segs = segs > kSumBlocks ? kSumBlocks : segs;
+    segs = segs > most ? most : segs;
+    return dim3((unsigned)slabs, (unsigned)(segs < 1 ? 1 : segs));
+}
+unsigned elementwise_grid(int64_t groups) {
+    const int64_t g = (groups + 255) / 256;
+    return (unsigned)(g > 256 * 16 ? 256 * 16 : g);
+}
+int sizes_check(const char* name, int64_t rows, int64_t n) {
+    EZL_REQUIRE(rows >= 0 && rows < (1LL << 31) && n > 0 && n % 8 == 0 && n < (1LL << 31) && (rows == 0 || n <= (1LL << 60) / rows), EZL_EUNSUPPORTED,
+                "%s: need n %% 8 == 0, rows and n < 2^31 (got %lld x %lld)", name, (long long)rows, (long long)n);
+    return EZL_OK;
+}
+
+}  // namespace
+
+int column_sums(const char* name, const ColumnSum* sums, int count, int blocks, int64_t n, hipStream_t stream) {
+    SumsArgs a = {};
+    for (int i = 0; i < count; ++i) a.s[i] = sums[i];
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((n + 63) / 64), (unsigned)count), dim3(kColsumThreads), 0, stream, a, blocks, (int)n);
+    EZL_LAUNCH_CHECK(name);
+    return EZL_OK;
+}
+
+extern "C" int ezl_dropout_add_fwd(const void* x, const void* bias, const void* residual, const ezl_dropout* drop, void* out, int64_t rows, int64_t n,
+                                   void* stream) {
+    const char* name = "ezl_dropout_add_fwd";
+    if (const int rc = sizes_check(name, rows, n)) return rc;
+    EZL_REQUIRE(rows == 0 || (x && out), EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(ezl_aligned16(x) && ezl_aligned16(bias) && ezl_aligned16(residual) && ezl_aligned16(out), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    DropAdd a = {(const bf16_t*)x, (const bf16_t*)bias, (const bf16_t*)residual, (bf16_t*)out, rows * (n / 8), (int)(n / 8), {}};
+    if (const int rc = drop_args(name, drop, a.drop)) return rc;
+    if (rows == 0) return EZL_OK;
+    const dim3 grid(elementwise_grid(a.groups));
+    hipStream_t st = (hipStream_t)stream;
+    if (a.drop.threshold && bias) hipLaunchKernelGGL((dropout_add_kernel<true, true>), grid, dim3(256), 0, st, a);
+    else if (a.drop.threshold) hipLaunchKernelGGL((dropout_add_kernel<true, false>), grid, dim3(256), 0, st, a);
+    else if (bias) hipLaunchKernelGGL((dropout_add_kernel<false, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((dropout_add_kernel<false, false>), grid, dim3(256), 0, st, a);
+    EZL_LAUNCH_CHECK("ezl_dropout_add_fwd");
+    return EZL_OK;
+}
+
+extern "C" int64_t ezl_column_sum_workspace_bytes(int64_t rows, int64_t n) {
+    return rows < 0 || n <= 0 ? 0 : (int64_t)sum_grid(rows, n).y * n * (int64_t)sizeof(float);
+}
+
+extern "C" int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void* dx, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
+                                   int64_t rows, int64_t n, void* stream) {
+    const char* name = "ezl_dropout_add_bwd";
+    if (const int rc = sizes_check(name, rows, n)) return rc;
+    EZL_REQUIRE(rows == 0 || (dy && dx), EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(ezl_aligned16(dy) && ezl_aligned16(dx) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    DropArgs d;
+    if (const int rc = drop_args(name, drop, d)) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (!wanted(dbias)) {
+        if (rows == 0) return EZL_OK;
+        const DropAdd a = {(const bf16_t*)dy, nullptr, nullptr, (bf16_t*)dx, rows * (n / 8), (int)(n / 8), d};
+        if (d.threshold) hipLaunchKernelGGL((dropout_add_kernel<true, false>), dim3(elementwise_grid(a.groups)), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((dropout_add_kernel<false, false>), dim3(elementwise_grid(a.groups)), dim3(256), 0, st, a);
+        EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
+        return EZL_OK;
+    }
+    EZL_REQUIRE(workspace && workspace_bytes >= ezl_column_sum_workspace_bytes(rows, n), EZL_EINVAL, "%s: workspace missing or too small", name);
+    const DropSum a = {(const bf16_t*)dy, (bf16_t*)dx, (float*)workspace, (int)rows, (int)n, d};
+    const dim3 grid = sum_grid(rows, n);
+    hipLaunchKernelGGL(dropout_sum_kernel, grid, dim3(256), 0, st, a);
+    EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
+    const ColumnSum s = column_sum((const float*)workspace, dbias);
+    return column_sums(name, &s, 1, (int)grid.y, n, st);
+}

@@ -1,0 +1,115 @@
+"""Where dropout takes its numbers from: a seed and a counter of the calls made so far (base_modules' `get_cuda_rng_tracker` role).
+
+The mask of a call follows from (seed, offset, step) and the elements' indices alone (`include/ezl.h`, ezl_dropout), so nothing random is kept but
+these numbers: the backward pass is given the forward's, and a recomputed forward replays them (`recording`, `replaying`).  Every call takes the next offset.
+Inside a captured graph the offset is frozen; there the kernels add a step that lies in device memory, which whoever replays the graph advances
+(`stepping`; `runner.GraphedStep` does).  Outside one the step is zero, and a graph's first is one, so the two never draw the same numbers.
+"""
+import contextlib
+import threading
+from typing import NamedTuple, Optional
+
+import torch
+
+
+class Draw(NamedTuple):
+    """The numbers of one call."""
+    seed: int
+    offset: int
+    step: Optional[torch.Tensor] = None  # int64 [1] on the GPU
+
+
+class _Thread(threading.local):
+    def __init__(self):
+        self.records, self.replays, self.steps = [], [], []
+
+
+_thread = _Thread()
+_lock = threading.Lock()
+_seed = None  # None: torch's, when the first call is made
+_calls = 0
+
+
+def manual_seed(seed):
+    """Starts the draws of this process anew."""
+    global _seed, _calls
+    with _lock:
+        _seed, _calls = int(seed), 0
+
+
+def get_state():
+    """(seed, number of calls): what a checkpoint of a training run has to keep."""
+    global _seed
+    with _lock:
+        if _seed is None:
+            _seed = torch.initial_seed()
+        return _seed, _calls
+
+
+def set_state(state):
+    global _seed, _calls
+    with _lock:
+        _seed, _calls = int(state[0]), int(state[1])
+
+
+def next_draw():
+    """The numbers of the next call of this thread: new ones, or those of the forward pass that is being recomputed."""
+    global _seed, _calls
+    if _thread.replays:
+        try:
+            draw = next(_thread.replays[-1])
+        except StopIteration:
+            raise RuntimeError("a recomputed forward makes more dropout calls than the forward it repeats") from None
+    else:
+        step = None
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            if not _thread.steps:
+                raise RuntimeError("dropout inside a captured graph draws the same mask on every replay unless its step advances: "
+                                   "capture with dropout.stepping() (runner.GraphedStep does)")
+            step = _thread.steps[-1]
+        with _lock:
+            if _seed is None:
+                _seed = torch.initial_seed()
+            draw = Draw((_seed + (_calls >> 32)) & 0xFFFFFFFFFFFFFFFF, _calls & 0xFFFFFFFF, step)
+            _calls += 1
+    for record in _thread.records:
+        record.append(draw)
+    return draw
+
+
+@contextlib.contextmanager
+def recording():
+    """-> the list of this thread's draws inside the block"""
+    draws = []
+    _thread.records.append(draws)
+    try:
+        yield draws
+    finally:
+        _thread.records.pop()
+
+
+@contextlib.contextmanager
+def replaying(draws):
+    """This thread's calls inside the block take `draws`, in order."""
+    _thread.replays.append(iter(draws))
+    try:
+        yield
+    finally:
+        _thread.replays.pop()
+
+
+@contextlib.contextmanager
+def stepping(step):
+    """Captured calls of this thread inside the block read `step` (int64 [1] on the GPU, 1 or more on every replay)."""
+    _thread.steps.append(step)
+    try:
+        yield
+    finally:
+        _thread.steps.pop()
+
+
+def threshold_of(p):
+    """An element is dropped where its 16-bit number is below this: p rounded to a multiple of 2^-16."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability has to be between 0 and 1, but got %r" % (p,))
+    return int(p * 65536 + 0.5)

@@ -14,6 +14,7 @@ import threading
 
 import torch
 
+from . import dropout as _dropout
 from . import kernels as K
 
 
@@ -219,6 +220,102 @@ def rmsnorm_pass(x, weight, eps):
 
 def add_rmsnorm(x, residual, weight, eps):
     return AddRMSNormFunction.apply(x, residual, weight, eps)
+
+
+# --------------------------------------------------------------------------------------------
+# layer norm, dropout and the residual sum: base_modules/layers/fused_layer_norm.py ('mixed_fused_norm'), hidden_dropout of llama/default_cfg.py:21
+# --------------------------------------------------------------------------------------------
+def _vector_target(param, needed):
+    """((f32, bf16, accumulate) for a kernel to write, gradient to return) of a vector parameter"""
+    if param is None or not needed:
+        return None, None
+    mg, acc = _main_grad_target(param)
+    grad = None if mg is not None else torch.empty_like(param)
+    return (mg, grad, acc), grad
+
+
+class NormFunction(torch.autograd.Function):
+    """y = norm(s), s = x or residual + dropout(x + x_bias); returns y, (x, y) with keep_input, or with a residual (s, y).  The gradient that
+    arrives for s (x) is added inside the norm's backward kernel."""
+
+    @staticmethod
+    def forward(ctx, kind, x, residual, x_bias, weight, bias, eps, threshold, draw, keep_input):
+        x = x.contiguous()
+        y, s, mean, rstd = K.norm_fwd(kind, x, weight, bias, eps, None if residual is None else residual.contiguous(), x_bias, threshold, draw)
+        ctx.kind, ctx.threshold, ctx.draw = kind, threshold, draw
+        ctx.pair = keep_input or residual is not None
+        ctx.has_residual = residual is not None
+        ctx.save_for_backward(x if s is None else s, weight, bias, x_bias, mean, rstd)
+        if residual is not None:
+            return s, y
+        return (x.view_as(x), y) if keep_input else y
+
+    @staticmethod
+    def backward(ctx, *grads):
+        s, weight, bias, x_bias, mean, rstd = ctx.saved_tensors
+        dsum, dy = grads if ctx.pair else (None, grads[0])
+        need = ctx.needs_input_grad
+        weight_to, dw = _vector_target(weight, need[4])
+        bias_to, db = _vector_target(bias, need[5])
+        x_bias_to, dxb = _vector_target(x_bias, need[3])
+        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to or (None, torch.empty_like(weight), False), bias_to,
+                              None if dsum is None else dsum.contiguous(), ctx.threshold, ctx.draw, x_bias_to)
+        return (None, dx if need[1] else None, dres if ctx.has_residual and need[2] else None, dxb, dw, db, None, None, None, None)
+
+
+def _draw_for(p, rng):
+    """(threshold, draw): `rng` is (seed, offset[, step]), or None for the next of this process."""
+    threshold = _dropout.threshold_of(p)
+    return threshold, (None if not threshold else _dropout.next_draw() if rng is None else rng)
+
+
+def layer_norm(x, weight, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension."""
+    return NormFunction.apply(K.LAYER_NORM, x, None, None, weight, bias, eps, 0, None, False)
+
+
+def layer_norm_pass(x, weight, bias=None, eps=1e-5):
+    """(x, layer_norm(x)): x as the residual branch, whose gradient is added in the norm's backward kernel."""
+    return NormFunction.apply(K.LAYER_NORM, x, None, None, weight, bias, eps, 0, None, True)
+
+
+def add_layer_norm(x, residual, weight, bias=None, eps=1e-5):
+    """(s, layer_norm(s)), s = x + residual"""
+    return NormFunction.apply(K.LAYER_NORM, x, residual, None, weight, bias, eps, 0, None, False)
+
+
+def dropout_add_layer_norm(x, residual, weight, norm_bias=None, eps=1e-5, bias=None, p=0.0, rng=None):
+    """(s, layer_norm(s)), s = residual + dropout(x + bias).  p is rounded to a multiple of 2^-16; rng: (seed, offset), or None for numbers of
+    this process's own (`easyllm_amd.dropout`)."""
+    threshold, draw = _draw_for(p, rng)
+    return NormFunction.apply(K.LAYER_NORM, x, residual, bias, weight, norm_bias, eps, threshold, draw, False)
+
+
+def dropout_add_rmsnorm(x, residual, weight, eps=1e-6, bias=None, p=0.0, rng=None):
+    """(s, rmsnorm(s)), s = residual + dropout(x + bias).  The norm is of s in fp32 (`add_rmsnorm` rounds it first)."""
+    threshold, draw = _draw_for(p, rng)
+    return NormFunction.apply(K.RMS_NORM, x, residual, bias, weight, None, eps, threshold, draw, False)
+
+
+class DropoutAddFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, bias, threshold, draw):
+        ctx.threshold, ctx.draw, ctx.bias = threshold, draw, bias
+        return K.dropout_add_fwd(x.contiguous(), bias, None if residual is None else residual.contiguous(), threshold, draw)
+
+    @staticmethod
+    def backward(ctx, dy):
+        bias_to, db = _vector_target(ctx.bias, ctx.needs_input_grad[2])
+        dx = dy
+        if bias_to is not None or (ctx.threshold and ctx.needs_input_grad[0]):
+            dx = K.dropout_add_bwd(dy.contiguous(), ctx.threshold, ctx.draw, bias_to)
+        return dx if ctx.needs_input_grad[0] else None, dy if ctx.needs_input_grad[1] else None, db, None, None
+
+
+def dropout_add(x, residual=None, bias=None, p=0.0, rng=None):
+    """residual + dropout(x + bias), residual and bias as far as given; p and rng as in `dropout_add_layer_norm`."""
+    threshold, draw = _draw_for(p, rng)
+    return DropoutAddFunction.apply(x, residual, bias, threshold, draw)
 
 
 # --------------------------------------------------------------------------------------------

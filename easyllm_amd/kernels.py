@@ -128,6 +128,125 @@ def rmsnorm_bwd_swapped(dy, x, weight, rstd, main_grad=None, accumulate=False):
     return dx, dw
 
 
+# ------------------------------------------------------------------------------------- dropout, layer norm
+def _here(*tensors):
+    """All on the current GPU: that is where the launch goes."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError("tensors on GPU %d, but GPU %d is current" % (t.get_device(), device))
+
+
+def _vector(t, n, name):
+    if t is not None:
+        _bf16c(t, name)
+        _need(t.dim() == 1 and t.shape[0] == n, name + " size mismatch")
+
+
+def _drop(threshold, draw):
+    """The C form of a draw (seed, offset[, step]) that drops `threshold` of 65536, None where it drops nothing."""
+    if not threshold:
+        return None
+    seed, offset, *step = draw
+    step = step[0] if step else None
+    _need(0 <= offset < 2 ** 32, "a draw's offset has 32 bits")
+    if step is not None:
+        _need(step.is_cuda and step.dtype is torch.int64 and step.numel() == 1, "a draw's step is an int64 [1] GPU tensor")
+        _here(step)
+    return ctypes.byref(_lib.Dropout(seed & 0xFFFFFFFFFFFFFFFF, offset, threshold, _p(step)))
+
+
+def _grad_target(target, n, what):
+    """(f32 or None, bf16 or None, accumulate) -> C form; None: no gradient wanted"""
+    if target is None:
+        return None
+    f32, bf16, accumulate = target
+    if f32 is not None:
+        _need(f32.is_cuda and f32.dtype is torch.float32 and f32.is_contiguous() and f32.numel() == n, "bad main_grad of the " + what)
+    else:
+        _vector(bf16, n, what + " gradient")
+    _here(f32, bf16)
+    return ctypes.byref(_lib.LayerGrad(_p(f32), _p(bf16), 1 if accumulate else 0))
+
+
+def dropout_add_fwd(x, bias, residual, threshold, draw):
+    """residual + dropout(x + bias); bias and residual may be None."""
+    _bf16c(x, "x")
+    n = x.shape[-1]
+    _vector(bias, n, "bias")
+    if residual is not None:
+        _bf16c(residual, "residual")
+        _need(residual.shape == x.shape, "residual shape mismatch")
+    _here(x, bias, residual)
+    out = torch.empty_like(x)
+    if x.numel():
+        _lib.call("ezl_dropout_add_fwd", _p(x), _p(bias), _p(residual), _drop(threshold, draw), _p(out), x.numel() // n, n, _stream())
+    return out
+
+
+def dropout_add_bwd(dy, threshold, draw, dbias=None):
+    """-> dx; the bias's gradient goes to dbias = (f32 or None, bf16 or None, accumulate)."""
+    _bf16c(dy, "dy")
+    _here(dy)
+    n = dy.shape[-1]
+    rows = dy.numel() // n
+    target = _grad_target(dbias, n, "bias")
+    ws_bytes = _lib.column_sum_workspace_bytes(rows, n) if target else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if target else None
+    dx = torch.empty_like(dy)
+    _lib.call("ezl_dropout_add_bwd", _p(dy), _drop(threshold, draw), _p(dx), target, _p(ws), ws_bytes, rows, n, _stream())
+    return dx
+
+
+LAYER_NORM, RMS_NORM = 0, 1
+
+
+def norm_fwd(kind, x, weight, bias, eps, residual=None, x_bias=None, threshold=0, draw=None):
+    """-> (y, sum, mean, rstd): the norm of x, or of sum = residual + dropout(x + x_bias).  RMS_NORM has no bias, no mean and needs a residual."""
+    _bf16c(x, "x")
+    h = x.shape[-1]
+    _vector(weight, h, "weight"); _vector(bias, h, "norm bias"); _vector(x_bias, h, "bias")
+    _here(x, weight, bias, residual, x_bias)
+    rows = x.numel() // h
+    y = torch.empty_like(x)
+    s = mean = None
+    if residual is not None:
+        _bf16c(residual, "residual")
+        _need(residual.shape == x.shape, "residual shape mismatch")
+        s = torch.empty_like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    rstd = stats[1]
+    if kind == LAYER_NORM:
+        mean = stats[0]
+    _lib.call("ezl_norm_fwd", kind, _p(x), _p(x_bias), _p(residual), _drop(threshold, draw), _p(weight), _p(bias), _p(y), _p(s), _p(mean), _p(rstd),
+              rows, h, float(eps), _stream())
+    return y, s, mean, rstd
+
+
+def norm_bwd(kind, dy, s, weight, mean, rstd, dweight, dbias=None, dsum=None, threshold=0, draw=None, dx_bias=None):
+    """-> (dx, dresidual), one tensor where nothing is dropped.  dweight, dbias, dx_bias: (f32 or None, bf16 or None, accumulate) that
+    receive the parameters' gradients; the last two may be None."""
+    _bf16c(dy, "dy"); _bf16c(s, "s")
+    h = s.shape[-1]
+    rows = s.numel() // h
+    _vector(weight, h, "weight")
+    for t in (mean, rstd):
+        _need(t is None or (t.dtype is torch.float32 and t.numel() == rows and t.is_contiguous()), "norm_bwd: bad statistics")
+    _need(dy.shape == s.shape, "norm_bwd: shape mismatch")
+    if dsum is not None:
+        _bf16c(dsum, "dsum")
+        _need(dsum.shape == s.shape, "norm_bwd: shape mismatch")
+    _here(dy, s, weight, mean, rstd, dsum)
+    dx = torch.empty_like(s)
+    drop = _drop(threshold, draw)
+    dres = torch.empty_like(s) if drop else None
+    ws_bytes = _lib.norm_bwd_workspace_bytes(rows, h)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=s.device)
+    _lib.call("ezl_norm_bwd", kind, _p(dy), _p(dsum), _p(s), _p(weight), _p(mean), _p(rstd), drop, _p(dx), _p(dres), _grad_target(dweight, h, "weight"),
+              _grad_target(dbias, h, "norm bias"), _grad_target(dx_bias, h, "bias"), _p(ws), ws_bytes, rows, h, _stream())
+    return dx, (dx if dres is None else dres)
+
+
 # ------------------------------------------------------------------------------------- SwiGLU
 def swiglu_fwd(gate, up):
     _bf16c(gate, "gate"); _bf16c(up, "up")

@@ -63,6 +63,50 @@ int64_t ezl_rmsnorm_bwd_noalloc_max_h(void);
 int ezl_rmsnorm_bwd_noalloc(const void* dy, const void* x, const void* weight, const void* rstd, const void* dresidual, void* dx,
                             void* dw_bf16, void* dw_f32, int accumulate, int64_t rows, int64_t h, void* stream);
 
+/* ---- dropout: hidden_dropout / embedding_dropout_prob (llama/default_cfg.py:21) --------------------------
+ * Elements 8 g .. 8 g + 7 of a tensor, in the order of its rows, take the 128 bits of Philox-4x32-10 at the counter (g low, g high, offset, step) under the key
+ * (seed low, seed high) as eight 16-bit numbers, the low half of a word first; an element is dropped where its number is below
+ * drop_of_65536, the others are scaled by 65536 / (65536 - drop_of_65536).  Nothing of it is stored: the backward call is given the same numbers.
+ * A step in device memory lets a captured graph draw anew on each replay. */
+typedef struct {
+    uint64_t seed;
+    uint32_t offset;
+    int32_t drop_of_65536; /* 0 .. 65536 */
+    const void* step;      /* device int64 (low 32 bits count), or NULL: 0 */
+} ezl_dropout;
+/* where a parameter's gradient goes: an fp32 buffer (overwritten, or added to when accumulate != 0), else a bf16 one, else
+ * (both NULL, where an entry point allows it) nowhere */
+typedef struct {
+    void *f32, *bf16;
+    int accumulate;
+} ezl_layer_grad;
+/* out = residual + dropout(x + bias) over [rows, n] bf16, n % 8 == 0; bias [n] and residual may be NULL (out may be residual or x); fp32
+ * arithmetic, one rounding.  drop NULL: nothing is dropped. */
+int ezl_dropout_add_fwd(const void* x, const void* bias, const void* residual, const ezl_dropout* drop, void* out, int64_t rows, int64_t n,
+                        void* stream);
+/* dx = what the draw left of dy, scaled (may be dy); dbias (HOST pointer, or NULL) = its column sums, taken before rounding.  (The residual's
+ * gradient is dy.)  workspace: ezl_column_sum_workspace_bytes(rows, n), 16-byte aligned; not needed without dbias. */
+int64_t ezl_column_sum_workspace_bytes(int64_t rows, int64_t n);
+int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void* dx, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
+                        int64_t rows, int64_t n, void* stream);
+
+/* ---- layer norm (base_modules/layers/fused_layer_norm.py, 'mixed_fused_norm'), and either norm behind dropout and the residual sum ----
+ * rows of h bf16, h % 8 == 0, h <= 8192.  kind: EZL_LAYER_NORM y = (s - mean) * rstd * weight + bias (bias may be NULL), EZL_RMS_NORM
+ * y = s * rstd * weight (bias NULL; with a residual, else ezl_rmsnorm_fwd); s = x, or with a residual s = residual + dropout(x + x_bias), x_bias and drop may be NULL.  sum_out, given with
+ * a residual and only then, receives s rounded; y and the statistics are of s as it was.  mean (layer norm only) and rstd: fp32 [rows], kept
+ * for backward.  A layer norm's weight may not be NULL. */
+#define EZL_LAYER_NORM 0
+#define EZL_RMS_NORM 1
+int ezl_norm_fwd(int kind, const void* x, const void* x_bias, const void* residual, const ezl_dropout* drop, const void* weight, const void* bias,
+                 void* y, void* sum_out, void* mean, void* rstd, int64_t rows, int64_t h, float eps, void* stream);
+/* s: the forward's x, or sum_out where it had a residual.  ds = gradient through the norm (+ dsum, the gradient of s from elsewhere, if given).  dx gets ds, or with
+ * `drop` what the draw left of it, scaled; dresidual (with `drop` and only then) gets ds: without, the two are one.  dweight, and dbias
+ * and dx_bias where wanted (HOST pointers, or NULL): column sums, added in a fixed order.  workspace: ezl_norm_bwd_workspace_bytes(rows, h) bytes, 16-byte aligned. */
+int64_t ezl_norm_bwd_workspace_bytes(int64_t rows, int64_t h);
+int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const void* s, const void* weight, const void* mean, const void* rstd,
+                 const ezl_dropout* drop, void* dx, void* dresidual, const ezl_layer_grad* dweight, const ezl_layer_grad* dbias,
+                 const ezl_layer_grad* dx_bias, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t h, void* stream);
+
 /* ---- SwiGLU: llama/transformer.py:220-222 + base_modules/layers/glu_activations.py:56-61 ---- */
 int ezl_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, void* stream);
 int ezl_swiglu_bwd(const void* dout, const void* gate, const void* up, void* dgate, void* dup, int64_t n, void* stream);
@@ -279,12 +323,7 @@ typedef struct {
     const void* position_ids;             /* int64 [b, s] or NULL */
     const void* cu_seqlens;               /* int32 [ndocs + 1] or NULL */
 } ezl_layer;
-/* where a parameter's gradient goes: an fp32 buffer (overwritten, or added to when accumulate != 0), else a bf16 one, else
- * (both NULL; not for the norms) nowhere */
-typedef struct {
-    void *f32, *bf16;
-    int accumulate;
-} ezl_layer_grad;
+/* a parameter without a gradient (both pointers NULL) is not allowed for the norms */
 enum { EZL_G_LN1, EZL_G_Q, EZL_G_K, EZL_G_V, EZL_G_O, EZL_G_LN2, EZL_G_GATE, EZL_G_UP, EZL_G_DOWN, EZL_G_BQ, EZL_G_BK, EZL_G_BV, EZL_G_COUNT };
 /* device bytes of the blocks below (256-byte aligned bases): which 0 = saved, 1 = forward temp, 2 = backward temp; -1: bad sizes */
 int64_t ezl_layer_bytes(const ezl_layer* layer, int which);
