@@ -32,6 +32,11 @@ class Dropout(ctypes.Structure):
     _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint32), ("drop_of_65536", ctypes.c_int32), ("step", _vp)]
 
 
+class Epilogue(ctypes.Structure):
+    """struct ezl_epilogue"""
+    _fields_ = [("bias", _vp), ("residual", _vp), ("pre", _vp), ("ldr", _i64), ("ldp", _i64), ("act", _i32)]
+
+
 _layerp = ctypes.POINTER(Layer)
 _dropp = ctypes.POINTER(Dropout)
 _gradp = ctypes.POINTER(LayerGrad)
@@ -68,6 +73,8 @@ SIGNATURES = {
     "ezl_bias_add": [_vp, _vp, _vp, _i64, _i64, _vp],
     "ezl_bias_grad": [_vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp],
     "ezl_gemm_bf16": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
+    "ezl_gemm_bf16_epilogue": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(Epilogue), _vp, _i64, _vp],
+    "ezl_act_bwd": [_i32, _vp, _vp, _vp, _gradp, _vp, _i64, _i64, _i64, _vp],
     "ezl_gemm_bf16_ksplit": [_i32, _vpp, _vpp, _vp, _i64, _i64, _i64p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
     "ezl_gemm_bf16_group": [_i32, _vpp, _vpp, _vpp, _i64p, _i64p, _i64, _i64p, _i64p, _i64p, _i32, _i32, _i32, ctypes.POINTER(_i32), _vp,
                             _i64, _vp],

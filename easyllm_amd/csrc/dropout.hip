@@ -1,4 +1,4 @@
-// Dropout with bias and residual sum, and the column sums of its backward pass (HBM-bound).
+// Dropout with bias and residual sum, the backward passes of it and of the activations, and their column sums (HBM-bound).
 #include "activation.h"
 #include "column_sums.h"
 #include "dropout.h"
@@ -84,6 +84,34 @@ __global__ __launch_bounds__(256) void dropout_sum_kernel(const DropSum a) {
     });
 }
 
+struct ActBwd {
+    const bf16_t *dy, *pre;
+    bf16_t* dpre;
+    float* partial;
+    int64_t groups;  // of 8 elements
+    int rows, n;
+};
+template <int ACT>
+__device__ __forceinline__ void act_bwd8(const ActBwd& a, int64_t at, float (&v)[8]) {
+    float p[8];
+    unpack8(ld_bf16x8(a.dy + at), v);
+    unpack8(ld_bf16x8(a.pre + at), p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= activation_slope(p[i], ACT);
+    st_bf16x8(a.dpre + at, pack8(v));
+}
+template <int ACT, bool SUMS>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const ActBwd a) {
+    if constexpr (SUMS) {
+        rows_with_column_sums(a.rows, a.n, a.partial, [&](int64_t at, float (&v)[8]) { act_bwd8<ACT>(a, at, v); });
+    } else {
+        for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < a.groups; g += (int64_t)gridDim.x * 256) {
+            float v[8];
+            act_bwd8<ACT>(a, g * 8, v);
+        }
+    }
+}
+
 struct SumsArgs {
     ColumnSum s[kColumnSums];
 };
@@ -165,6 +193,32 @@ extern "C" int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void
     const dim3 grid = sum_grid(rows, n);
     hipLaunchKernelGGL(dropout_sum_kernel, grid, dim3(256), 0, st, a);
     EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
+    const ColumnSum s = column_sum((const float*)workspace, dbias);
+    return column_sums(name, &s, 1, (int)grid.y, n, st);
+}
+
+extern "C" int ezl_act_bwd(int act, const void* dy, const void* pre, void* dpre, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
+                           int64_t rows, int64_t n, void* stream) {
+    const char* name = "ezl_act_bwd";
+    EZL_REQUIRE(act == kActGelu || act == kActGeluTanh, EZL_EINVAL, "%s: act must be EZL_ACT_GELU or EZL_ACT_GELU_TANH", name);
+    if (const int rc = sizes_check(name, rows, n)) return rc;
+    EZL_REQUIRE(rows == 0 || (dy && pre && dpre), EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(ezl_aligned16(dy) && ezl_aligned16(pre) && ezl_aligned16(dpre) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    hipStream_t st = (hipStream_t)stream;
+    const ActBwd a = {(const bf16_t*)dy, (const bf16_t*)pre, (bf16_t*)dpre, (float*)workspace, rows * (n / 8), (int)rows, (int)n};
+    if (!wanted(dbias)) {
+        if (rows == 0) return EZL_OK;
+        const dim3 grid(elementwise_grid(a.groups));
+        if (act == kActGelu) hipLaunchKernelGGL((act_bwd_kernel<kActGelu, false>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((act_bwd_kernel<kActGeluTanh, false>), grid, dim3(256), 0, st, a);
+        EZL_LAUNCH_CHECK("ezl_act_bwd");
+        return EZL_OK;
+    }
+    EZL_REQUIRE(workspace && workspace_bytes >= ezl_column_sum_workspace_bytes(rows, n), EZL_EINVAL, "%s: workspace missing or too small", name);
+    const dim3 grid = sum_grid(rows, n);
+    if (act == kActGelu) hipLaunchKernelGGL((act_bwd_kernel<kActGelu, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((act_bwd_kernel<kActGeluTanh, true>), grid, dim3(256), 0, st, a);
+    EZL_LAUNCH_CHECK("ezl_act_bwd");
     const ColumnSum s = column_sum((const float*)workspace, dbias);
     return column_sums(name, &s, 1, (int)grid.y, n, st);
 }

@@ -30,6 +30,7 @@
 // tiles of gemm_small.hip (see choose_plan).
 #include "gemm_tile.h"
 #include "gemm_list.h"
+#include "../../include/ezl.h"
 
 #include <math.h>
 
@@ -95,10 +96,10 @@ struct SchedPhase {
 // accesses per flop).  A 64-wide K tile is worked off in four phases (k half, M half): a phase issues 16 MFMAs on 4 A and
 // 4 B fragments while the fragments of the next phase are read from LDS into the other register set.
 //
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL>
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, class EPI = NoEpilogue>
 __global__ __launch_bounds__(512) void gemm_d2l_kernel(const bf16_t* __restrict__ A, const bf16_t* __restrict__ B, OutT* __restrict__ C,
                                                        int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int accumulate,
-                                                       int tiles_m, int tiles_n, const SplitPlan plan, const KSegments seg) {
+                                                       int tiles_m, int tiles_n, const SplitPlan plan, const KSegments seg, const EPI epi) {
     constexpr int NW = 8, WAVES_N = 4;
     __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * DTILE];  // A0 B0 A1 B1
     const int tid = threadIdx.x, lane = tid & 63;
@@ -236,6 +237,10 @@ __global__ __launch_bounds__(512) void gemm_d2l_kernel(const bf16_t* __restrict_
     }
     const int mrem = M - m0 < BM ? M - m0 : BM, nrem = N - n0;
     OutT* Ct = C + (int64_t)m0 * ldc + n0;
+    if constexpr (std::is_same_v<EPI, Epilogue>) {
+        store_tile_epilogue<8, 4>(acc, Ct, ldc, mrem, nrem, arow, brow, lane, epi.at(m0, n0));
+        return;
+    }
     if (N % 8 == 0 && ldc % (16 / (int)sizeof(OutT)) == 0 && ((uintptr_t)C & 15) == 0 && ldc < (1 << 21) / ((int)sizeof(OutT) / 2)) {
         store_tile_flags<8, 4, OutT, true, A_KC && B_KC>(acc, Ct, ldc, mrem, nrem, arow, brow, lane, accumulate);
         return;
@@ -293,11 +298,11 @@ __global__ __launch_bounds__(512) void gemm_d2l_kernel(const bf16_t* __restrict_
 // as 128 x 128 tiles in 453 us, as these in 387; its gate and up products (704 tiles) as 256 x 128 tiles in 208, as these in 155.  (One
 // product in a list of one would save the form without it, but costs 6 us a launch: a tile's scalar loads depend on one another.)
 struct NoList {};
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, bool LIST = false, int TBM = 256>
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, bool LIST = false, int TBM = 256, class EPI = NoEpilogue>
 __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restrict__ A, const bf16_t* __restrict__ B, OutT* __restrict__ C,
                                                          int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int accumulate,
                                                          int tiles_m, int tiles_n, int items, const SplitPlan plan, const KSegments seg,
-                                                         const std::conditional_t<LIST, GemmSmallArgs, NoList> list) {
+                                                         const std::conditional_t<LIST, GemmSmallArgs, NoList> list, const EPI epi) {
     static_assert(!LIST || (A_KC == B_KC && !MULTI), "lists are of forward products or weight gradients");
     constexpr int TM = TBM / 32, NA = TM, NB = 8;  // MFMA tiles of a wave, one below the other; wave loads of an A and a B tile
     constexpr int ASTAGE = TBM * BK;
@@ -558,7 +563,12 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
         } else {
             const int mrem = M - it.m0 < TBM ? M - it.m0 : TBM;
             OutT* Ct = C + (int64_t)it.m0 * ld + it.n0;
-            store_tile_flags<TM, 8, OutT, true, A_KC && B_KC>(acc, Ct, ld, mrem, N - it.n0, arow, brow, lane, accumulate);
+            if constexpr (std::is_same_v<EPI, Epilogue>) {
+                Epilogue e = epi;
+                int l = lane;
+                asm volatile("" : "+s"(e.ldr), "+s"(e.ldp), "+v"(l));  // (nor what these make)
+                store_tile_epilogue<TM, 8>(acc, Ct, ld, mrem, N - it.n0, arow, brow, l, e.at(it.m0, it.n0));
+            } else store_tile_flags<TM, 8, OutT, true, A_KC && B_KC>(acc, Ct, ld, mrem, N - it.n0, arow, brow, lane, accumulate);
         }
         if (!more) break;
         it = next;
@@ -595,9 +605,9 @@ __device__ __forceinline__ f32x4 sum_partials(const float* __restrict__ src, siz
 // product, tiles x shares: 1531 x 4096, 128 of 192 rows x 2 16.3 -> 10.2; 2048 x 768, 24 x 10 18.0 -> 10.4; 1167 x 1024, 20 x 12 17.1 -> 9.3; 4000 x 2048, 128 x 2
 // 22.3 -> 12.8; fp32, 50304 x 1024, 20 x 2 5.8 -> 4.6.)
 constexpr int kReduceRows = 4;  // rows of a block
-template <typename OutT, int TBM>
+template <typename OutT, int TBM, class EPI = NoEpilogue>
 __global__ __launch_bounds__(256) void gemm_split_reduce_kernel(OutT* __restrict__ C, int M, int N, int64_t ldc, int accumulate,
-                                                                int tiles_m, int tiles_n, const SplitPlan plan) {
+                                                                int tiles_m, int tiles_n, const SplitPlan plan, const EPI epi) {
     constexpr int PIECES = TBM / kReduceRows;
     const int t = blockIdx.x / PIECES;  // split tile
     int tm, tn;
@@ -606,6 +616,11 @@ __global__ __launch_bounds__(256) void gemm_split_reduce_kernel(OutT* __restrict
     const int row = tm * TBM + rl, col = tn * BN + cl;
     if (row >= M || col >= N) return;
     f32x4 v = sum_partials(plan.partial + (size_t)t * plan.nsplit * (TBM * BN) + (size_t)rl * BN + cl, TBM * BN, plan.nsplit);
+    if constexpr (std::is_same_v<EPI, Epilogue>) {
+        float x[4] = {v[0], v[1], v[2], v[3]};
+        store_epilogue<4>(x, C, ldc, row, col, epi);
+        return;
+    }
     if (accumulate & kRoundResult) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (float)(bf16_t)v[e];
@@ -981,7 +996,7 @@ void launch_list_256(GemmSmallArgs& a, int count, void* workspace, int64_t works
     const int items = plan.full + plan.rest * plan.nsplit;
 #define EZL_LIST(KTAIL)                                                                                                                 \
     hipLaunchKernelGGL((gemm_w4_kernel<KC, KC, OutT, false, KTAIL, true>), w4_grid(items), dim3(256), 0, st, nullptr, nullptr,       \
-                       (OutT*)nullptr, 0, 0, a.K, (int64_t)0, (int64_t)0, (int64_t)0, 0, 0, 0, items, plan, KSegments(), a)
+                       (OutT*)nullptr, 0, 0, a.K, (int64_t)0, (int64_t)0, (int64_t)0, 0, 0, 0, items, plan, KSegments(), a, NoEpilogue())
     if (a.K % BK == 0) EZL_LIST(false);
     else EZL_LIST(true);
 #undef EZL_LIST
@@ -994,9 +1009,9 @@ void launch_list_256(GemmSmallArgs& a, int count, void* workspace, int64_t works
 
 // large tiles: the 4-wave kernel in either height, or the 8-wave one.  ktot: length of the whole reduction, from which the workspace was sized (the K tiles of
 // several pairs can be one or two more)
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL>
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, class EPI = NoEpilogue>
 void launch_large(int kind, bool lines, int64_t ktot, const void* A, const void* B, void* C, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int accumulate,
-                  void* workspace, int64_t workspace_bytes, const KSegments& seg, hipStream_t st) {
+                  void* workspace, int64_t workspace_bytes, const KSegments& seg, hipStream_t st, const EPI& epi = EPI()) {
     const int nk = MULTI ? seg.nk : (K + BK - 1) / BK;
     // (fp32 input gradients stay with the 8-wave kernel)
     constexpr bool HAS_W4 = A_KC ? B_KC || sizeof(OutT) == 2 : !B_KC;
@@ -1011,8 +1026,8 @@ void launch_large(int kind, bool lines, int64_t ktot, const void* A, const void*
     w4 = w4 && (kind == kTile192x256 || w4_pays(form, plan, nk, ldb));
     if constexpr (HAS_W4) {
 #define EZL_W4(TBM)                                                                                                                            \
-    hipLaunchKernelGGL((gemm_w4_kernel<A_KC, B_KC, OutT, MULTI, KTAIL, false, TBM>), w4_grid(items), dim3(256), 0, st, (const bf16_t*)A,     \
-                       (const bf16_t*)B, (OutT*)C, M, N, K, lda, ldb, ldc, accumulate, tiles_m, tiles_n, items, plan, seg, NoList())
+    hipLaunchKernelGGL((gemm_w4_kernel<A_KC, B_KC, OutT, MULTI, KTAIL, false, TBM, EPI>), w4_grid(items), dim3(256), 0, st, (const bf16_t*)A, \
+                       (const bf16_t*)B, (OutT*)C, M, N, K, lda, ldb, ldc, accumulate, tiles_m, tiles_n, items, plan, seg, NoList(), epi)
         if (w4 && kind == kTile192x256) {
             if constexpr (HAS_192) EZL_W4(192);
         } else if (w4) {
@@ -1021,11 +1036,11 @@ void launch_large(int kind, bool lines, int64_t ktot, const void* A, const void*
 #undef EZL_W4
     }
     if (!w4)
-        hipLaunchKernelGGL((gemm_d2l_kernel<A_KC, B_KC, OutT, MULTI, KTAIL>), dim3((unsigned)items), dim3(512), 0, st, (const bf16_t*)A,
-                           (const bf16_t*)B, (OutT*)C, M, N, K, lda, ldb, ldc, accumulate, tiles_m, tiles_n, plan, seg);
+        hipLaunchKernelGGL((gemm_d2l_kernel<A_KC, B_KC, OutT, MULTI, KTAIL, EPI>), dim3((unsigned)items), dim3(512), 0, st, (const bf16_t*)A,
+                           (const bf16_t*)B, (OutT*)C, M, N, K, lda, ldb, ldc, accumulate, tiles_m, tiles_n, plan, seg, epi);
 #define EZL_REDUCE(TBM)                                                                                                                    \
-    hipLaunchKernelGGL((gemm_split_reduce_kernel<OutT, TBM>), dim3((unsigned)(plan.rest * (TBM / kReduceRows))), dim3(256), 0, st, (OutT*)C, M, N, ldc, \
-                       accumulate, tiles_m, tiles_n, plan)
+    hipLaunchKernelGGL((gemm_split_reduce_kernel<OutT, TBM, EPI>), dim3((unsigned)(plan.rest * (TBM / kReduceRows))), dim3(256), 0, st, (OutT*)C, M, N, ldc, \
+                       accumulate, tiles_m, tiles_n, plan, epi)
     if (plan.nsplit > 1) {
         if (kind == kTile192x256) EZL_REDUCE(192);
         else EZL_REDUCE(256);
@@ -1037,9 +1052,9 @@ template <typename OutT>
 bool small_stores_ok(int64_t ldc) {
     return ldc * (int64_t)sizeof(OutT) * 256 < (1LL << 31);
 }
-template <bool A_KC, bool B_KC, typename OutT>
+template <bool A_KC, bool B_KC, typename OutT, class EPI = NoEpilogue>
 void launch(const void* A, const void* B, void* C, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int accumulate,
-            void* workspace, int64_t workspace_bytes, hipStream_t st) {
+            void* workspace, int64_t workspace_bytes, hipStream_t st, const EPI& epi = EPI()) {
     constexpr int form = A_KC ? (B_KC ? (sizeof(OutT) == 4 ? 4 : 0) : 1) : (sizeof(OutT) == 4 ? 2 : 3);
     constexpr Class cls = !A_KC ? kWeightGradient : (B_KC ? kForward : kInputGradient);
     const bool lines = whole_lines(cls, M, N, K);
@@ -1053,15 +1068,16 @@ void launch(const void* A, const void* B, void* C, int M, int N, int K, int64_t 
                 a.p[0] = {(const bf16_t*)A, (const bf16_t*)B, C, lda, ldb, ldc, M, N, 0, 0, 0, accumulate};
                 a.K = K;
                 a.partial = (float*)workspace;
-                gemm_small_launch(form, false, plan, a, 1, st);
+                if constexpr (std::is_same_v<EPI, Epilogue>) gemm_small_launch(form, false, plan, a, 1, st, &epi);
+                else gemm_small_launch(form, false, plan, a, 1, st);
                 return;
             }
         }
     }
     if (K % BK == 0)
-        launch_large<A_KC, B_KC, OutT, false, false>(kind, lines, K, A, B, C, M, N, K, lda, ldb, ldc, accumulate, workspace, workspace_bytes, KSegments(), st);
+        launch_large<A_KC, B_KC, OutT, false, false>(kind, lines, K, A, B, C, M, N, K, lda, ldb, ldc, accumulate, workspace, workspace_bytes, KSegments(), st, epi);
     else
-        launch_large<A_KC, B_KC, OutT, false, true>(kind, lines, K, A, B, C, M, N, K, lda, ldb, ldc, accumulate, workspace, workspace_bytes, KSegments(), st);
+        launch_large<A_KC, B_KC, OutT, false, true>(kind, lines, K, A, B, C, M, N, K, lda, ldb, ldc, accumulate, workspace, workspace_bytes, KSegments(), st, epi);
 }
 
 // C = 0 for an empty reduction (a fill kernel rather than a memset node, so the call can be captured into a graph)
@@ -1140,6 +1156,28 @@ extern "C" int ezl_gemm_bf16(const void* A, const void* B, void* C, int64_t M, i
     return EZL_OK;
 }
 
+// y = act(A B^T + bias) + residual: the forward form with an epilogue.
+extern "C" int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
+                                      const ezl_epilogue* epilogue, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* name = "ezl_gemm_bf16_epilogue";
+    EZL_REQUIRE(M >= 0 && N >= 0 && K > 0 && epilogue, EZL_EINVAL, "%s: negative size, empty reduction or no epilogue", name);
+    const Epilogue e = {(const bf16_t*)epilogue->bias, (const bf16_t*)epilogue->residual, (bf16_t*)epilogue->pre, epilogue->residual ? epilogue->ldr : 0,
+                        epilogue->pre ? epilogue->ldp : 0, epilogue->act};
+    EZL_REQUIRE(e.act == kActNone || e.act == kActGelu || e.act == kActGeluTanh, EZL_EINVAL, "%s: act must be EZL_ACT_NONE, EZL_ACT_GELU or EZL_ACT_GELU_TANH", name);
+    if (M == 0 || N == 0) return EZL_OK;
+    EZL_REQUIRE(C, EZL_EINVAL, "%s: null pointer", name);
+    if (const int rc = check_operands(A, B, M, N, K, lda, ldb, ldc, 1, 1)) return rc;
+    // (16-byte stores at 31-bit byte offsets inside a tile)
+    EZL_REQUIRE(N % 8 == 0 && ldc % 8 == 0 && e.ldr % 8 == 0 && e.ldp % 8 == 0 && ldc < (1LL << 21) && e.ldr < (1LL << 21) && e.ldp < (1LL << 21), EZL_EUNSUPPORTED,
+                "%s: N and row strides must be multiples of 8, strides below 2^21", name);
+    EZL_REQUIRE((!e.residual || e.ldr >= N) && (!e.pre || e.ldp >= N), EZL_EINVAL, "%s: leading dimension too small", name);
+    EZL_REQUIRE(ezl_aligned16(C) && ezl_aligned16(e.bias) && ezl_aligned16(e.residual) && ezl_aligned16(e.pre) && ezl_aligned16(workspace), EZL_EINVAL,
+                "%s: pointers must be 16-byte aligned", name);
+    launch<true, true, bf16_t, Epilogue>(A, B, C, (int)M, (int)N, (int)K, lda, ldb, ldc, 0, workspace, workspace_bytes, (hipStream_t)stream, e);
+    EZL_LAUNCH_CHECK("ezl_gemm_bf16_epilogue");
+    return EZL_OK;
+}
+
 int gemm_forward_add(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
     EZL_REQUIRE(M > 0 && N > 0 && K > 0 && C, EZL_EINVAL, "ezl_gemm_bf16: null pointer or empty product");
     if (const int rc = check_operands(A, B, M, N, K, K, K, N, 1, 1)) return rc;
@@ -1210,7 +1248,8 @@ extern "C" int ezl_gemm_bf16_ksplit(int count, const void* const* A, const void*
         }
     }
     (tail ? launch_large<true, false, bf16_t, true, true> : launch_large<true, false, bf16_t, true, false>)(
-        kind, whole_lines(kInputGradient, M, N, ktot), ktot, A[0], B[0], C, (int)M, (int)N, (int)K[0], lda, ldb, ldc, accumulate, workspace, workspace_bytes, seg, (hipStream_t)stream);
+        kind, whole_lines(kInputGradient, M, N, ktot), ktot, A[0], B[0], C, (int)M, (int)N, (int)K[0], lda, ldb, ldc, accumulate, workspace, workspace_bytes, seg, (hipStream_t)stream,
+        NoEpilogue());
     EZL_LAUNCH_CHECK("ezl_gemm_bf16_ksplit");
     return EZL_OK;
 }

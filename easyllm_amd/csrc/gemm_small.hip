@@ -38,11 +38,12 @@ template <typename OutT>
 __device__ __forceinline__ bool vector_stores(const GemmProblem& p) {
     return p.N % 8 == 0 && p.ldc % (16 / (int)sizeof(OutT)) == 0 && ((uintptr_t)p.C & 15) == 0;
 }
-template <bool FORWARD, int TM, int TN, typename OutT>
-__device__ __forceinline__ void store_tile(const f32x4 (&acc)[TM][TN], const GemmProblem& p, int m0, int n0, int row0, int col0, int lane) {
+template <bool FORWARD, int TM, int TN, typename OutT, class EPI>
+__device__ __forceinline__ void store_tile(const f32x4 (&acc)[TM][TN], const GemmProblem& p, int m0, int n0, int row0, int col0, int lane, const EPI& epi) {
     OutT* C = (OutT*)p.C + (int64_t)m0 * p.ldc + n0;
     const int mrem = p.M - m0 < 256 ? p.M - m0 : 256, nrem = p.N - n0;  // (no tile is taller: the range fits 31 bits)
-    if (vector_stores<OutT>(p)) store_tile_flags<TM, TN, OutT, true, FORWARD>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, p.accumulate);
+    if constexpr (std::is_same_v<EPI, Epilogue>) store_tile_epilogue<TM, TN>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, epi.at(m0, n0));
+    else if (vector_stores<OutT>(p)) store_tile_flags<TM, TN, OutT, true, FORWARD>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, p.accumulate);
     else store_tile_flags<TM, TN, OutT, false, FORWARD>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, p.accumulate);
 }
 
@@ -80,8 +81,8 @@ __device__ __forceinline__ void zero_acc(f32x4 (&acc)[TM][TN]) {
 // 144 KiB) let the wave loads of a K tile (12) go out over both phases, one every fifth MFMA (the address unit needs 48 of the
 // 64 MFMA slots of a K tile), two K tiles ahead of their use; a stage is free from the barrier in front of its K tile's second
 // phase on, because that phase works on fragments already in registers.
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, int TBM, int TBN>
-__global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs args) {
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, bool KTAIL, int TBM, int TBN, class EPI = NoEpilogue>
+__global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs args, const EPI epi) {
     constexpr int TM = TBM / 32, TN = TBN / 32;
     constexpr int STAGE = (TBM + TBN) * BK;
     __shared__ __attribute__((aligned(1024))) bf16_t smem[3 * STAGE];
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs a
     }
     phase_b(smem, smem, no{}, no{});
     if (args.nsplit > 1) store_partial<TM, TN, TBM, TBN>(acc, args, tile, part, arow, brow, lane);
-    else store_tile<A_KC && B_KC, TM, TN, OutT>(acc, p, m0, n0, arow, brow, lane);
+    else store_tile<A_KC && B_KC, TM, TN, OutT>(acc, p, m0, n0, arow, brow, lane, epi);
 }
 
 // =================================================================================================
@@ -203,8 +204,8 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs a
 // =================================================================================================
 // One barrier per K tile and no hand-laid schedule: the CU's other workgroups cover a wave's waits.  128: two stages (64 KiB),
 // two workgroups per CU.  64: four stages (64 KiB); such launches are latency-bound and a deep queue of loads is what helps.
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI, int TB, int ST>
-__global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs args) {
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, int TB, int ST, class EPI = NoEpilogue>
+__global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs args, const EPI epi) {
     constexpr int T = TB / 32;  // MFMA tiles per wave and direction
     constexpr int STAGE = 2 * TB * BK;
     __shared__ __attribute__((aligned(1024))) bf16_t smem[ST * STAGE];
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs ar
         free_stage = free_stage + 1 == ST ? 0 : free_stage + 1;
     }
     if (args.nsplit > 1) store_partial<T, T, TB, TB>(acc, args, tile, part, arow, brow, lane);
-    else store_tile<A_KC && B_KC, T, T, OutT>(acc, p, m0, n0, arow, brow, lane);
+    else store_tile<A_KC && B_KC, T, T, OutT>(acc, p, m0, n0, arow, brow, lane, epi);
 }
 
 // =================================================================================================
@@ -274,8 +275,8 @@ __global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs ar
 // Few tiles and a long reduction (a weight gradient of a narrow layer): each wave multiplies the whole tile over every eighth
 // K tile out of its own 16 KiB of LDS, with no barrier in the loop, so eight K tiles are in flight per workgroup; the eight
 // sums are added in wave order at the end.
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI>
-__global__ __launch_bounds__(512) void gemm_64_waves_kernel(const GemmSmallArgs args) {
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, class EPI = NoEpilogue>
+__global__ __launch_bounds__(512) void gemm_64_waves_kernel(const GemmSmallArgs args, const EPI epi) {
     constexpr int NW = 8, STAGE = 2 * 64 * BK;
     __shared__ __attribute__((aligned(1024))) bf16_t smem[NW * STAGE];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -346,12 +347,12 @@ __global__ __launch_bounds__(512) void gemm_64_waves_kernel(const GemmSmallArgs 
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[0][q][r] += x[r];
         }
-    store_tile<A_KC && B_KC, 1, 2, OutT>(sum, p, m0, n0, (wave >> 1) * 16, (wave & 1) * 32, lane);
+    store_tile<A_KC && B_KC, 1, 2, OutT>(sum, p, m0, n0, (wave >> 1) * 16, (wave & 1) * 32, lane, epi);
 }
 
 // C tile (=|+=) sum of the nsplit fp32 partial tiles, added in index order; a thread owns 8 consecutive columns of one row
-template <typename OutT>
-__global__ __launch_bounds__(256) void small_reduce_kernel(const GemmSmallArgs args, int tbm, int tbn, int first_tile) {
+template <typename OutT, class EPI = NoEpilogue>
+__global__ __launch_bounds__(256) void small_reduce_kernel(const GemmSmallArgs args, int tbm, int tbn, int first_tile, const EPI epi) {
     const int per_tile = tbm * tbn / 2048;  // workgroups per tile
     const int local = blockIdx.x / per_tile, tile = first_tile + local;
     const GemmProblem p = problem_of(args, tile);
@@ -371,6 +372,10 @@ __global__ __launch_bounds__(256) void small_reduce_kernel(const GemmSmallArgs a
         const f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) { v[r] += x[r]; v[4 + r] += y[r]; }
+    }
+    if constexpr (std::is_same_v<EPI, Epilogue>) {
+        store_epilogue<8>(v, (bf16_t*)p.C, p.ldc, row, col, epi);
+        return;
     }
     if (p.accumulate & kRoundResult) {
 #pragma unroll
@@ -401,24 +406,24 @@ __global__ __launch_bounds__(256) void small_reduce_kernel(const GemmSmallArgs a
     }
 }
 
-template <bool A_KC, bool B_KC, typename OutT, bool MULTI>
-void launch_kind(int kind, const GemmSmallArgs& a, bool tail, hipStream_t st) {
+template <bool A_KC, bool B_KC, typename OutT, bool MULTI, class EPI = NoEpilogue>
+void launch_kind(int kind, const GemmSmallArgs& a, bool tail, hipStream_t st, const EPI& epi = EPI()) {
     const dim3 grid((unsigned)(a.ntiles * a.nsplit));
     switch (kind) {
 #define EZL_WIDE(BM_, BN_)                                                                                                                 \
-    if (tail) hipLaunchKernelGGL((gemm_wide_kernel<A_KC, B_KC, OutT, MULTI, true, BM_, BN_>), grid, dim3(256), 0, st, a);                  \
-    else hipLaunchKernelGGL((gemm_wide_kernel<A_KC, B_KC, OutT, MULTI, false, BM_, BN_>), grid, dim3(256), 0, st, a);                      \
+    if (tail) hipLaunchKernelGGL((gemm_wide_kernel<A_KC, B_KC, OutT, MULTI, true, BM_, BN_, EPI>), grid, dim3(256), 0, st, a, epi);        \
+    else hipLaunchKernelGGL((gemm_wide_kernel<A_KC, B_KC, OutT, MULTI, false, BM_, BN_, EPI>), grid, dim3(256), 0, st, a, epi);            \
     break
         case kTile256x128: EZL_WIDE(256, 128);
         case kTile192x128: EZL_WIDE(192, 128);
 #undef EZL_WIDE
-        case kTile128: hipLaunchKernelGGL((gemm_square_kernel<A_KC, B_KC, OutT, MULTI, 128, 2>), grid, dim3(256), 0, st, a); break;
-        case kTile64: hipLaunchKernelGGL((gemm_square_kernel<A_KC, B_KC, OutT, MULTI, 64, 4>), grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL((gemm_64_waves_kernel<A_KC, B_KC, OutT, MULTI>), grid, dim3(512), 0, st, a); break;
+        case kTile128: hipLaunchKernelGGL((gemm_square_kernel<A_KC, B_KC, OutT, MULTI, 128, 2, EPI>), grid, dim3(256), 0, st, a, epi); break;
+        case kTile64: hipLaunchKernelGGL((gemm_square_kernel<A_KC, B_KC, OutT, MULTI, 64, 4, EPI>), grid, dim3(256), 0, st, a, epi); break;
+        default: hipLaunchKernelGGL((gemm_64_waves_kernel<A_KC, B_KC, OutT, MULTI, EPI>), grid, dim3(512), 0, st, a, epi); break;
     }
     if (a.nsplit > 1) {
         const int tbm = (int)gemm_kind_bm(kind), tbn = (int)gemm_kind_bn(kind);
-        hipLaunchKernelGGL((small_reduce_kernel<OutT>), dim3((unsigned)(a.ntiles * (tbm * tbn / 2048))), dim3(256), 0, st, a, tbm, tbn, 0);
+        hipLaunchKernelGGL((small_reduce_kernel<OutT, EPI>), dim3((unsigned)(a.ntiles * (tbm * tbn / 2048))), dim3(256), 0, st, a, tbm, tbn, 0, epi);
     }
 }
 
@@ -444,15 +449,16 @@ void gemm_tile_grids(const GemmPlan& plan, GemmSmallArgs& a, int count) {
 void gemm_small_reduce(int kind, bool fp32, int first_tile, const GemmSmallArgs& a, hipStream_t stream) {
     const int bm = (int)gemm_kind_bm(kind), bn = (int)gemm_kind_bn(kind);
     const dim3 grid((unsigned)((a.ntiles - first_tile) * (bm * bn / 2048)));
-    if (fp32) hipLaunchKernelGGL((small_reduce_kernel<float>), grid, dim3(256), 0, stream, a, bm, bn, first_tile);
-    else hipLaunchKernelGGL((small_reduce_kernel<bf16_t>), grid, dim3(256), 0, stream, a, bm, bn, first_tile);
+    if (fp32) hipLaunchKernelGGL((small_reduce_kernel<float>), grid, dim3(256), 0, stream, a, bm, bn, first_tile, NoEpilogue());
+    else hipLaunchKernelGGL((small_reduce_kernel<bf16_t>), grid, dim3(256), 0, stream, a, bm, bn, first_tile, NoEpilogue());
 }
 
-void gemm_small_launch(int form, bool multi, const GemmPlan& plan, GemmSmallArgs& a, int count, hipStream_t stream) {
+void gemm_small_launch(int form, bool multi, const GemmPlan& plan, GemmSmallArgs& a, int count, hipStream_t stream, const Epilogue* epilogue) {
     gemm_tile_grids(plan, a, count);
     bool tail = a.K % BK != 0;
     if (multi) tail = tail || a.seg.K1 % BK != 0 || a.seg.K2 % BK != 0;
-    if (form == 0) launch_kind<true, true, bf16_t, false>(plan.kind, a, tail, stream);
+    if (epilogue) launch_kind<true, true, bf16_t, false, Epilogue>(plan.kind, a, tail, stream, *epilogue);
+    else if (form == 0) launch_kind<true, true, bf16_t, false>(plan.kind, a, tail, stream);
     else if (form == 1 && multi) launch_kind<true, false, bf16_t, true>(plan.kind, a, tail, stream);
     else if (form == 1) launch_kind<true, false, bf16_t, false>(plan.kind, a, tail, stream);
     else if (form == 4) launch_kind<true, true, float, false>(plan.kind, a, tail, stream);

@@ -1,5 +1,6 @@
 // Device code shared by the GEMM kernels (gemm.hip, gemm_small.hip): operand tiles in LDS, MFMA fragments, K segments.
 #pragma once
+#include "activation.h"
 #include "common.h"
 
 #include <type_traits>
@@ -20,6 +21,21 @@ struct KSegments {
 // Kernels take it in the bits of `accumulate`: the product is rounded to bf16 first (logits that are handed out in fp32; with bit 0, a forward product
 // added to a bf16 tensor as a launch of its own would add the two).
 constexpr int kRoundResult = 2;
+
+// What a forward product's values go through on their way from the accumulators to a bf16 C: y = act(v + bias) + residual, fp32 up to the one
+// rounding; v + bias also goes to `pre` (rounded: the activation's backward reads it).  bias [N], residual (may be C) and pre [M, N] may
+// be null.  Rows start on 16 bytes, N is a multiple of 8.
+struct NoEpilogue {};
+struct Epilogue {
+    const bf16_t *bias, *residual;
+    bf16_t* pre;
+    int64_t ldr, ldp;
+    int act;
+    // as seen from row m, column n on
+    __device__ __forceinline__ Epilogue at(int64_t m, int64_t n) const {
+        return {bias ? bias + n : nullptr, residual ? residual + m * ldr + n : nullptr, pre ? pre + m * ldp + n : nullptr, ldr, ldp, act};
+    }
+};
 
 namespace {
 
@@ -335,7 +351,97 @@ __device__ __forceinline__ void store_tile_impl(const f32x4 (&acc)[TM][TN], OutT
     }
 }
 
-// as above with the kernel's flags: bit 0 accumulate, kRoundResult (only where the form has it: MAY_ROUND; an fp32 result has it without bit 0, a bf16
+// The same for a forward product with an epilogue (pointers at the tile's corner): bias, residual and pre are buffers like C, a lane's bias is read
+// once, a row's residual in front of the stores of the row before it.
+template <int ACT, int TM, int TN>
+__device__ __forceinline__ void store_tile_act(const f32x4 (&acc)[TM][TN], bf16_t* C, int64_t ldc, int mrem, int nrem, int row0, int col0, int lane,
+                                               const Epilogue& e) {
+    constexpr uint32_t kOut = 0x80000000u;
+    const auto matrix = [&](const bf16_t* p, int64_t ld) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(p)), 0, (uint32_t)(((int64_t)(mrem - 1) * ld + nrem) * 2), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc), rbuf = matrix(e.residual, e.ldr), pbuf = matrix(e.pre, e.ldp);
+    const bool has_residual = e.residual != nullptr, has_pre = e.pre != nullptr;
+    const int g = lane >> 4;
+    uint32_t col_off[TN / 2];
+    bf16x8 bias[TN / 2];
+#pragma unroll
+    for (int jp = 0; jp < TN / 2; ++jp) {
+        const int col = col0 + (2 * jp + (g & 1)) * 16 + 8 * (g >> 1);
+        col_off[jp] = col < nrem ? (uint32_t)col * 2 : kOut;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) bias[jp][r] = (bf16_t)0.0f;
+        if (e.bias && col < nrem) bias[jp] = ld_bf16x8(e.bias + col);
+    }
+    const uint32_t row = (uint32_t)(row0 + (lane & 15));
+    // (256 rows span less than 2 GiB: past the last column an offset stays out of range)
+    const auto offset = [&](int i, int jp, int64_t ld) { return col_off[jp] + row * (uint32_t)(ld * 2) + i * (uint32_t)(32 * ld); };
+    u32x4 old[2][TN / 2];
+    const auto fetch = [&](int i) {
+#pragma unroll
+        for (int jp = 0; jp < TN / 2; ++jp) old[i & 1][jp] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rbuf, offset(i, jp, e.ldr), 0, 0));
+    };
+    if (has_residual) fetch(0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        if (has_residual && i + 1 < TM) fetch(i + 1);
+#pragma unroll
+        for (int jp = 0; jp < TN / 2; ++jp) {
+            const f32x4 va = from_agprs<TM * TN>(acc[i][2 * jp]), vb = from_agprs<TM * TN>(acc[i][2 * jp + 1]);
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(va[r]), __float_as_uint(vb[r]), false, false);
+                v[r] = __uint_as_float(sw[0]);
+                v[4 + r] = __uint_as_float(sw[1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] += (float)bias[jp][r];
+            if (has_pre) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(v)), pbuf, offset(i, jp, e.ldp), 0, 0);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = activation(v[r], ACT);
+            if (has_residual) {
+                const bf16x8 o = __builtin_bit_cast(bf16x8, old[i & 1][jp]);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] += (float)o[r];
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(v)), cbuf, offset(i, jp, ldc), 0, 0);
+            if constexpr (TM * TN >= 48) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+template <int TM, int TN>
+__device__ __forceinline__ void store_tile_epilogue(const f32x4 (&acc)[TM][TN], bf16_t* C, int64_t ldc, int mrem, int nrem, int row0, int col0, int lane,
+                                                    const Epilogue& e) {
+    if (e.act == kActGelu) store_tile_act<kActGelu, TM, TN>(acc, C, ldc, mrem, nrem, row0, col0, lane, e);
+    else if (e.act == kActGeluTanh) store_tile_act<kActGeluTanh, TM, TN>(acc, C, ldc, mrem, nrem, row0, col0, lane, e);
+    else store_tile_act<kActNone, TM, TN>(acc, C, ldc, mrem, nrem, row0, col0, lane, e);
+}
+// N consecutive values of row m from column n on (whole: the kernels that add partial tiles)
+template <int N>
+__device__ __forceinline__ void store_epilogue(float (&v)[N], bf16_t* C, int64_t ldc, int64_t m, int64_t n, const Epilogue& e) {
+    typedef bf16_t vec __attribute__((ext_vector_type(N)));
+    const auto add = [&](const bf16_t* p) {
+        const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] += (float)x[r];
+    };
+    const auto store = [&](bf16_t* p) {
+        vec x;
+#pragma unroll
+        for (int r = 0; r < N; ++r) x[r] = (bf16_t)v[r];
+        *reinterpret_cast<vec*>(p) = x;
+    };
+    if (e.bias) add(e.bias + n);
+    if (e.pre) store(e.pre + m * e.ldp + n);
+    if (e.act)
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = activation(v[r], e.act);
+    if (e.residual) add(e.residual + m * e.ldr + n);
+    store(C + m * ldc + n);
+}
+
+// as store_tile_impl with the kernel's flags: bit 0 accumulate, kRoundResult (only where the form has it: MAY_ROUND; an fp32 result has it without bit 0, a bf16
 // one, which is rounded as it is stored, with it)
 template <int TM, int TN, typename OutT, bool VEC, bool MAY_ROUND>
 __device__ __forceinline__ void store_tile_flags(const f32x4 (&acc)[TM][TN], OutT* C, int64_t ldc, int mrem, int nrem, int row0, int col0,
@@ -379,8 +485,9 @@ struct GemmPlan {
 };
 // form 0: A, B k-contiguous, bf16 result; 1: A k-contiguous, bf16 result (multi: over K segments); 2 / 3: neither, fp32 / bf16
 // result; 4: as 0 with an fp32 result.  Sets the tile grids in `a` and launches; 256 rows of every problem's C must span less than 2 GiB.
+// epilogue (form 0, one product, N a multiple of 8, rows on 16 bytes): null, or what its values go through
 __attribute__((visibility("hidden"))) void gemm_small_launch(int form, bool multi, const GemmPlan& plan, GemmSmallArgs& a, int count,
-                                                             hipStream_t stream);
+                                                             hipStream_t stream, const Epilogue* epilogue = nullptr);
 // tile grids of a launch on tiles of that plan's shape (K is set)
 __attribute__((visibility("hidden"))) void gemm_tile_grids(const GemmPlan& plan, GemmSmallArgs& a, int count);
 // results (fp32, else bf16) of tiles first_tile.. of a launch from their partial tiles (a.partial: of first_tile on, a.nsplit of each)

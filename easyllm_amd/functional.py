@@ -140,6 +140,51 @@ def bias_add(x, bias):
     return BiasAddFunction.apply(x, bias)
 
 
+class LinearActFunction(torch.autograd.Function):
+    """act(x W^T + bias) + residual in one product.  With an activation, what goes into it is kept for backward, in bf16: half the bytes of fp32, and its
+    rounding moves the slope by less than the gradient's own, which the products behind it take in bf16 anyway."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        need = ctx.needs_input_grad
+        x2d = x.reshape(-1, x.shape[-1])
+        r2d = None if residual is None else residual.reshape(-1, weight.shape[0])
+        if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
+            raise ValueError("residual shape mismatch")
+        y, pre = K.linear_act_fwd(x2d, weight, bias, act, r2d, act != "none" and (need[0] or need[1] or need[2]))
+        ctx.act = act
+        ctx.save_for_backward(x, weight, bias, pre)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        d = dy.reshape(-1, dy.shape[-1]).contiguous()
+        bias_to, db = _vector_target(bias, need[2])
+        if pre is not None:
+            d = K.act_bwd(ctx.act, d, pre, bias_to)
+        elif bias_to is not None:
+            mg, grad, acc = bias_to
+            db = K.bias_grad(d, main_grad=mg, accumulate=acc)
+        if need[0]:
+            dx = K.linear_dgrad(d, weight).view(x.shape)
+        if need[1]:
+            mg, acc = _main_grad_target(weight)
+            dw = K.linear_wgrad(d, x.reshape(-1, x.shape[-1]), out=mg, accumulate=acc)
+            dw = dw if mg is None else None
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None):
+    """act(x weight^T + bias) + residual, fp32 up to one rounding.  activation: None or 'none', 'gelu' (exact), 'gelu_tanh'."""
+    activation = activation or "none"
+    if activation not in K.ACTIVATIONS:
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(K.ACTIVATIONS), activation))
+    return LinearActFunction.apply(x, weight, bias, residual, activation)
+
+
 # --------------------------------------------------------------------------------------------
 # RMSNorm (+ fused residual add): base_modules/layers/fused_layer_norm.py:49-71, transformer.py:786
 # --------------------------------------------------------------------------------------------

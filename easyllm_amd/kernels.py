@@ -610,6 +610,44 @@ def linear_wgrad_multi(dy2ds, x2d, outs, accumulates):
     return res
 
 
+ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def linear_act_fwd(x2d, w, bias=None, act="none", residual=None, want_pre=False):
+    """-> (act(x2d @ w^T + bias) + residual, the bf16 x2d @ w^T + bias or None).  residual [T, out] may have strided rows."""
+    lda, ldb = _rows_ld(x2d, "x"), _rows_ld(w, "w")
+    (T, n_in), (n, w_in) = x2d.shape, w.shape
+    _need(n_in == w_in, "linear_act: inner dimensions differ")
+    _need(n_in > 0 and n % 8 == 0, "linear_act: needs an input, and a width that is a multiple of 8")
+    _vector(bias, n, "bias")
+    ldr = 0
+    if residual is not None:
+        ldr = _rows_ld(residual, "residual")
+        _need(residual.shape == (T, n), "residual shape mismatch")
+    _here(x2d, w, bias, residual)
+    out = torch.empty((T, n), dtype=BF16, device=x2d.device)
+    pre = torch.empty((T, n), dtype=BF16, device=x2d.device) if want_pre else None
+    epilogue = _lib.Epilogue(_p(bias), _p(residual), _p(pre), ldr, n, ACTIVATIONS[act])
+    ws, ws_bytes = _gemm_workspace(T, n, n_in, out.device)
+    _lib.call("ezl_gemm_bf16_epilogue", _p(x2d), _p(w), _p(out), T, n, n_in, lda, ldb, n, ctypes.byref(epilogue), _p(ws), ws_bytes, _stream())
+    return out, pre
+
+
+def act_bwd(act, dy, pre, dbias=None):
+    """-> dy * act'(pre); its column sums go to dbias = (f32 or None, bf16 or None, accumulate)."""
+    _bf16c(dy, "dy"); _bf16c(pre, "pre")
+    _need(dy.shape == pre.shape, "act_bwd: shape mismatch")
+    _here(dy, pre)
+    n = dy.shape[-1]
+    rows = dy.numel() // n
+    target = _grad_target(dbias, n, "bias")
+    ws_bytes = _lib.column_sum_workspace_bytes(rows, n) if target else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if target else None
+    dpre = torch.empty_like(dy)
+    _lib.call("ezl_act_bwd", ACTIVATIONS[act], _p(dy), _p(pre), _p(dpre), target, _p(ws), ws_bytes, rows, n, _stream())
+    return dpre
+
+
 def bias_add(x, bias):
     _bf16c(x, "x"); _bf16c(bias, "bias")
     n = x.shape[-1]

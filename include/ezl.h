@@ -182,6 +182,25 @@ int ezl_cast_f32_to_bf16(const void* in, void* out, int64_t n, void* stream);
 int64_t ezl_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int ezl_gemm_bf16(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
                   int a_kc, int b_kc, int out_dtype, int accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+/* C = act(A B^T + bias) + residual, the forward form (a_kc = b_kc = 1, bf16 C, K > 0) with what stands behind a product in its epilogue: fp32 from
+ * the reduction to the one rounding.  bias [N], residual [M, N] (rows ldr elements apart; may be C) may be NULL; pre [M, N] (rows ldp apart), if given,
+ * receives A B^T + bias rounded, which ezl_act_bwd reads.  N and the row strides are multiples of 8, C and the pointers here on 16 bytes, row strides below 2^21.
+ * EZL_ACT_GELU x Phi(x), Phi the normal distribution function; EZL_ACT_GELU_TANH x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2. */
+#define EZL_ACT_NONE 0
+#define EZL_ACT_GELU 1
+#define EZL_ACT_GELU_TANH 2
+typedef struct {
+    const void *bias, *residual;
+    void* pre;
+    int64_t ldr, ldp;
+    int act;
+} ezl_epilogue; /* HOST struct */
+int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
+                           const ezl_epilogue* epilogue, void* workspace, int64_t workspace_bytes, void* stream);
+/* dpre = dy * act'(pre) over [rows, n], n % 8 == 0 (may be dy or pre); dbias (HOST pointer, or NULL) = its column sums, taken before rounding, with a workspace of
+ * ezl_column_sum_workspace_bytes(rows, n).  act: EZL_ACT_GELU or EZL_ACT_GELU_TANH. */
+int ezl_act_bwd(int act, const void* dy, const void* pre, void* dpre, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
+                int64_t rows, int64_t n, void* stream);
 /* C (=|+=) sum_i A[i] * B[i] over `count` operand pairs with common M, N and leading dimensions and reduction lengths K[i]:
  * the input gradient sum_i dy_i W_i of the linears that share one input -- q/k/v (transformer.py:419-426) and gate/up
  * (:217-221), which the reference leaves to autograd as one matmul per linear (column_parallel_linear.py:68) plus adds.
