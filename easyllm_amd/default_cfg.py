@@ -41,6 +41,7 @@ TRANSFORMER_LAYER_DEFAULTS = {
     "initializer": {"type": "normal", "kwargs": {"sigma": 0.02}},
     "output_initializer": {"type": "scaled_normal", "kwargs": {"sigma": 0.02, "num_layers": 32}},
     "qkv_pack": False, "attention_qkv_bias": False, "attention_o_bias": False,
+    "mlp_bias": False,  # not in the reference: biases of the plain MLP's products (glu_activation None)
 }
 
 

@@ -1,6 +1,6 @@
 """Host-side mirror of the reference's base layers, backed by the HIP kernels:
 
-  RMSNorm / build_layer_norm ....... base_modules/layers/fused_layer_norm.py:20-71, 143-155
+  RMSNorm / MixedFusedLayerNorm / build_layer_norm ... base_modules/layers/fused_layer_norm.py:20-71, 143-155
   ColumnParallelLinear ............. base_modules/layers/column_parallel_linear.py:158-266
   RowParallelLinear ................ base_modules/layers/row_parallel_linear.py:13-132
   VocabParallelEmbedding ........... base_modules/layers/vocab_parallel_emb.py:30-137
@@ -123,6 +123,58 @@ class RMSNorm(torch.nn.Module):
         _require_bf16(x, "RMSNorm")
         return F_.add_rmsnorm(x, residual, self.weight, self.eps)
 
+    def forward_with_dropout_residual(self, x, residual, p, bias=None):
+        """(s, norm(s)), s = residual + dropout(x + bias), in one kernel"""
+        if self.layernorm_tp_auto_sync or self.sequence_parallel:
+            dist_env.sync_tp_duplicated_parameter(self.weight)
+        _require_bf16(x, "RMSNorm")
+        return F_.dropout_add_rmsnorm(x, residual, self.weight, self.eps, bias=bias, p=p)
+
+
+class MixedFusedLayerNorm(torch.nn.Module):
+    """Layer norm with weight and bias ('mixed_fused_norm'); the constructor and the fused forms of RMSNorm."""
+
+    def __init__(self, sync_tp_duplicated_parameters, normalized_shape, eps=1e-5, use_flash_attn=False, bf16=True,
+                 hf_mode=False, sequence_parallel=False, params_dtype=None):
+        super().__init__()
+        if isinstance(normalized_shape, numbers.Integral):
+            normalized_shape = (normalized_shape,)
+        self.normalized_shape = torch.Size(normalized_shape)
+        self.eps = eps
+        dtype = get_torch_dtype(params_dtype) if params_dtype is not None else (torch.bfloat16 if bf16 else torch.float32)
+        self.weight = Parameter(torch.ones(*normalized_shape, dtype=dtype, device=_param_device()))
+        self.bias = Parameter(torch.zeros(*normalized_shape, dtype=dtype, device=_param_device()))
+        self.layernorm_tp_auto_sync = sync_tp_duplicated_parameters
+        self.sequence_parallel = sequence_parallel
+
+    def reset_parameters(self):
+        torch.nn.init.ones_(self.weight)
+        torch.nn.init.zeros_(self.bias)
+
+    def _sync(self, x):
+        if self.layernorm_tp_auto_sync or self.sequence_parallel:
+            dist_env.sync_tp_duplicated_parameter(self.weight)
+            dist_env.sync_tp_duplicated_parameter(self.bias)
+        _require_bf16(x, "MixedFusedLayerNorm")
+
+    def forward(self, input):
+        self._sync(input)
+        return F_.layer_norm(input, self.weight, self.bias, self.eps)
+
+    def forward_keep_input(self, x):
+        """(x, norm(x)), as RMSNorm's"""
+        self._sync(x)
+        return F_.layer_norm_pass(x, self.weight, self.bias, self.eps)
+
+    def forward_with_residual(self, x, residual):
+        """(x + residual, norm(x + residual)) in one kernel"""
+        return self.forward_with_dropout_residual(x, residual, 0.0)
+
+    def forward_with_dropout_residual(self, x, residual, p, bias=None):
+        """(s, norm(s)), s = residual + dropout(x + bias), in one kernel"""
+        self._sync(x)
+        return F_.dropout_add_layer_norm(x, residual, self.weight, self.bias, self.eps, bias=bias, p=p)
+
 
 class LayerSpec(object):
     """Deferred constructor, the shape of deepspeed.pipe.LayerSpec used by llama/llama.py:142-190."""
@@ -137,12 +189,12 @@ class LayerSpec(object):
 
 
 def build_layer_norm(cfg_ln, layer_spec=False):
-    if cfg_ln["type"] == "rms_norm":
-        if layer_spec:
-            return LayerSpec(RMSNorm, **cfg_ln["kwargs"])
-        return RMSNorm(**cfg_ln["kwargs"])
-    # 'mixed_fused_norm' (LayerNorm with bias) is never selected by the llama configs
-    raise NotImplementedError(cfg_ln["type"])
+    types = {"rms_norm": RMSNorm, "mixed_fused_norm": MixedFusedLayerNorm}
+    if cfg_ln["type"] not in types:
+        raise NotImplementedError(cfg_ln["type"])
+    if layer_spec:
+        return LayerSpec(types[cfg_ln["type"]], **cfg_ln["kwargs"])
+    return types[cfg_ln["type"]](**cfg_ln["kwargs"])
 
 
 # ---- linears ----------------------------------------------------------------------------------

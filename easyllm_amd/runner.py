@@ -9,6 +9,7 @@ number of accumulation steps and ZeRO partitioning are DeepSpeed's and are not r
 import torch
 
 from .registry import MODULE_ZOO_REGISTRY
+from . import dropout as _dropout
 from . import functional as _F
 from . import kernels as _K
 from . import llama as _llama  # (registers the model builders)
@@ -101,6 +102,7 @@ class GraphedStep:
     time; new token ids / labels of the same shape are copied into the static input buffers by `__call__`.  The loss is
     returned as a device tensor that the next replay overwrites.  The token-id range check of the embedding cannot
     raise inside a graph: its flag is read back after every replay and raised one call late, as in the deferred mode.
+    Dropout draws anew on every replay: its captured calls read a step in device memory that `__call__` advances.
     """
 
     def __init__(self, model, inputs, labels, accumulate=False, warmup=2):
@@ -135,7 +137,8 @@ class GraphedStep:
             p.grad = None
         del functional.CAPTURED_ID_FLAGS[:]
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        self._step = torch.zeros(1, dtype=torch.int64, device="cuda")
+        with _dropout.recording() as self._draws, _dropout.stepping(self._step), torch.cuda.graph(self.graph):
             self.loss = one_step()
         self._flags = list(functional.CAPTURED_ID_FLAGS)
         del functional.CAPTURED_ID_FLAGS[:]
@@ -164,6 +167,8 @@ class GraphedStep:
                 if getattr(p, "main_grad_fresh", False):
                     p.main_grad.zero_()
                     p.main_grad_fresh = False
+        if self._draws:
+            self._step.add_(1)
         self.graph.replay()
         for host, (flag, _) in zip(self._host_flags, self._flags):
             host.copy_(flag, non_blocking=True)

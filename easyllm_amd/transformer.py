@@ -18,7 +18,8 @@ import torch
 
 from . import dist_env
 from . import functional as F_
-from .layers import (ColumnParallelLinear, RMSNorm, RowParallelLinear, GLU_ACTIVATIONS, build_layer_norm,
+from .dropout import threshold_of
+from .layers import (ColumnParallelLinear, MixedFusedLayerNorm, RMSNorm, RowParallelLinear, GLU_ACTIVATIONS, build_layer_norm,
                      get_initializer_from_cfg, get_torch_dtype)
 from .positional_embeddings import RotaryEmbedding, apply_rotary_pos_emb
 
@@ -97,28 +98,42 @@ class FlashAttention(torch.nn.Module):
 
 
 class ParallelMLP(torch.nn.Module):
-    """down_proj(silu(gate_proj(x)) * up_proj(x)); returns (output, output_bias)."""
+    """down_proj(silu(gate_proj(x)) * up_proj(x)), or with glu_activation None down_proj(gelu(up_proj(x))), the products with their biases where
+    mlp_bias is set and the activation in the first one's epilogue (exact; with the tanh where bias_gelu_fusion or use_openai_gelu ask for
+    it).  Returns (output, output_bias); with `residual`, which the plain form takes, the whole sum and None."""
 
     def __init__(self, init_method, output_layer_init_method, hidden_size=1024, intermediate_size=4096,
                  use_cpu_initialization=False, params_dtype=torch.half, bias_gelu_fusion=False, glu_activation=None,
-                 use_openai_gelu=False, onnx_safe=False, sync_tp_duplicated_parameters=True, sequence_parallel=False):
+                 use_openai_gelu=False, onnx_safe=False, sync_tp_duplicated_parameters=True, sequence_parallel=False, mlp_bias=False):
         super().__init__()
         self.sequence_parallel = sequence_parallel
-        common = dict(gather_output=False, init_method=init_method, skip_bias_add=True, bias=False,
+        self.glu = glu_activation is not None
+        if self.glu and glu_activation not in GLU_ACTIVATIONS:
+            raise NotImplementedError("glu_activation=%r: the llama step uses 'silu' (default_cfg.py:163)" % (glu_activation,))
+        if self.glu and mlp_bias:
+            raise NotImplementedError("mlp_bias: the products of a gated MLP have no biases")
+        common = dict(gather_output=False, init_method=init_method, skip_bias_add=True, bias=mlp_bias,
                       use_cpu_initialization=use_cpu_initialization, params_dtype=params_dtype,
                       sequence_parallel=sequence_parallel)
-        self.gate_proj = ColumnParallelLinear(hidden_size, intermediate_size, **common)
+        if self.glu:
+            self.gate_proj = ColumnParallelLinear(hidden_size, intermediate_size, **common)
         self.up_proj = ColumnParallelLinear(hidden_size, intermediate_size, **common)
-        if glu_activation not in GLU_ACTIVATIONS:
-            raise NotImplementedError("glu_activation=%r: the llama step uses 'silu' (default_cfg.py:163)" % (glu_activation,))
-        self.activation_func = GLU_ACTIVATIONS[glu_activation]
+        self.activation_func = GLU_ACTIVATIONS[glu_activation] if self.glu else None
+        self.activation = None if self.glu else "gelu_tanh" if bias_gelu_fusion or use_openai_gelu else "gelu"
         self.down_proj = RowParallelLinear(intermediate_size, hidden_size, input_is_parallel=True,
-                                           init_method=output_layer_init_method, skip_bias_add=True, bias=False,
+                                           init_method=output_layer_init_method, skip_bias_add=True, bias=mlp_bias,
                                            use_cpu_initialization=use_cpu_initialization, params_dtype=params_dtype,
                                            sync_tp_duplicated_parameters=sync_tp_duplicated_parameters,
                                            sequence_parallel=sequence_parallel)
 
-    def forward(self, hidden_states):
+    def forward(self, hidden_states, residual=None):
+        if not self.glu:
+            h1 = F_.linear_act(hidden_states, self.up_proj.weight, self.up_proj.bias, self.activation)
+            if residual is None:
+                return self.down_proj(h1)
+            return F_.linear_act(h1, self.down_proj.weight, self.down_proj.bias, residual=residual), None
+        if residual is not None:
+            raise ValueError("a gated MLP leaves the residual sum to the layer")
         # gate_proj and up_proj share their input: one fan-out op (input gradient accumulated in the GEMM)
         h1, h2 = F_.fan_out_linear(hidden_states, self.gate_proj.weight, self.up_proj.weight)
         h1 = self.activation_func.fused_mul(h1, h2)
@@ -248,7 +263,7 @@ class ParallelTransformerLayer(torch.nn.Module):
                  onnx_safe=None, sync_tp_duplicated_parameters=False, hidden_dropout=0, bias_dropout_fusion=False,
                  intermediate_size=4096, seq_length=1024, micro_batch_size=1, sequence_parallel=False, use_flash_attn=False,
                  initializer=None, output_initializer=None, use_matmul=False, qkv_pack=False, attention_qkv_bias=False,
-                 attention_o_bias=False):
+                 attention_o_bias=False, mlp_bias=False):
         super().__init__()
         assert layer_type in ("encoder", "decoder")
         assert position_embedding_type in _POSITION_TYPES and self_attn_mask_type in _MASK_TYPES
@@ -261,7 +276,7 @@ class ParallelTransformerLayer(torch.nn.Module):
             raise NotImplementedError("fp32 residual stream is not built (default_cfg.py:32 default is False)")
         self.fp32_residual_connection = False
         self.sequence_parallel = sequence_parallel
-        assert hidden_dropout == 0, "hidden dropout is 0 in every llama config (default_cfg.py:21)"
+        threshold_of(hidden_dropout)  # (raises for what is no probability)
         self.hidden_dropout = hidden_dropout
         self.bias_dropout_fusion = bias_dropout_fusion
         self.input_layernorm = build_layer_norm(layer_norm)
@@ -284,7 +299,7 @@ class ParallelTransformerLayer(torch.nn.Module):
             intermediate_size=intermediate_size, use_cpu_initialization=use_cpu_initialization, params_dtype=params_dtype,
             bias_gelu_fusion=bias_gelu_fusion, glu_activation=glu_activation, use_openai_gelu=use_openai_gelu,
             onnx_safe=onnx_safe, sync_tp_duplicated_parameters=sync_tp_duplicated_parameters,
-            sequence_parallel=sequence_parallel)
+            sequence_parallel=sequence_parallel, mlp_bias=mlp_bias)
         self.alibi = None
         # Layers of up to this many forward FLOPs make all their launches in one native call (see _native_inputs).
         self.native_call_flops = 1e12
@@ -296,9 +311,11 @@ class ParallelTransformerLayer(torch.nn.Module):
         code) exceeds the kernels' own time: two layers at h = 256 on 1024 tokens, forward + loss + backward, 1.6 ms of which
         0.57 are kernels.  1e12 FLOPs are 0.8 ms of kernels, where the host is ahead either way; larger layers keep the
         composed form, whose activations and gradients are freed one by one.  Only the plain layer qualifies: its own
-        submodules, unhooked, separate q / k / v projections with all biases or none, no o or down bias, no key padding mask."""
+        submodules, unhooked, separate q / k / v projections with all biases or none, no o or down bias, no key padding mask, RMSNorm, a gated
+        MLP, nothing dropped."""
         attn, mlp = self.self_attn, self.mlp
-        if (type(attn) is not ParallelAttention or type(mlp) is not ParallelMLP or attn.qkv_pack or self.apply_residual_connection_post_layernorm
+        if (type(attn) is not ParallelAttention or type(mlp) is not ParallelMLP or attn.qkv_pack or not mlp.glu or (self.training and self.hidden_dropout > 0)
+                or self.apply_residual_connection_post_layernorm
                 or (attention_mask is not None and cu_seqlens is None) or not hidden_states.is_cuda
                 or hidden_states.dtype is not torch.bfloat16 or hidden_states.dim() != 3):
             return None
@@ -341,18 +358,31 @@ class ParallelTransformerLayer(torch.nn.Module):
         hidden_states, layernorm_output = self.input_layernorm.forward_keep_input(hidden_states)
         attention_output, attention_bias = self.self_attn(layernorm_output, attention_mask, cu_seqlens, position_ids,
                                                           layer_past=layer_past, get_key_value=get_key_value, alibi=self.alibi)
-        if attention_bias is not None:
-            attention_output = F_.bias_add(attention_output, attention_bias)
+        dropout_p = self.hidden_dropout if self.training else 0.0
+        norm_takes_bias = dropout_p > 0 or isinstance(self.post_attention_layernorm, MixedFusedLayerNorm)  # (and the dropout in front of it)
+        if attention_bias is not None and not norm_takes_bias:
+            attention_output, attention_bias = F_.bias_add(attention_output, attention_bias), None
         if self.apply_residual_connection_post_layernorm:
-            layernorm_input = F_.add(attention_output, layernorm_output)
+            if dropout_p > 0 or attention_bias is not None:
+                layernorm_input = F_.dropout_add(attention_output, layernorm_output, attention_bias, dropout_p)
+            else:
+                layernorm_input = F_.add(attention_output, layernorm_output)
             layernorm_output = self.post_attention_layernorm(layernorm_input)
             residual = layernorm_output
+        elif norm_takes_bias:
+            layernorm_input, layernorm_output = self.post_attention_layernorm.forward_with_dropout_residual(attention_output, hidden_states, dropout_p,
+                                                                                                            attention_bias)
+            residual = layernorm_input
         else:
             # residual add (:786) + post-attention RMSNorm (:787) in one kernel
             layernorm_input, layernorm_output = self.post_attention_layernorm.forward_with_residual(attention_output,
                                                                                                      hidden_states)
             residual = layernorm_input
-        mlp_output, _ = self.mlp(layernorm_output)
+        if dropout_p == 0 and not getattr(self.mlp, "glu", True) and are_plain(((self.mlp, ParallelMLP), (self.mlp.down_proj, RowParallelLinear))):
+            return self.mlp(layernorm_output, residual=residual)[0]  # the sum in the second product's epilogue
+        mlp_output, mlp_bias = self.mlp(layernorm_output)
+        if dropout_p > 0 or mlp_bias is not None:
+            return F_.dropout_add(mlp_output, residual, mlp_bias, dropout_p)
         return F_.add(mlp_output, residual)  # :797
 
 

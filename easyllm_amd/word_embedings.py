@@ -3,6 +3,7 @@ import torch
 
 from . import dist_env
 from . import functional as F_
+from .dropout import threshold_of
 from .layers import VocabParallelEmbedding, get_initializer_from_cfg, get_torch_dtype
 
 
@@ -18,7 +19,8 @@ class Embedding(torch.nn.Module):
         self.pretrain_causal_attention = pretrain_causal_attention
         if position_embedding_type == "absolute":
             raise NotImplementedError("learned absolute positions are not used by the llama configs (rotary)")
-        assert embedding_dropout_prob == 0, "embedding dropout is 0 in every llama config"
+        threshold_of(embedding_dropout_prob)  # (raises for what is no probability)
+        self.embedding_dropout_prob = embedding_dropout_prob
         self.word_embeddings = VocabParallelEmbedding(vocab_size, hidden_size, init_method=self.init_method,
                                                       use_bnb_optimizer=use_bnb_optimizer,
                                                       use_cpu_initialization=use_cpu_initialization,
@@ -27,7 +29,10 @@ class Embedding(torch.nn.Module):
         self.sequence_parallel = sequence_parallel
 
     def forward(self, input_ids, position_ids, sequence_first=False):
-        embeddings = self.word_embeddings(input_ids, sequence_first=True) if sequence_first else self.word_embeddings(input_ids)  # [b, s, h]
+        dropping = self.training and self.embedding_dropout_prob > 0
+        embeddings = self.word_embeddings(input_ids, sequence_first=True) if sequence_first and not dropping else self.word_embeddings(input_ids)  # [b, s, h]
+        if dropping:
+            embeddings = F_.dropout_add(embeddings, p=self.embedding_dropout_prob)
         if self.sequence_parallel:
             embeddings = dist_env.scatter_to_sequence_parallel_region(embeddings)
         return embeddings
