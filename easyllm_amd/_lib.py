@@ -166,10 +166,12 @@ def rmsnorm_bwd_workspace_bytes(rows, h):
     return load().ezl_rmsnorm_bwd_workspace_bytes(rows, h)
 
 
+@functools.lru_cache(maxsize=1024)
 def column_sum_workspace_bytes(rows, n):
     return load().ezl_column_sum_workspace_bytes(rows, n)
 
 
+@functools.lru_cache(maxsize=1024)
 def norm_bwd_workspace_bytes(rows, h):
     return load().ezl_norm_bwd_workspace_bytes(rows, h)
 

@@ -75,12 +75,16 @@ __device__ __forceinline__ void rows_with_column_sums(int rows, int n, float* pa
     for (int j = threadIdx.x; j < 512; j += 256)
         if (blockIdx.x * 512 + j < n) partial[(int64_t)blockIdx.y * n + blockIdx.x * 512 + j] = fold[0][j] + fold[1][j] + fold[2][j] + fold[3][j];
 }
+template <bool DROP>
 __global__ __launch_bounds__(256) void dropout_sum_kernel(const DropSum a) {
-    const uint32_t step = drop_step(a.drop);
+    uint32_t step = 0;
+    if constexpr (DROP) step = drop_step(a.drop);
     rows_with_column_sums(a.rows, a.n, a.partial, [&](int64_t at, float (&v)[8]) {
         unpack8(ld_bf16x8(a.dy + at), v);
-        drop8(v, at >> 3, a.drop, step);
-        st_bf16x8(a.dx + at, pack8(v));
+        if constexpr (DROP) {
+            drop8(v, at >> 3, a.drop, step);
+            st_bf16x8(a.dx + at, pack8(v));
+        }
     });
 }
 
@@ -175,7 +179,8 @@ extern "C" int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void
                                    int64_t rows, int64_t n, void* stream) {
     const char* name = "ezl_dropout_add_bwd";
     if (const int rc = sizes_check(name, rows, n)) return rc;
-    EZL_REQUIRE(rows == 0 || (dy && dx), EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(rows == 0 || (dy && (dx != nullptr) == (drop != nullptr)), EZL_EINVAL, "%s: null pointer, or a dx without drop", name);
+    EZL_REQUIRE(drop || wanted(dbias), EZL_EINVAL, "%s: nothing to do", name);
     EZL_REQUIRE(ezl_aligned16(dy) && ezl_aligned16(dx) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
     DropArgs d;
     if (const int rc = drop_args(name, drop, d)) return rc;
@@ -183,15 +188,15 @@ extern "C" int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void
     if (!wanted(dbias)) {
         if (rows == 0) return EZL_OK;
         const DropAdd a = {(const bf16_t*)dy, nullptr, nullptr, (bf16_t*)dx, rows * (n / 8), (int)(n / 8), d};
-        if (d.threshold) hipLaunchKernelGGL((dropout_add_kernel<true, false>), dim3(elementwise_grid(a.groups)), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((dropout_add_kernel<false, false>), dim3(elementwise_grid(a.groups)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((dropout_add_kernel<true, false>), dim3(elementwise_grid(a.groups)), dim3(256), 0, st, a);
         EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
         return EZL_OK;
     }
     EZL_REQUIRE(workspace && workspace_bytes >= ezl_column_sum_workspace_bytes(rows, n), EZL_EINVAL, "%s: workspace missing or too small", name);
     const DropSum a = {(const bf16_t*)dy, (bf16_t*)dx, (float*)workspace, (int)rows, (int)n, d};
     const dim3 grid = sum_grid(rows, n);
-    hipLaunchKernelGGL(dropout_sum_kernel, grid, dim3(256), 0, st, a);
+    if (drop) hipLaunchKernelGGL(dropout_sum_kernel<true>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(dropout_sum_kernel<false>, grid, dim3(256), 0, st, a);
     EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
     const ColumnSum s = column_sum((const float*)workspace, dbias);
     return column_sums(name, &s, 1, (int)grid.y, n, st);

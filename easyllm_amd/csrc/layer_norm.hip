@@ -9,6 +9,8 @@
 #include "column_sums.h"
 #include "dropout.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kMaxH = 8192;
@@ -17,24 +19,29 @@ struct NormFwd {
     const bf16_t *x, *x_bias, *res, *w, *b;
     bf16_t *y, *sum;
     float *mean, *rstd;
-    int T, h, tpr;
+    int T, h;
     float eps;
     DropArgs drop;
 };
 
-// tpr threads (whole waves) per row, 256 / tpr rows per block; thread t holds the chunks of 8 columns at (c * tpr + t) * 8.
-template <int NCHUNK, bool CENTER, bool RES, bool DROP>
+// A row is shared by NSPLIT waves: wave part p owns the NCHUNK * 512 columns from p * NCHUNK * 512 on, lane l the 8 columns at l * 8 of each 512.  A
+// wave's next row is loaded before the current one is worked on, and where a wave holds whole rows no barrier ties it to others.  Rate of the bytes read and
+// written, x + residual -> sum + y: 16384 x 5120 5.4 TB/s, 8192 x 8192 5.5, 32768 x 1024 6.2; a copy of 2 GiB runs at 5.0.  (A block per row that loads,
+// reduces and stores in turn, up to 512 threads: 4.6, 5.5, 5.9.  Streaming hints on any of the loads or stores: within 1 %.)
+template <int NCHUNK, int NSPLIT, bool CENTER, bool RES, bool DROP>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(const NormFwd a) {
-    __shared__ float red[2][4][4];  // [parity][row slot][wave in slot]
-    const int tpr = a.tpr, h = a.h;
-    const int slot = threadIdx.x / tpr, tin = threadIdx.x % tpr, wis = tin >> 6, nws = tpr >> 6, lane = threadIdx.x & 63;
-    const int rpb = 256 / tpr;
+    constexpr int RPB = 4 / NSPLIT;
+    __shared__ float cell[2][RPB][NSPLIT];
+    const int lane = threadIdx.x & 63, h = a.h;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = wave / NSPLIT, part = wave % NSPLIT;
+    const int col0 = (part * NCHUNK * 64 + lane) * 8;
     bf16x8 wv[NCHUNK], bv[NCHUNK], xb[NCHUNK];
 #pragma unroll
     for (int c = 0; c < NCHUNK; ++c) {
-        const int col = (c * tpr + tin) * 8;
+        const int col = col0 + c * 512;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bv[c][i] = xb[c][i] = (bf16_t)0.0f;
+        for (int i = 0; i < 8; ++i) wv[c][i] = bv[c][i] = xb[c][i] = (bf16_t)0.0f;
         if (col < h) {
             wv[c] = ld_bf16x8(a.w + col);
             if (CENTER && a.b) bv[c] = ld_bf16x8(a.b + col);
@@ -46,41 +53,57 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(const NormFwd a) {
     int parity = 0;
     auto row_sum = [&](float v) {
         v = wave_sum(v);
-        if (nws > 1) {
-            if (lane == 0) red[parity][slot][wis] = v;
+        if constexpr (NSPLIT > 1) {
+            if (lane == 0) cell[parity][slot][part] = v;
             __syncthreads();
-            v = 0.f;
-            for (int i = 0; i < nws; ++i) v += red[parity][slot][i];
+            v = cell[parity][slot][0];
+#pragma unroll
+            for (int q = 1; q < NSPLIT; ++q) v += cell[parity][slot][q];
             parity ^= 1;
         }
         return v;
     };
     const float inv_h = 1.0f / (float)h;
-    // every thread of the block runs the same number of iterations (barriers inside)
-    for (int row0 = blockIdx.x * rpb; row0 < a.T; row0 += gridDim.x * rpb) {
+    bf16x8 nx[NCHUNK], nr[NCHUNK];
+    auto fetch = [&](int row) {
+        const int64_t at = (int64_t)row * h + col0;
+#pragma unroll
+        for (int c = 0; c < NCHUNK; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) nx[c][i] = nr[c][i] = (bf16_t)0.0f;
+            if (row < a.T && col0 + c * 512 < h) {
+                nx[c] = ld_bf16x8(a.x + at + c * 512);
+                if (RES) nr[c] = ld_bf16x8(a.res + at + c * 512);
+            }
+        }
+    };
+    fetch(blockIdx.x * RPB + slot);
+    for (int row0 = blockIdx.x * RPB; row0 < a.T; row0 += gridDim.x * RPB) {
         const int row = row0 + slot;
         const bool live = row < a.T;
-        const int64_t base = (int64_t)row * h;
+        const int64_t at = (int64_t)row * h + col0;
+        bf16x8 x[NCHUNK], r[NCHUNK];
+#pragma unroll
+        for (int c = 0; c < NCHUNK; ++c) {
+            x[c] = nx[c];
+            r[c] = nr[c];
+        }
+        if (row0 + (int)gridDim.x * RPB < a.T) fetch(row + gridDim.x * RPB);
         float v[NCHUNK][8];
         float s1 = 0.f;
 #pragma unroll
         for (int c = 0; c < NCHUNK; ++c) {
-            const int col = (c * tpr + tin) * 8;
-            if (live && col < h) {
-                unpack8(ld_bf16x8(a.x + base + col), v[c]);
-                if constexpr (RES) {
-                    float r[8];
-                    unpack8(ld_bf16x8(a.res + base + col), r);
+            unpack8(x[c], v[c]);
+            if constexpr (RES) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[c][i] += (float)xb[c][i];
-                    if constexpr (DROP) drop8(v[c], (base + col) >> 3, a.drop, step);
+                for (int i = 0; i < 8; ++i) v[c][i] += (float)xb[c][i];
+                if constexpr (DROP) drop8(v[c], (at + c * 512) >> 3, a.drop, step);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[c][i] += r[i];
-                    st_bf16x8(a.sum + base + col, pack8(v[c]));
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s1 += CENTER ? v[c][i] : v[c][i] * v[c][i];
+                for (int i = 0; i < 8; ++i) v[c][i] += (float)r[c][i];
+                if (live && col0 + c * 512 < h) st_bf16x8(a.sum + at + c * 512, pack8(v[c]));
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s1 += CENTER ? v[c][i] : v[c][i] * v[c][i];
         }
         s1 = row_sum(s1) * inv_h;
         float mean = 0.f, var = s1;
@@ -89,7 +112,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(const NormFwd a) {
             float s2 = 0.f;
 #pragma unroll
             for (int c = 0; c < NCHUNK; ++c)
-                if (live && (c * tpr + tin) * 8 < h)
+                if (col0 + c * 512 < h)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         v[c][i] -= mean;
@@ -98,20 +121,18 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(const NormFwd a) {
             var = row_sum(s2) * inv_h;
         }
         const float rs = rsqrtf(var + a.eps);
-        if (live && tin == 0) {
+        if (live && part == 0 && lane == 0) {
             a.rstd[row] = rs;
             if (CENTER) a.mean[row] = mean;
         }
 #pragma unroll
-        for (int c = 0; c < NCHUNK; ++c) {
-            const int col = (c * tpr + tin) * 8;
-            if (live && col < h) {
+        for (int c = 0; c < NCHUNK; ++c)
+            if (live && col0 + c * 512 < h) {
                 float o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[i] = v[c][i] * rs * (float)wv[c][i] + (float)bv[c][i];
-                st_bf16x8(a.y + base + col, pack8(o));
+                st_bf16x8(a.y + at + c * 512, pack8(o));
             }
-        }
     }
 }
 
@@ -121,17 +142,16 @@ struct NormBwd {
     bf16_t *dx, *dres;
     float *dw, *db, *dxb;  // partial rows
     int T, h;
-    bool stream;
     DropArgs drop;
 };
 
-// A row is shared by NSPLIT waves: wave part p owns the NCHUNK * 512 columns from p * NCHUNK * 512 on, lane l the 8 columns at l * 8 of each 512.  The
-// operands of a wave's next row are loaded before the current row is worked on.  Each wave keeps the column sums of its lanes' columns over the rows it
-// visits; the rows of a block are folded through LDS in a fixed order and one partial row per block goes to HBM.
+// Rows, columns and loads ahead as in the forward kernel.  Each wave keeps the column sums of its lanes' columns over the rows it
+// visits; the waves of a block that hold the same columns are added through LDS in a fixed order and one partial row per block goes to HBM.
 template <int NCHUNK, int NSPLIT, bool CENTER, bool DROP, bool XB>
 __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(const NormBwd a) {
     constexpr int RPB = 4 / NSPLIT, NSUMS = 1 + CENTER + XB;
-    extern __shared__ float fold[];  // h floats
+    constexpr bool AHEAD = NCHUNK < 4 || NSUMS < 3;  // dsum is loaded a row ahead too, where the registers hold it
+    extern __shared__ float fold[];  // RPB rows of h
     __shared__ float cell[2][RPB][NSPLIT][2];  // [parity][row slot][part]
     const int lane = threadIdx.x & 63, h = a.h;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -168,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(const NormBwd a) {
             if (live && col0 + c * 512 < h) {
                 ns[c] = ld_bf16x8_nt(a.s + at + c * 512);
                 ndy[c] = ld_bf16x8_nt(a.dy + at + c * 512);
-                if (a.dsum) nds[c] = ld_bf16x8_nt(a.dsum + at + c * 512);
+                if (AHEAD && a.dsum) nds[c] = ld_bf16x8_nt(a.dsum + at + c * 512);
             }
         }
     };
@@ -182,6 +202,7 @@ __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(const NormBwd a) {
             sr[c] = ns[c];
             dyr[c] = ndy[c];
             dsr[c] = nds[c];
+            if (!AHEAD && a.dsum && live && col0 + c * 512 < h) dsr[c] = ld_bf16x8_nt(a.dsum + (int64_t)row * h + col0 + c * 512);
         }
         const float rs = nrs, mean = nmean;
         if (row0 + (int)gridDim.x * RPB < a.T) fetch(row + gridDim.x * RPB);
@@ -227,70 +248,80 @@ __global__ __launch_bounds__(256, 2) void norm_bwd_kernel(const NormBwd a) {
                     if constexpr (CENTER) acc[1][c][i] += dyv;
                 }
                 if constexpr (DROP) {
-                    if (a.stream) st_bf16x8_nt(a.dres + at + c * 512, pack8(o));
-                    else st_bf16x8(a.dres + at + c * 512, pack8(o));
+                    st_bf16x8(a.dres + at + c * 512, pack8(o));
                     drop8(o, (at + c * 512) >> 3, a.drop, step);
                 }
                 if constexpr (XB)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) acc[NSUMS - 1][c][i] += o[i];
-                if (a.stream) st_bf16x8_nt(a.dx + at + c * 512, pack8(o));
-                else st_bf16x8(a.dx + at + c * 512, pack8(o));
+                st_bf16x8(a.dx + at + c * 512, pack8(o));
             }
         }
     }
     float* const out[3] = {a.dw, CENTER ? a.db : a.dxb, a.dxb};
 #pragma unroll
     for (int q = 0; q < NSUMS; ++q) {
-        __syncthreads();
-        for (int s2 = 0; s2 < RPB; ++s2) {  // row slot 0 stores, the others add in turn
-            if (slot == s2) {
+        float* const dst = RPB > 1 ? fold + slot * h : out[q] + (int64_t)blockIdx.x * h;  // (a block of one row: its waves' columns are apart)
+        if (RPB > 1 && q > 0) __syncthreads();
 #pragma unroll
-                for (int c = 0; c < NCHUNK; ++c) {
-                    const int col = col0 + c * 512;
-                    if (col < h) {
+        for (int c = 0; c < NCHUNK; ++c) {
+            const int col = col0 + c * 512;
+            if (col < h)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (s2 == 0) fold[col + i] = acc[q][c][i];
-                            else fold[col + i] += acc[q][c][i];
-                        }
-                    }
-                }
-            }
-            __syncthreads();
+                for (int k = 0; k < 8; k += 4) *reinterpret_cast<f32x4*>(dst + col + k) = f32x4{acc[q][c][k], acc[q][c][k + 1], acc[q][c][k + 2], acc[q][c][k + 3]};
         }
-        for (int j = threadIdx.x; j < h; j += 256) out[q][(size_t)blockIdx.x * h + j] = fold[j];
+        if constexpr (RPB > 1) {
+            __syncthreads();
+            for (int j = threadIdx.x * 4; j < h; j += 1024) {
+                f32x4 v = *reinterpret_cast<const f32x4*>(fold + j);
+#pragma unroll
+                for (int s2 = 1; s2 < RPB; ++s2) v += *reinterpret_cast<const f32x4*>(fold + s2 * h + j);
+                *reinterpret_cast<f32x4*>(out[q] + (int64_t)blockIdx.x * h + j) = v;
+            }
+        }
     }
 }
 
-constexpr int64_t kBwdBlocks = 512;  // partial rows at most: two blocks per CU
+constexpr int64_t kFwdBlocks = 4096, kBwdBlocks = 512;  // at most
+
+// waves that share a row, and with it rows of a block of four
+int split_of(int64_t h) { return h <= 2048 ? 1 : (h <= 4096 ? 2 : 4); }
+
+// launch(NCHUNK, NSPLIT) for rows of h
+template <class L>
+void by_width(int64_t h, L&& launch) {
+    const int split = split_of(h), nchunk = ((int)h + 512 * split - 1) / (512 * split);
+    typedef std::integral_constant<int, 1> one;
+    typedef std::integral_constant<int, 2> two;
+    typedef std::integral_constant<int, 3> three;
+    typedef std::integral_constant<int, 4> four;
+    if (split == 1 && nchunk == 1) launch(one{}, one{});
+    else if (split == 1 && nchunk == 2) launch(two{}, one{});
+    else if (split == 1 && nchunk == 3) launch(three{}, one{});
+    else if (split == 1) launch(four{}, one{});
+    else if (split == 2 && nchunk == 3) launch(three{}, two{});
+    else if (split == 2) launch(four{}, two{});
+    else if (nchunk == 3) launch(three{}, four{});
+    else launch(four{}, four{});
+}
+unsigned blocks_for(int64_t rows, int64_t h, int64_t most) {
+    const int rpb = 4 / split_of(h);
+    const int64_t blocks = (rows + rpb - 1) / rpb;
+    return (unsigned)(blocks > most ? most : (blocks < 1 ? 1 : blocks));
+}
 
 template <bool CENTER, bool RES, bool DROP>
-void launch_fwd(int nchunk, unsigned grid, unsigned threads, const NormFwd& a, hipStream_t st) {
-    if (nchunk == 1) hipLaunchKernelGGL((norm_fwd_kernel<1, CENTER, RES, DROP>), dim3(grid), dim3(threads), 0, st, a);
-    else if (nchunk == 2) hipLaunchKernelGGL((norm_fwd_kernel<2, CENTER, RES, DROP>), dim3(grid), dim3(threads), 0, st, a);
-    else hipLaunchKernelGGL((norm_fwd_kernel<4, CENTER, RES, DROP>), dim3(grid), dim3(threads), 0, st, a);
+void launch_fwd(const NormFwd& a, hipStream_t st) {
+    by_width(a.h, [&](auto nc, auto ns) {
+        hipLaunchKernelGGL((norm_fwd_kernel<decltype(nc)::value, decltype(ns)::value, CENTER, RES, DROP>), dim3(blocks_for(a.T, a.h, kFwdBlocks)), dim3(256), 0, st, a);
+    });
 }
-
-int bwd_split(int64_t h) { return h <= 2048 ? 1 : (h <= 4096 ? 2 : 4); }
-
 template <bool CENTER, bool DROP, bool XB>
 void launch_bwd(unsigned grid, const NormBwd& a, hipStream_t st) {
-    const size_t smem = (size_t)a.h * sizeof(float);
-#define EZL_BWD(NC, NS) hipLaunchKernelGGL((norm_bwd_kernel<NC, NS, CENTER, DROP, XB>), dim3(grid), dim3(256), smem, st, a)
-    const int split = bwd_split(a.h), nchunk = (a.h + 512 * split - 1) / (512 * split);
-    if (split == 1) {
-        if (nchunk == 1) EZL_BWD(1, 1);
-        else if (nchunk == 2) EZL_BWD(2, 1);
-        else EZL_BWD(4, 1);
-    } else if (split == 2) {
-        if (nchunk == 3) EZL_BWD(3, 2);
-        else EZL_BWD(4, 2);
-    } else {
-        if (nchunk == 3) EZL_BWD(3, 4);
-        else EZL_BWD(4, 4);
-    }
-#undef EZL_BWD
+    by_width(a.h, [&](auto nc, auto ns) {
+        hipLaunchKernelGGL((norm_bwd_kernel<decltype(nc)::value, decltype(ns)::value, CENTER, DROP, XB>), dim3(grid), dim3(256),
+                           decltype(ns)::value == 4 ? 0 : (size_t)a.h * (4 / decltype(ns)::value) * sizeof(float), st, a);
+    });
 }
 
 }  // namespace
@@ -309,23 +340,16 @@ extern "C" int ezl_norm_fwd(int kind, const void* x, const void* x_bias, const v
     EZL_REQUIRE(ezl_aligned16(x) && ezl_aligned16(x_bias) && ezl_aligned16(residual) && ezl_aligned16(weight) && ezl_aligned16(bias) && ezl_aligned16(y) && ezl_aligned16(sum_out),
                 EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
     NormFwd a = {(const bf16_t*)x, (const bf16_t*)x_bias, (const bf16_t*)residual, (const bf16_t*)weight, (const bf16_t*)bias, (bf16_t*)y, (bf16_t*)sum_out,
-                 (float*)mean, (float*)rstd, (int)rows, (int)h, 0, eps, {}};
+                 (float*)mean, (float*)rstd, (int)rows, (int)h, eps, {}};
     if (const int rc = drop_args(name, drop, a.drop)) return rc;
     if (rows == 0) return EZL_OK;
     hipStream_t st = (hipStream_t)stream;
-    int tpr = ((int)h / 8 + 63) / 64 * 64;
-    if (tpr > 256) tpr = 256;
-    a.tpr = tpr;
-    const int nchunk = ((int)h + tpr * 8 - 1) / (tpr * 8), rpb = 256 / tpr;
-    int64_t grid = (rows + rpb - 1) / rpb;
-    if (grid > 256 * 16) grid = 256 * 16;
-    const unsigned threads = (unsigned)(rpb * tpr);  // whole row slots only
     const bool dropping = drop && drop->drop_of_65536 > 0;
-    if (layer && !residual) launch_fwd<true, false, false>(nchunk, (unsigned)grid, threads, a, st);
-    else if (layer && !dropping) launch_fwd<true, true, false>(nchunk, (unsigned)grid, threads, a, st);
-    else if (layer) launch_fwd<true, true, true>(nchunk, (unsigned)grid, threads, a, st);
-    else if (!dropping) launch_fwd<false, true, false>(nchunk, (unsigned)grid, threads, a, st);
-    else launch_fwd<false, true, true>(nchunk, (unsigned)grid, threads, a, st);
+    if (layer && !residual) launch_fwd<true, false, false>(a, st);
+    else if (layer && !dropping) launch_fwd<true, true, false>(a, st);
+    else if (layer) launch_fwd<true, true, true>(a, st);
+    else if (!dropping) launch_fwd<false, true, false>(a, st);
+    else launch_fwd<false, true, true>(a, st);
     EZL_LAUNCH_CHECK("ezl_norm_fwd");
     return EZL_OK;
 }
@@ -352,20 +376,21 @@ extern "C" int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const vo
     EZL_REQUIRE(workspace && workspace_bytes >= ezl_norm_bwd_workspace_bytes(rows, h), EZL_EINVAL, "%s: workspace missing or too small", name);
     float* part = (float*)workspace;
     NormBwd a = {(const bf16_t*)dy, (const bf16_t*)dsum, (const bf16_t*)s, (const bf16_t*)weight, (const float*)mean, (const float*)rstd, (bf16_t*)dx,
-                 (bf16_t*)dresidual, part, part + kBwdBlocks * h, part + 2 * kBwdBlocks * h, (int)rows, (int)h, false, {}};
+                 (bf16_t*)dresidual, part, part + kBwdBlocks * h, part + 2 * kBwdBlocks * h, (int)rows, (int)h, {}};
     if (const int rc = drop_args(name, drop, a.drop)) return rc;
-    a.stream = ezl_streams(rows * h * (drop ? 4 : 2));
     hipStream_t st = (hipStream_t)stream;
-    const int rpb = 4 / bwd_split(h);
-    int64_t grid = (rows + rpb - 1) / rpb;
-    grid = grid > kBwdBlocks ? kBwdBlocks : (grid < 1 ? 1 : grid);  // (no rows still give zero sums)
+    // Every block leaves partial rows of h floats, which few rows feel, and wide ones, which cost most per block; the others gain by two blocks per CU.  256
+    // against 512, us: 1167 x 1000 9.1, 9.6; 4000 x 2048 20.7, 21.6 (with dropout and a bias 26.1, 27.2); 8000 x 2048 30.8, 29.9; 2048 x 4096 22.5, 24.4; 4096 x 5120 42.6,
+    // 39.3; 16384 x 5120 138, 116; 32768 x 1024 50.5, 48.9 (67.5, 63.0); 4096 x 8192 53.0, 56.0; 8192 x 8192 91.8, 95.7.
+    const bool few = rows * split_of(h) <= 8192 || h > 6144;
+    const unsigned grid = blocks_for(rows, h, few ? kBwdBlocks / 2 : kBwdBlocks);  // (no rows still give zero sums)
     const bool xb = wanted(dx_bias);
 #define EZL_LAUNCH_BWD(L)                                          \
     do {                                                           \
-        if (drop && xb) launch_bwd<L, true, true>((unsigned)grid, a, st);        \
-        else if (drop) launch_bwd<L, true, false>((unsigned)grid, a, st);        \
-        else if (xb) launch_bwd<L, false, true>((unsigned)grid, a, st);          \
-        else launch_bwd<L, false, false>((unsigned)grid, a, st);                 \
+        if (drop && xb) launch_bwd<L, true, true>(grid, a, st);        \
+        else if (drop) launch_bwd<L, true, false>(grid, a, st);        \
+        else if (xb) launch_bwd<L, false, true>(grid, a, st);          \
+        else launch_bwd<L, false, false>(grid, a, st);                 \
     } while (0)
     if (layer) EZL_LAUNCH_BWD(true);
     else EZL_LAUNCH_BWD(false);

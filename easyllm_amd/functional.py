@@ -166,8 +166,7 @@ class LinearActFunction(torch.autograd.Function):
         if pre is not None:
             d = K.act_bwd(ctx.act, d, pre, bias_to)
         elif bias_to is not None:
-            mg, grad, acc = bias_to
-            db = K.bias_grad(d, main_grad=mg, accumulate=acc)
+            K.dropout_add_bwd(d, 0, None, bias_to)  # (nothing dropped: the column sums alone)
         if need[0]:
             dx = K.linear_dgrad(d, weight).view(x.shape)
         if need[1]:
@@ -274,9 +273,11 @@ def _vector_target(param, needed):
     """((f32, bf16, accumulate) for a kernel to write, gradient to return) of a vector parameter"""
     if param is None or not needed:
         return None, None
+    if getattr(param, "main_grad", None) is None:
+        grad = torch.empty_like(param)
+        return (None, grad, False), grad
     mg, acc = _main_grad_target(param)
-    grad = None if mg is not None else torch.empty_like(param)
-    return (mg, grad, acc), grad
+    return (mg, None, acc), None
 
 
 class NormFunction(torch.autograd.Function):
@@ -303,7 +304,7 @@ class NormFunction(torch.autograd.Function):
         weight_to, dw = _vector_target(weight, need[4])
         bias_to, db = _vector_target(bias, need[5])
         x_bias_to, dxb = _vector_target(x_bias, need[3])
-        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to or (None, torch.empty_like(weight), False), bias_to,
+        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to if need[4] else (None, torch.empty_like(weight), False), bias_to,
                               None if dsum is None else dsum.contiguous(), ctx.threshold, ctx.draw, x_bias_to)
         return (None, dx if need[1] else None, dres if ctx.has_residual and need[2] else None, dxb, dw, db, None, None, None, None)
 
@@ -311,7 +312,7 @@ class NormFunction(torch.autograd.Function):
 def _draw_for(p, rng):
     """(threshold, draw): `rng` is (seed, offset[, step]), or None for the next of this process."""
     threshold = _dropout.threshold_of(p)
-    return threshold, (None if not threshold else _dropout.next_draw() if rng is None else rng)
+    return threshold, K.prepared_draw(threshold, _dropout.next_draw() if threshold and rng is None else rng)
 
 
 def layer_norm(x, weight, bias=None, eps=1e-5):
@@ -351,10 +352,8 @@ class DropoutAddFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         bias_to, db = _vector_target(ctx.bias, ctx.needs_input_grad[2])
-        dx = dy
-        if bias_to is not None or (ctx.threshold and ctx.needs_input_grad[0]):
-            dx = K.dropout_add_bwd(dy.contiguous(), ctx.threshold, ctx.draw, bias_to)
-        return dx if ctx.needs_input_grad[0] else None, dy if ctx.needs_input_grad[1] else None, db, None, None
+        dx = K.dropout_add_bwd(dy.contiguous(), ctx.threshold, ctx.draw, bias_to) if ctx.needs_input_grad[0] or bias_to else None
+        return dx, dy if ctx.needs_input_grad[1] else None, db, None, None
 
 
 def dropout_add(x, residual=None, bias=None, p=0.0, rng=None):

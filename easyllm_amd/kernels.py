@@ -129,31 +129,42 @@ def rmsnorm_bwd_swapped(dy, x, weight, rstd, main_grad=None, accumulate=False):
 
 
 # ------------------------------------------------------------------------------------- dropout, layer norm
-def _here(*tensors):
-    """All on the current GPU: that is where the launch goes."""
+# (Forward and backward of a small call are the host's work: checks of several tensors are one call here, and a draw's C form is made once.)
+def _ready(**tensors):
+    """Contiguous bf16 tensors (or None) of the current GPU, where the launch goes."""
     device = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise ValueError("tensors on GPU %d, but GPU %d is current" % (t.get_device(), device))
+    for name, t in tensors.items():
+        if t is not None and not (t.dtype is BF16 and t.get_device() == device and t.is_contiguous()):
+            _bf16c(t, name)
+            raise ValueError("%s is on GPU %d, but GPU %d is current" % (name, t.get_device(), device))
 
 
-def _vector(t, n, name):
-    if t is not None:
-        _bf16c(t, name)
-        _need(t.dim() == 1 and t.shape[0] == n, name + " size mismatch")
+def _here(t, name):
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("%s is not on the current GPU" % name)
 
 
-def _drop(threshold, draw):
-    """The C form of a draw (seed, offset[, step]) that drops `threshold` of 65536, None where it drops nothing."""
+def _vectors(n, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.shape != (n,):
+            raise ValueError(name + " size mismatch")
+
+
+def prepared_draw(threshold, draw):
+    """The C form of a draw (seed, offset[, step]) that drops `threshold` of 65536, None where it drops nothing; itself where it has that form."""
     if not threshold:
         return None
+    if type(draw) is _lib.Dropout:
+        return draw
     seed, offset, *step = draw
     step = step[0] if step else None
     _need(0 <= offset < 2 ** 32, "a draw's offset has 32 bits")
     if step is not None:
         _need(step.is_cuda and step.dtype is torch.int64 and step.numel() == 1, "a draw's step is an int64 [1] GPU tensor")
-        _here(step)
-    return ctypes.byref(_lib.Dropout(seed & 0xFFFFFFFFFFFFFFFF, offset, threshold, _p(step)))
+        _here(step, "a draw's step")
+    c = _lib.Dropout(seed & 0xFFFFFFFFFFFFFFFF, offset, threshold, _p(step))
+    c.holds = step  # (the memory that its address is of)
+    return c
 
 
 def _grad_target(target, n, what):
@@ -161,40 +172,46 @@ def _grad_target(target, n, what):
     if target is None:
         return None
     f32, bf16, accumulate = target
-    if f32 is not None:
-        _need(f32.is_cuda and f32.dtype is torch.float32 and f32.is_contiguous() and f32.numel() == n, "bad main_grad of the " + what)
-    else:
-        _vector(bf16, n, what + " gradient")
-    _here(f32, bf16)
-    return ctypes.byref(_lib.LayerGrad(_p(f32), _p(bf16), 1 if accumulate else 0))
+    if f32 is None:
+        _need(bf16.dtype is BF16 and bf16.shape == (n,) and bf16.is_contiguous(), "bad gradient of the " + what)
+        _here(bf16, "the gradient of the " + what)
+        return _lib.LayerGrad(None, bf16.data_ptr(), 0)
+    _need(f32.dtype is torch.float32 and f32.is_contiguous() and f32.numel() == n, "bad main_grad of the " + what)
+    _here(f32, "the main_grad of the " + what)
+    return _lib.LayerGrad(f32.data_ptr(), None, 1 if accumulate else 0)
+
+
+def _rows(t):
+    n = t.shape[-1]
+    _need(n > 0, "rows of no width")
+    return t.numel() // n, n
 
 
 def dropout_add_fwd(x, bias, residual, threshold, draw):
     """residual + dropout(x + bias); bias and residual may be None."""
-    _bf16c(x, "x")
-    n = x.shape[-1]
-    _vector(bias, n, "bias")
-    if residual is not None:
-        _bf16c(residual, "residual")
-        _need(residual.shape == x.shape, "residual shape mismatch")
-    _here(x, bias, residual)
+    _ready(x=x, bias=bias, residual=residual)
+    rows, n = _rows(x)
+    _vectors(n, bias=bias)
+    _need(residual is None or residual.shape == x.shape, "residual shape mismatch")
     out = torch.empty_like(x)
-    if x.numel():
-        _lib.call("ezl_dropout_add_fwd", _p(x), _p(bias), _p(residual), _drop(threshold, draw), _p(out), x.numel() // n, n, _stream())
+    _lib.call("ezl_dropout_add_fwd", x.data_ptr(), _p(bias), _p(residual), prepared_draw(threshold, draw), out.data_ptr(), rows, n, _stream())
     return out
 
 
 def dropout_add_bwd(dy, threshold, draw, dbias=None):
-    """-> dx; the bias's gradient goes to dbias = (f32 or None, bf16 or None, accumulate)."""
-    _bf16c(dy, "dy")
-    _here(dy)
-    n = dy.shape[-1]
-    rows = dy.numel() // n
+    """-> dx (dy itself where nothing is dropped); the bias's gradient goes to dbias = (f32 or None, bf16 or None, accumulate)."""
+    _ready(dy=dy)
+    rows, n = _rows(dy)
+    drop = prepared_draw(threshold, draw)
     target = _grad_target(dbias, n, "bias")
-    ws_bytes = _lib.column_sum_workspace_bytes(rows, n) if target else 0
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if target else None
-    dx = torch.empty_like(dy)
-    _lib.call("ezl_dropout_add_bwd", _p(dy), _drop(threshold, draw), _p(dx), target, _p(ws), ws_bytes, rows, n, _stream())
+    if drop is None and target is None:
+        return dy
+    ws_bytes, ws = 0, None
+    if target:
+        ws_bytes = _lib.column_sum_workspace_bytes(rows, n)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
+    dx = torch.empty_like(dy) if drop else dy
+    _lib.call("ezl_dropout_add_bwd", dy.data_ptr(), drop, dx.data_ptr() if drop else None, target, _p(ws), ws_bytes, rows, n, _stream())
     return dx
 
 
@@ -203,47 +220,39 @@ LAYER_NORM, RMS_NORM = 0, 1
 
 def norm_fwd(kind, x, weight, bias, eps, residual=None, x_bias=None, threshold=0, draw=None):
     """-> (y, sum, mean, rstd): the norm of x, or of sum = residual + dropout(x + x_bias).  RMS_NORM has no bias, no mean and needs a residual."""
-    _bf16c(x, "x")
-    h = x.shape[-1]
-    _vector(weight, h, "weight"); _vector(bias, h, "norm bias"); _vector(x_bias, h, "bias")
-    _here(x, weight, bias, residual, x_bias)
-    rows = x.numel() // h
+    _ready(x=x, weight=weight, bias=bias, residual=residual, x_bias=x_bias)
+    rows, h = _rows(x)
+    _vectors(h, weight=weight, bias=bias, x_bias=x_bias)
     y = torch.empty_like(x)
     s = mean = None
     if residual is not None:
-        _bf16c(residual, "residual")
         _need(residual.shape == x.shape, "residual shape mismatch")
         s = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    rstd = stats[1]
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
     if kind == LAYER_NORM:
-        mean = stats[0]
-    _lib.call("ezl_norm_fwd", kind, _p(x), _p(x_bias), _p(residual), _drop(threshold, draw), _p(weight), _p(bias), _p(y), _p(s), _p(mean), _p(rstd),
-              rows, h, float(eps), _stream())
+        mean = torch.empty_like(rstd)
+    _lib.call("ezl_norm_fwd", kind, x.data_ptr(), _p(x_bias), _p(residual), prepared_draw(threshold, draw), _p(weight), _p(bias), y.data_ptr(), _p(s), _p(mean),
+              rstd.data_ptr(), rows, h, float(eps), _stream())
     return y, s, mean, rstd
 
 
 def norm_bwd(kind, dy, s, weight, mean, rstd, dweight, dbias=None, dsum=None, threshold=0, draw=None, dx_bias=None):
     """-> (dx, dresidual), one tensor where nothing is dropped.  dweight, dbias, dx_bias: (f32 or None, bf16 or None, accumulate) that
     receive the parameters' gradients; the last two may be None."""
-    _bf16c(dy, "dy"); _bf16c(s, "s")
-    h = s.shape[-1]
-    rows = s.numel() // h
-    _vector(weight, h, "weight")
+    _ready(dy=dy, s=s, weight=weight, dsum=dsum)
+    rows, h = _rows(s)
+    _vectors(h, weight=weight)
     for t in (mean, rstd):
-        _need(t is None or (t.dtype is torch.float32 and t.numel() == rows and t.is_contiguous()), "norm_bwd: bad statistics")
-    _need(dy.shape == s.shape, "norm_bwd: shape mismatch")
-    if dsum is not None:
-        _bf16c(dsum, "dsum")
-        _need(dsum.shape == s.shape, "norm_bwd: shape mismatch")
-    _here(dy, s, weight, mean, rstd, dsum)
+        _need(t is None or (t.dtype is torch.float32 and t.shape == (rows,) and t.is_contiguous() and t.device == s.device), "norm_bwd: bad statistics")
+    _need(dy.shape == s.shape and (dsum is None or dsum.shape == s.shape), "norm_bwd: shape mismatch")
     dx = torch.empty_like(s)
-    drop = _drop(threshold, draw)
+    drop = prepared_draw(threshold, draw)
     dres = torch.empty_like(s) if drop else None
     ws_bytes = _lib.norm_bwd_workspace_bytes(rows, h)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=s.device)
-    _lib.call("ezl_norm_bwd", kind, _p(dy), _p(dsum), _p(s), _p(weight), _p(mean), _p(rstd), drop, _p(dx), _p(dres), _grad_target(dweight, h, "weight"),
-              _grad_target(dbias, h, "norm bias"), _grad_target(dx_bias, h, "bias"), _p(ws), ws_bytes, rows, h, _stream())
+    _lib.call("ezl_norm_bwd", kind, dy.data_ptr(), _p(dsum), s.data_ptr(), weight.data_ptr(), _p(mean), rstd.data_ptr(), drop, dx.data_ptr(), _p(dres),
+              _grad_target(dweight, h, "weight"), _grad_target(dbias, h, "norm bias"), _grad_target(dx_bias, h, "bias"), ws.data_ptr(), ws_bytes, rows, h,
+              _stream())
     return dx, (dx if dres is None else dres)
 
 
@@ -619,27 +628,27 @@ def linear_act_fwd(x2d, w, bias=None, act="none", residual=None, want_pre=False)
     (T, n_in), (n, w_in) = x2d.shape, w.shape
     _need(n_in == w_in, "linear_act: inner dimensions differ")
     _need(n_in > 0 and n % 8 == 0, "linear_act: needs an input, and a width that is a multiple of 8")
-    _vector(bias, n, "bias")
+    _ready(bias=bias)
+    _vectors(n, bias=bias)
+    _here(x2d, "x"); _here(w, "weight")
     ldr = 0
     if residual is not None:
         ldr = _rows_ld(residual, "residual")
         _need(residual.shape == (T, n), "residual shape mismatch")
-    _here(x2d, w, bias, residual)
+        _here(residual, "residual")
     out = torch.empty((T, n), dtype=BF16, device=x2d.device)
     pre = torch.empty((T, n), dtype=BF16, device=x2d.device) if want_pre else None
     epilogue = _lib.Epilogue(_p(bias), _p(residual), _p(pre), ldr, n, ACTIVATIONS[act])
     ws, ws_bytes = _gemm_workspace(T, n, n_in, out.device)
-    _lib.call("ezl_gemm_bf16_epilogue", _p(x2d), _p(w), _p(out), T, n, n_in, lda, ldb, n, ctypes.byref(epilogue), _p(ws), ws_bytes, _stream())
+    _lib.call("ezl_gemm_bf16_epilogue", _p(x2d), _p(w), _p(out), T, n, n_in, lda, ldb, n, epilogue, _p(ws), ws_bytes, _stream())
     return out, pre
 
 
 def act_bwd(act, dy, pre, dbias=None):
     """-> dy * act'(pre); its column sums go to dbias = (f32 or None, bf16 or None, accumulate)."""
-    _bf16c(dy, "dy"); _bf16c(pre, "pre")
+    _ready(dy=dy, pre=pre)
     _need(dy.shape == pre.shape, "act_bwd: shape mismatch")
-    _here(dy, pre)
-    n = dy.shape[-1]
-    rows = dy.numel() // n
+    rows, n = _rows(dy)
     target = _grad_target(dbias, n, "bias")
     ws_bytes = _lib.column_sum_workspace_bytes(rows, n) if target else 0
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device) if target else None

@@ -85,7 +85,7 @@ typedef struct {
 int ezl_dropout_add_fwd(const void* x, const void* bias, const void* residual, const ezl_dropout* drop, void* out, int64_t rows, int64_t n,
                         void* stream);
 /* dx = what the draw left of dy, scaled (may be dy); dbias (HOST pointer, or NULL) = its column sums, taken before rounding.  (The residual's
- * gradient is dy.)  workspace: ezl_column_sum_workspace_bytes(rows, n), 16-byte aligned; not needed without dbias. */
+ * gradient is dy.)  Without drop dx is dy too: dx NULL, the column sums alone.  workspace: ezl_column_sum_workspace_bytes(rows, n), 16-byte aligned; not needed without dbias. */
 int64_t ezl_column_sum_workspace_bytes(int64_t rows, int64_t n);
 int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void* dx, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
                         int64_t rows, int64_t n, void* stream);

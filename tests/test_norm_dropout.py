@@ -118,11 +118,13 @@ def test_dropout_add_refuses():
     refused(-1, "drop_of_65536", *fwd(d=drop(-1)))
     refused(-1, "step", *fwd(d=drop(step=A + 4)))
     bwd = lambda dy=A, d=None, dx=A, g=None, ws=None, size=0: ("ezl_dropout_add_bwd", dy, d, dx, g, ws, size, 2, 64, None)  # noqa: E731
-    refused(-1, "null", *bwd(dy=None))
-    refused(-1, "null", *bwd(dx=None))
-    refused(-1, "workspace", *bwd(g=grad(f32=A)))
-    refused(-1, "workspace", *bwd(g=grad(bf16=A), ws=A, size=_lib.column_sum_workspace_bytes(2, 64) - 1))
-    refused(-1, "aligned", *bwd(g=grad(bf16=A), ws=A + 4, size=1 << 20))
+    refused(-1, "null", *bwd(dy=None, d=drop()))
+    refused(-1, "null", *bwd(dx=None, d=drop()))
+    refused(-1, "without drop", *bwd(g=grad(f32=A), ws=A, size=1 << 20))
+    refused(-1, "nothing to do", *bwd(dx=None))
+    refused(-1, "workspace", *bwd(d=drop(), g=grad(f32=A)))
+    refused(-1, "workspace", *bwd(dx=None, g=grad(bf16=A), ws=A, size=_lib.column_sum_workspace_bytes(2, 64) - 1))
+    refused(-1, "aligned", *bwd(dx=None, g=grad(bf16=A), ws=A + 4, size=1 << 20))
 
 
 def test_norm_refuses():
