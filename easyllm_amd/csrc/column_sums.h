@@ -14,6 +14,7 @@ inline ColumnSum column_sum(const float* partials, const ezl_layer_grad* g) {
     if (!wanted(g)) return {partials, nullptr, nullptr, 0};
     return {partials, g->f32 ? nullptr : g->bf16, g->f32, g->f32 && g->accumulate};
 }
+constexpr int64_t kMaxRows = (1LL << 31) - (1 << 16);  // row numbers are 32-bit, with room for one step past the last
 constexpr int kColumnSums = 3;
 // `count` of them (partials null: not there), in index order whatever the launch
 __attribute__((visibility("hidden"))) int column_sums(const char* name, const ColumnSum* sums, int count, int blocks, int64_t n, hipStream_t stream);

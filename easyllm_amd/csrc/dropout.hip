@@ -137,8 +137,8 @@ unsigned elementwise_grid(int64_t groups) {
     return (unsigned)(g > 256 * 16 ? 256 * 16 : g);
 }
 int sizes_check(const char* name, int64_t rows, int64_t n) {
-    EZL_REQUIRE(rows >= 0 && rows < (1LL << 31) && n > 0 && n % 8 == 0 && n < (1LL << 31) && (rows == 0 || n <= (1LL << 60) / rows), EZL_EUNSUPPORTED,
-                "%s: need n %% 8 == 0, rows and n < 2^31 (got %lld x %lld)", name, (long long)rows, (long long)n);
+    EZL_REQUIRE(rows >= 0 && rows <= kMaxRows && n > 0 && n % 8 == 0 && n <= kMaxRows && (rows == 0 || n <= (1LL << 60) / rows), EZL_EUNSUPPORTED,
+                "%s: need n %% 8 == 0, rows and n <= %lld (got %lld x %lld)", name, (long long)kMaxRows, (long long)rows, (long long)n);
     return EZL_OK;
 }
 

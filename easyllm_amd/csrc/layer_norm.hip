@@ -331,8 +331,8 @@ extern "C" int ezl_norm_fwd(int kind, const void* x, const void* x_bias, const v
     const char* name = "ezl_norm_fwd";
     const bool layer = kind == EZL_LAYER_NORM;
     EZL_REQUIRE(layer || kind == EZL_RMS_NORM, EZL_EINVAL, "%s: kind must be EZL_LAYER_NORM or EZL_RMS_NORM", name);
-    EZL_REQUIRE(rows >= 0 && rows < (1LL << 31) && h > 0 && h % 8 == 0 && h <= kMaxH, EZL_EUNSUPPORTED, "%s: need h %% 8 == 0, h <= %d and rows < 2^31 (got %lld x %lld)",
-                name, kMaxH, (long long)rows, (long long)h);
+    EZL_REQUIRE(rows >= 0 && rows <= kMaxRows && h > 0 && h % 8 == 0 && h <= kMaxH, EZL_EUNSUPPORTED, "%s: need h %% 8 == 0, h <= %d and rows <= %lld (got %lld x %lld)",
+                name, kMaxH, (long long)kMaxRows, (long long)rows, (long long)h);
     EZL_REQUIRE((residual != nullptr) == (sum_out != nullptr) || rows == 0, EZL_EINVAL, "%s: residual and sum_out go together", name);
     EZL_REQUIRE(residual || (layer && !x_bias && !drop) || rows == 0, EZL_EINVAL, "%s: x_bias, drop and EZL_RMS_NORM need a residual", name);
     EZL_REQUIRE(layer || !bias, EZL_EINVAL, "%s: an RMSNorm has no bias", name);
@@ -365,8 +365,8 @@ extern "C" int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const vo
     const char* name = "ezl_norm_bwd";
     const bool layer = kind == EZL_LAYER_NORM;
     EZL_REQUIRE(layer || kind == EZL_RMS_NORM, EZL_EINVAL, "%s: kind must be EZL_LAYER_NORM or EZL_RMS_NORM", name);
-    EZL_REQUIRE(rows >= 0 && rows < (1LL << 31) && h > 0 && h % 8 == 0 && h <= kMaxH, EZL_EUNSUPPORTED, "%s: need h %% 8 == 0, h <= %d and rows < 2^31 (got %lld x %lld)",
-                name, kMaxH, (long long)rows, (long long)h);
+    EZL_REQUIRE(rows >= 0 && rows <= kMaxRows && h > 0 && h % 8 == 0 && h <= kMaxH, EZL_EUNSUPPORTED, "%s: need h %% 8 == 0, h <= %d and rows <= %lld (got %lld x %lld)",
+                name, kMaxH, (long long)kMaxRows, (long long)rows, (long long)h);
     EZL_REQUIRE(weight && (rows == 0 || (dy && s && rstd && dx && (mean || !layer))), EZL_EINVAL, "%s: null pointer", name);
     EZL_REQUIRE(wanted(dweight), EZL_EINVAL, "%s: dweight is always written", name);
     EZL_REQUIRE(layer || !wanted(dbias), EZL_EINVAL, "%s: an RMSNorm has no bias", name);

@@ -3,7 +3,8 @@
 The mask of a call follows from (seed, offset, step) and the elements' indices alone (`include/ezl.h`, ezl_dropout), so nothing random is kept but
 these numbers: the backward pass is given the forward's, and a recomputed forward replays them (`recording`, `replaying`).  Every call takes the next offset.
 Inside a captured graph the offset is frozen; there the kernels add a step that lies in device memory, which whoever replays the graph advances
-(`stepping`; `runner.GraphedStep` does).  Outside one the step is zero, and a graph's first is one, so the two never draw the same numbers.
+(`stepping`; `runner.GraphedStep` does), between a replay's end and the next one's start.  Outside one the step is zero, and a graph's first is one, so the two
+never draw the same numbers.  Ranks that hold different data are seeded apart by whoever starts them (`manual_seed`).
 """
 import contextlib
 import threading
@@ -62,7 +63,7 @@ def next_draw():
             raise RuntimeError("a recomputed forward makes more dropout calls than the forward it repeats") from None
     else:
         step = None
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             if not _thread.steps:
                 raise RuntimeError("dropout inside a captured graph draws the same mask on every replay unless its step advances: "
                                    "capture with dropout.stepping() (runner.GraphedStep does)")

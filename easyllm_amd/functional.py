@@ -285,7 +285,8 @@ class NormFunction(torch.autograd.Function):
     arrives for s (x) is added inside the norm's backward kernel."""
 
     @staticmethod
-    def forward(ctx, kind, x, residual, x_bias, weight, bias, eps, threshold, draw, keep_input):
+    def forward(ctx, x, residual, x_bias, weight, bias, how):
+        kind, eps, threshold, draw, keep_input = how
         x = x.contiguous()
         y, s, mean, rstd = K.norm_fwd(kind, x, weight, bias, eps, None if residual is None else residual.contiguous(), x_bias, threshold, draw)
         ctx.kind, ctx.threshold, ctx.draw = kind, threshold, draw
@@ -301,12 +302,12 @@ class NormFunction(torch.autograd.Function):
         s, weight, bias, x_bias, mean, rstd = ctx.saved_tensors
         dsum, dy = grads if ctx.pair else (None, grads[0])
         need = ctx.needs_input_grad
-        weight_to, dw = _vector_target(weight, need[4])
-        bias_to, db = _vector_target(bias, need[5])
-        x_bias_to, dxb = _vector_target(x_bias, need[3])
-        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to if need[4] else (None, torch.empty_like(weight), False), bias_to,
+        weight_to, dw = _vector_target(weight, need[3])
+        bias_to, db = _vector_target(bias, need[4])
+        x_bias_to, dxb = _vector_target(x_bias, need[2])
+        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to if need[3] else (None, torch.empty_like(weight), False), bias_to,
                               None if dsum is None else dsum.contiguous(), ctx.threshold, ctx.draw, x_bias_to)
-        return (None, dx if need[1] else None, dres if ctx.has_residual and need[2] else None, dxb, dw, db, None, None, None, None)
+        return dx if need[0] else None, dres if ctx.has_residual and need[1] else None, dxb, dw, db, None
 
 
 def _draw_for(p, rng):
@@ -317,30 +318,30 @@ def _draw_for(p, rng):
 
 def layer_norm(x, weight, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension."""
-    return NormFunction.apply(K.LAYER_NORM, x, None, None, weight, bias, eps, 0, None, False)
+    return NormFunction.apply(x, None, None, weight, bias, (K.LAYER_NORM, eps, 0, None, False))
 
 
 def layer_norm_pass(x, weight, bias=None, eps=1e-5):
     """(x, layer_norm(x)): x as the residual branch, whose gradient is added in the norm's backward kernel."""
-    return NormFunction.apply(K.LAYER_NORM, x, None, None, weight, bias, eps, 0, None, True)
+    return NormFunction.apply(x, None, None, weight, bias, (K.LAYER_NORM, eps, 0, None, True))
 
 
 def add_layer_norm(x, residual, weight, bias=None, eps=1e-5):
     """(s, layer_norm(s)), s = x + residual"""
-    return NormFunction.apply(K.LAYER_NORM, x, residual, None, weight, bias, eps, 0, None, False)
+    return NormFunction.apply(x, residual, None, weight, bias, (K.LAYER_NORM, eps, 0, None, False))
 
 
 def dropout_add_layer_norm(x, residual, weight, norm_bias=None, eps=1e-5, bias=None, p=0.0, rng=None):
-    """(s, layer_norm(s)), s = residual + dropout(x + bias).  p is rounded to a multiple of 2^-16; rng: (seed, offset), or None for numbers of
-    this process's own (`easyllm_amd.dropout`)."""
+    """(s, layer_norm(s)), s = residual + dropout(x + bias).  p is rounded to a multiple of 2^-16; rng: (seed, offset) or (seed, offset,
+    step), an int64 [1] GPU tensor that holds still until the backward pass has run, or None for numbers of this process's own (`easyllm_amd.dropout`)."""
     threshold, draw = _draw_for(p, rng)
-    return NormFunction.apply(K.LAYER_NORM, x, residual, bias, weight, norm_bias, eps, threshold, draw, False)
+    return NormFunction.apply(x, residual, bias, weight, norm_bias, (K.LAYER_NORM, eps, threshold, draw, False))
 
 
 def dropout_add_rmsnorm(x, residual, weight, eps=1e-6, bias=None, p=0.0, rng=None):
     """(s, rmsnorm(s)), s = residual + dropout(x + bias).  The norm is of s in fp32 (`add_rmsnorm` rounds it first)."""
     threshold, draw = _draw_for(p, rng)
-    return NormFunction.apply(K.RMS_NORM, x, residual, bias, weight, None, eps, threshold, draw, False)
+    return NormFunction.apply(x, residual, bias, weight, None, (K.RMS_NORM, eps, threshold, draw, False))
 
 
 class DropoutAddFunction(torch.autograd.Function):

@@ -130,11 +130,12 @@ def rmsnorm_bwd_swapped(dy, x, weight, rstd, main_grad=None, accumulate=False):
 
 # ------------------------------------------------------------------------------------- dropout, layer norm
 # (Forward and backward of a small call are the host's work: checks of several tensors are one call here, and a draw's C form is made once.)
-def _ready(**tensors):
+def _ready(tensors, names):
     """Contiguous bf16 tensors (or None) of the current GPU, where the launch goes."""
     device = torch._C._cuda_getDevice()
-    for name, t in tensors.items():
+    for t in tensors:
         if t is not None and not (t.dtype is BF16 and t.get_device() == device and t.is_contiguous()):
+            name = names.split()[[u is t for u in tensors].index(True)]
             _bf16c(t, name)
             raise ValueError("%s is on GPU %d, but GPU %d is current" % (name, t.get_device(), device))
 
@@ -144,10 +145,10 @@ def _here(t, name):
         raise ValueError("%s is not on the current GPU" % name)
 
 
-def _vectors(n, **tensors):
-    for name, t in tensors.items():
+def _vectors(n, tensors, names):
+    for t in tensors:
         if t is not None and t.shape != (n,):
-            raise ValueError(name + " size mismatch")
+            raise ValueError(names.split()[[u is t for u in tensors].index(True)] + " size mismatch")
 
 
 def prepared_draw(threshold, draw):
@@ -189,9 +190,9 @@ def _rows(t):
 
 def dropout_add_fwd(x, bias, residual, threshold, draw):
     """residual + dropout(x + bias); bias and residual may be None."""
-    _ready(x=x, bias=bias, residual=residual)
+    _ready((x, bias, residual), "x bias residual")
     rows, n = _rows(x)
-    _vectors(n, bias=bias)
+    _vectors(n, (bias,), "bias")
     _need(residual is None or residual.shape == x.shape, "residual shape mismatch")
     out = torch.empty_like(x)
     _lib.call("ezl_dropout_add_fwd", x.data_ptr(), _p(bias), _p(residual), prepared_draw(threshold, draw), out.data_ptr(), rows, n, _stream())
@@ -200,7 +201,7 @@ def dropout_add_fwd(x, bias, residual, threshold, draw):
 
 def dropout_add_bwd(dy, threshold, draw, dbias=None):
     """-> dx (dy itself where nothing is dropped); the bias's gradient goes to dbias = (f32 or None, bf16 or None, accumulate)."""
-    _ready(dy=dy)
+    _ready((dy,), "dy")
     rows, n = _rows(dy)
     drop = prepared_draw(threshold, draw)
     target = _grad_target(dbias, n, "bias")
@@ -220,9 +221,9 @@ LAYER_NORM, RMS_NORM = 0, 1
 
 def norm_fwd(kind, x, weight, bias, eps, residual=None, x_bias=None, threshold=0, draw=None):
     """-> (y, sum, mean, rstd): the norm of x, or of sum = residual + dropout(x + x_bias).  RMS_NORM has no bias, no mean and needs a residual."""
-    _ready(x=x, weight=weight, bias=bias, residual=residual, x_bias=x_bias)
+    _ready((x, weight, bias, residual, x_bias), "x weight norm_bias residual bias")
     rows, h = _rows(x)
-    _vectors(h, weight=weight, bias=bias, x_bias=x_bias)
+    _vectors(h, (weight, bias, x_bias), "weight norm_bias bias")
     y = torch.empty_like(x)
     s = mean = None
     if residual is not None:
@@ -239,9 +240,9 @@ def norm_fwd(kind, x, weight, bias, eps, residual=None, x_bias=None, threshold=0
 def norm_bwd(kind, dy, s, weight, mean, rstd, dweight, dbias=None, dsum=None, threshold=0, draw=None, dx_bias=None):
     """-> (dx, dresidual), one tensor where nothing is dropped.  dweight, dbias, dx_bias: (f32 or None, bf16 or None, accumulate) that
     receive the parameters' gradients; the last two may be None."""
-    _ready(dy=dy, s=s, weight=weight, dsum=dsum)
+    _ready((dy, s, weight, dsum), "dy s weight dsum")
     rows, h = _rows(s)
-    _vectors(h, weight=weight)
+    _vectors(h, (weight,), "weight")
     for t in (mean, rstd):
         _need(t is None or (t.dtype is torch.float32 and t.shape == (rows,) and t.is_contiguous() and t.device == s.device), "norm_bwd: bad statistics")
     _need(dy.shape == s.shape and (dsum is None or dsum.shape == s.shape), "norm_bwd: shape mismatch")
@@ -628,8 +629,8 @@ def linear_act_fwd(x2d, w, bias=None, act="none", residual=None, want_pre=False)
     (T, n_in), (n, w_in) = x2d.shape, w.shape
     _need(n_in == w_in, "linear_act: inner dimensions differ")
     _need(n_in > 0 and n % 8 == 0, "linear_act: needs an input, and a width that is a multiple of 8")
-    _ready(bias=bias)
-    _vectors(n, bias=bias)
+    _ready((bias,), "bias")
+    _vectors(n, (bias,), "bias")
     _here(x2d, "x"); _here(w, "weight")
     ldr = 0
     if residual is not None:
@@ -646,7 +647,7 @@ def linear_act_fwd(x2d, w, bias=None, act="none", residual=None, want_pre=False)
 
 def act_bwd(act, dy, pre, dbias=None):
     """-> dy * act'(pre); its column sums go to dbias = (f32 or None, bf16 or None, accumulate)."""
-    _ready(dy=dy, pre=pre)
+    _ready((dy, pre), "dy pre")
     _need(dy.shape == pre.shape, "act_bwd: shape mismatch")
     rows, n = _rows(dy)
     target = _grad_target(dbias, n, "bias")

@@ -80,7 +80,7 @@ typedef struct {
     void *f32, *bf16;
     int accumulate;
 } ezl_layer_grad;
-/* out = residual + dropout(x + bias) over [rows, n] bf16, n % 8 == 0; bias [n] and residual may be NULL (out may be residual or x); fp32
+/* out = residual + dropout(x + bias) over [rows, n] bf16, n % 8 == 0, rows and n up to 2^31 - 2^16; bias [n] and residual may be NULL (out may be residual or x); fp32
  * arithmetic, one rounding.  drop NULL: nothing is dropped. */
 int ezl_dropout_add_fwd(const void* x, const void* bias, const void* residual, const ezl_dropout* drop, void* out, int64_t rows, int64_t n,
                         void* stream);
@@ -91,7 +91,7 @@ int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void* dx, const
                         int64_t rows, int64_t n, void* stream);
 
 /* ---- layer norm (base_modules/layers/fused_layer_norm.py, 'mixed_fused_norm'), and either norm behind dropout and the residual sum ----
- * rows of h bf16, h % 8 == 0, h <= 8192.  kind: EZL_LAYER_NORM y = (s - mean) * rstd * weight + bias (bias may be NULL), EZL_RMS_NORM
+ * rows of h bf16, h % 8 == 0, h <= 8192, up to 2^31 - 2^16 of them.  kind: EZL_LAYER_NORM y = (s - mean) * rstd * weight + bias (bias may be NULL), EZL_RMS_NORM
  * y = s * rstd * weight (bias NULL; with a residual, else ezl_rmsnorm_fwd); s = x, or with a residual s = residual + dropout(x + x_bias), x_bias and drop may be NULL.  sum_out, given with
  * a residual and only then, receives s rounded; y and the statistics are of s as it was.  mean (layer norm only) and rstd: fp32 [rows], kept
  * for backward.  A layer norm's weight may not be NULL. */

@@ -233,7 +233,14 @@ def test_the_wrappers_refuse(F):
                 lambda: F.linear_act(x.cpu(), w.cpu())):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             bad()
-    assert F.linear_act(x[:0], w, rnd(72), "gelu").shape == (0, 72)
+
+
+def test_an_empty_batch(F):
+    x, w, b, r = (rnd(*s, seed=i).requires_grad_(True) for i, s in enumerate(((0, 64), (72, 64), (72,), (0, 72))))
+    for act in (None, "gelu"):
+        y = F.linear_act(x, w, b, act, r)
+        got = torch.autograd.grad(y, (x, w, b, r), torch.empty_like(y))
+        assert y.shape == (0, 72) and [g.shape for g in got] == [t.shape for t in (x, w, b, r)] and not got[1].any() and not got[2].any()
 
 
 def test_a_captured_product_on_another_stream(F):

@@ -108,7 +108,7 @@ def grad(f32=None, bf16=None):
 
 def test_dropout_add_refuses():
     fwd = lambda x=A, b=None, r=None, d=None, o=A, rows=2, n=64: ("ezl_dropout_add_fwd", x, b, r, d, o, rows, n, None)  # noqa: E731
-    for args in (dict(n=60), dict(n=0), dict(rows=-1), dict(rows=2 ** 31), dict(n=2 ** 31)):
+    for args in (dict(n=60), dict(n=0), dict(rows=-1), dict(rows=2 ** 31 - 1), dict(n=2 ** 31)):
         refused(-2, "n % 8", *fwd(**args))
     for args in (dict(x=None), dict(o=None)):
         refused(-1, "null", *fwd(**args))
@@ -131,7 +131,7 @@ def test_norm_refuses():
     def fwd(kind=0, x=A, xb=None, r=None, d=None, w=A, b=None, y=A, s=None, mean=A, rstd=A, rows=2, h=64):
         return ("ezl_norm_fwd", kind, x, xb, r, d, w, b, y, s, mean, rstd, rows, h, 1e-5, None)
     refused(-1, "kind", *fwd(kind=2))
-    for args in (dict(h=60), dict(h=0), dict(h=8200), dict(rows=-1), dict(rows=2 ** 31)):
+    for args in (dict(h=60), dict(h=0), dict(h=8200), dict(rows=-1), dict(rows=2 ** 31 - 1)):
         refused(-2, "h % 8", *fwd(**args))
     for args in (dict(x=None), dict(w=None), dict(y=None), dict(rstd=None), dict(mean=None)):
         refused(-1, "null", *fwd(**args))
@@ -149,7 +149,7 @@ def test_norm_refuses():
     def bwd(kind=0, dy=A, ds=None, s=A, w=A, mean=A, rstd=A, d=None, dx=A, dr=None, gw=grad(f32=A), gb=None, gx=None, ws=A, size=size, rows=2, h=64):
         return ("ezl_norm_bwd", kind, dy, ds, s, w, mean, rstd, d, dx, dr, gw, gb, gx, ws, size, rows, h, None)
     refused(-1, "kind", *bwd(kind=-1))
-    for args in (dict(h=60), dict(h=8200), dict(rows=2 ** 31)):
+    for args in (dict(h=60), dict(h=8200), dict(rows=2 ** 31 - 1)):
         refused(-2, "h % 8", *bwd(**args))
     for args in (dict(dy=None), dict(s=None), dict(w=None), dict(mean=None), dict(rstd=None), dict(dx=None)):
         refused(-1, "null", *bwd(**args))

@@ -178,6 +178,20 @@ def test_no_rows(K):
     assert K.dropout_add_fwd(x, w, None, 100, (1, 2)).shape == (0, 64)
     K.dropout_add_bwd(x, 100, (1, 2), (None, dxb, False))
     assert not dxb.any()
+    dxb.fill_(5)
+    K.dropout_add_bwd(x, 0, None, (None, dxb, False))
+    assert not dxb.any()
+
+
+def test_one_row_without_a_batch(F):
+    x, r, w, b = (rnd(264, seed=i).requires_grad_(True) for i in range(4))
+    s, y = F.dropout_add_layer_norm(x, r, w, b, p=0.5, rng=(1, 2))
+    two = [t.detach().view(1, -1).requires_grad_(True) for t in (x, r)]
+    s2, y2 = F.dropout_add_layer_norm(*two, w, b, p=0.5, rng=(1, 2))
+    assert torch.equal(s, s2[0]) and torch.equal(y, y2[0])
+    got, want = torch.autograd.grad((y, s), (x, r, w, b), (x, r)), torch.autograd.grad((y2, s2), (*two, w, b), two)
+    for a, c in zip(got, want):
+        assert torch.equal(a, c.view_as(a))
 
 
 @pytest.mark.parametrize("rows,n", [(1, 8), (3, 64), (5, 520), (1167, 1000), (7, 8192), (2, 13704), (517, 5120), (4099, 256)])
