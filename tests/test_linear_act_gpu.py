@@ -68,8 +68,11 @@ def check_forward(K, M, N, Kd, act, bias, residual, seed=0, want_pre=True, strid
     close(y, a, slack, "y")
 
 
-# the smallest, odd ones, and every tile shape, whole and split, with and without a K tail (asked for below)
-SHAPES = [(1, 8, 8), (1, 11008, 4096), (8, 264, 1000), (17, 72, 4104), (64, 64, 64), (100, 520, 688), (389, 520, 256), (1000, 1032, 776), (389, 520, 1024),
+# up to 16 rows (a kernel of their own up to K = 6144) at each number of K blocks a wave owns, the smallest, odd ones, and every tile shape, whole and
+# split, with and without a K tail (asked for below)
+ROWS = [(1, 8, 8), (1, 11008, 4096), (8, 264, 1000), (16, 16, 512), (16, 24, 520), (5, 520, 1032), (3, 16384, 64), (16, 4104, 1544), (2, 72, 2560), (7, 1000, 3080),
+        (9, 8200, 4104), (16, 520, 5128), (15, 4096, 6144), (16, 520, 6152), (16, 32776, 72)]
+SHAPES = ROWS + [(17, 72, 4104), (64, 64, 64), (100, 520, 688), (389, 520, 256), (1000, 1032, 776), (389, 520, 1024),
           (389, 520, 4096), (389, 5120, 256), (389, 5120, 776), (600, 2048, 4096), (389, 5120, 1024), (389, 8192, 776), (1000, 1032, 4096), (4104, 2048, 256),
           (600, 5120, 4096), (1000, 5504, 1024), (1000, 5504, 776), (389, 2752, 4096), (4000, 8192, 256), (4000, 8192, 776), (2500, 5120, 256), (4104, 2048, 776),
           (389, 5120, 11008), (4096, 4096, 4096)]
@@ -96,7 +99,7 @@ def test_forward_without_some_of_it(K, M, N, Kd, bias, residual, want_pre):
     check_forward(K, M, N, Kd, "gelu", bias, residual, want_pre=want_pre)
 
 
-@pytest.mark.parametrize("M,N,Kd", [(3, 264, 64), (300, 520, 1000), (1100, 4096, 4096)])
+@pytest.mark.parametrize("M,N,Kd", [(3, 264, 64), (16, 4104, 1000), (300, 520, 1000), (1100, 4096, 4096)])
 def test_forward_of_strided_rows(K, M, N, Kd):
     print("strided", M, N, Kd, flush=True)
     check_forward(K, M, N, Kd, "gelu_tanh", True, True, strided=True)
@@ -106,7 +109,7 @@ def test_nothing_is_written_past_the_results_edges(K):
     """Rows and columns next to a result that is a part of a larger buffer stay as they are (through the C ABI: row strides of its own)."""
     import ctypes
     from easyllm_amd import _lib
-    for M, N, Kd in ((70, 72, 128), (300, 520, 1000), (1000, 4104, 4096)):
+    for M, N, Kd in ((5, 72, 136), (16, 8200, 4096), (70, 72, 128), (300, 520, 1000), (1000, 4104, 4096)):
         x, w, b = rnd(M, Kd, seed=1), rnd(N, Kd, seed=2), rnd(N, seed=3)
         full = torch.full((2, M + 300, N + 24), 77.0, dtype=torch.bfloat16, device="cuda")
         res = full[0].clone()
@@ -126,7 +129,7 @@ def test_nothing_is_written_past_the_results_edges(K):
 def test_the_residual_may_be_the_result(K):
     import ctypes
     from easyllm_amd import _lib
-    for M, N, Kd in ((70, 72, 128), (1000, 1032, 776), (2048, 4096, 4096), (1531, 4096, 11008)):
+    for M, N, Kd in ((9, 4104, 1000), (70, 72, 128), (1000, 1032, 776), (2048, 4096, 4096), (1531, 4096, 11008)):
         x, w, r = rnd(M, Kd, seed=1), rnd(N, Kd, seed=2), rnd(M, N, seed=3)
         want, _ = K.linear_act_fwd(x, w, None, "none", r)
         size = _lib.gemm_workspace_bytes(M, N, Kd)
@@ -152,6 +155,19 @@ def test_activations_over_their_whole_range(K):
         d = K.act_bwd(act, torch.ones_like(v), v)
         slope = act64(v.double().clamp(-200, 200), act)[1]
         close(d, slope, 2.0 ** -18 + slope.abs() * 2.0 ** -14, act + " slope")
+
+
+def test_what_is_not_finite_stays_in_its_place(K):
+    """An infinity in a weight or an input reaches the results it is part of, as itself, and no other; rows and columns and k past the operands' ends count for nothing."""
+    for M, N, Kd in ((5, 40, 72), (16, 520, 1000), (40, 72, 72), (300, 520, 1000)):
+        x, w = rnd(M, Kd, seed=1).abs() + 1, rnd(N, Kd, seed=2).abs() + 1
+        w[N - 1, 0] = float("inf")
+        x[M - 1, Kd - 1] = float("nan")
+        y, _ = K.linear_act_fwd(x, w, None, "gelu", None)
+        want = torch.full((M, N), False, device="cuda")
+        want[:, N - 1] = True
+        want[M - 1] = True
+        assert torch.equal(~torch.isfinite(y), want) and (y[:M - 1, N - 1] == float("inf")).all() and torch.isnan(y[M - 1]).all()
 
 
 def test_slopes_against_differences(K):
