@@ -270,12 +270,11 @@ def add_rmsnorm(x, residual, weight, eps):
 # layer norm, dropout and the residual sum: base_modules/layers/fused_layer_norm.py ('mixed_fused_norm'), hidden_dropout of llama/default_cfg.py:21
 # --------------------------------------------------------------------------------------------
 def _vector_target(param, needed):
-    """((f32, bf16, accumulate) for a kernel to write, gradient to return) of a vector parameter"""
+    """(where a kernel writes it, gradient to return) of a vector parameter that the forward has read"""
     if param is None or not needed:
         return None, None
     if getattr(param, "main_grad", None) is None:
-        grad = torch.empty_like(param)
-        return (None, grad, False), grad
+        return K.new_gradient(param)
     mg, acc = _main_grad_target(param)
     return (mg, None, acc), None
 
@@ -305,7 +304,9 @@ class NormFunction(torch.autograd.Function):
         weight_to, dw = _vector_target(weight, need[3])
         bias_to, db = _vector_target(bias, need[4])
         x_bias_to, dxb = _vector_target(x_bias, need[2])
-        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to if need[3] else (None, torch.empty_like(weight), False), bias_to,
+        if weight_to is None:  # (the kernel writes it in any case)
+            weight_to, unwanted = K.new_gradient(weight)
+        dx, dres = K.norm_bwd(ctx.kind, dy.contiguous(), s, weight, mean, rstd, weight_to, bias_to,
                               None if dsum is None else dsum.contiguous(), ctx.threshold, ctx.draw, x_bias_to)
         return dx if need[0] else None, dres if ctx.has_residual and need[1] else None, dxb, dw, db, None
 

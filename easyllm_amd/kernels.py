@@ -169,9 +169,9 @@ def prepared_draw(threshold, draw):
 
 
 def _grad_target(target, n, what):
-    """(f32 or None, bf16 or None, accumulate) -> C form; None: no gradient wanted"""
-    if target is None:
-        return None
+    """(f32 or None, bf16 or None, accumulate) -> C form; itself where it has that form; None: no gradient wanted"""
+    if target is None or type(target) is _lib.LayerGrad:
+        return target
     f32, bf16, accumulate = target
     if f32 is None:
         _need(bf16.dtype is BF16 and bf16.shape == (n,) and bf16.is_contiguous(), "bad gradient of the " + what)
@@ -180,6 +180,12 @@ def _grad_target(target, n, what):
     _need(f32.dtype is torch.float32 and f32.is_contiguous() and f32.numel() == n, "bad main_grad of the " + what)
     _here(f32, "the main_grad of the " + what)
     return _lib.LayerGrad(f32.data_ptr(), None, 1 if accumulate else 0)
+
+
+def new_gradient(param):
+    """(C form, bf16 tensor) of an overwritten gradient of a vector parameter that a kernel has read"""
+    grad = torch.empty_like(param)
+    return _lib.LayerGrad(None, grad.data_ptr(), 0), grad
 
 
 def _rows(t):
@@ -243,8 +249,9 @@ def norm_bwd(kind, dy, s, weight, mean, rstd, dweight, dbias=None, dsum=None, th
     _ready((dy, s, weight, dsum), "dy s weight dsum")
     rows, h = _rows(s)
     _vectors(h, (weight,), "weight")
-    for t in (mean, rstd):
-        _need(t is None or (t.dtype is torch.float32 and t.shape == (rows,) and t.is_contiguous() and t.device == s.device), "norm_bwd: bad statistics")
+    for t in (rstd, mean):
+        if t is not None and not (t.dtype is torch.float32 and t.shape == (rows,) and t.is_contiguous() and t.get_device() == s.get_device()):
+            raise ValueError("norm_bwd: bad statistics")
     _need(dy.shape == s.shape and (dsum is None or dsum.shape == s.shape), "norm_bwd: shape mismatch")
     dx = torch.empty_like(s)
     drop = prepared_draw(threshold, draw)

@@ -340,6 +340,21 @@ def test_main_grads_and_frozen_parameters(F):
     sum_near(xb.main_grad, dy.double() * factor((50, h), 0.5, 1, 1), torch.zeros(50, h, device="cuda").double() + 1e-6, "dbias")
 
 
+@pytest.mark.parametrize("frozen", ["w", "nb", "xb", "x", "r", "w nb xb"])
+def test_gradients_do_not_change_with_what_is_frozen(F, frozen):
+    names = ("x", "r", "w", "nb", "xb")
+    t = dict(zip(names, (rnd(70, 1032, seed=1), rnd(70, 1032, seed=2), rnd(1032, seed=3), rnd(1032, seed=4), rnd(1032, seed=5))))
+    d = rnd(70, 1032, seed=6), rnd(70, 1032, seed=7)
+
+    def grads(wanted):
+        v = {n: a.clone().requires_grad_(n in wanted) for n, a in t.items()}
+        s, y = F.dropout_add_layer_norm(v["x"], v["r"], v["w"], v["nb"], bias=v["xb"], p=0.25, rng=(8, 9))
+        return dict(zip(wanted, torch.autograd.grad((s, y), [v[n] for n in wanted], d)))
+    every, some = grads(names), grads([n for n in names if n not in frozen.split()])
+    for n, g in some.items():
+        assert torch.equal(g, every[n]), n
+
+
 def test_results_do_not_depend_on_the_launch_or_the_stream(F):
     x, r, w, nb = rnd(1500, 1032, seed=1).requires_grad_(True), rnd(1500, 1032, seed=2), rnd(1032, seed=3).requires_grad_(True), rnd(1032, seed=4)
     dy = rnd(1500, 1032, seed=5)
