@@ -16,5 +16,5 @@ inline ColumnSum column_sum(const float* partials, const ezl_layer_grad* g) {
 }
 constexpr int64_t kMaxRows = (1LL << 31) - (1 << 16);  // row numbers are 32-bit, with room for one step past the last
 constexpr int kColumnSums = 3;
-// `count` of them (partials null: not there), in index order whatever the launch
+// `count` of them, the rows of each in index order, one after the other where two targets share memory
 __attribute__((visibility("hidden"))) int column_sums(const char* name, const ColumnSum* sums, int count, int blocks, int64_t n, hipStream_t stream);

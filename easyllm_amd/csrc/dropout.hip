@@ -145,6 +145,14 @@ int sizes_check(const char* name, int64_t rows, int64_t n) {
 }  // namespace
 
 int column_sums(const char* name, const ColumnSum* sums, int count, int blocks, int64_t n, hipStream_t stream) {
+    // (one parameter in two places has one buffer, which is overwritten first and added to then)
+    for (int i = 1; i < count; ++i)
+        for (int j = 0; j < i; ++j)
+            if (sums[i].f32 && sums[j].f32 && (char*)sums[i].f32 < (char*)sums[j].f32 + 4 * n && (char*)sums[j].f32 < (char*)sums[i].f32 + 4 * n) {
+                for (int k = 0; k < count; ++k)
+                    if (const int rc = column_sums(name, sums + k, 1, blocks, n, stream)) return rc;
+                return EZL_OK;
+            }
     SumsArgs a = {};
     for (int i = 0; i < count; ++i) a.s[i] = sums[i];
     hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((n + 63) / 64), (unsigned)count), dim3(kColsumThreads), 0, stream, a, blocks, (int)n);

@@ -79,8 +79,8 @@ def sync_tp_duplicated_parameter(param):
 
 
 class _RngTracker(object):
-    """`get_cuda_rng_tracker().fork()` guards dropout in the reference (transformer.py:489); with
-    dropout 0 and one rank there is no state to switch."""
+    """`get_cuda_rng_tracker().fork()` guards attention dropout in the reference (transformer.py:489), which is 0 here; the
+    other dropouts' numbers are handed out call by call (dropout.py), so there is no state to switch."""
 
     @contextlib.contextmanager
     def fork(self, name="model-parallel-rng"):

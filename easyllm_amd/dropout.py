@@ -1,7 +1,8 @@
 """Where dropout takes its numbers from: a seed and a counter of the calls made so far (base_modules' `get_cuda_rng_tracker` role).
 
 The mask of a call follows from (seed, offset, step) and the elements' indices alone (`include/ezl.h`, ezl_dropout), so nothing random is kept but
-these numbers: the backward pass is given the forward's, and a recomputed forward replays them (`recording`, `replaying`).  Every call takes the next offset.
+these numbers: the backward pass is given the forward's, and a recomputed forward replays them (`recording`, `replaying`; `checkpointing.checkpoint` does, other
+recomputations have to).  Every call takes the next offset.
 Inside a captured graph the offset is frozen; there the kernels add a step that lies in device memory, which whoever replays the graph advances
 (`stepping`; `runner.GraphedStep` does), between a replay's end and the next one's start.  Outside one the step is zero, and a graph's first is one, so the two
 never draw the same numbers.  Ranks that hold different data are seeded apart by whoever starts them (`manual_seed`).

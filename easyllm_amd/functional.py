@@ -149,8 +149,11 @@ class LinearActFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         x2d = x.reshape(-1, x.shape[-1])
         r2d = None if residual is None else residual.reshape(-1, weight.shape[0])
-        if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
-            raise ValueError("residual shape mismatch")
+        if residual is not None:
+            if residual.shape != (*x.shape[:-1], weight.shape[0]):
+                raise ValueError("residual shape mismatch")
+            if r2d.stride(1) != 1 or r2d.stride(0) < r2d.shape[1]:
+                r2d = r2d.contiguous()
         y, pre = K.linear_act_fwd(x2d, weight, bias, act, r2d, act != "none" and (need[0] or need[1] or need[2]))
         ctx.act = act
         ctx.save_for_backward(x, weight, bias, pre)

@@ -223,6 +223,12 @@ def test_gradients_through_the_public_call(F, act, bias, residual):
         assert torch.equal(got["r"], dy)
 
 
+def test_residuals_of_other_layouts(F):
+    x, w = rnd(40, 64, seed=1), rnd(72, 64, seed=2)
+    for r in (rnd(72, seed=3).expand(40, 72), rnd(72, 40, seed=3).t(), rnd(40, 144, seed=3)[:, ::2]):
+        assert torch.equal(F.linear_act(x, w, None, "gelu", r), F.linear_act(x, w, None, "gelu", r.contiguous()))
+
+
 def test_main_grads_and_frozen_parameters(F):
     x, w, b = rnd(50, 64, seed=1).requires_grad_(True), rnd(72, 64, seed=2).requires_grad_(True), rnd(72, seed=3).requires_grad_(True)
     dy = rnd(50, 72, seed=4)

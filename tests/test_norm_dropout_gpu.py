@@ -340,6 +340,27 @@ def test_main_grads_and_frozen_parameters(F):
     sum_near(xb.main_grad, dy.double() * factor((50, h), 0.5, 1, 1), torch.zeros(50, h, device="cuda").double() + 1e-6, "dbias")
 
 
+def test_one_parameter_in_several_places(F):
+    """Its fp32 buffer takes the gradients one after the other: overwritten once where it is fresh, then added to."""
+    h = 2056
+    x, r, p = rnd(300, h, seed=1).requires_grad_(True), rnd(300, h, seed=2), rnd(h, seed=3).requires_grad_(True)
+    d = rnd(300, h, seed=4)
+
+    def call(q):
+        s, y = F.dropout_add_layer_norm(x, r, q[0], q[1], bias=q[2], p=0.1, rng=(1, 1))
+        return torch.autograd.grad((y, s), q, (d, d))
+    apart = [p.detach().clone().requires_grad_(True) for _ in range(3)]
+    want = sum(g.double() for g in call(apart))
+    for fresh in (True, False):
+        p.main_grad, p.main_grad_fresh = torch.full((h,), 7.0, device="cuda"), fresh
+        s, y = F.dropout_add_layer_norm(x, r, p, p, bias=p, p=0.1, rng=(1, 1))
+        torch.autograd.backward((y, s), (d, d))
+        off = (p.main_grad.double() - want - (0 if fresh else 7)).abs()
+        # the three are rounded to bf16 in `want`, 2^-8 each of at most
+        assert bool((off <= 2.0 ** -8 * sum(g.double().abs() for g in call(apart)) + 1e-3).all()), off.max()
+        p.main_grad = None
+
+
 @pytest.mark.parametrize("frozen", ["w", "nb", "xb", "x", "r", "w nb xb"])
 def test_gradients_do_not_change_with_what_is_frozen(F, frozen):
     names = ("x", "r", "w", "nb", "xb")
