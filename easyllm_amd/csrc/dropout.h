@@ -5,6 +5,7 @@
 // take the 128 bits of the counter (g low, g high, offset, step) under the key `seed` as eight 16-bit numbers, the low half of a word first, and
 // an element is dropped where its number is below drop_of_65536.  16 bits an element: the share is a multiple of 2^-16 (and
 // kept elements are scaled by what is exactly its counterpart), one generator call serves the 16 bytes of a lane's vector.
+// (32 bits, two calls: 8192 x 8192 forward with a residual 73.5 -> 74.8 us, backward 43.0 -> 49.7, the norm's backward 131 -> 142.)
 #pragma once
 #include "common.h"
 
