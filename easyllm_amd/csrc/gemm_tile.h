@@ -25,7 +25,7 @@ constexpr int kRoundResult = 2;
 // What a forward product's values go through on their way from the accumulators to a bf16 C: y = act(v + bias) + residual, fp32 up to the one
 // rounding; v + bias also goes to `pre` (rounded: the activation's backward reads it).  bias [N], residual (may be C) and pre [M, N] may
 // be null.  Rows start on 16 bytes, N is a multiple of 8.  What it costs beside the product alone, us: 4096 x 11008 x 4096 272, with bias and residual 288, GELU 286
-(with the tanh 276), both outputs 296 (291); 16384 x 4096 x 1024 119, 151, 141 (127), 164 (142), where a pass of its own over the result takes 54 and more.
+// (with the tanh 276), both outputs 296 (291); 16384 x 4096 x 1024 119, 151, 141 (127), 164 (142), where a pass of its own over the result takes 54 and more.
 struct NoEpilogue {};
 struct Epilogue {
     const bf16_t *bias, *residual;
