@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kWaves * 64) void gemm_rows_kernel(const bf16_t* __
         // above goes past the loads (seen as wrong last elements; tests/test_mfma_wait_states.py looks for such reads).
         asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a0), "+v"(a1));
         sums[buf][wave][lane] = a0 + a1;
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): written; the next tile's loads stay on the way across the barrier
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // written; the next tile's loads stay on the way across the barrier
         wave_barrier();
         // a register q of lane l is C[l & 15][16 tile + 4 (l >> 4) + q].  (A buffer is written again two tiles on, behind a barrier that its reader has passed.)
         const int n = tile * 16 + g * 4;
