@@ -93,6 +93,8 @@ __global__ __launch_bounds__(256) void dropout_sum_kernel(const DropSum a) {
     });
 }
 
+// pre is kept in bf16 (half the bytes of fp32; what its rounding moves the slope by is below dpre's own) and dpre is written in bf16, the operand of both gradients'
+// products.  Against 64 bits dx and dW come out 0.0024 off where a single rounding leaves 0.0017 (norms of 1531 x 4096 x 11008); the bias's gradient is summed before dpre is rounded.
 struct ActBwd {
     const bf16_t *dy, *pre;
     bf16_t* dpre;
@@ -205,6 +207,7 @@ extern "C" int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void
         EZL_LAUNCH_CHECK("ezl_dropout_add_bwd");
         return EZL_OK;
     }
+    EZL_REQUIRE(n <= kMaxSumColumns, EZL_EUNSUPPORTED, "%s: column sums of n <= %lld (got %lld)", name, (long long)kMaxSumColumns, (long long)n);
     EZL_REQUIRE(workspace && workspace_bytes >= ezl_column_sum_workspace_bytes(rows, n), EZL_EINVAL, "%s: workspace missing or too small", name);
     const DropSum a = {(const bf16_t*)dy, (bf16_t*)dx, (float*)workspace, (int)rows, (int)n, d};
     const dim3 grid = sum_grid(rows, n);
@@ -232,6 +235,7 @@ extern "C" int ezl_act_bwd(int act, const void* dy, const void* pre, void* dpre,
         EZL_LAUNCH_CHECK("ezl_act_bwd");
         return EZL_OK;
     }
+    EZL_REQUIRE(n <= kMaxSumColumns, EZL_EUNSUPPORTED, "%s: column sums of n <= %lld (got %lld)", name, (long long)kMaxSumColumns, (long long)n);
     EZL_REQUIRE(workspace && workspace_bytes >= ezl_column_sum_workspace_bytes(rows, n), EZL_EINVAL, "%s: workspace missing or too small", name);
     const dim3 grid = sum_grid(rows, n);
     if (act == kActGelu) hipLaunchKernelGGL((act_bwd_kernel<kActGelu, true>), grid, dim3(256), 0, st, a);

@@ -5,7 +5,8 @@
 //   ds = rstd (g - [mean(g)] - xhat mean(g xhat)) + dsum, g = dy w;   dw = sum dy xhat, db = sum dy, dx = dropout'(ds), dx_bias = sum dx
 //
 // A row is held in registers (h <= 8192) and read from HBM once: the variance is of the centred values, not a difference of two large sums.
-// y and the statistics are of the fp32 sum; the backward pass has the sum as it was stored, in bf16.
+// y and the statistics are of the fp32 sum.  The backward pass has the sum as it was stored, in bf16: dw and ds come out up to 0.0026 off 64 bits where one rounding
+// leaves 0.0018, and the sum made anew from x, the mask and the residual would be a quarter more to read.
 #include "column_sums.h"
 #include "dropout.h"
 

@@ -84,7 +84,7 @@ typedef struct {
  * arithmetic, one rounding.  drop NULL: nothing is dropped. */
 int ezl_dropout_add_fwd(const void* x, const void* bias, const void* residual, const ezl_dropout* drop, void* out, int64_t rows, int64_t n,
                         void* stream);
-/* dx = what the draw left of dy, scaled (may be dy); dbias (HOST pointer, or NULL) = its column sums, taken before rounding.  (The residual's
+/* dx = what the draw left of dy, scaled (may be dy); dbias (HOST pointer, or NULL) = its column sums, taken before rounding, n up to 2^27.  (The residual's
  * gradient is dy.)  Without drop dx is dy too: dx NULL, the column sums alone.  workspace: ezl_column_sum_workspace_bytes(rows, n), 16-byte aligned; not needed without dbias. */
 int64_t ezl_column_sum_workspace_bytes(int64_t rows, int64_t n);
 int ezl_dropout_add_bwd(const void* dy, const ezl_dropout* drop, void* dx, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
@@ -197,7 +197,7 @@ typedef struct {
 } ezl_epilogue; /* HOST struct */
 int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
                            const ezl_epilogue* epilogue, void* workspace, int64_t workspace_bytes, void* stream);
-/* dpre = dy * act'(pre) over [rows, n], n % 8 == 0 (may be dy or pre); dbias (HOST pointer, or NULL) = its column sums, taken before rounding, with a workspace of
+/* dpre = dy * act'(pre) over [rows, n], n % 8 == 0 (may be dy or pre); dbias (HOST pointer, or NULL) = its column sums, taken before rounding, n up to 2^27, with a workspace of
  * ezl_column_sum_workspace_bytes(rows, n).  act: EZL_ACT_GELU or EZL_ACT_GELU_TANH. */
 int ezl_act_bwd(int act, const void* dy, const void* pre, void* dpre, const ezl_layer_grad* dbias, void* workspace, int64_t workspace_bytes,
                 int64_t rows, int64_t n, void* stream);

@@ -127,6 +127,12 @@ def test_dropout_add_refuses():
     refused(-1, "aligned", *bwd(dx=None, g=grad(bf16=A), ws=A + 4, size=1 << 20))
 
 
+def test_column_sums_of_more_columns_than_a_launch_has_threads_for_are_refused():
+    n = 2 ** 27 + 8
+    refused(-2, "column sums", "ezl_dropout_add_bwd", A, drop(), A, grad(f32=A), A, 1 << 50, 1, n, None)
+    refused(-2, "column sums", "ezl_act_bwd", 1, A, A, A, grad(bf16=A), A, 1 << 50, 1, n, None)
+
+
 def test_norm_refuses():
     def fwd(kind=0, x=A, xb=None, r=None, d=None, w=A, b=None, y=A, s=None, mean=A, rstd=A, rows=2, h=64):
         return ("ezl_norm_fwd", kind, x, xb, r, d, w, b, y, s, mean, rstd, rows, h, 1e-5, None)
