@@ -45,7 +45,7 @@ def hf_to_megatron_llama(dt, model, pack=False):
         if "model.embed_tokens" in key:
             out["1.word_embeddings.weight"] = value
         elif "model.norm" in key:
-            out["%d.weight" % (L + 4)] = value
+            out["%d.%s" % (L + 4, key.rpartition(".")[2])] = value
         elif "lm_head" in key:
             out["%d.word_embeddings.weight" % (L + 5)] = value
         elif "layers" in key:
@@ -61,10 +61,8 @@ def hf_to_megatron_llama(dt, model, pack=False):
                     assert k_key in dt and v_key in dt, \
                         "Pack mode only suport q_proj, k_proj, v_proj in one checkpoint, please re-formula your checkpoint file."
                     out[prefix + "self_attn.wqkv." + kind] = [value, dt[k_key], dt[v_key]]
-                elif hf_name.startswith("self_attn"):
+                else:  # (utils.py:206-215 knows MLP and norm entries as weights only; layer norm and mlp_bias have both)
                     out[prefix + name + "." + kind] = value
-                else:  # MLP and norm entries are weights only (utils.py:206-215)
-                    out[prefix + name + ".weight"] = value
         else:
             logger.info("unuse keys %s", key)
     return out
@@ -144,7 +142,8 @@ def internlm2_to_llama2(dt, model, pack=False):
 
 
 def megatron_to_hf_llama(state_dict, num_layers):
-    """Inverse of `hf_to_megatron_llama` (unpacked form) for export; `inv_freq` buffers are dropped."""
+    """Inverse of `hf_to_megatron_llama` (unpacked form) for export; `inv_freq` buffers are dropped.  Layer norms and a plain MLP keep their
+    tensors' names, biases included, though no Hugging Face llama class reads them."""
     out = {}
     for key, value in state_dict.items():
         key = key[len("module."):] if key.startswith("module.") else key
@@ -155,7 +154,7 @@ def megatron_to_hf_llama(state_dict, num_layers):
         if idx == 1:
             out["model.embed_tokens.weight"] = value
         elif idx == num_layers + 4:
-            out["model.norm.weight"] = value
+            out["model.norm." + rest] = value
         elif idx == num_layers + 5:
             out["lm_head.weight"] = value
         elif 3 <= idx < num_layers + 3:
@@ -208,14 +207,32 @@ def _find_param(name, model):
     return None, None
 
 
+def _has_no_place(name, model):
+    """Whether this model holds the norm or MLP that a tensor belongs to, and not the tensor (layers may live elsewhere or be left out, and biases of
+    the attention's projections are passed by)."""
+    name = name[len("module."):] if name.startswith("module.") else name
+    index, part = name.split(".")[:2]
+    holder = index if part in ("weight", "bias") else index + "." + part
+    for candidate in (holder, "module." + holder):
+        try:
+            model.get_submodule(candidate)
+            return part != "self_attn"
+        except AttributeError:
+            pass
+    return False
+
+
 def copy_into_model(dt, model, tp_rank=0, tp_world_size=1, init_set=None):
     """Copies converted tensors into the model's parameters; returns the set of names that were initialised.
     A parameter with more rows than the checkpoint (padded vocabulary) keeps the checkpoint rows and fills the rest with
-    0.1 x the checkpoint row of smallest sum, as the reference does (utils.py:290-296)."""
+    0.1 x the checkpoint row of smallest sum, as the reference does (utils.py:290-296).  A norm's or an MLP's tensor that the model has no
+    place for (a bias, the gate of a plain MLP) is an error."""
     init_set = set() if init_set is None else init_set
     for name, value in dt.items():
         param, module = _find_param(name, model)
         if param is None:
+            if _has_no_place(name, model):
+                raise ValueError("Name %s -- the model has no such parameter" % name)
             continue
         tensor = slice_for_rank(value, module, tuple(param.shape), tp_rank, tp_world_size)
         with torch.no_grad():
