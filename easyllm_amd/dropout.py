@@ -61,7 +61,7 @@ def next_draw():
         try:
             draw = next(_thread.replays[-1])
         except StopIteration:
-            raise RuntimeError("a recomputed forward makes more dropout calls than the forward it repeats") from None
+            raise RuntimeError("a repeated forward makes more dropout calls than the forward whose numbers it takes") from None
     else:
         step = None
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
@@ -92,12 +92,17 @@ def recording():
 
 @contextlib.contextmanager
 def replaying(draws):
-    """This thread's calls inside the block take `draws`, in order."""
-    _thread.replays.append(iter(draws))
+    """This thread's calls inside the block take `draws`, in order and all of them."""
+    draws = list(draws)
+    left = iter(draws)
+    _thread.replays.append(left)
     try:
         yield
     finally:
         _thread.replays.pop()
+    unused = sum(1 for _ in left)
+    if unused:  # (a mask of the forward's that the repetition has not applied)
+        raise RuntimeError("a repeated forward made %d of %d dropout calls of the forward whose numbers it takes" % (len(draws) - unused, len(draws)))
 
 
 @contextlib.contextmanager
