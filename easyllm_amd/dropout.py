@@ -5,7 +5,8 @@ these numbers: the backward pass is given the forward's, and a recomputed forwar
 recomputations have to).  Every call takes the next offset.
 Inside a captured graph the offset is frozen; there the kernels add a step that lies in device memory, which whoever replays the graph advances
 (`stepping`; `runner.GraphedStep` does), between a replay's end and the next one's start.  Outside one the step is zero, and a graph's first is one, so the two
-never draw the same numbers.  Ranks that hold different data are seeded apart by whoever starts them (`manual_seed`).
+never draw the same numbers.  A captured graph keeps the numbers it was captured with: it is captured behind `manual_seed` or `set_state`, and a run that
+is to go on where it stopped keeps `get_state` and each `GraphedStep.dropout_state`.  Ranks that hold different data are seeded apart by whoever starts them (`manual_seed`).
 """
 import contextlib
 import threading
@@ -30,17 +31,21 @@ _thread = _Thread()
 _lock = threading.Lock()
 _seed = None  # None: torch's, when the first call is made
 _calls = 0
+_generation = 0  # how often the draws were started anew or somewhere else
 
 
 def manual_seed(seed):
     """Starts the draws of this process anew."""
-    global _seed, _calls
-    with _lock:
-        _seed, _calls = int(seed), 0
+    set_state((seed, 0))
+
+
+def generation():
+    """Another number after every `manual_seed` and `set_state`, which a captured graph does not follow."""
+    return _generation
 
 
 def get_state():
-    """(seed, number of calls): what a checkpoint of a training run has to keep."""
+    """(seed, number of calls): what a checkpoint of a training run has to keep, beside the `dropout_state` of each captured step."""
     global _seed
     with _lock:
         if _seed is None:
@@ -49,9 +54,10 @@ def get_state():
 
 
 def set_state(state):
-    global _seed, _calls
+    global _seed, _calls, _generation
     with _lock:
         _seed, _calls = int(state[0]), int(state[1])
+        _generation += 1
 
 
 def next_draw():

@@ -6,6 +6,8 @@ gradients landing in fp32 `main_grad` buffers (DeepSpeed's bf16 optimizer accumu
 The optimizer step with global-norm clipping that follows lives in optimizer.py; loss scaling by the
 number of accumulation steps and ZeRO partitioning are DeepSpeed's and are not reproduced.
 """
+import contextlib
+
 import torch
 
 from .registry import MODULE_ZOO_REGISTRY
@@ -102,10 +104,12 @@ class GraphedStep:
     time; new token ids / labels of the same shape are copied into the static input buffers by `__call__`.  The loss is
     returned as a device tensor that the next replay overwrites.  The token-id range check of the embedding cannot
     raise inside a graph: its flag is read back after every replay and raised one call late, as in the deferred mode.
-    Dropout draws anew on every replay: its captured calls read a step in device memory that `__call__` advances.
+    Dropout draws anew on every replay: its captured calls read a step in device memory that `__call__` advances.  A run that is resumed restores
+    `dropout.set_state` first and captures with `dropout_state`, what the interrupted run's step returned from `dropout_state()`: the replays then go on
+    where they stopped.  (Without it they draw numbers that no step had.)
     """
 
-    def __init__(self, model, inputs, labels, accumulate=False, warmup=2):
+    def __init__(self, model, inputs, labels, accumulate=False, warmup=2, dropout_state=None):
         from . import functional
         self.model = model
         self.inputs = _tree_map(lambda t: t.clone(), inputs)
@@ -126,19 +130,29 @@ class GraphedStep:
                 zero_main_grads(model)
             return forward_step(model, self.inputs, self.labels)
 
+        self._replays = 0 if dropout_state is None else int(dropout_state["step"])
+        self._dropout_generation = _dropout.generation()
+
+        def draws_of(step):
+            """New numbers, or those of the step that goes on, which take none of the process's."""
+            if dropout_state is None:
+                return contextlib.nullcontext()
+            return _dropout.replaying([_dropout.Draw(int(seed), int(offset), step) for seed, offset in dropout_state["draws"]])
+
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(warmup):
-                one_step()
+                with draws_of(None):
+                    one_step()
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         for p in model.parameters():
             p.grad = None
         del functional.CAPTURED_ID_FLAGS[:]
         self.graph = torch.cuda.CUDAGraph()
-        self._step = torch.zeros(1, dtype=torch.int64, device="cuda")
-        with _dropout.recording() as self._draws, _dropout.stepping(self._step), torch.cuda.graph(self.graph):
+        self._step = torch.full((1,), self._replays, dtype=torch.int64, device="cuda")
+        with _dropout.recording() as self._draws, _dropout.stepping(self._step), draws_of(self._step), torch.cuda.graph(self.graph):
             self.loss = one_step()
         self._flags = list(functional.CAPTURED_ID_FLAGS)
         del functional.CAPTURED_ID_FLAGS[:]
@@ -159,7 +173,14 @@ class GraphedStep:
             for host, (_, n) in zip(self._host_flags, self._flags):
                 functional._raise_for_id_flag(int(host.item()), self.inputs[0] if isinstance(self.inputs, (tuple, list)) else self.inputs, n)
 
+    def dropout_state(self):
+        """Plain values: what a checkpoint of the run has to keep for `dropout_state=` of the step that goes on from it."""
+        return {"step": self._replays, "draws": [(d.seed, d.offset) for d in self._draws]}
+
     def __call__(self, inputs=None, labels=None):
+        if self._draws and self._dropout_generation != _dropout.generation():
+            raise RuntimeError("dropout was seeded or its state restored behind the capture, whose numbers stay what they were: capture again "
+                               "(with the dropout_state of the step that is to go on)")
         self._check_previous()
         _tree_copy(*zip(*[(own, new) for own, new in ((self.inputs, inputs), (self.labels, labels)) if new is not None] or [((), ())]))
         if self._accumulate:
@@ -169,6 +190,7 @@ class GraphedStep:
                     p.main_grad_fresh = False
         if self._draws:
             self._step.add_(1)
+            self._replays += 1
         self.graph.replay()
         for host, (flag, _) in zip(self._host_flags, self._flags):
             host.copy_(flag, non_blocking=True)
