@@ -2,7 +2,7 @@
 
 The mask of a call follows from (seed, offset, step) and the elements' indices alone (`include/ezl.h`, ezl_dropout), so nothing random is kept but
 these numbers: the backward pass is given the forward's, and a recomputed forward replays them (`recording`, `replaying`; `checkpointing.checkpoint` does, other
-recomputations have to).  Every call takes the next offset.
+recomputations have to, or are refused).  Every call takes the next offset.
 Inside a captured graph the offset is frozen; there the kernels add a step that lies in device memory, which whoever replays the graph advances
 (`stepping`; `runner.GraphedStep` does), between a replay's end and the next one's start.  Outside one the step is zero, and a graph's first is one, so the two
 never draw the same numbers.  A captured graph keeps the numbers it was captured with: it is captured behind `manual_seed` or `set_state`, and a run that
@@ -69,6 +69,9 @@ def next_draw():
         except StopIteration:
             raise RuntimeError("a repeated forward makes more dropout calls than the forward whose numbers it takes") from None
     else:
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("dropout draws new numbers inside a backward pass, where a recomputed forward has to take those of the forward it repeats: "
+                               "record the forward's (dropout.recording()) and repeat it under dropout.replaying(), as checkpointing.checkpoint does")
         step = None
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             if not _thread.steps:
