@@ -29,13 +29,22 @@ class _Thread(threading.local):
 
 _thread = _Thread()
 _lock = threading.Lock()
-_seed = None  # None: torch's, when the first call is made
+_seed = None
+_given = False  # whether it is the caller's; else torch's
 _calls = 0
 _generation = 0  # how often the draws were started anew or somewhere else
 
 
+def _follow_torch():
+    """Without a seed of dropout's own the draws start anew where torch's seed has changed.  (Lock held.)"""
+    global _seed, _calls
+    if not _given and _seed != torch.initial_seed():
+        _seed, _calls = torch.initial_seed(), 0
+
+
 def manual_seed(seed):
-    """Starts the draws of this process anew."""
+    """Starts the draws of this process anew.  Until it or `set_state` is called, another seed given to `torch.manual_seed` does (the same one again does
+    not: the draws go on)."""
     set_state((seed, 0))
 
 
@@ -46,23 +55,21 @@ def generation():
 
 def get_state():
     """(seed, number of calls): what a checkpoint of a training run has to keep, beside the `dropout_state` of each captured step."""
-    global _seed
     with _lock:
-        if _seed is None:
-            _seed = torch.initial_seed()
+        _follow_torch()
         return _seed, _calls
 
 
 def set_state(state):
-    global _seed, _calls, _generation
+    global _seed, _given, _calls, _generation
     with _lock:
-        _seed, _calls = int(state[0]), int(state[1])
+        _seed, _given, _calls = int(state[0]), True, int(state[1])
         _generation += 1
 
 
 def next_draw():
     """The numbers of the next call of this thread: new ones, or those of the forward pass that is being recomputed."""
-    global _seed, _calls
+    global _calls
     if _thread.replays:
         try:
             draw = next(_thread.replays[-1])
@@ -79,8 +86,7 @@ def next_draw():
                                    "capture with dropout.stepping() (runner.GraphedStep does)")
             step = _thread.steps[-1]
         with _lock:
-            if _seed is None:
-                _seed = torch.initial_seed()
+            _follow_torch()
             draw = Draw((_seed + (_calls >> 32)) & 0xFFFFFFFFFFFFFFFF, _calls & 0xFFFFFFFF, step)
             _calls += 1
     for record in _thread.records:
