@@ -145,8 +145,8 @@ class LinearActFunction(torch.autograd.Function):
     rounding moves the slope by less than the gradient's own, which the products behind it take in bf16 anyway."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        need = ctx.needs_input_grad
+    def forward(ctx, x, weight, bias, residual, act, training):
+        need = ctx.needs_input_grad  # (also where gradients are off: a parameter's flag)
         x2d = x.reshape(-1, x.shape[-1])
         r2d = None if residual is None else residual.reshape(-1, weight.shape[0])
         if residual is not None:
@@ -154,7 +154,7 @@ class LinearActFunction(torch.autograd.Function):
                 raise ValueError("residual shape mismatch")
             if r2d.stride(1) != 1 or r2d.stride(0) < r2d.shape[1]:
                 r2d = r2d.contiguous()
-        y, pre = K.linear_act_fwd(x2d, weight, bias, act, r2d, act != "none" and (need[0] or need[1] or need[2]))
+        y, pre = K.linear_act_fwd(x2d, weight, bias, act, r2d, training and act != "none" and (need[0] or need[1] or need[2]))
         ctx.act = act
         ctx.save_for_backward(x, weight, bias, pre)
         return y.view(*x.shape[:-1], weight.shape[0])
@@ -176,7 +176,7 @@ class LinearActFunction(torch.autograd.Function):
             mg, acc = _main_grad_target(weight)
             dw = K.linear_wgrad(d, x.reshape(-1, x.shape[-1]), out=mg, accumulate=acc)
             dw = dw if mg is None else None
-        return dx, dw, db, dy if need[3] else None, None
+        return dx, dw, db, dy if need[3] else None, None, None
 
 
 def linear_act(x, weight, bias=None, activation=None, residual=None):
@@ -184,7 +184,7 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
     activation = activation or "none"
     if activation not in K.ACTIVATIONS:
         raise ValueError("activation must be one of %s, got %r" % (", ".join(K.ACTIVATIONS), activation))
-    return LinearActFunction.apply(x, weight, bias, residual, activation)
+    return LinearActFunction.apply(x, weight, bias, residual, activation, torch.is_grad_enabled())
 
 
 # --------------------------------------------------------------------------------------------
