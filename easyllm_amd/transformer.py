@@ -126,12 +126,23 @@ class ParallelMLP(torch.nn.Module):
                                            sync_tp_duplicated_parameters=sync_tp_duplicated_parameters,
                                            sequence_parallel=sequence_parallel)
 
+    def _activated(self, x, bias):
+        """The activation as a pass of its own, PyTorch's: behind a hooked or replaced projection, whose result has to be seen without it."""
+        x = x if bias is None else F_.bias_add(x, bias)
+        return torch.nn.functional.gelu(x, approximate="tanh" if self.activation == "gelu_tanh" else "none")
+
     def forward(self, hidden_states, residual=None):
         if not self.glu:
-            h1 = F_.linear_act(hidden_states, self.up_proj.weight, self.up_proj.bias, self.activation)
+            if is_plain(self.up_proj, ColumnParallelLinear):
+                h1 = F_.linear_act(hidden_states, self.up_proj.weight, self.up_proj.bias, self.activation)
+            else:
+                h1 = self._activated(*self.up_proj(hidden_states))
             if residual is None:
                 return self.down_proj(h1)
-            return F_.linear_act(h1, self.down_proj.weight, self.down_proj.bias, residual=residual), None
+            if is_plain(self.down_proj, RowParallelLinear):
+                return F_.linear_act(h1, self.down_proj.weight, self.down_proj.bias, residual=residual), None
+            output, bias = self.down_proj(h1)
+            return F_.dropout_add(output, residual, bias), None
         if residual is not None:
             raise ValueError("a gated MLP leaves the residual sum to the layer")
         # gate_proj and up_proj share their input: one fan-out op (input gradient accumulated in the GEMM)
