@@ -145,8 +145,11 @@ class ParallelMLP(torch.nn.Module):
             return F_.dropout_add(output, residual, bias), None
         if residual is not None:
             raise ValueError("a gated MLP leaves the residual sum to the layer")
-        # gate_proj and up_proj share their input: one fan-out op (input gradient accumulated in the GEMM)
-        h1, h2 = F_.fan_out_linear(hidden_states, self.gate_proj.weight, self.up_proj.weight)
+        if are_plain(((self.gate_proj, ColumnParallelLinear), (self.up_proj, ColumnParallelLinear))):
+            # gate_proj and up_proj share their input: one fan-out op (input gradient accumulated in the GEMM)
+            h1, h2 = F_.fan_out_linear(hidden_states, self.gate_proj.weight, self.up_proj.weight)
+        else:
+            h1, h2 = self.gate_proj(hidden_states)[0], self.up_proj(hidden_states)[0]
         h1 = self.activation_func.fused_mul(h1, h2)
         return self.down_proj(h1)
 
@@ -227,12 +230,11 @@ class ParallelAttention(torch.nn.Module):
         # hidden_states [s, b, h]
         if layer_past is not None or get_key_value:
             raise NotImplementedError("KV-cache inference is outside the training step")
-        if not self.qkv_pack and self.q_proj.bias is None:
-            query_layer, key_layer, value_layer = F_.fan_out_linear(hidden_states, self.q_proj.weight, self.k_proj.weight,
-                                                                    self.v_proj.weight)
-        elif not self.qkv_pack:
+        if not self.qkv_pack:
             projections = (self.q_proj, self.k_proj, self.v_proj)
-            if self._adds_all_biases(projections):  # one launch where that is faster, one input gradient
+            if all(p.bias is None for p in projections) and are_plain([(p, ColumnParallelLinear) for p in projections]):
+                query_layer, key_layer, value_layer = F_.fan_out_linear(hidden_states, *(p.weight for p in projections))
+            elif self._adds_all_biases(projections):  # one launch where that is faster, one input gradient
                 ys = F_.fan_out_linear(hidden_states, *(p.weight for p in projections))
                 query_layer, key_layer, value_layer = (F_.bias_add(y, p.bias) for y, p in zip(ys, projections))
             else:

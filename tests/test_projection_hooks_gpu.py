@@ -8,7 +8,9 @@ import torch
 pytestmark = pytest.mark.gpu
 
 PLAIN = dict(glu_activation=None, mlp_bias=True)
-STACKS = {"plain MLP, biases": (dict(PLAIN), "up_proj"), "plain MLP, tanh": (dict(glu_activation=None, use_openai_gelu=True), "up_proj")}
+STACKS = {"plain MLP, biases": (dict(PLAIN), "up_proj"), "plain MLP, tanh": (dict(glu_activation=None, use_openai_gelu=True), "up_proj"),
+          "gated MLP, gate": ({}, "gate_proj"), "gated MLP, up": ({}, "up_proj"), "attention, q": ({}, "q_proj"), "attention, v": ({}, "v_proj"),
+          "attention, k with a bias": (dict(attention_qkv_bias=True), "k_proj"), "packed projections": (dict(qkv_pack=True), "wqkv")}
 
 
 def build(layer):
@@ -64,28 +66,34 @@ def test_a_hook_sees_the_projections_own_call(name):
 
 @pytest.mark.parametrize("name", STACKS)
 def test_what_a_hook_returns_counts(name):
+    """Twice the projection, against the projection itself through a hook: the same launches, other values."""
     params, part = STACKS[name]
     layer = build(params).get_submodule("3")
-    want, _ = run(layer)
-    hook = find(layer, part).register_forward_hook(lambda m, i, o: (o[0] * 2, o[1]))
-    got, grads = run(layer)
-    hook.remove()
-    assert not close(got, want) and all(torch.isfinite(g).all() for g in grads)
+    results = []
+    for factor in (1, 2):
+        hook = find(layer, part).register_forward_hook(lambda m, i, o: (o[0] * factor, o[1]))
+        results.append(run(layer))
+        hook.remove()
+    (one, _), (two, grads) = results
+    assert not torch.equal(one, two) and all(torch.isfinite(g).all() for g in grads)
 
 
 @pytest.mark.parametrize("name", STACKS)
 def test_a_projection_of_another_class_is_called(name):
     params, part = STACKS[name]
     layer = build(params).get_submodule("3")
-    want, _ = run(layer)
     module = find(layer, part)
 
     class Adapted(type(module)):
+        share = 0
+
         def forward(self, x):
             y, bias = super().forward(x)
-            return y + 3 * y.detach().roll(1, -1), bias
+            return y + self.share * y.detach().roll(1, -1), bias
     module.__class__ = Adapted
-    assert not close(run(layer)[0], want)
+    without, _ = run(layer)
+    Adapted.share = 3
+    assert not torch.equal(run(layer)[0], without)
 
 
 def test_a_residual_does_not_pass_a_hooked_down_projection_by():
