@@ -9,6 +9,7 @@ checkpoint variants of DeepSpeed are not reproduced.
 import torch
 
 from . import dropout
+from .first_order import first_order
 
 
 class _CheckpointFunction(torch.autograd.Function):
@@ -23,6 +24,7 @@ class _CheckpointFunction(torch.autograd.Function):
         return outputs
 
     @staticmethod
+    @first_order
     def backward(ctx, *grads):
         args = list(ctx.others)
         detached = []

@@ -16,6 +16,7 @@ import torch
 
 from . import dropout as _dropout
 from . import kernels as K
+from .first_order import first_order
 
 
 def _main_grad_target(param):
@@ -41,6 +42,7 @@ class LinearFunction(torch.autograd.Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         dy2d = dy.reshape(-1, dy.shape[-1])
@@ -74,6 +76,7 @@ class LinearFp32OutputFunction(torch.autograd.Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         return LinearFunction.backward(ctx, K.cast_f32_to_bf16(dy.contiguous()))
 
@@ -94,6 +97,7 @@ class FanOutLinearFunction(torch.autograd.Function):
         return tuple(y.view(*x.shape[:-1], y.shape[1]) for y in K.linear_fwd_multi(x2d, weights))
 
     @staticmethod
+    @first_order
     def backward(ctx, *dys):
         x, *weights = ctx.saved_tensors
         x2d = x.reshape(-1, x.shape[-1])
@@ -130,6 +134,7 @@ class BiasAddFunction(torch.autograd.Function):
         return K.bias_add(x.contiguous(), bias)
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         mg, acc = _main_grad_target(ctx.bias)
         db = K.bias_grad(dy.contiguous(), main_grad=mg, accumulate=acc)
@@ -160,6 +165,7 @@ class LinearActFunction(torch.autograd.Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, weight, bias, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -212,6 +218,7 @@ class RMSNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, weight, rstd = ctx.saved_tensors
         mg, acc = _main_grad_target(weight)
@@ -230,6 +237,7 @@ class AddRMSNormFunction(torch.autograd.Function):
         return s, y
 
     @staticmethod
+    @first_order
     def backward(ctx, dsum, dy):
         s, weight, rstd = ctx.saved_tensors
         mg, acc = _main_grad_target(weight)
@@ -249,6 +257,7 @@ class RMSNormPassFunction(torch.autograd.Function):
         return xc.view_as(xc), y
 
     @staticmethod
+    @first_order
     def backward(ctx, dres, dy):
         x, weight, rstd = ctx.saved_tensors
         mg, acc = _main_grad_target(weight)
@@ -300,6 +309,7 @@ class NormFunction(torch.autograd.Function):
         return (x.view_as(x), y) if keep_input else y
 
     @staticmethod
+    @first_order
     def backward(ctx, *grads):
         s, weight, bias, x_bias, mean, rstd = ctx.saved_tensors
         dsum, dy = grads if ctx.pair else (None, grads[0])
@@ -355,6 +365,7 @@ class DropoutAddFunction(torch.autograd.Function):
         return K.dropout_add_fwd(x.contiguous(), bias, None if residual is None else residual.contiguous(), threshold, draw)
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         bias_to, db = _vector_target(ctx.bias, ctx.needs_input_grad[2])
         dx = K.dropout_add_bwd(dy.contiguous(), ctx.threshold, ctx.draw, bias_to) if ctx.needs_input_grad[0] or bias_to else None
@@ -377,6 +388,7 @@ class SwiGLUFunction(torch.autograd.Function):
         return K.swiglu_fwd(gate, up)
 
     @staticmethod
+    @first_order
     def backward(ctx, dout):
         gate, up = ctx.saved_tensors
         return K.swiglu_bwd(dout.contiguous(), gate, up)
@@ -398,6 +410,7 @@ class RotaryFunction(torch.autograd.Function):
         return K.rope_apply(x, cos, sin, position_ids)
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         cos, sin, position_ids = ctx.saved_tensors
         if dy.stride(3) != 1 or dy.stride(2) != dy.shape[3]:
@@ -418,6 +431,7 @@ class RotaryPairFunction(torch.autograd.Function):
         return K.rope_apply_pair(q, k, cos, sin, position_ids)
 
     @staticmethod
+    @first_order
     def backward(ctx, dq, dk):
         cos, sin, position_ids = ctx.saved_tensors
         if dq.stride(3) != 1 or dq.stride(2) != dq.shape[3]:
@@ -446,6 +460,7 @@ class FlashAttnFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, dout):
         q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
         if dout.stride(3) != 1 or dout.stride(2) != dout.shape[3]:
@@ -470,6 +485,7 @@ class RowsGatherFunction(torch.autograd.Function):
         return K.rows_gather(x, idx, out_sb)
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         (idx_back,) = ctx.saved_tensors
         if dy.stride(3) != 1 or dy.stride(2) != dy.shape[3]:
@@ -508,6 +524,7 @@ class DecoderLayerFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, saved, cos, sin, position_ids, cu_seqlens, *params = ctx.saved_tensors
         desc = K.layer_desc(x.shape, *ctx.plan, params[:9], params[9:] or None, cos, sin, position_ids, cu_seqlens)
@@ -556,6 +573,7 @@ class EmbeddingFunction(torch.autograd.Function):
         return out, flag
 
     @staticmethod
+    @first_order
     def backward(ctx, dout, _dflag):
         ids, weight = ctx.saved_tensors
         mg, acc = _main_grad_target(weight)
@@ -720,6 +738,7 @@ class Transpose01Function(torch.autograd.Function):
         return K.transpose01(x.contiguous())
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         return K.transpose01(dy.contiguous())
 
@@ -751,6 +770,7 @@ class ToFp32Function(torch.autograd.Function):
         return K.cast_bf16_to_f32(x.contiguous())
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         return K.cast_f32_to_bf16(dy.contiguous())
 
@@ -775,6 +795,7 @@ class VocabParallelCrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         logits, target, lse = ctx.saved_tensors
         g = K.ce_bwd(logits, target, lse, grad_out.contiguous().float(), ctx.cut_size)
@@ -802,6 +823,7 @@ class FusedCrossEntropyLossFunction(torch.autograd.Function):
         return K.ce_reduce(loss_rows, weights, count)
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_out):
         if not ctx.saved_tensors:  # (only the mask asked for a gradient, and has none)
             return (None,) * 7
