@@ -311,6 +311,14 @@ unsigned blocks_for(int64_t rows, int64_t h, int64_t most) {
     return (unsigned)(blocks > most ? most : (blocks < 1 ? 1 : blocks));
 }
 
+// Every block leaves partial rows of h floats, which few rows feel, and wide ones, which cost most per block; the others gain by two blocks per CU.  256
+// against 512, us: 1167 x 1000 9.1, 9.6; 4000 x 2048 20.7, 21.6 (with dropout and a bias 26.1, 27.2); 8000 x 2048 30.8, 29.9; 2048 x 4096 22.5, 24.4; 4096 x 5120 42.6,
+// 39.3; 16384 x 5120 138, 116; 32768 x 1024 50.5, 48.9 (67.5, 63.0); 4096 x 8192 53.0, 56.0; 8192 x 8192 91.8, 95.7.
+unsigned bwd_blocks(int64_t rows, int64_t h) {
+    const bool few = rows * split_of(h) <= 8192 || h > 6144;
+    return blocks_for(rows, h, few ? kBwdBlocks / 2 : kBwdBlocks);  // (no rows still give zero sums)
+}
+
 template <bool CENTER, bool RES, bool DROP>
 void launch_fwd(const NormFwd& a, hipStream_t st) {
     by_width(a.h, [&](auto nc, auto ns) {
@@ -356,8 +364,7 @@ extern "C" int ezl_norm_fwd(int kind, const void* x, const void* x_bias, const v
 }
 
 extern "C" int64_t ezl_norm_bwd_workspace_bytes(int64_t rows, int64_t h) {
-    (void)rows;
-    return kColumnSums * kBwdBlocks * h * (int64_t)sizeof(float);
+    return rows < 0 || h <= 0 ? 0 : kColumnSums * bwd_blocks(rows, h) * h * (int64_t)sizeof(float);
 }
 
 extern "C" int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const void* s, const void* weight, const void* mean, const void* rstd,
@@ -375,16 +382,13 @@ extern "C" int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const vo
     EZL_REQUIRE(ezl_aligned16(dy) && ezl_aligned16(dsum) && ezl_aligned16(s) && ezl_aligned16(weight) && ezl_aligned16(dx) && ezl_aligned16(dresidual) && ezl_aligned16(workspace),
                 EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
     EZL_REQUIRE(workspace && workspace_bytes >= ezl_norm_bwd_workspace_bytes(rows, h), EZL_EINVAL, "%s: workspace missing or too small", name);
+    const unsigned grid = bwd_blocks(rows, h);
+    const int64_t set = grid * h;  // partial rows of one sum
     float* part = (float*)workspace;
     NormBwd a = {(const bf16_t*)dy, (const bf16_t*)dsum, (const bf16_t*)s, (const bf16_t*)weight, (const float*)mean, (const float*)rstd, (bf16_t*)dx,
-                 (bf16_t*)dresidual, part, part + kBwdBlocks * h, part + 2 * kBwdBlocks * h, (int)rows, (int)h, {}};
+                 (bf16_t*)dresidual, part, part + set, part + 2 * set, (int)rows, (int)h, {}};
     if (const int rc = drop_args(name, drop, a.drop)) return rc;
     hipStream_t st = (hipStream_t)stream;
-    // Every block leaves partial rows of h floats, which few rows feel, and wide ones, which cost most per block; the others gain by two blocks per CU.  256
-    // against 512, us: 1167 x 1000 9.1, 9.6; 4000 x 2048 20.7, 21.6 (with dropout and a bias 26.1, 27.2); 8000 x 2048 30.8, 29.9; 2048 x 4096 22.5, 24.4; 4096 x 5120 42.6,
-    // 39.3; 16384 x 5120 138, 116; 32768 x 1024 50.5, 48.9 (67.5, 63.0); 4096 x 8192 53.0, 56.0; 8192 x 8192 91.8, 95.7.
-    const bool few = rows * split_of(h) <= 8192 || h > 6144;
-    const unsigned grid = blocks_for(rows, h, few ? kBwdBlocks / 2 : kBwdBlocks);  // (no rows still give zero sums)
     const bool xb = wanted(dx_bias);
 #define EZL_LAUNCH_BWD(L)                                          \
     do {                                                           \
