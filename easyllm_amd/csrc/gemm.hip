@@ -1174,7 +1174,7 @@ extern "C" int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int
     EZL_REQUIRE((!e.residual || e.ldr >= N) && (!e.pre || e.ldp >= N), EZL_EINVAL, "%s: leading dimension too small", name);
     EZL_REQUIRE(ezl_aligned16(C) && ezl_aligned16(e.bias) && ezl_aligned16(e.residual) && ezl_aligned16(e.pre) && ezl_aligned16(workspace), EZL_EINVAL,
                 "%s: pointers must be 16-byte aligned", name);
-    if (gemm_rows_pays(M, K)) {
+    if (gemm_rows_pays(M, N, K)) {
         gemm_rows_launch(A, B, C, (int)M, (int)N, (int)K, lda, ldb, ldc, e, (hipStream_t)stream);
         EZL_LAUNCH_CHECK("ezl_gemm_bf16_epilogue");
         return EZL_OK;

@@ -82,6 +82,7 @@ __global__ __launch_bounds__(kWaves * 64) void gemm_rows_kernel(const bf16_t* __
 }  // namespace
 
 void gemm_rows_launch(const void* X, const void* W, void* C, int M, int N, int K, int64_t ldx, int64_t ldw, int64_t ldc, const Epilogue& epi, hipStream_t st) {
+    static_assert(kRowsMaxK <= 10 * 64 * kWaves, "blocks of K in registers");
     const int tiles = (N + 15) / 16, kb = (K + 64 * kWaves - 1) / (64 * kWaves);
     // One workgroup per CU where it has 24 loads per wave and more on the way, two where fewer: 8 rows, 8192 x 1000 6.2 -> 5.7 us, but 11008 x 4096 21.6 -> 24.2.
     const int most = kb <= 2 ? 512 : 256;
@@ -96,8 +97,7 @@ void gemm_rows_launch(const void* X, const void* W, void* C, int M, int N, int K
         case 4: EZL_ROWS(4);
         case 5: case 6: EZL_ROWS(6);
         case 7: case 8: EZL_ROWS(8);
-        case 9: case 10: EZL_ROWS(10);
-        default: EZL_ROWS(12);
+        default: EZL_ROWS(10);
     }
 #undef EZL_ROWS
 }
