@@ -157,8 +157,9 @@ class LinearActFunction(torch.autograd.Function):
         if residual is not None:
             if residual.shape != (*x.shape[:-1], weight.shape[0]):
                 raise ValueError("residual shape mismatch")
-            if r2d.stride(1) != 1 or r2d.stride(0) < r2d.shape[1]:
-                r2d = r2d.contiguous()
+            step = r2d.stride(0)
+            if r2d.stride(1) != 1 or step < r2d.shape[1] or step % 8 or step >= 2 ** 21 or r2d.data_ptr() % 16:  # (what the kernel does not read in place)
+                r2d = r2d.clone(memory_format=torch.contiguous_format)
         y, pre = K.linear_act_fwd(x2d, weight, bias, act, r2d, training and act != "none" and (need[0] or need[1] or need[2]))
         ctx.act = act
         ctx.save_for_backward(x, weight, bias, pre)
