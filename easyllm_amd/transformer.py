@@ -362,26 +362,36 @@ class ParallelTransformerLayer(torch.nn.Module):
         scale = core.softmax_scale if core.softmax_scale is not None else d ** -0.5
         return hidden_states, ((nq, nk, d), f, (ln1.eps, ln2.eps), scale), cos, sin, position_ids, cu_seqlens, params
 
+    @staticmethod
+    def _passes_by(norm):
+        """Whether the norm's own call may be passed by, for the sum in front of it or its input's gradient in its kernels."""
+        return type(norm) in (RMSNorm, MixedFusedLayerNorm) and is_plain(norm, type(norm))
+
     def forward(self, hidden_states, attention_mask, cu_seqlens=None, position_ids=None, layer_past=None,
                 get_key_value=False):
         if layer_past is None and not get_key_value:
             native = self._native_inputs(hidden_states, attention_mask, cu_seqlens, position_ids)
             if native is not None:
                 return F_.decoder_layer(*native)
-        hidden_states, layernorm_output = self.input_layernorm.forward_keep_input(hidden_states)
+        if self._passes_by(self.input_layernorm):
+            hidden_states, layernorm_output = self.input_layernorm.forward_keep_input(hidden_states)
+        else:
+            layernorm_output = self.input_layernorm(hidden_states)
         attention_output, attention_bias = self.self_attn(layernorm_output, attention_mask, cu_seqlens, position_ids,
                                                           layer_past=layer_past, get_key_value=get_key_value, alibi=self.alibi)
         dropout_p = self.hidden_dropout if self.training else 0.0
+        post_norm = self.apply_residual_connection_post_layernorm
         norm_takes_bias = dropout_p > 0 or isinstance(self.post_attention_layernorm, MixedFusedLayerNorm)  # (and the dropout in front of it)
         if attention_bias is not None and not norm_takes_bias:
             attention_output, attention_bias = F_.bias_add(attention_output, attention_bias), None
-        if self.apply_residual_connection_post_layernorm:
+        if post_norm or not self._passes_by(self.post_attention_layernorm):
+            residual = layernorm_output if post_norm else hidden_states
             if dropout_p > 0 or attention_bias is not None:
-                layernorm_input = F_.dropout_add(attention_output, layernorm_output, attention_bias, dropout_p)
+                layernorm_input = F_.dropout_add(attention_output, residual, attention_bias, dropout_p)
             else:
-                layernorm_input = F_.add(attention_output, layernorm_output)
+                layernorm_input = F_.add(attention_output, residual)
             layernorm_output = self.post_attention_layernorm(layernorm_input)
-            residual = layernorm_output
+            residual = layernorm_output if post_norm else layernorm_input
         elif norm_takes_bias:
             layernorm_input, layernorm_output = self.post_attention_layernorm.forward_with_dropout_residual(attention_output, hidden_states, dropout_p,
                                                                                                             attention_bias)
@@ -416,4 +426,4 @@ class ParallelTransformerLayerPipe(ParallelTransformerLayer):
         raise RuntimeError("Received more inputs than understood.")
 
 
-passed_by_when_plain(RMSNorm, ColumnParallelLinear, RowParallelLinear, RotaryEmbedding, FlashAttention, ParallelMLP, ParallelAttention)
+passed_by_when_plain(RMSNorm, MixedFusedLayerNorm, ColumnParallelLinear, RowParallelLinear, RotaryEmbedding, FlashAttention, ParallelMLP, ParallelAttention)

@@ -1,4 +1,4 @@
-"""Hooks on a layer's projections, and projections that stand in for them, are not passed by.
+"""Hooks on a layer's projections and norms, and modules that stand in for them, are not passed by.
 
 Tolerance, before any run: without a hook the two differ by a few roundings to bf16 in what is stored between the products, 2^-9 of its size each: 1 % of the
 result's norm is five times that and more."""
@@ -13,11 +13,11 @@ STACKS = {"plain MLP, biases": (dict(PLAIN), "up_proj"), "plain MLP, tanh": (dic
           "attention, k with a bias": (dict(attention_qkv_bias=True), "k_proj"), "packed projections": (dict(qkv_pack=True), "wqkv")}
 
 
-def build(layer):
+def build(layer, **kw):
     from easyllm_amd import runner
     torch.manual_seed(5)
     cfg = dict(num_layers=1, hidden_size=256, num_attention_heads=4, intermediate_size=712, vocab_size=520, seq_length=96, bf16=True,
-               checkpoint_activations=False, fp32_logits=False, transformer_layer_params=dict(layer))
+               checkpoint_activations=False, fp32_logits=False, transformer_layer_params=dict(layer), **{k: dict(v) if isinstance(v, dict) else v for k, v in kw.items()})
     model = runner.build_model({"type": "llama_custom", "kwargs": cfg}).cuda()
     with torch.no_grad():
         for p in model.parameters():
@@ -27,7 +27,7 @@ def build(layer):
 
 
 def find(layer, name):
-    return getattr(layer.mlp if hasattr(layer.mlp, name) else layer.self_attn, name)
+    return next(getattr(m, name) for m in (layer, layer.mlp, layer.self_attn) if hasattr(m, name))
 
 
 def close(a, b):
@@ -105,3 +105,55 @@ def test_a_residual_does_not_pass_a_hooked_down_projection_by():
     got, bias2 = mlp(x, residual=r)
     hook.remove()
     assert len(seen) == 1 and bias is None and bias2 is None and close(got, want)
+
+
+LN = dict(layer_norm_params={"type": "mixed_fused_norm"})
+NORMED = {"RMSNorm": ({}, {}), "layer norm": (LN, {}), "layer norm, output bias": (LN, dict(PLAIN, attention_o_bias=True)),
+          "RMSNorm, dropout": (dict(hidden_dropout=0.25), {}), "layer norm, dropout, output bias": (dict(LN, hidden_dropout=0.25), dict(PLAIN, attention_o_bias=True)),
+          "layer norm, residual behind it": (LN, dict(apply_residual_connection_post_layernorm=True))}
+
+
+@pytest.mark.parametrize("part", ["input_layernorm", "post_attention_layernorm"])
+@pytest.mark.parametrize("name", NORMED)
+def test_a_hook_sees_the_norms_own_call(name, part):
+    """What goes in (for the second the residual sum, rounded), what comes out, and what the hook makes of it."""
+    from easyllm_amd import dropout
+    model, params = NORMED[name]
+    layer = build(params, **model).get_submodule("3")
+    with dropout.recording() as draws:
+        want, want_grads = run(layer)
+    norm, seen, factor = find(layer, part), [], 1
+
+    def hook(m, i, o):
+        seen.append((i[0].detach().clone(), o.detach().clone()))
+        return o * factor
+    handle = norm.register_forward_hook(hook)
+    with dropout.replaying(draws):
+        got, grads = run(layer)
+    factor = 2
+    with dropout.replaying(draws):
+        twice, _ = run(layer)
+    handle.remove()
+    assert len(seen) == 2
+    x, y = seen[0]
+    x = x.double()
+    if type(norm).__name__ == "RMSNorm":
+        ref = x * (x.square().mean(-1, keepdim=True) + norm.eps).rsqrt() * norm.weight.double()
+    else:
+        ref = torch.nn.functional.layer_norm(x, (256,), norm.weight.double(), norm.bias.double(), norm.eps)
+    assert close(y, ref) and close(got, want) and all(close(a, b) for a, b in zip(grads, want_grads))
+    assert not torch.equal(twice, got)  # (the same launches; behind another norm twice as much may be nearly the same)
+
+
+@pytest.mark.parametrize("name", NORMED)
+def test_a_norm_of_another_class_is_called(name):
+    """One that knows none of the fused forms."""
+    model, params = NORMED[name]
+    layer = build(params, **model).get_submodule("3")
+
+    class Scale(torch.nn.Module):
+        def forward(self, x):
+            return x * 0.5
+    layer.input_layernorm, layer.post_attention_layernorm = Scale(), Scale()
+    y, grads = run(layer)
+    assert torch.isfinite(y).all() and all(torch.isfinite(g).all() for g in grads)
