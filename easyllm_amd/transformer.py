@@ -64,6 +64,21 @@ def is_plain(module, cls):
     return are_plain(((module, cls),))
 
 
+def fused_form(norm, name):
+    """The norm's method of that name, which takes the sum in front of it or its input's gradient into its kernels, or None where it would pass the norm's own call
+    by: a hook, a forward of another kind, a class without the method."""
+    if (torch.nn.modules.module._has_any_global_hook() or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks
+            or norm._backward_pre_hooks):
+        return None
+    method = getattr(norm, name, None)
+    for cls in (RMSNorm, MixedFusedLayerNorm):
+        if isinstance(norm, cls):
+            here, defined = (lambda n: getattr(getattr(norm, n), "__func__", None)), dict(_METHODS[cls])
+            if here("forward") is not defined["forward"] and here(name) is defined[name]:
+                return None
+    return method
+
+
 class FlashAttention(torch.nn.Module):
     """Causal softmax(q k^T * scale) v over packed documents (the flash_attn_varlen_* seam)."""
 
@@ -362,19 +377,15 @@ class ParallelTransformerLayer(torch.nn.Module):
         scale = core.softmax_scale if core.softmax_scale is not None else d ** -0.5
         return hidden_states, ((nq, nk, d), f, (ln1.eps, ln2.eps), scale), cos, sin, position_ids, cu_seqlens, params
 
-    @staticmethod
-    def _passes_by(norm):
-        """Whether the norm's own call may be passed by, for the sum in front of it or its input's gradient in its kernels."""
-        return type(norm) in (RMSNorm, MixedFusedLayerNorm) and is_plain(norm, type(norm))
-
     def forward(self, hidden_states, attention_mask, cu_seqlens=None, position_ids=None, layer_past=None,
                 get_key_value=False):
         if layer_past is None and not get_key_value:
             native = self._native_inputs(hidden_states, attention_mask, cu_seqlens, position_ids)
             if native is not None:
                 return F_.decoder_layer(*native)
-        if self._passes_by(self.input_layernorm):
-            hidden_states, layernorm_output = self.input_layernorm.forward_keep_input(hidden_states)
+        keep_input = fused_form(self.input_layernorm, "forward_keep_input")
+        if keep_input is not None:
+            hidden_states, layernorm_output = keep_input(hidden_states)
         else:
             layernorm_output = self.input_layernorm(hidden_states)
         attention_output, attention_bias = self.self_attn(layernorm_output, attention_mask, cu_seqlens, position_ids,
@@ -384,7 +395,8 @@ class ParallelTransformerLayer(torch.nn.Module):
         norm_takes_bias = dropout_p > 0 or isinstance(self.post_attention_layernorm, MixedFusedLayerNorm)  # (and the dropout in front of it)
         if attention_bias is not None and not norm_takes_bias:
             attention_output, attention_bias = F_.bias_add(attention_output, attention_bias), None
-        if post_norm or not self._passes_by(self.post_attention_layernorm):
+        add_norm = None if post_norm else fused_form(self.post_attention_layernorm, "forward_with_dropout_residual" if norm_takes_bias else "forward_with_residual")
+        if add_norm is None:
             residual = layernorm_output if post_norm else hidden_states
             if dropout_p > 0 or attention_bias is not None:
                 layernorm_input = F_.dropout_add(attention_output, residual, attention_bias, dropout_p)
@@ -392,14 +404,10 @@ class ParallelTransformerLayer(torch.nn.Module):
                 layernorm_input = F_.add(attention_output, residual)
             layernorm_output = self.post_attention_layernorm(layernorm_input)
             residual = layernorm_output if post_norm else layernorm_input
-        elif norm_takes_bias:
-            layernorm_input, layernorm_output = self.post_attention_layernorm.forward_with_dropout_residual(attention_output, hidden_states, dropout_p,
-                                                                                                            attention_bias)
-            residual = layernorm_input
         else:
-            # residual add (:786) + post-attention RMSNorm (:787) in one kernel
-            layernorm_input, layernorm_output = self.post_attention_layernorm.forward_with_residual(attention_output,
-                                                                                                     hidden_states)
+            # dropout, residual add (:786) and post-attention norm (:787) in one kernel
+            layernorm_input, layernorm_output = (add_norm(attention_output, hidden_states, dropout_p, attention_bias) if norm_takes_bias
+                                                 else add_norm(attention_output, hidden_states))
             residual = layernorm_input
         if dropout_p == 0 and not getattr(self.mlp, "glu", True) and are_plain(((self.mlp, ParallelMLP), (self.mlp.down_proj, RowParallelLinear))):
             return self.mlp(layernorm_output, residual=residual)[0]  # the sum in the second product's epilogue

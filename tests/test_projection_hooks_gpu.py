@@ -157,3 +157,25 @@ def test_a_norm_of_another_class_is_called(name):
     layer.input_layernorm, layer.post_attention_layernorm = Scale(), Scale()
     y, grads = run(layer)
     assert torch.isfinite(y).all() and all(torch.isfinite(g).all() for g in grads)
+
+
+@pytest.mark.parametrize("part", ["input_layernorm", "post_attention_layernorm"])
+@pytest.mark.parametrize("name", ["RMSNorm", "layer norm", "RMSNorm, dropout"])
+@pytest.mark.parametrize("how", ["subclass", "instance", "class"])
+def test_a_norm_with_a_forward_of_its_own_is_called(name, part, how, monkeypatch):
+    model, params = NORMED[name]
+    layer = build(params, **model).get_submodule("3")
+    norm, calls = find(layer, part), []
+    original = type(norm).forward
+
+    def forward(self, x):
+        calls.append(x.shape)
+        return original(self, x)
+    if how == "subclass":
+        norm.__class__ = type("Other", (type(norm),), {"forward": forward})
+    elif how == "class":
+        monkeypatch.setattr(type(norm), "forward", forward)
+    else:
+        monkeypatch.setattr(norm, "forward", lambda x: forward(norm, x))
+    run(layer)
+    assert calls == [(40, 2, 256)] * (2 if how == "class" else 1)
