@@ -5,8 +5,10 @@
 //   ds = rstd (g - [mean(g)] - xhat mean(g xhat)) + dsum, g = dy w;   dw = sum dy xhat, db = sum dy, dx = dropout'(ds), dx_bias = sum dx
 //
 // A row is held in registers (h <= 8192) and read from HBM once: the variance is of the centred values, not a difference of two large sums.
-// y and the statistics are of the fp32 sum.  The backward pass has the sum as it was stored, in bf16: dw and ds come out up to 0.0026 off 64 bits where one rounding
-// leaves 0.0018, and the sum made anew from x, the mask and the residual would be a quarter more to read.
+// y and the statistics are of the fp32 sum.  The backward pass has the sum as it was stored, in bf16, and dw's terms dy xhat carry that rounding, |s| rstd 2^-9 at most
+// (ds, where xhat enters with a mean over the row only, shows nothing of it).  dw against 64 bits, norms: 0.0022 to 0.0028 for rows around zero where one rounding
+// leaves 0.0017; 0.013 where a row's mean is ten times its spread and 0.10 at a hundred times, as far as a norm of the stored sum would be off in y.  The sum made anew from x,
+// the mask and the residual would be a quarter more to read, its remainder kept in 8 bits a tenth more to move in both passes.
 #include "column_sums.h"
 #include "dropout.h"
 
@@ -27,8 +29,9 @@ struct NormFwd {
 
 // A row is shared by NSPLIT waves: wave part p owns the NCHUNK * 512 columns from p * NCHUNK * 512 on, lane l the 8 columns at l * 8 of each 512.  A
 // wave's next row is loaded before the current one is worked on, and where a wave holds whole rows no barrier ties it to others.  Rate of the bytes read and
-// written, x + residual -> sum + y: 16384 x 5120 5.4 TB/s, 8192 x 8192 5.5, 32768 x 1024 6.2; a copy of 2 GiB runs at 5.0.  (A block per row that loads,
-// reduces and stores in turn, up to 512 threads: 4.6, 5.5, 5.9.  Streaming hints on any of the loads or stores: within 1 %.)
+// written, x + residual -> sum + y, call after call: 16384 x 5120 5.4 TB/s, 8192 x 8192 5.3, 32768 x 1024 6.2; a copy of 2 GiB runs at 5.0.  (Between backward passes of
+// the same size 4.5, 150 us with dropout and a bias for 126, while those take 142 us for 173: each finds some of what the other left in the last-level cache.)  (A block per row
+// that loads, reduces and stores in turn, up to 512 threads: 4.6, 5.5, 5.9.  Streaming hints on any of the loads or stores: within 1 %.)
 template <int NCHUNK, int NSPLIT, bool CENTER, bool RES, bool DROP>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(const NormFwd a) {
     constexpr int RPB = 4 / NSPLIT;
