@@ -247,9 +247,10 @@ class ParallelAttention(torch.nn.Module):
             raise NotImplementedError("KV-cache inference is outside the training step")
         if not self.qkv_pack:
             projections = (self.q_proj, self.k_proj, self.v_proj)
-            if all(p.bias is None for p in projections) and are_plain([(p, ColumnParallelLinear) for p in projections]):
+            plain = are_plain([(p, ColumnParallelLinear) for p in projections])
+            if plain and all(p.bias is None for p in projections):
                 query_layer, key_layer, value_layer = F_.fan_out_linear(hidden_states, *(p.weight for p in projections))
-            elif self._adds_all_biases(projections):  # one launch where that is faster, one input gradient
+            elif plain and all(p.bias is not None and not p.skip_bias_add for p in projections):  # one launch where that is faster, one input gradient
                 ys = F_.fan_out_linear(hidden_states, *(p.weight for p in projections))
                 query_layer, key_layer, value_layer = (F_.bias_add(y, p.bias) for y, p in zip(ys, projections))
             else:
@@ -349,6 +350,8 @@ class ParallelTransformerLayer(torch.nn.Module):
             return None
         q, k, v, o, gate, up, down = attn.q_proj, attn.k_proj, attn.v_proj, attn.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj
         ln1, ln2, core, rotary = self.input_layernorm, self.post_attention_layernorm, attn.core_attention_flash, attn.rotary_emb
+        if any(type(p) is not ColumnParallelLinear for p in (q, k, v, gate, up)) or type(o) is not RowParallelLinear or type(down) is not RowParallelLinear:
+            return None  # (they need not have a weight)
         nq, nk = attn.num_attention_heads_per_partition, attn.num_kv_attention_heads_per_partition
         d, f = attn.hidden_size_per_attention_head, gate.weight.shape[0]
         s, b, h = hidden_states.shape

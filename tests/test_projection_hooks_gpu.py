@@ -96,6 +96,28 @@ def test_a_projection_of_another_class_is_called(name):
     assert not torch.equal(run(layer)[0], without)
 
 
+@pytest.mark.parametrize("name", [*STACKS, "gated MLP, down", "attention, o"])
+def test_a_projection_that_wraps_another_is_called(name):
+    """It has no weight of its own to go by."""
+    params, part = STACKS.get(name) or ({}, {"gated MLP, down": "down_proj", "attention, o": "o_proj"}[name])
+    layer = build(params).get_submodule("3")
+    want, want_grads = run(layer)
+    module, calls = find(layer, part), []
+
+    class Wrapped(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            calls.append(x.shape)
+            return self.inner(x)
+    holder = next(m for m in (layer.mlp, layer.self_attn) if hasattr(m, part))
+    setattr(holder, part, Wrapped(module))
+    got, grads = run(layer)
+    assert len(calls) == 1 and close(got, want) and all(close(a, b) for a, b in zip(grads, want_grads))
+
+
 def test_a_residual_does_not_pass_a_hooked_down_projection_by():
     mlp = build(PLAIN).get_submodule("3").mlp
     x, r = (torch.randn(40, 256, device="cuda").bfloat16() for _ in range(2))
