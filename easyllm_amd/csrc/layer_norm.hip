@@ -6,7 +6,7 @@
 //
 // A row is held in registers (h <= 8192) and read from HBM once: the variance is of the centred values, not a difference of two large sums.
 // y and the statistics are of the fp32 sum.  The backward pass has the sum as it was stored, in bf16, and dw's terms dy xhat carry that rounding, |s| rstd 2^-9 at most
-// (ds, where xhat enters with a mean over the row only, shows nothing of it).  dw against 64 bits, norms: 0.0022 to 0.0028 for rows around zero where one rounding
+// (ds, where xhat enters with a mean over the row only, hardly shows it: 0.0025 at a hundred times below).  dw against 64 bits, norms: 0.0022 to 0.0028 for rows around zero where one rounding
 // leaves 0.0017; 0.013 where a row's mean is ten times its spread and 0.10 at a hundred times, as far as a norm of the stored sum would be off in y.  The gradient is that
 // of the tensor that the call returned.  (The sum made anew from x, the mask and the residual leaves dw at one rounding everywhere and costs the backward pass a quarter more to read: 16384 x 5120
 // 117 -> 146 us, with dropout and a bias 173 -> 206.)
