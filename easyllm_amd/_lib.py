@@ -37,7 +37,24 @@ class Epilogue(ctypes.Structure):
     _fields_ = [("bias", _vp), ("residual", _vp), ("pre", _vp), ("ldr", _i64), ("ldp", _i64), ("act", _i32)]
 
 
+class RotarySide(ctypes.Structure):
+    """struct ezl_rotary_side"""
+    _fields_ = [("x", _vp), ("out", _vp), ("heads", _i64), ("seq_stride", _i64), ("batch_stride", _i64), ("head_stride", _i64)]
+
+
+class Adam8Tensor(ctypes.Structure):
+    """struct ezl_adam8_tensor"""
+    _fields_ = [(n, _vp) for n in ("master", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "grad", "param_bf16")] + [("n", _i64), ("number", ctypes.c_uint32)]
+
+
+class Adam8(ctypes.Structure):
+    """struct ezl_adam8"""
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("step", _i64), ("seed", ctypes.c_uint64), ("bias_correction", _i32)]
+
+
 _layerp = ctypes.POINTER(Layer)
+_sidep = ctypes.POINTER(RotarySide)
+_adam8p = ctypes.POINTER(Adam8Tensor)
 _dropp = ctypes.POINTER(Dropout)
 _gradp = ctypes.POINTER(LayerGrad)
 
@@ -57,6 +74,11 @@ SIGNATURES = {
     "ezl_rope_table": [_vp, _vp, _vp, _i64, _i64, _f32, _vp],
     "ezl_rope_apply": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "ezl_rope_apply_pair": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
+    "ezl_rotary": [_sidep, _sidep, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f32, _i32, _vp],
+    "ezl_gate_fwd": [_i32, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "ezl_adamw8_list": [_i32, _adam8p, ctypes.POINTER(Adam8), _vp, _vp],
+    "ezl_moments8_list": [_i32, _adam8p, _vpp, _vpp, _vp],
     "ezl_ids_in_range": [_vp, _i64, _i64, _vp, _vp],
     "ezl_ids_in_range_host_flag": [_vp, _i64, _i64, _vp, _vp],
     "ezl_embed_gather": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],

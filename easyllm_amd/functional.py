@@ -399,6 +399,50 @@ def swiglu(gate, up):
     return SwiGLUFunction.apply(gate.contiguous(), up.contiguous())
 
 
+class GatedMLPFunction(torch.autograd.Function):
+    """down(act(gate x) * up x).  The two products' results are kept for backward (bf16), what they make together is not: the backward pass computes it
+    again where it needs it, for the down projection's weight gradient."""
+
+    @staticmethod
+    def forward(ctx, x, gate_weight, up_weight, down_weight, act):
+        x2d = x.reshape(-1, x.shape[-1])
+        gate, up = K.linear_fwd_multi(x2d, (gate_weight, up_weight))
+        y = K.linear_fwd(K.gate_fwd(act, gate, up), down_weight)
+        ctx.act = act
+        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, gate, up)
+        return y.view(*x.shape[:-1], down_weight.shape[0])
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dy):
+        x, gate_weight, up_weight, down_weight, gate, up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        x2d, dy2d = x.reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
+        if not dy2d.is_contiguous():
+            dy2d = dy2d.contiguous()
+        dgate, dup, mid = K.gate_bwd(ctx.act, K.linear_dgrad(dy2d, down_weight), gate, up, need[3])
+        grads = [None, None, None]
+        if need[3]:
+            mg, acc = _main_grad_target(down_weight)
+            dw = K.linear_wgrad(dy2d, mid, out=mg, accumulate=acc)
+            grads[2] = dw if mg is None else None
+        wanted = [i for i in range(2) if need[1 + i]]
+        if wanted:
+            targets = [_main_grad_target((gate_weight, up_weight)[i]) for i in wanted]
+            dws = K.linear_wgrad_multi([(dgate, dup)[i] for i in wanted], x2d, [mg for mg, _ in targets], [acc for _, acc in targets])
+            for i, (mg, _), dw in zip(wanted, targets, dws):
+                grads[i] = dw if mg is None else None
+        dx = K.linear_dgrad_multi([dgate, dup], [gate_weight, up_weight]).view(x.shape) if need[0] else None
+        return (dx, *grads, None)
+
+
+def gated_mlp(x, gate_weight, up_weight, down_weight, activation="silu"):
+    """(act(x gate^T) * (x up^T)) down^T; activation: 'silu', 'gelu' (exact), 'gelu_tanh' or 'relu'.  x [..., h], weights [f, h], [f, h], [h', f]."""
+    if activation not in K.GATES:
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(K.GATES), activation))
+    return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation)
+
+
 # --------------------------------------------------------------------------------------------
 # rotary embedding: llama/positional_embeddings.py:105-122
 # --------------------------------------------------------------------------------------------
@@ -445,6 +489,38 @@ class RotaryPairFunction(torch.autograd.Function):
 
 def apply_rotary_pair(q, k, cos, sin, position_ids=None):
     return RotaryPairFunction.apply(q, k, cos, sin, position_ids)
+
+
+class RotaryEmbedFunction(torch.autograd.Function):
+    """(q, k) turned by their positions; backward turns both gradients the other way, times the same scale."""
+
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, position_ids, interleaved, scale):
+        ctx.how = interleaved, scale
+        ctx.save_for_backward(inv_freq, position_ids)
+        return K.rotary(_rotary_rows(q), _rotary_rows(k), inv_freq, position_ids, interleaved, scale)
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dq, dk):
+        inv_freq, position_ids = ctx.saved_tensors
+        gq, gk = K.rotary(_rotary_rows(dq), _rotary_rows(dk), inv_freq, position_ids, *ctx.how, backward=True)
+        return gq, gk, None, None, None, None
+
+
+def _rotary_rows(x):
+    return x if x is None or x.dim() != 4 or K.rotary_in_place_ok(x) else x.contiguous()
+
+
+def rotary_embed(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0):
+    """q [s, b, nq, d] and k [s, b, nk, d] (or None) turned by their positions -> (q, k), contiguous.
+
+    The first 2 len(inv_freq) elements of a head are pairs (j, j + len(inv_freq)), or (2 j, 2 j + 1) if `interleaved`, turned by position * inv_freq[j] and
+    multiplied by `scale`; the rest of it is copied.  Angles are computed in 64 bits from fp32 or fp64 frequencies, so positions (int64 [b, s], any strides; None: the place in
+    the sequence) have no limit that a table would set."""
+    if inv_freq.requires_grad:
+        raise ValueError("rotary_embed: frequencies are not learnt")
+    return RotaryEmbedFunction.apply(q, k, inv_freq, position_ids, bool(interleaved), float(scale))
 
 
 # --------------------------------------------------------------------------------------------

@@ -281,6 +281,29 @@ def swiglu_bwd(dout, gate, up):
     return dgate, dup
 
 
+# ------------------------------------------------------------------------------------- gated MLP
+GATES = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+def gate_fwd(act, gate, up):
+    """act(gate) * up"""
+    _ready((gate, up), "gate up")
+    _need(gate.shape == up.shape, "gate/up shape mismatch")
+    out = torch.empty_like(gate)
+    _lib.call("ezl_gate_fwd", GATES[act], _p(gate), _p(up), _p(out), gate.numel(), _stream())
+    return out
+
+
+def gate_bwd(act, dout, gate, up, want_out=False):
+    """-> (dgate, dup, act(gate) * up or None)"""
+    _ready((dout, gate, up), "dout gate up")
+    _need(gate.shape == up.shape == dout.shape, "gate_bwd shape mismatch")
+    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    out = torch.empty_like(gate) if want_out else None
+    _lib.call("ezl_gate_bwd", GATES[act], _p(dout), _p(gate), _p(up), _p(dgate), _p(dup), _p(out), gate.numel(), _stream())
+    return dgate, dup, out
+
+
 # ------------------------------------------------------------------------------------- RoPE
 def rope_table(inv_freq, npos, scale_factor=1.0):
     _need(inv_freq.is_cuda and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(), "inv_freq must be fp32 on the GPU")
@@ -338,6 +361,45 @@ def rope_apply_pair(q, k, cos, sin, position_ids=None, backward=False):
     _lib.call("ezl_rope_apply_pair", _p(q), _p(qo), nq, qs, qos, _p(k), _p(ko), k.shape[2], ks, kos, _p(cos), _p(sin),
               _p(position_ids), s, b, d, cos.shape[0], 1 if backward else 0, _stream())
     return qo, ko
+
+
+def _rotary_side(x, out):
+    s, b, heads, d = x.shape
+    st = x.stride()
+    return _lib.RotarySide(x.data_ptr(), out.data_ptr(), heads, st[0], st[1], st[2])
+
+
+def rotary_in_place_ok(x):
+    """Whether the kernel reads x [s, b, heads, d] where it lies: rows of whole 16 bytes, each on its own strides."""
+    st = x.stride()
+    return st[3] == 1 and st[0] % 8 == 0 and st[1] % 8 == 0 and st[2] % 8 == 0 and x.data_ptr() % 16 == 0
+
+
+def rotary(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0, backward=False):
+    """q [s, b, nq, d], k [s, b, nk, d] or None -> both turned (contiguous), k None where it is."""
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None:
+            continue
+        if not (t.dtype is BF16 and t.is_cuda and t.dim() == 4):
+            raise ValueError("%s must be a bf16 [s, b, heads, d] GPU tensor" % name)
+        _here(t, name)
+        _need(rotary_in_place_ok(t), "rotary: strides must be multiples of 8, the last 1")
+    s, b, _, d = q.shape
+    _need(k is None or (k.shape[0] == s and k.shape[1] == b and k.shape[3] == d), "rotary: q / k shapes differ")
+    _need(inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.is_cuda,
+          "inv_freq must be a contiguous fp32 or fp64 [turned / 2] GPU tensor")
+    _here(inv_freq, "inv_freq")
+    _need(0 < 2 * inv_freq.numel() <= d and d % 8 == 0, "rotary: a frequency for each pair of the head's elements, at most half of them; the head's width a multiple of 8")
+    pos = (0, 0)
+    if position_ids is not None:
+        _need(position_ids.is_cuda and position_ids.dtype is torch.int64 and tuple(position_ids.shape) == (b, s), "position_ids must be int64 [b, s]")
+        _here(position_ids, "position_ids")
+        pos = position_ids.stride()
+    q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=BF16, device=k.device)
+    _lib.call("ezl_rotary", _rotary_side(q, q_out), None if k is None else _rotary_side(k, k_out), inv_freq.data_ptr(), 1 if inv_freq.dtype is torch.float64 else 0,
+              _p(position_ids), pos[1], pos[0], s, b, d, 2 * inv_freq.numel(), 1 if interleaved else 0, float(scale), 1 if backward else 0, _stream())
+    return q_out, k_out
 
 
 def ids_in_range_flag(ids, limit, host_flag=None):
@@ -943,6 +1005,52 @@ def adamw_list(masters, exp_avgs, exp_avg_sqs, grads, params, lr, beta1, beta2, 
     _lib.call("ezl_adamw_list", len(ns), _pointers(masters), _pointers(exp_avgs), _pointers(exp_avg_sqs), _pointers(grads), _pointers(params),
               (ctypes.c_int64 * len(ns))(*ns), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(step),
               1 if bias_correction else 0, _p(norm_coef), _stream())
+
+
+def _adam8_tensors(states, grads=None, params=None):
+    """The C forms of states {master, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, number}; without gradients only the moments are looked at."""
+    out = (_lib.Adam8Tensor * len(states))()
+    for i, st in enumerate(states):
+        n = st["exp_avg"].numel()
+        for name, length in (("exp_avg", n), ("exp_avg_sq", n), ("exp_avg_scale", (n + 255) // 256), ("exp_avg_sq_scale", (n + 255) // 256)):
+            t = st[name]
+            if not (t.dtype is torch.uint8 and t.is_contiguous() and t.is_cuda and t.numel() == length):
+                raise ValueError("%s must be a contiguous uint8 GPU tensor of %d values" % (name, length))
+            _here(t, name)
+            setattr(out[i], name, t.data_ptr())
+        out[i].n = n
+        if grads is None:
+            continue
+        for t, name in ((st["master"], "master"), (grads[i], "grad")):
+            _f32c(t, name)
+            _here(t, name)
+            _need(t.numel() == n, "adamw8_list: size mismatch")
+        if params[i] is not None:
+            _bf16c(params[i], "param")
+            _here(params[i], "param")
+            _need(params[i].numel() == n, "param size mismatch")
+        out[i].master, out[i].grad, out[i].param_bf16 = st["master"].data_ptr(), grads[i].data_ptr(), _p(params[i])
+        number = int(st["number"])
+        _need(0 <= number < 2 ** 32, "a tensor's number has 32 bits")
+        out[i].number = number
+    return out
+
+
+def adamw8_list(states, grads, params, lr, beta1, beta2, eps, weight_decay, step, bias_correction=True, norm_coef=None, seed=0):
+    """adamw_list for moments of 8 bits, rounded at random by the counter (seed, step, number, place)."""
+    _need(len(grads) == len(states) == len(params), "adamw8_list: the lists need one entry per tensor")
+    if norm_coef is not None:
+        _f32c(norm_coef, "norm_coef")
+        _need(norm_coef.numel() == 2, "norm_coef must hold (norm, coefficient)")
+    how = _lib.Adam8(lr, beta1, beta2, eps, weight_decay, step, seed & 0xFFFFFFFFFFFFFFFF, 1 if bias_correction else 0)
+    _lib.call("ezl_adamw8_list", len(states), _adam8_tensors(states, grads, params), how, _p(norm_coef), _stream())
+
+
+def moments8_list(states):
+    """[(exp_avg, exp_avg_sq)] as flat bf16 tensors, exact"""
+    outs = [tuple(torch.empty(st["exp_avg"].numel(), dtype=BF16, device=st["exp_avg"].device) for _ in range(2)) for st in states]
+    _lib.call("ezl_moments8_list", len(states), _adam8_tensors(states), _pointers([m for m, _ in outs]), _pointers([v for _, v in outs]), _stream())
+    return outs
 
 
 # ------------------------------------------------------------------------------------- one decoder layer per call

@@ -111,6 +111,15 @@ int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const void* s, cons
 int ezl_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, void* stream);
 int ezl_swiglu_bwd(const void* dout, const void* gate, const void* up, void* dgate, void* dup, int64_t n, void* stream);
 
+/* ---- gated MLPs with SiLU, either GELU or ReLU: out = act(gate) * up over n bf16 values (n % 8 == 0), and dgate = dout * up * act'(gate),
+ *      dup = dout * act(gate) (dgate may be gate or dout, dup up); out, if given, receives act(gate) * up again ---- */
+#define EZL_GATE_SILU 0
+#define EZL_GATE_GELU 1
+#define EZL_GATE_GELU_TANH 2
+#define EZL_GATE_RELU 3
+int ezl_gate_fwd(int act, const void* gate, const void* up, void* out, int64_t n, void* stream);
+int ezl_gate_bwd(int act, const void* dout, const void* gate, const void* up, void* dgate, void* dup, void* out, int64_t n, void* stream);
+
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----
  * table: cos/sin fp32 [npos, half_dim], theta = (p / scale_factor) * inv_freq[j].
  * apply: x/out bf16 [s*b rows (s-major), nheads, d] with row strides in elements (out may alias x);
@@ -120,6 +129,18 @@ int ezl_rope_table(const void* inv_freq, void* cos_out, void* sin_out, int64_t n
 int ezl_rope_apply(const void* x, void* out, const void* cos_table, const void* sin_table, const void* position_ids, int64_t s,
                    int64_t b, int64_t nheads, int64_t d, int64_t in_row_stride, int64_t out_row_stride, int64_t npos,
                    int backward, void* stream);
+/* Positions of either pairing, without a table: of every head's d elements the first `turned` (even) are pairs (j, j + turned / 2), or with
+ * `interleaved` (2 j, 2 j + 1), that are turned by position * inv_freq[j] (turned / 2 fp32 values, or fp64; the product and its reduction are in fp64) and
+ * multiplied by scale; the others are copied.  backward != 0 turns the other way (the gradient).  A side is x [s, b, heads, d] with its strides in elements
+ * (multiples of 8, 0 allowed) and a contiguous out [s, b, heads, d]; k (HOST pointers both) may be NULL.  position_ids int64 with its strides, any value below 2^31 or so (an
+ * angle is off by position * 2^-52), or NULL (position = s index). */
+typedef struct {
+    const void* x;
+    void* out;
+    int64_t heads, seq_stride, batch_stride, head_stride;
+} ezl_rotary_side; /* HOST struct */
+int ezl_rotary(const ezl_rotary_side* q, const ezl_rotary_side* k, const void* inv_freq, int inv_freq_f64, const void* position_ids, int64_t pos_seq_stride,
+               int64_t pos_batch_stride, int64_t s, int64_t b, int64_t d, int64_t turned, int interleaved, float scale, int backward, void* stream);
 /* range test of the position ids that index the tables (the reference's cos[position_ids], positional_embeddings.py:109-117,
  * fails on an index past the table): ORs 1 into *bad_flag (device int32) if some id >= limit, 2 if some id < 0.  The apply
  * kernels themselves clamp. */
@@ -317,6 +338,34 @@ int ezl_sumsq_list(int count, const void* const* x, const int64_t* n, void* part
 int ezl_adamw_list(int count, void* const* master, void* const* exp_avg, void* const* exp_avg_sq, const void* const* grad,
                    void* const* param_bf16, const int64_t* n, float lr, float beta1, float beta2, float eps, float weight_decay,
                    int64_t step, int bias_correction, const void* norm_coef, void* stream);
+
+/* ---- AdamW with moments of 8 bits (the reference's yaml type AdamW8bit, optimizer_helper.py) ----
+ * Elements in blocks of 256.  A moment's block has a scale e: the exponent field of its largest |x|, as it is with 2^20 added to the fp32 bits
+ * (255: not finite, the whole block reads as NaN).  A value's code is (bits of |x| 2^(K - e) + 16 r + 8) >> 20 with a random 16-bit r, so that it is right on
+ * average: exp_avg K = 15, 7 bits and the sign above; exp_avg_sq K = 31, 8 bits, at least 1 where x > 0.  A code c stands for the fp32 number of the bits
+ * c << 20, times 2^(e - K).  Elements 4 i .. 4 i + 3 of block 2 j, then of block 2 j + 1, take the eight 16-bit numbers (low half of a word first) that Philox-4x32-10 makes of
+ * the counter (64 j + i low, high, number, step) under the key `seed`; both moments the same.
+ * The update is ezl_adamw_list's, from the moments before they are rounded; every product and sum is rounded by itself. */
+typedef struct {
+    void* master;                                /* fp32 [n] */
+    void *exp_avg, *exp_avg_sq;                  /* codes: uint8 [n] */
+    void *exp_avg_scale, *exp_avg_sq_scale;      /* uint8 [ceil(n / 256)] */
+    const void* grad;                            /* fp32 [n] */
+    void* param_bf16;                            /* bf16 [n], or NULL */
+    int64_t n;
+    uint32_t number;                             /* tells the tensors of a seed apart */
+} ezl_adam8_tensor;
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;
+    uint64_t seed;
+    int bias_correction;
+} ezl_adam8;
+/* tensors and how are HOST memory.  Codes, scales and fp32 buffers on 16 bytes, the bf16 weight on 8.  One launch per 40 tensors; one that shares memory with an earlier one
+ * starts a new launch. */
+int ezl_adamw8_list(int count, const ezl_adam8_tensor* tensors, const ezl_adam8* how, const void* norm_coef, void* stream);
+/* the moments as bf16 values (exact: they have four significant bits); only the codes, the scales and n of a tensor are looked at */
+int ezl_moments8_list(int count, const ezl_adam8_tensor* tensors, void* const* exp_avg_bf16, void* const* exp_avg_sq_bf16, void* stream);
 
 /* ---- packed-sequence sample index (host code, no GPU): llm/data/cores/helpers.cpp:36-122 `build_location_idx`
  *      (python twin llm/data/nlp_dataset.py:424-463) ----

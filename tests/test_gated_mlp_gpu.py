@@ -1,0 +1,129 @@
+"""act(x gate^T) * (x up^T), times down^T, forward and backward, against 64-bit arithmetic.
+
+Tolerances, before any run.  E = 2^-24.  A sum of K products of bf16 values is off by at most 2 (K + 4) E times the sum of their magnitudes ("size").  An activation's slope is
+below 1.13 and its second derivative below 1.2 (ReLU's jumps: gates within their error of zero are left out by taking the larger of both slopes), its own arithmetic adds 2^-15 of its value.
+Roundings to bf16 are 2^-8 of a value: of gate and up where the backward pass reads them, of the products between the launches, of the results."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+E, H = 2.0 ** -24, 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def F():
+    from easyllm_amd import functional
+    return functional
+
+
+def rnd(*shape, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).bfloat16()
+
+
+def act64(a, act):
+    """act(a), act'(a) in fp64"""
+    if act == "silu":
+        s = torch.sigmoid(a)
+        return a * s, s * (1 + a * (1 - s))
+    if act == "gelu":
+        cdf = 0.5 * torch.special.erfc(-a / math.sqrt(2))
+        return a * cdf, cdf + a * torch.exp(-0.5 * a * a) / math.sqrt(2 * math.pi)
+    if act == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        s = torch.sigmoid(2 * c * (a + 0.044715 * a ** 3))
+        return a * s, s + a * s * (1 - s) * 2 * c * (1 + 3 * 0.044715 * a * a)
+    return a.clamp_min(0), (a > 0).double()
+
+
+def near(got, ref, slack, what):
+    off = (got.double() - ref).abs() - ref.abs() * H - slack * (1 + H)
+    assert got.shape == ref.shape and bool((off <= 0).all()), "%s: %g beyond its tolerance" % (what, off.max().item())
+
+
+def product(a, a_err, b, b_err=None):
+    """a b in fp64, and how far a product in fp32 of values that far off may be from it"""
+    k = a.shape[1]
+    err = a_err @ b.abs() if a_err is not None else 0
+    if b_err is not None:
+        err = err + (a.abs() + (0 if a_err is None else a_err)) @ b_err
+    return a @ b, err + (a.abs() @ b.abs()) * (2 * (k + 4) * E)
+
+
+def expected(x, wg, wu, wd, dy, act):
+    """name -> (reference, slack)"""
+    x, wg, wu, wd = (t.detach().double() for t in (x, wg, wu, wd))
+    (g, g_err), (u, u_err) = product(x, None, wg.t()), product(x, None, wu.t())
+    a, slope = act64(g, act)
+    # forward: gate and up may be rounded on their way to the gate
+    g1, u1 = g_err + g.abs() * H, u_err + u.abs() * H
+    a_err = 1.2 * g1 + a.abs() * 2.0 ** -15
+    mid = a * u
+    mid_err = a_err * u.abs() + (a.abs() + a_err) * u1
+    mid_err = mid_err + (mid.abs() + mid_err) * H
+    out = {"y": product(mid, mid_err, wd.t())}
+    if dy is not None:
+        dy = dy.double()
+        d, d_err = product(dy, None, wd)
+        d_err = d_err + d.abs() * H
+        slope_err = 1.2 * g1 + slope.abs() * 2.0 ** -15
+        if act == "relu":
+            slope_err = slope_err * 0 + (g.abs() <= g1)
+        du = d * a
+        du_err = d_err * a.abs() + (d.abs() + d_err) * a_err
+        du_err = du_err + (du.abs() + du_err) * H
+        dg = d * u * slope
+        dg_err = d_err * (u * slope).abs() + (d.abs() + d_err) * (u1 * slope.abs() + (u.abs() + u1) * slope_err)
+        dg_err = dg_err + (dg.abs() + dg_err) * H
+        one, two = product(dg, dg_err, wg), product(du, du_err, wu)
+        out.update(x=(one[0] + two[0], one[1] + two[1]), gate=product(dg.t(), dg_err.t(), x), up=product(du.t(), du_err.t(), x),
+                   down=product(dy.t(), None, mid, mid_err))
+    return out
+
+
+def check(F, T, h, f, act, h_out=None, seed=0, train=True, shape=None):
+    h_out = h_out or h
+    x = rnd(T, h, seed=seed).view(*(shape or (T,)), h).requires_grad_(train)
+    wg, wu = (rnd(f, h, seed=seed + 1 + i, scale=1.5 * h ** -0.5).requires_grad_(train) for i in range(2))
+    wd = rnd(h_out, f, seed=seed + 3, scale=f ** -0.5).requires_grad_(train)
+    dy = rnd(T, h_out, seed=seed + 4) if train else None
+    with torch.set_grad_enabled(train):
+        y = F.gated_mlp(x, wg, wu, wd, activation=act)
+    assert y.shape == (*x.shape[:-1], h_out)
+    want = expected(x.reshape(-1, h), wg, wu, wd, dy, act)
+    near(y.reshape(-1, h_out), *want["y"], "y")
+    if train:
+        grads = torch.autograd.grad(y, (x, wg, wu, wd), dy.view(y.shape))
+        for name, g in zip(("x", "gate", "up", "down"), grads):
+            near(g.reshape(want[name][0].shape), *want[name], name)
+
+
+SHAPES = [(1, 8, 8), (1, 64, 64), (2, 256, 688), (5, 1000, 24), (8, 512, 1368), (16, 264, 1000), (17, 72, 520), (33, 128, 16), (64, 64, 136), (100, 520, 264), (257, 768, 2048),
+          (389, 256, 688), (389, 1032, 2776), (300, 72, 1048), (1000, 776, 1032), (1024, 2048, 5504), (2500, 520, 4104), (513, 4096, 1024)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T,h,f", SHAPES)
+def test_forward_and_backward(F, T, h, f, act):
+    print("gated", T, h, f, act, flush=True)
+    check(F, T, h, f, act)
+
+
+@pytest.mark.parametrize("T,h,f,h_out", [(1, 4096, 11008, 4096), (4, 5120, 13696, 5120), (16, 4096, 4096, 1024), (40, 2048, 5504, 512), (1531, 1024, 2816, 1024)])
+def test_forward_alone(F, T, h, f, h_out):
+    print("gated", T, h, f, h_out, flush=True)
+    for act in ("silu", "gelu"):
+        check(F, T, h, f, act, h_out=h_out, train=False)
+
+
+def test_shapes_around_the_rows(F):
+    check(F, 6 * 35, 64, 80, "silu", shape=(6, 35))
+    check(F, 30, 64, 80, "silu", shape=(2, 3, 5))
+    x = rnd(0, 4, 64).requires_grad_()
+    ws = [rnd(80, 64).requires_grad_(), rnd(80, 64).requires_grad_(), rnd(64, 80).requires_grad_()]
+    y = F.gated_mlp(x, *ws)
+    assert y.shape == (0, 4, 64)
+    grads = torch.autograd.grad(y.float().sum(), [x, *ws])
+    assert grads[0].shape == x.shape and all(not bool(g.any()) and g.shape == w.shape for g, w in zip(grads[1:], ws))
