@@ -1007,49 +1007,57 @@ def adamw_list(masters, exp_avgs, exp_avg_sqs, grads, params, lr, beta1, beta2, 
               1 if bias_correction else 0, _p(norm_coef), _stream())
 
 
-def _adam8_tensors(states, grads=None, params=None):
-    """The C forms of states {master, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, number}; without gradients only the moments are looked at."""
-    out = (_lib.Adam8Tensor * len(states))()
-    for i, st in enumerate(states):
-        n = st["exp_avg"].numel()
-        for name, length in (("exp_avg", n), ("exp_avg_sq", n), ("exp_avg_scale", (n + 255) // 256), ("exp_avg_sq_scale", (n + 255) // 256)):
-            t = st[name]
-            if not (t.dtype is torch.uint8 and t.is_contiguous() and t.is_cuda and t.numel() == length):
-                raise ValueError("%s must be a contiguous uint8 GPU tensor of %d values" % (name, length))
-            _here(t, name)
-            setattr(out[i], name, t.data_ptr())
-        out[i].n = n
-        if grads is None:
-            continue
-        for t, name in ((st["master"], "master"), (grads[i], "grad")):
-            _f32c(t, name)
-            _here(t, name)
-            _need(t.numel() == n, "adamw8_list: size mismatch")
-        if params[i] is not None:
-            _bf16c(params[i], "param")
-            _here(params[i], "param")
-            _need(params[i].numel() == n, "param size mismatch")
-        out[i].master, out[i].grad, out[i].param_bf16 = st["master"].data_ptr(), grads[i].data_ptr(), _p(params[i])
-        number = int(st["number"])
-        _need(0 <= number < 2 ** 32, "a tensor's number has 32 bits")
-        out[i].number = number
-    return out
+_ADAM8_MOMENTS = "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"
+
+
+def _adam8_moments(st, device):
+    """(the addresses of a state's codes and scales, number of values)"""
+    m, v, ms, vs = ts = st["exp_avg"], st["exp_avg_sq"], st["exp_avg_scale"], st["exp_avg_sq_scale"]
+    n = m.numel()
+    blocks = (n + 255) // 256
+    for t, length in zip(ts, (n, n, blocks, blocks)):
+        if not (t.dtype is torch.uint8 and t.get_device() == device and t.numel() == length and t.is_contiguous()):
+            raise ValueError("%s must be a contiguous uint8 tensor of %d values on the current GPU" % (_ADAM8_MOMENTS[[u is t for u in ts].index(True)], length))
+    return (m.data_ptr(), v.data_ptr(), ms.data_ptr(), vs.data_ptr()), n
 
 
 def adamw8_list(states, grads, params, lr, beta1, beta2, eps, weight_decay, step, bias_correction=True, norm_coef=None, seed=0):
-    """adamw_list for moments of 8 bits, rounded at random by the counter (seed, step, number, place)."""
+    """adamw_list for states {master, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, number} with moments of 8 bits, rounded at random by the counter
+    (seed, step, number, place)."""
     _need(len(grads) == len(states) == len(params), "adamw8_list: the lists need one entry per tensor")
+    device = torch._C._cuda_getDevice()
     if norm_coef is not None:
         _f32c(norm_coef, "norm_coef")
+        _here(norm_coef, "norm_coef")
         _need(norm_coef.numel() == 2, "norm_coef must hold (norm, coefficient)")
+    tensors = (_lib.Adam8Tensor * len(states))()
+    for i, (st, grad, param) in enumerate(zip(states, grads, params)):
+        moments, n = _adam8_moments(st, device)
+        master, number = st["master"], st["number"]
+        for t, name in ((master, "master"), (grad, "grad")):
+            if not (t.dtype is torch.float32 and t.get_device() == device and t.numel() == n and t.is_contiguous()):
+                raise ValueError("%s must be a contiguous fp32 tensor of %d values on the current GPU" % (name, n))
+        if param is not None and not (param.dtype is BF16 and param.get_device() == device and param.numel() == n and param.is_contiguous()):
+            raise ValueError("param must be a contiguous bf16 tensor of %d values on the current GPU" % n)
+        if not 0 <= number < 2 ** 32:
+            raise ValueError("a tensor's number has 32 bits")
+        tensors[i] = (master.data_ptr(), *moments, grad.data_ptr(), None if param is None else param.data_ptr(), n, number)
     how = _lib.Adam8(lr, beta1, beta2, eps, weight_decay, step, seed & 0xFFFFFFFFFFFFFFFF, 1 if bias_correction else 0)
-    _lib.call("ezl_adamw8_list", len(states), _adam8_tensors(states, grads, params), how, _p(norm_coef), _stream())
+    _lib.call("ezl_adamw8_list", len(states), tensors, how, _p(norm_coef), _stream())
 
 
 def moments8_list(states):
-    """[(exp_avg, exp_avg_sq)] as flat bf16 tensors, exact"""
-    outs = [tuple(torch.empty(st["exp_avg"].numel(), dtype=BF16, device=st["exp_avg"].device) for _ in range(2)) for st in states]
-    _lib.call("ezl_moments8_list", len(states), _adam8_tensors(states), _pointers([m for m, _ in outs]), _pointers([v for _, v in outs]), _stream())
+    """[(exp_avg, exp_avg_sq)] as bf16 tensors of the master weights' shapes, exact"""
+    device = torch._C._cuda_getDevice()
+    tensors = (_lib.Adam8Tensor * len(states))()
+    outs = []
+    for i, st in enumerate(states):
+        moments, n = _adam8_moments(st, device)
+        _need(st["master"].numel() == n, "moments8_list: size mismatch")
+        tensors[i] = (None, *moments, None, None, n, 0)
+        shape = st["master"].shape
+        outs.append((torch.empty(shape, dtype=BF16, device=st["exp_avg"].device), torch.empty(shape, dtype=BF16, device=st["exp_avg"].device)))
+    _lib.call("ezl_moments8_list", len(states), tensors, _pointers([m for m, _ in outs]), _pointers([v for _, v in outs]), _stream())
     return outs
 
 

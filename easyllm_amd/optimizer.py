@@ -137,7 +137,7 @@ def adamw_8bit_step(states, grads, weights, lr, betas=(0.9, 0.999), eps=1e-8, we
 
 def moments_8bit(states):
     """[(exp_avg, exp_avg_sq)] of a list of such states, as bf16 tensors of the master weights' shapes (exact: a moment of 8 bits has four significant ones)."""
-    return [tuple(t.view(st["master"].shape) for t in pair) for st, pair in zip(states, K.moments8_list(states))]
+    return K.moments8_list(states)
 
 
 def build_optimizer(cfg_optim, model, deepspeed=True):

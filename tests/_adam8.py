@@ -35,7 +35,7 @@ def encode(x, r, top, bits, least):
         scaled = (magnitude.astype(np.uint32).view(np.float32).astype(np.float64) * 2.0 ** (top - e[:, None])).astype(np.float32)  # (one rounding, of denormals)
     code = ((scaled.view(np.uint32).astype(np.int64) + 16 * blocks(r) + 8) >> 20).reshape(-1)[:n]
     code = np.where((x > 0) & (code < least), least, code)
-    code = np.where(x < 0, code | (1 << bits) & 0xFF, code)
+    code = np.where(np.signbit(x), code | (1 << bits) & 0xFF, code)
     return np.where(np.repeat(e, 256)[:n] == 255, 0, code).astype(np.uint8), e.astype(np.uint8)
 
 
