@@ -75,8 +75,9 @@ SIGNATURES = {
     "ezl_rope_apply": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "ezl_rope_apply_pair": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "ezl_rotary": [_sidep, _sidep, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f32, _i32, _vp],
-    "ezl_gate_fwd": [_i32, _vp, _vp, _vp, _i64, _vp],
-    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gated_fwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
+    "ezl_gated_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
+    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "ezl_adamw8_list": [_i32, _adam8p, ctypes.POINTER(Adam8), _vp, _vp],
     "ezl_moments8_list": [_i32, _adam8p, _vpp, _vpp, _vp],
     "ezl_ids_in_range": [_vp, _i64, _i64, _vp, _vp],
@@ -133,6 +134,7 @@ _SPECIAL = {
     "ezl_attn_bwd_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
     "ezl_attn_plan": ([_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64], _i32),
     "ezl_gemm_workspace_bytes": ([_i64, _i64, _i64], _i64),
+    "ezl_gated_workspace_bytes": ([_i64, _i64, _i64], _i64),
     "ezl_gemm_group_workspace_bytes": ([_i32, _i64p, _i64p, _i64], _i64),
     "ezl_gemm_group_form_workspace_bytes": ([_i32, _i32, _i64p, _i64p, _i64], _i64),
     "ezl_gemm_searches": ([], _i64),
@@ -219,6 +221,11 @@ def attn_plan(backward, ndocs, total_tokens, s_len, nq, nk, d):
 @functools.lru_cache(maxsize=1024)  # a function of the sizes alone
 def gemm_workspace_bytes(M, N, K):
     return load().ezl_gemm_workspace_bytes(M, N, K)
+
+
+@functools.lru_cache(maxsize=1024)
+def gated_workspace_bytes(M, f, K):
+    return load().ezl_gated_workspace_bytes(M, f, K)
 
 
 @functools.lru_cache(maxsize=1024)

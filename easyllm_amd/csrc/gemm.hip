@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
         }
         // (scalar registers: the buffer bases are made of them)
         it.m0 = __builtin_amdgcn_readfirstlane(tm * TBM);
-        it.n0 = __builtin_amdgcn_readfirstlane(tn * BN);
+        it.n0 = __builtin_amdgcn_readfirstlane(tn * (kPairs<EPI> ? BN / 2 : BN));
         it.kt0 = __builtin_amdgcn_readfirstlane(it.kt0);
         it.nk = __builtin_amdgcn_readfirstlane(it.nk);
         it.slot = __builtin_amdgcn_readfirstlane(it.slot);
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
     Item it = item_of(u);
 
     TileLoader<A_KC, TBM, 4, KTAIL> la;
-    TileLoader<B_KC, BN, 4, KTAIL> lb;
+    TileLoader<B_KC, BN, 4, KTAIL, kPairs<EPI>> lb;
     la.init(lane, wave, rows_left(it), a_stride(it));
     lb.init(lane, wave, cols_left(it), b_stride(it));
 
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
         if constexpr (f < 8) fb[buf][f] = rb.template read<f>(sB, ks);
         else fa[buf][f - 8] = ra.template read<f - 8>(sA, ks);
     };
-    __amdgpu_buffer_rsrc_t ga, gb;
+    __amdgpu_buffer_rsrc_t ga, gb, gb2;
     int kva = BK, kvb = BK;
     auto a_base = [&](const Item& x, int t) {
         t += x.kt0;
@@ -437,12 +437,14 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
             const bf16_t *Ab, *Bb;
             pick_segment<MULTI>(A, B, K, seg, t, kvb, Ab, Bb);
             gb = lb.base(Bb + x.b_blk + (int64_t)t * bstep);
+            if constexpr (kPairs<EPI>) gb2 = lb.base(epi.B2 + x.b_blk + (int64_t)t * bstep);
         }
     };
     // load l of a tile pair: l < NA piece l of the A tile, else of the B tile
     auto issue_load = [&](bf16_t* sA, bf16_t* sB, auto L) {
         constexpr int l = decltype(L)::value;
         if constexpr (l < NA) la.template issue_at<l>(ga, sA, lane, wave, kva);
+        else if constexpr (kPairs<EPI>) lb.template issue_pair_at<l - NA>(gb, gb2, sB, lane, wave, kvb);
         else lb.template issue_at<l - NA>(gb, sB, lane, wave, kvb);
     };
 
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
     // newer than the A tile that is waited for: the B tile behind the next, and where an item begins the stores of the one before (a count
     // holds at most 63)
     typedef std::integral_constant<int, NB> ahead;
-    constexpr int STORES = TM * 8 * (int)sizeof(OutT) / 4;
+    constexpr int STORES = kPairs<EPI> ? TM * 2 : TM * 8 * (int)sizeof(OutT) / 4;  // (the least there are: a gated product that keeps its parts has three times those)
     typedef std::integral_constant<int, NB + STORES <= 63 ? NB + STORES : 63> ahead_and_stores;
     auto flip = [&]() {
         const int x = a0, y = b0;
@@ -569,6 +571,11 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
                 int l = lane;
                 asm volatile("" : "+s"(e.ldr), "+s"(e.ldp), "+v"(l));  // (nor what these make)
                 store_tile_epilogue<TM, 8>(acc, Ct, ld, mrem, N - it.n0, arow, brow, l, e.at(it.m0, it.n0));
+            } else if constexpr (kGate<EPI>) {
+                EPI e = epi;
+                int l = lane;
+                asm volatile("" : "+s"(e.ld), "+v"(l));
+                store_tile_gate<EPI, TM, 8>(acc, Ct, ld, mrem, N - it.n0, arow, kPairs<EPI> ? brow / 2 : brow, l, e.at(it.m0, it.n0));
             } else store_tile_flags<TM, 8, OutT, true, A_KC && B_KC>(acc, Ct, ld, mrem, N - it.n0, arow, brow, lane, accumulate);
         }
         if (!more) break;
@@ -1081,6 +1088,39 @@ void launch(const void* A, const void* B, void* C, int M, int N, int K, int64_t 
         launch_large<A_KC, B_KC, OutT, false, true>(kind, lines, K, A, B, C, M, N, K, lda, ldb, ldc, accumulate, workspace, workspace_bytes, KSegments(), st, epi);
 }
 
+// The two forms of a gated MLP: the 4-wave kernel or the smaller tiles, planned as the product that they are (forward: of twice the columns, in whole blocks of 16).
+int64_t gate_columns(bool pairs, int64_t N) { return pairs ? (N + 15) / 16 * 32 : N; }
+template <class EPI>
+void launch_gate(const void* A, const void* B, void* C, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, void* workspace, int64_t workspace_bytes, hipStream_t st, const EPI& epi) {
+    constexpr bool B_KC = kPairs<EPI>;
+    constexpr Class cls = B_KC ? kForward : kInputGradient;
+    const int64_t columns = gate_columns(B_KC, N);
+    const bool lines = whole_lines(cls, M, columns, K);
+    const int nk = (K + BK - 1) / BK;
+    GemmPlan plan = choose_plan(cls, M, columns, K, workspace ? workspace_bytes : 0);
+    if (gemm_kind_large(plan.kind) && nk < 2) plan = {kTile256x128, 1};  // (the 4-wave kernel's items have two K tiles or more)
+    if (!gemm_kind_large(plan.kind)) {
+        GemmSmallArgs a = {};
+        a.p[0] = {(const bf16_t*)A, (const bf16_t*)B, C, lda, ldb, ldc, M, N, 0, 0, 0, 0};
+        a.K = K;
+        a.partial = (float*)workspace;
+        gemm_small_gate_launch<EPI>(plan, a, st, epi);
+        return;
+    }
+    const bool tail = K % BK != 0;
+    const int kind = tail ? (int)kTile256 : plan.kind;  // (the 192 x 256 tiles are planned for whole K tiles only)
+    const int cols = gemm_gate_cols<EPI>(kind), bm = (int)gemm_kind_bm(kind);
+    const int tiles_m = (M + bm - 1) / bm, tiles_n = (N + cols - 1) / cols;
+    const SplitPlan split = make_plan(kind, lines, (int64_t)tiles_m * tiles_n, nk, workspace, workspace_bytes);
+    const int items = split.full + split.rest * split.nsplit;
+#define EZL_W4(KTAIL, TBM)                                                                                                                                         hipLaunchKernelGGL((gemm_w4_kernel<true, B_KC, bf16_t, false, KTAIL, false, TBM, EPI>), w4_grid(items), dim3(256), 0, st, (const bf16_t*)A, (const bf16_t*)B,                        (bf16_t*)C, M, N, K, lda, ldb, ldc, 0, tiles_m, tiles_n, items, split, KSegments(), NoList(), epi)
+    if (kind == kTile192x256) EZL_W4(false, 192);
+    else if (tail) EZL_W4(true, 256);
+    else EZL_W4(false, 256);
+#undef EZL_W4
+    if (split.nsplit > 1) gemm_gate_reduce<EPI>(kind, split.partial, split.nsplit, split.full, tiles_m, tiles_n, (bf16_t*)C, ldc, M, N, st, epi);
+}
+
 // C = 0 for an empty reduction (a fill kernel rather than a memset node, so the call can be captured into a graph)
 template <typename OutT>
 __global__ __launch_bounds__(256) void zero_c_kernel(OutT* __restrict__ C, int64_t M, int64_t N, int64_t ldc) {
@@ -1181,6 +1221,42 @@ extern "C" int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int
     }
     launch<true, true, bf16_t, Epilogue>(A, B, C, (int)M, (int)N, (int)K, lda, ldb, ldc, 0, workspace, workspace_bytes, (hipStream_t)stream, e);
     EZL_LAUNCH_CHECK("ezl_gemm_bf16_epilogue");
+    return EZL_OK;
+}
+
+extern "C" int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K) { return M <= 0 || f <= 0 || K <= 0 ? 0 : plan_bytes(M, gate_columns(true, f), K); }
+
+extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* gate, void* up, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* name = "ezl_gated_fwd";
+    EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
+    EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
+    EZL_REQUIRE(!gate == !up, EZL_EINVAL, "%s: gate and up are kept together or not at all", name);
+    if (M == 0 || f == 0) return EZL_OK;
+    EZL_REQUIRE(out && up_weight, EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
+    if (const int rc = check_operands(x, gate_weight, M, f, K, ldx, ldw, f, 1, 1)) return rc;
+    EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    launch_gate<GateForward>(x, gate_weight, out, (int)M, (int)f, (int)K, ldx, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
+                             {(const bf16_t*)up_weight, (bf16_t*)gate, (bf16_t*)up, f, act});
+    EZL_LAUNCH_CHECK(name);
+    return EZL_OK;
+}
+
+extern "C" int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy,
+                             int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* name = "ezl_gated_bwd";
+    EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
+    EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
+    if (M == 0 || f == 0) return EZL_OK;
+    EZL_REQUIRE(gate && up && dgate && dup, EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
+    if (const int rc = check_operands(dy, down_weight, M, f, K, lddy, ldw, f, 1, 0)) return rc;
+    EZL_REQUIRE(ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) && ezl_aligned16(workspace), EZL_EINVAL,
+                "%s: pointers must be 16-byte aligned", name);
+    launch_gate<GateBackward>(dy, down_weight, dgate, (int)M, (int)f, (int)K, lddy, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
+                              {(const bf16_t*)gate, (const bf16_t*)up, (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, f, act});
+    EZL_LAUNCH_CHECK(name);
     return EZL_OK;
 }
 

@@ -43,6 +43,7 @@ __device__ __forceinline__ void store_tile(const f32x4 (&acc)[TM][TN], const Gem
     OutT* C = (OutT*)p.C + (int64_t)m0 * p.ldc + n0;
     const int mrem = p.M - m0 < 256 ? p.M - m0 : 256, nrem = p.N - n0;  // (no tile is taller: the range fits 31 bits)
     if constexpr (std::is_same_v<EPI, Epilogue>) store_tile_epilogue<TM, TN>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, epi.at(m0, n0));
+    else if constexpr (kGate<EPI>) store_tile_gate<EPI, TM, TN>(acc, C, p.ldc, mrem, nrem, row0, kPairs<EPI> ? col0 / 2 : col0, lane, epi.at(m0, n0));
     else if (vector_stores<OutT>(p)) store_tile_flags<TM, TN, OutT, true, FORWARD>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, p.accumulate);
     else store_tile_flags<TM, TN, OutT, false, FORWARD>(acc, C, p.ldc, mrem, nrem, row0, col0, lane, p.accumulate);
 }
@@ -93,10 +94,10 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs a
     const GemmProblem p = problem_of(args, tile);
     int tm, tn;
     tile_of(tile - p.first, p.tiles_m, p.tiles_n, tm, tn);
-    const int m0 = tm * TBM, n0 = tn * TBN;
+    const int m0 = tm * TBM, n0 = tn * (kPairs<EPI> ? TBN / 2 : TBN);
     const int arow = (wave >> 1) * (TBM / 2), brow = (wave & 1) * (TBN / 2);
     TileLoader<A_KC, TBM, 4, KTAIL> la;
-    TileLoader<B_KC, TBN, 4, KTAIL> lb;
+    TileLoader<B_KC, TBN, 4, KTAIL, kPairs<EPI>> lb;
     const int64_t a_blk = A_KC ? (int64_t)m0 * p.lda : (int64_t)m0;
     const int64_t b_blk = B_KC ? (int64_t)n0 * p.ldb : (int64_t)n0;
     la.init(lane, wave, p.M - m0, p.lda);
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs a
         if constexpr (f < TN) fb[buf][f] = sfrag<B_KC, TBN>(sA + TBM * BK, brow + f * 16, ks, lane);
         else fa[buf][f - TN] = sfrag<A_KC, TBM>(sA, arow + (f - TN) * 16, ks, lane);
     };
-    __amdgpu_buffer_rsrc_t ga, gb;
+    __amdgpu_buffer_rsrc_t ga, gb, gb2;
     int kv = BK;
     auto tile_bases = [&](int t) {
         const bf16_t *Ab, *Bb;
@@ -127,10 +128,12 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(const GemmSmallArgs a
         pick_segment<MULTI>(p.A, p.B, args.K, args.seg, t, kv, Ab, Bb);
         ga = la.base(Ab + a_blk + (int64_t)t * astep);
         gb = lb.base(Bb + b_blk + (int64_t)t * bstep);
+        if constexpr (kPairs<EPI>) gb2 = lb.base(epi.B2 + b_blk + (int64_t)t * bstep);
     };
     auto issue_load = [&](bf16_t* st, auto L) {
         constexpr int l = decltype(L)::value;
         if constexpr (l < NA) la.template issue_at<l>(ga, st, lane, wave, kv);
+        else if constexpr (kPairs<EPI>) lb.template issue_pair_at<l - NA>(gb, gb2, st + TBM * BK, lane, wave, kv);
         else lb.template issue_at<l - NA>(gb, st + TBM * BK, lane, wave, kv);
     };
     auto issue_tile = [&](int t, bf16_t* st) {
@@ -216,10 +219,10 @@ __global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs ar
     const GemmProblem p = problem_of(args, tile);
     int tm, tn;
     tile_of(tile - p.first, p.tiles_m, p.tiles_n, tm, tn);
-    const int m0 = tm * TB, n0 = tn * TB;
+    const int m0 = tm * TB, n0 = tn * (kPairs<EPI> ? TB / 2 : TB);
     const int arow = (wave >> 1) * (TB / 2), brow = (wave & 1) * (TB / 2);
     TileLoader<A_KC, TB, 4, true> la;
-    TileLoader<B_KC, TB, 4, true> lb;
+    TileLoader<B_KC, TB, 4, true, kPairs<EPI>> lb;
     const int64_t a_blk = A_KC ? (int64_t)m0 * p.lda : (int64_t)m0;
     const int64_t b_blk = B_KC ? (int64_t)n0 * p.ldb : (int64_t)n0;
     la.init(lane, wave, p.M - m0, p.lda);
@@ -234,7 +237,10 @@ __global__ __launch_bounds__(256) void gemm_square_kernel(const GemmSmallArgs ar
         t += kt0;
         pick_segment<MULTI>(p.A, p.B, args.K, args.seg, t, kv, Ab, Bb);
         la.issue(la.base(Ab + a_blk + (int64_t)t * astep), smem + stage * STAGE, lane, wave, kv);
-        lb.issue(lb.base(Bb + b_blk + (int64_t)t * bstep), smem + stage * STAGE + TB * BK, lane, wave, kv);
+        if constexpr (kPairs<EPI>)
+            lb.issue_pair(lb.base(lb.first(Bb, epi.B2, wave) + b_blk + (int64_t)t * bstep), lb.base(epi.B2 + b_blk + (int64_t)t * bstep), smem + stage * STAGE + TB * BK, lane, wave, kv);
+        else
+            lb.issue(lb.base(Bb + b_blk + (int64_t)t * bstep), smem + stage * STAGE + TB * BK, lane, wave, kv);
     };
     constexpr int NLD = decltype(la)::NI + decltype(lb)::NI;
 #pragma unroll
@@ -286,9 +292,9 @@ __global__ __launch_bounds__(512) void gemm_64_waves_kernel(const GemmSmallArgs 
     const GemmProblem p = problem_of(args, tile);
     int tm, tn;
     tile_of(tile - p.first, p.tiles_m, p.tiles_n, tm, tn);
-    const int m0 = tm * 64, n0 = tn * 64;
+    const int m0 = tm * 64, n0 = tn * (kPairs<EPI> ? 32 : 64);
     TileLoader<A_KC, 64, 1, true> la;
-    TileLoader<B_KC, 64, 1, true> lb;
+    TileLoader<B_KC, 64, 1, true, kPairs<EPI>> lb;
     const int64_t a_blk = A_KC ? (int64_t)m0 * p.lda : (int64_t)m0;
     const int64_t b_blk = B_KC ? (int64_t)n0 * p.ldb : (int64_t)n0;
     la.init(lane, 0, p.M - m0, p.lda);
@@ -301,7 +307,10 @@ __global__ __launch_bounds__(512) void gemm_64_waves_kernel(const GemmSmallArgs 
         int kv;
         pick_segment<MULTI>(p.A, p.B, args.K, args.seg, t, kv, Ab, Bb);
         la.issue(la.base(Ab + a_blk + (int64_t)t * astep), smem + wave * STAGE, lane, 0, kv);
-        lb.issue(lb.base(Bb + b_blk + (int64_t)t * bstep), smem + wave * STAGE + 64 * BK, lane, 0, kv);
+        if constexpr (kPairs<EPI>)
+            lb.issue_pair(lb.base(Bb + b_blk + (int64_t)t * bstep), lb.base(epi.B2 + b_blk + (int64_t)t * bstep), smem + wave * STAGE + 64 * BK, lane, 0, kv);
+        else
+            lb.issue(lb.base(Bb + b_blk + (int64_t)t * bstep), smem + wave * STAGE + 64 * BK, lane, 0, kv);
     };
     f32x4 acc[4][4];
     zero_acc(acc);
@@ -406,6 +415,72 @@ __global__ __launch_bounds__(256) void small_reduce_kernel(const GemmSmallArgs a
     }
 }
 
+// Sums of the partial tiles of a gated MLP's launch, in index order, and the epilogue: a thread owns four columns of a row of the result.
+template <class EPI>
+__global__ __launch_bounds__(256) void gate_reduce_kernel(const float* __restrict__ partial, int nsplit, int first_tile, int tiles_m, int tiles_n, int tbm, int tbn, bf16_t* __restrict__ C,
+                                                          int64_t ldc, int M, int N, const EPI epi) {
+    const int cols = kPairs<EPI> ? tbn / 2 : tbn, per_tile = tbm * cols / 1024;  // workgroups of a tile
+    const int local = blockIdx.x / per_tile;
+    int tm, tn;
+    tile_of(first_tile + local, tiles_m, tiles_n, tm, tn);
+    const int e = ((blockIdx.x - local * per_tile) * 256 + threadIdx.x) * 4, rl = e / cols, cl = e - rl * cols;
+    const int row = tm * tbm + rl, col = tn * cols + cl;
+    if (row >= M || col >= N) return;
+    const size_t stride = (size_t)tbm * tbn;
+    const float* src = partial + (size_t)local * nsplit * stride + (size_t)rl * tbn;
+    const auto sum = [&](int at) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int q = 0; q < nsplit; ++q) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(src + q * stride + at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += x[r];
+        }
+        return v;
+    };
+    const auto with = [&](auto ACT) {
+        constexpr int act = decltype(ACT)::value;
+        const auto store = [&](bf16_t* to, const f32x4& v) {
+            bf16x4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = (bf16_t)v[r];
+            *reinterpret_cast<bf16x4*>(to) = o;
+        };
+        if constexpr (kPairs<EPI>) {
+            const int at = (cl >> 4) * 32 + (cl & 15);
+            const f32x4 g = sum(at), u = sum(at + 16);
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = gate_value<act>(g[r]) * u[r];
+            if (epi.gate) {
+                store(epi.gate + (int64_t)row * epi.ld + col, g);
+                store(epi.up + (int64_t)row * epi.ld + col, u);
+            }
+            store(C + (int64_t)row * ldc + col, y);
+        } else {
+            const f32x4 d = sum(cl);
+            const int64_t at = (int64_t)row * epi.ld + col;
+            const bf16x4 g = *reinterpret_cast<const bf16x4*>(epi.gate + at), u = *reinterpret_cast<const bf16x4*>(epi.up + at);
+            f32x4 dg, du, mid;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float y, slope;
+                gate_value_slope<act>((float)g[r], y, slope);
+                dg[r] = d[r] * (float)u[r] * slope;
+                du[r] = d[r] * y;
+                mid[r] = y * (float)u[r];
+            }
+            store(epi.dgate + at, dg);
+            store(epi.dup + at, du);
+            if (epi.mid) store(epi.mid + at, mid);
+        }
+    };
+    if (epi.act == EZL_GATE_SILU) with(std::integral_constant<int, EZL_GATE_SILU>{});
+    else if (epi.act == EZL_GATE_GELU) with(std::integral_constant<int, EZL_GATE_GELU>{});
+    else if (epi.act == EZL_GATE_GELU_TANH) with(std::integral_constant<int, EZL_GATE_GELU_TANH>{});
+    else with(std::integral_constant<int, EZL_GATE_RELU>{});
+}
+
 template <bool A_KC, bool B_KC, typename OutT, bool MULTI, class EPI = NoEpilogue>
 void launch_kind(int kind, const GemmSmallArgs& a, bool tail, hipStream_t st, const EPI& epi = EPI()) {
     const dim3 grid((unsigned)(a.ntiles * a.nsplit));
@@ -421,7 +496,10 @@ void launch_kind(int kind, const GemmSmallArgs& a, bool tail, hipStream_t st, co
         case kTile64: hipLaunchKernelGGL((gemm_square_kernel<A_KC, B_KC, OutT, MULTI, 64, 4, EPI>), grid, dim3(256), 0, st, a, epi); break;
         default: hipLaunchKernelGGL((gemm_64_waves_kernel<A_KC, B_KC, OutT, MULTI, EPI>), grid, dim3(512), 0, st, a, epi); break;
     }
-    if (a.nsplit > 1) {
+    if constexpr (kGate<EPI>) {
+        if (a.nsplit > 1) gemm_gate_reduce<EPI>(kind, a.partial, a.nsplit, 0, a.p[0].tiles_m, a.p[0].tiles_n, (bf16_t*)a.p[0].C, a.p[0].ldc, a.p[0].M, a.p[0].N, st, epi);
+        return;
+    } else if (a.nsplit > 1) {
         const int tbm = (int)gemm_kind_bm(kind), tbn = (int)gemm_kind_bn(kind);
         hipLaunchKernelGGL((small_reduce_kernel<OutT, EPI>), dim3((unsigned)(a.ntiles * (tbm * tbn / 2048))), dim3(256), 0, st, a, tbm, tbn, 0, epi);
     }
@@ -452,6 +530,25 @@ void gemm_small_reduce(int kind, bool fp32, int first_tile, const GemmSmallArgs&
     if (fp32) hipLaunchKernelGGL((small_reduce_kernel<float>), grid, dim3(256), 0, stream, a, bm, bn, first_tile, NoEpilogue());
     else hipLaunchKernelGGL((small_reduce_kernel<bf16_t>), grid, dim3(256), 0, stream, a, bm, bn, first_tile, NoEpilogue());
 }
+
+template <class EPI>
+void gemm_gate_reduce(int kind, const float* partial, int nsplit, int first_tile, int tiles_m, int tiles_n, bf16_t* C, int64_t ldc, int M, int N, hipStream_t stream, const EPI& epilogue) {
+    const int bm = (int)gemm_kind_bm(kind), bn = (int)gemm_kind_bn(kind);
+    const dim3 grid((unsigned)((tiles_m * tiles_n - first_tile) * (bm * gemm_gate_cols<EPI>(kind) / 1024)));
+    hipLaunchKernelGGL((gate_reduce_kernel<EPI>), grid, dim3(256), 0, stream, partial, nsplit, first_tile, tiles_m, tiles_n, bm, bn, C, ldc, M, N, epilogue);
+}
+template <class EPI>
+void gemm_small_gate_launch(const GemmPlan& plan, GemmSmallArgs& a, hipStream_t stream, const EPI& epilogue) {
+    gemm_tile_grids(plan, a, 1);
+    GemmProblem& p = a.p[0];
+    p.tiles_n = (p.N + gemm_gate_cols<EPI>(plan.kind) - 1) / gemm_gate_cols<EPI>(plan.kind);
+    a.ntiles = p.tiles_m * p.tiles_n;
+    launch_kind<true, kPairs<EPI>, bf16_t, false, EPI>(plan.kind, a, a.K % BK != 0, stream, epilogue);
+}
+template void gemm_small_gate_launch<GateForward>(const GemmPlan&, GemmSmallArgs&, hipStream_t, const GateForward&);
+template void gemm_small_gate_launch<GateBackward>(const GemmPlan&, GemmSmallArgs&, hipStream_t, const GateBackward&);
+template void gemm_gate_reduce<GateForward>(int, const float*, int, int, int, int, bf16_t*, int64_t, int, int, hipStream_t, const GateForward&);
+template void gemm_gate_reduce<GateBackward>(int, const float*, int, int, int, int, bf16_t*, int64_t, int, int, hipStream_t, const GateBackward&);
 
 void gemm_small_launch(int form, bool multi, const GemmPlan& plan, GemmSmallArgs& a, int count, hipStream_t stream, const Epilogue* epilogue) {
     gemm_tile_grids(plan, a, count);

@@ -2,6 +2,7 @@
 #pragma once
 #include "activation.h"
 #include "common.h"
+#include "gate.h"
 
 #include <type_traits>
 
@@ -37,6 +38,33 @@ struct Epilogue {
         return {bias ? bias + n : nullptr, residual ? residual + m * ldr + n : nullptr, pre ? pre + m * ldp + n : nullptr, ldr, ldp, act};
     }
 };
+
+// The first products of a gated MLP as one: C = act(A B^T) * (A B2^T), forward form, B and B2 alike.  A tile's columns are taken 16 of B, the same 16 of B2, and so on: the two
+// accumulators of a result lie in one lane, and a tile of 256 columns makes 128 of C.  gate and up (both or neither) receive the two products, rounded, for the backward pass; C is made of them
+// unrounded.
+struct GateForward {
+    const bf16_t* B2;
+    bf16_t *gate, *up;
+    int64_t ld;  // of gate and up
+    int act;
+    __device__ __forceinline__ GateForward at(int64_t m, int64_t n) const { return {B2, gate ? gate + m * ld + n : nullptr, up ? up + m * ld + n : nullptr, ld, act}; }
+};
+// The way back through it behind the input gradient d = A B of the down projection: dgate = d * up * act'(gate), dup = d * act(gate), and mid (may be null) =
+// act(gate) * up once more, which the down projection's weight gradient reads.  d itself is stored nowhere.  All [M, N], rows ld apart.
+struct GateBackward {
+    const bf16_t *gate, *up;
+    bf16_t *dgate, *dup, *mid;
+    int64_t ld;
+    int act;
+    __device__ __forceinline__ GateBackward at(int64_t m, int64_t n) const {
+        const int64_t o = m * ld + n;
+        return {gate + o, up + o, dgate + o, dup + o, mid ? mid + o : nullptr, ld, act};
+    }
+};
+template <class EPI>
+constexpr bool kPairs = std::is_same_v<EPI, GateForward>;
+template <class EPI>
+constexpr bool kGate = kPairs<EPI> || std::is_same_v<EPI, GateBackward>;
 
 namespace {
 
@@ -80,8 +108,10 @@ __device__ __forceinline__ int kmajor_swizzle(int krow) {
 // reads into a full drain (lgkmcnt(0)); with buffer loads the waits inside the K loop are exact counts.
 constexpr uint32_t kBufBytes = 0x80000000u;  // every tile is addressed as a 2 GiB buffer: an offset of kBufBytes reads as zero
 
-template <bool KC, int R, int NW, bool KTAIL>
+// PAIRS (k-contiguous): the tile's rows are 16 rows of one operand, the same 16 of a second one, and so on.
+template <bool KC, int R, int NW, bool KTAIL, bool PAIRS = false>
 struct TileLoader {
+    static_assert(KC || !PAIRS, "pairs are of k-contiguous operands");
     static constexpr int NI = R / 8 / NW;
     static constexpr int CPR = R / 8;       // k-major: chunks per k row
     uint32_t off[NI];  // byte offsets from (operand base + k advance - 4096)
@@ -107,7 +137,8 @@ struct TileLoader {
             if (KC) {
                 const int row = 8 * q + (lane >> 3);
                 const int c = (lane & 7) ^ ((row >> 1) & 7);
-                const int gr = row < dim ? row : dim - 1;
+                const int own = PAIRS ? (row >> 5) * 16 + (row & 15) : row;
+                const int gr = own < dim ? own : dim - 1;
                 e = (int64_t)gr * ld + c * 8;
             } else {
                 const int krow = k_row(wave, i, lane);
@@ -139,6 +170,21 @@ struct TileLoader {
         if constexpr (I < NI) {
             issue_at<I>(g, stage, lane, wave, kv);
             issue<I + 1>(g, stage, lane, wave, kv);
+        }
+    }
+    // PAIRS: a wave load is eight rows of one operand, two in a row are of the same.  Where a wave has only two, they are the operand that first() names, given as g.
+    static __device__ __forceinline__ const bf16_t* first(const bf16_t* a, const bf16_t* b, int wave) { return NI % 4 != 0 && (wave & 1) ? b : a; }
+    template <int I>
+    __device__ __forceinline__ void issue_pair_at(__amdgpu_buffer_rsrc_t g, __amdgpu_buffer_rsrc_t g2, bf16_t* stage, int lane, int wave, int kv) const {
+        static_assert(NI % 4 == 0 || NI == 2, "whole pairs of wave loads");
+        if constexpr (NI % 4 == 0 && (I >> 1 & 1)) issue_at<I>(g2, stage, lane, wave, kv);
+        else issue_at<I>(g, stage, lane, wave, kv);
+    }
+    template <int I = 0>
+    __device__ __forceinline__ void issue_pair(__amdgpu_buffer_rsrc_t g, __amdgpu_buffer_rsrc_t g2, bf16_t* stage, int lane, int wave, int kv) const {
+        if constexpr (I < NI) {
+            issue_pair_at<I>(g, g2, stage, lane, wave, kv);
+            issue_pair<I + 1>(g, g2, stage, lane, wave, kv);
         }
     }
 };
@@ -442,6 +488,147 @@ __device__ __forceinline__ void store_epilogue(float (&v)[N], bf16_t* C, int64_t
     store(C + m * ldc + n);
 }
 
+// The same for the two forms of a gated MLP.  Forward: acc[i][2 b], acc[i][2 b + 1] are the gate's and the up projection's columns col0 + 16 b .. (of C).  Lanes l and l ^ 16 trade halves
+// of two neighbouring blocks as above; where a wave has one block only, its stores are 8 bytes.
+template <int ACT, int TM, int TN>
+__device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], bf16_t* C, int64_t ldc, int mrem, int nrem, int row0, int col0, int lane, const GateForward& e) {
+    constexpr uint32_t kOut = 0x80000000u;
+    constexpr int NB = TN / 2;  // blocks of 16 columns
+    constexpr bool WIDE = NB % 2 == 0;
+    const auto matrix = [&](bf16_t* p, int64_t ld) {
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(p), 0, (uint32_t)(((int64_t)(mrem - 1) * ld + nrem) * 2), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc), gbuf = matrix(e.gate, e.ld), ubuf = matrix(e.up, e.ld);
+    const bool keep = e.gate != nullptr;
+    const int g = lane >> 4;
+    uint32_t col_off[WIDE ? NB / 2 : NB];
+#pragma unroll
+    for (int b = 0; b < (WIDE ? NB / 2 : NB); ++b) {
+        const int col = WIDE ? col0 + (2 * b + (g & 1)) * 16 + 8 * (g >> 1) : col0 + b * 16 + 4 * g;
+        col_off[b] = col < nrem ? (uint32_t)col * 2 : kOut;
+    }
+    const uint32_t row = (uint32_t)(row0 + (lane & 15));
+    const auto offset = [&](int i, int b, int64_t ld) { return col_off[b] + row * (uint32_t)(ld * 2) + i * (uint32_t)(32 * ld); };
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int b = 0; b < NB / 2; ++b) {
+                const f32x4 ga = from_agprs<TM * TN>(acc[i][4 * b]), ua = from_agprs<TM * TN>(acc[i][4 * b + 1]);
+                const f32x4 gb = from_agprs<TM * TN>(acc[i][4 * b + 2]), ub = from_agprs<TM * TN>(acc[i][4 * b + 3]);
+                const auto out = [&](const f32x4& a, const f32x4& c, __amdgpu_buffer_rsrc_t to, int64_t ld) {
+                    float v[8];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[r]), __float_as_uint(c[r]), false, false);
+                        v[r] = __uint_as_float(sw[0]);
+                        v[4 + r] = __uint_as_float(sw[1]);
+                    }
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(v)), to, offset(i, b, ld), 0, 0);
+                };
+                if (keep) {
+                    out(ga, gb, gbuf, e.ld);
+                    out(ua, ub, ubuf, e.ld);
+                }
+                f32x4 ya, yb;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    ya[r] = gate_value<ACT>(ga[r]) * ua[r];
+                    yb[r] = gate_value<ACT>(gb[r]) * ub[r];
+                }
+                out(ya, yb, cbuf, ldc);
+                if constexpr (TM * TN >= 48) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const f32x4 ga = acc[i][2 * b], ua = acc[i][2 * b + 1];
+                const auto out = [&](const f32x4& a, __amdgpu_buffer_rsrc_t to, int64_t ld) {
+                    bf16x4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = (bf16_t)a[r];
+                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), to, offset(i, b, ld), 0, 0);
+                };
+                if (keep) {
+                    out(ga, gbuf, e.ld);
+                    out(ua, ubuf, e.ld);
+                }
+                f32x4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = gate_value<ACT>(ga[r]) * ua[r];
+                out(y, cbuf, ldc);
+            }
+        }
+    }
+}
+// Backward: acc is d; a row's gate and up are fetched in front of the stores of the row before it.
+template <int ACT, int TM, int TN>
+__device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], int mrem, int nrem, int row0, int col0, int lane, const GateBackward& e) {
+    constexpr uint32_t kOut = 0x80000000u;
+    const auto matrix = [&](const bf16_t* p) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(p)), 0, (uint32_t)(((int64_t)(mrem - 1) * e.ld + nrem) * 2), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t gbuf = matrix(e.gate), ubuf = matrix(e.up), dgbuf = matrix(e.dgate), dubuf = matrix(e.dup), midbuf = matrix(e.mid);
+    const bool want_mid = e.mid != nullptr;
+    const int g = lane >> 4;
+    uint32_t off[TN / 2];
+#pragma unroll
+    for (int jp = 0; jp < TN / 2; ++jp) {
+        const int col = col0 + (2 * jp + (g & 1)) * 16 + 8 * (g >> 1);
+        off[jp] = (col < nrem ? (uint32_t)col * 2 : kOut) + (uint32_t)(row0 + (lane & 15)) * (uint32_t)(e.ld * 2);
+    }
+    const uint32_t row_step = (uint32_t)(32 * e.ld);
+    u32x4 old_g[2][TN / 2], old_u[2][TN / 2];
+    const auto fetch = [&](int i) {
+#pragma unroll
+        for (int jp = 0; jp < TN / 2; ++jp) {
+            old_g[i & 1][jp] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gbuf, off[jp] + i * row_step, 0, 0));
+            old_u[i & 1][jp] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ubuf, off[jp] + i * row_step, 0, 0));
+        }
+    };
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        if (i + 1 < TM) fetch(i + 1);
+#pragma unroll
+        for (int jp = 0; jp < TN / 2; ++jp) {
+            const f32x4 va = from_agprs<TM * TN>(acc[i][2 * jp]), vb = from_agprs<TM * TN>(acc[i][2 * jp + 1]);
+            float d[8], dg[8], du[8], mid[8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(va[r]), __float_as_uint(vb[r]), false, false);
+                d[r] = __uint_as_float(sw[0]);
+                d[4 + r] = __uint_as_float(sw[1]);
+            }
+            const bf16x8 gate = __builtin_bit_cast(bf16x8, old_g[i & 1][jp]), up = __builtin_bit_cast(bf16x8, old_u[i & 1][jp]);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                float y, slope;
+                gate_value_slope<ACT>((float)gate[r], y, slope);
+                dg[r] = d[r] * (float)up[r] * slope;
+                du[r] = d[r] * y;
+                mid[r] = y * (float)up[r];
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(dg)), dgbuf, off[jp] + i * row_step, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(du)), dubuf, off[jp] + i * row_step, 0, 0);
+            if (want_mid) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(mid)), midbuf, off[jp] + i * row_step, 0, 0);
+            if constexpr (TM * TN >= 48) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+template <class EPI, int TM, int TN>
+__device__ __forceinline__ void store_tile_gate(const f32x4 (&acc)[TM][TN], bf16_t* C, int64_t ldc, int mrem, int nrem, int row0, int col0, int lane, const EPI& e) {
+    const auto with = [&](auto ACT) {
+        if constexpr (kPairs<EPI>) store_gate_forward<decltype(ACT)::value, TM, TN>(acc, C, ldc, mrem, nrem, row0, col0, lane, e);
+        else store_gate_backward<decltype(ACT)::value, TM, TN>(acc, mrem, nrem, row0, col0, lane, e);
+    };
+    if (e.act == EZL_GATE_SILU) with(std::integral_constant<int, EZL_GATE_SILU>{});
+    else if (e.act == EZL_GATE_GELU) with(std::integral_constant<int, EZL_GATE_GELU>{});
+    else if (e.act == EZL_GATE_GELU_TANH) with(std::integral_constant<int, EZL_GATE_GELU_TANH>{});
+    else with(std::integral_constant<int, EZL_GATE_RELU>{});
+}
+
 // as store_tile_impl with the kernel's flags: bit 0 accumulate, kRoundResult (only where the form has it: MAY_ROUND; an fp32 result has it without bit 0, a bf16
 // one, which is rounded as it is stored, with it)
 template <int TM, int TN, typename OutT, bool VEC, bool MAY_ROUND>
@@ -489,6 +676,16 @@ struct GemmPlan {
 // epilogue (form 0, one product, N a multiple of 8, rows on 16 bytes): null, or what its values go through
 __attribute__((visibility("hidden"))) void gemm_small_launch(int form, bool multi, const GemmPlan& plan, GemmSmallArgs& a, int count,
                                                              hipStream_t stream, const Epilogue* epilogue = nullptr);
+// the same for the forms of a gated MLP, of one product: forward (form 0, a.p[0].N columns of the result) or behind an input gradient (form 1)
+template <class EPI>
+__attribute__((visibility("hidden"))) void gemm_small_gate_launch(const GemmPlan& plan, GemmSmallArgs& a, hipStream_t stream, const EPI& epilogue);
+// adds a gated launch's partial tiles (of first_tile on, tiles_m x tiles_n of the plan's shape in all) and does what their epilogue does
+template <class EPI>
+__attribute__((visibility("hidden"))) void gemm_gate_reduce(int kind, const float* partial, int nsplit, int first_tile, int tiles_m, int tiles_n, bf16_t* C, int64_t ldc, int M, int N,
+                                                            hipStream_t stream, const EPI& epilogue);
+// columns of a gated launch's result that a tile of that shape makes
+template <class EPI>
+constexpr int gemm_gate_cols(int kind) { return kKindCols[kind] / (kPairs<EPI> ? 2 : 1); }
 // tile grids of a launch on tiles of that plan's shape (K is set)
 __attribute__((visibility("hidden"))) void gemm_tile_grids(const GemmPlan& plan, GemmSmallArgs& a, int count);
 // results (fp32, else bf16) of tiles first_tile.. of a launch from their partial tiles (a.partial: of first_tile on, a.nsplit of each)

@@ -399,48 +399,93 @@ def swiglu(gate, up):
     return SwiGLUFunction.apply(gate.contiguous(), up.contiguous())
 
 
-class GatedMLPFunction(torch.autograd.Function):
-    """down(act(gate x) * up x).  The two products' results are kept for backward (bf16), what they make together is not: the backward pass computes it
-    again where it needs it, for the down projection's weight gradient."""
+def _gate_weights(gate_weight, up_weight):
+    """Both with the same row stride, as the kernel reads them."""
+    if gate_weight.stride() == up_weight.stride():
+        return gate_weight, up_weight
+    return gate_weight.contiguous(), up_weight.contiguous()
+
+
+def _gated_products_bwd(x, gate_weight, up_weight, dgate, dup, need):
+    """(dx, dgate_weight, dup_weight), as far as needed"""
+    x2d = x.reshape(-1, x.shape[-1])
+    grads = [None, None]
+    wanted = [i for i in range(2) if need[1 + i]]
+    if wanted:
+        targets = [_main_grad_target((gate_weight, up_weight)[i]) for i in wanted]
+        dws = K.linear_wgrad_multi([(dgate, dup)[i] for i in wanted], x2d, [mg for mg, _ in targets], [acc for _, acc in targets])
+        for i, (mg, _), dw in zip(wanted, targets, dws):
+            grads[i] = dw if mg is None else None
+    dx = K.linear_dgrad_multi([dgate, dup], [gate_weight, up_weight]).view(x.shape) if need[0] else None
+    return (dx, *grads)
+
+
+class GatedLinearFunction(torch.autograd.Function):
+    """act(gate x) * up x, both products kept for backward in bf16 (half the bytes of fp32; the gradients that are made of them go through bf16 products anyway)."""
 
     @staticmethod
-    def forward(ctx, x, gate_weight, up_weight, down_weight, act):
+    def forward(ctx, x, gate_weight, up_weight, act, training):
         x2d = x.reshape(-1, x.shape[-1])
-        gate, up = K.linear_fwd_multi(x2d, (gate_weight, up_weight))
-        y = K.linear_fwd(K.gate_fwd(act, gate, up), down_weight)
+        keep = training and any(ctx.needs_input_grad[:3])
+        mid, gate, up = K.gated_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), keep)
+        ctx.act = act
+        ctx.save_for_backward(x, gate_weight, up_weight, gate, up)
+        return mid.view(*x.shape[:-1], mid.shape[1])
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dmid):
+        x, gate_weight, up_weight, gate, up = ctx.saved_tensors
+        dgate, dup = K.gate_bwd(ctx.act, dmid.reshape(gate.shape).contiguous(), gate, up)
+        return (*_gated_products_bwd(x, gate_weight, up_weight, dgate, dup, ctx.needs_input_grad), None, None)
+
+
+class GatedMLPFunction(torch.autograd.Function):
+    """down(act(gate x) * up x).  The two products' results are kept for backward (bf16), what they make together is not: the backward pass makes it again in the
+    launch that takes the output's gradient through the down projection and the gate, for the down projection's weight gradient."""
+
+    @staticmethod
+    def forward(ctx, x, gate_weight, up_weight, down_weight, act, training):
+        x2d = x.reshape(-1, x.shape[-1])
+        keep = training and any(ctx.needs_input_grad[:4])
+        mid, gate, up = K.gated_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), keep)
+        y = K.linear_fwd(mid, down_weight)
         ctx.act = act
         ctx.save_for_backward(x, gate_weight, up_weight, down_weight, gate, up)
-        return y.view(*x.shape[:-1], down_weight.shape[0])
+        return y.view(*x.shape[:-1], y.shape[1])
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
         x, gate_weight, up_weight, down_weight, gate, up = ctx.saved_tensors
         need = ctx.needs_input_grad
-        x2d, dy2d = x.reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
+        dy2d = dy.reshape(-1, dy.shape[-1])
         if not dy2d.is_contiguous():
             dy2d = dy2d.contiguous()
-        dgate, dup, mid = K.gate_bwd(ctx.act, K.linear_dgrad(dy2d, down_weight), gate, up, need[3])
-        grads = [None, None, None]
+        dgate, dup, mid = K.gated_bwd(ctx.act, dy2d, down_weight, gate, up, need[3])
+        dw = None
         if need[3]:
             mg, acc = _main_grad_target(down_weight)
             dw = K.linear_wgrad(dy2d, mid, out=mg, accumulate=acc)
-            grads[2] = dw if mg is None else None
-        wanted = [i for i in range(2) if need[1 + i]]
-        if wanted:
-            targets = [_main_grad_target((gate_weight, up_weight)[i]) for i in wanted]
-            dws = K.linear_wgrad_multi([(dgate, dup)[i] for i in wanted], x2d, [mg for mg, _ in targets], [acc for _, acc in targets])
-            for i, (mg, _), dw in zip(wanted, targets, dws):
-                grads[i] = dw if mg is None else None
-        dx = K.linear_dgrad_multi([dgate, dup], [gate_weight, up_weight]).view(x.shape) if need[0] else None
-        return (dx, *grads, None)
+            dw = dw if mg is None else None
+        return (*_gated_products_bwd(x, gate_weight, up_weight, dgate, dup, need), dw, None, None)
+
+
+def _check_gate(activation):
+    if activation not in K.GATES:
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(K.GATES), activation))
+
+
+def gated_linear(x, gate_weight, up_weight, activation="silu"):
+    """act(x gate^T) * (x up^T), one launch, fp32 up to one rounding; activation: 'silu', 'gelu' (exact), 'gelu_tanh' or 'relu'.  x [..., h], weights [f, h]."""
+    _check_gate(activation)
+    return GatedLinearFunction.apply(x, gate_weight, up_weight, activation, torch.is_grad_enabled())
 
 
 def gated_mlp(x, gate_weight, up_weight, down_weight, activation="silu"):
-    """(act(x gate^T) * (x up^T)) down^T; activation: 'silu', 'gelu' (exact), 'gelu_tanh' or 'relu'.  x [..., h], weights [f, h], [f, h], [h', f]."""
-    if activation not in K.GATES:
-        raise ValueError("activation must be one of %s, got %r" % (", ".join(K.GATES), activation))
-    return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation)
+    """gated_linear(x, gate_weight, up_weight, activation) down^T; down [h', f].  Of the tensors between x and the result the backward pass keeps two, x gate^T and x up^T."""
+    _check_gate(activation)
+    return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation, torch.is_grad_enabled())
 
 
 # --------------------------------------------------------------------------------------------

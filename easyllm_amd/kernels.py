@@ -285,23 +285,46 @@ def swiglu_bwd(dout, gate, up):
 GATES = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 
-def gate_fwd(act, gate, up):
-    """act(gate) * up"""
+def gated_fwd(act, x2d, gate_weight, up_weight, keep=False):
+    """-> (act(x2d @ gate_weight^T) * (x2d @ up_weight^T), and with `keep` the two products, else None, None)"""
+    ldx, ldw = _rows_ld(x2d, "x"), _rows_ld(gate_weight, "gate weight")
+    (T, n_in), (f, w_in) = x2d.shape, gate_weight.shape
+    _need(up_weight.shape == gate_weight.shape and _rows_ld(up_weight, "up weight") == ldw, "gated: the two weights must be alike")
+    _need(n_in == w_in and n_in > 0 and f % 8 == 0, "gated: inner dimensions differ or are empty, or the width is no multiple of 8")
+    _here(x2d, "x"); _here(gate_weight, "gate weight"); _here(up_weight, "up weight")
+    out = torch.empty((T, f), dtype=BF16, device=x2d.device)
+    gate = up = None
+    if keep:
+        gate, up = torch.empty_like(out), torch.empty_like(out)
+    nbytes = _lib.gated_workspace_bytes(T, f, n_in)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x2d.device) if nbytes else None
+    _lib.call("ezl_gated_fwd", GATES[act], x2d.data_ptr(), gate_weight.data_ptr(), up_weight.data_ptr(), out.data_ptr(), _p(gate), _p(up), T, f, n_in, ldx, ldw, _p(ws), nbytes,
+              _stream())
+    return out, gate, up
+
+
+def gated_bwd(act, dy2d, down_weight, gate, up, want_mid=False):
+    """with d = dy2d @ down_weight -> (d * up * act'(gate), d * act(gate), act(gate) * up or None)"""
+    lddy, ldw = _rows_ld(dy2d, "dy"), _rows_ld(down_weight, "down weight")
+    (T, n_out), f = dy2d.shape, down_weight.shape[1]
     _ready((gate, up), "gate up")
-    _need(gate.shape == up.shape, "gate/up shape mismatch")
-    out = torch.empty_like(gate)
-    _lib.call("ezl_gate_fwd", GATES[act], _p(gate), _p(up), _p(out), gate.numel(), _stream())
-    return out
-
-
-def gate_bwd(act, dout, gate, up, want_out=False):
-    """-> (dgate, dup, act(gate) * up or None)"""
-    _ready((dout, gate, up), "dout gate up")
-    _need(gate.shape == up.shape == dout.shape, "gate_bwd shape mismatch")
+    _here(dy2d, "dy"); _here(down_weight, "down weight")
+    _need(down_weight.shape[0] == n_out and gate.shape == up.shape == (T, f), "gated_bwd: shape mismatch")
     dgate, dup = torch.empty_like(gate), torch.empty_like(up)
-    out = torch.empty_like(gate) if want_out else None
-    _lib.call("ezl_gate_bwd", GATES[act], _p(dout), _p(gate), _p(up), _p(dgate), _p(dup), _p(out), gate.numel(), _stream())
-    return dgate, dup, out
+    mid = torch.empty_like(gate) if want_mid else None
+    ws, nbytes = _gemm_workspace(T, f, n_out, dy2d.device)
+    _lib.call("ezl_gated_bwd", GATES[act], dy2d.data_ptr(), down_weight.data_ptr(), gate.data_ptr(), up.data_ptr(), dgate.data_ptr(), dup.data_ptr(), _p(mid), T, f, n_out, lddy, ldw,
+              _p(ws), nbytes, _stream())
+    return dgate, dup, mid
+
+
+def gate_bwd(act, d, gate, up):
+    """-> (d * up * act'(gate), d * act(gate))"""
+    _ready((d, gate, up), "d gate up")
+    _need(gate.shape == up.shape == d.shape, "gate_bwd shape mismatch")
+    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    _lib.call("ezl_gate_bwd", GATES[act], _p(d), _p(gate), _p(up), _p(dgate), _p(dup), gate.numel(), _stream())
+    return dgate, dup
 
 
 # ------------------------------------------------------------------------------------- RoPE

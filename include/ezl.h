@@ -111,14 +111,24 @@ int ezl_norm_bwd(int kind, const void* dy, const void* dsum, const void* s, cons
 int ezl_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, void* stream);
 int ezl_swiglu_bwd(const void* dout, const void* gate, const void* up, void* dgate, void* dup, int64_t n, void* stream);
 
-/* ---- gated MLPs with SiLU, either GELU or ReLU: out = act(gate) * up over n bf16 values (n % 8 == 0), and dgate = dout * up * act'(gate),
- *      dup = dout * act(gate) (dgate may be gate or dout, dup up); out, if given, receives act(gate) * up again ---- */
+/* ---- gated MLPs with SiLU, either GELU or ReLU (ParallelMLP with a gate, llama/transformer.py:217-225): the products with what stands around them ---- */
 #define EZL_GATE_SILU 0
 #define EZL_GATE_GELU 1
 #define EZL_GATE_GELU_TANH 2
 #define EZL_GATE_RELU 3
-int ezl_gate_fwd(int act, const void* gate, const void* up, void* out, int64_t n, void* stream);
-int ezl_gate_bwd(int act, const void* dout, const void* gate, const void* up, void* dgate, void* dup, void* out, int64_t n, void* stream);
+/* out[M, f] = act(x gate_weight^T) * (x up_weight^T) in one launch, fp32 from the reductions to the one rounding: x [M, K] (rows ldx elements apart), both weights [f, K] (rows
+ * ldw apart).  gate and up (both or neither) receive the two products, rounded, for the backward pass.  out, gate, up contiguous; f % 8 == 0, below 2^21; K % 8 == 0, not 0.
+ * workspace as for ezl_gemm_bf16, ezl_gated_workspace_bytes(M, f, K) bytes. */
+int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K);
+int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* gate, void* up, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+/* Its way back behind a down projection, from dy [M, K] (rows lddy apart) and down_weight [K, f] (rows ldw apart), in one launch: with d = dy down_weight, dgate = d * up * act'(gate),
+ * dup = d * act(gate), and mid (may be NULL) = act(gate) * up again, which the down projection's weight gradient dy^T mid reads; d itself is not stored.  All [M, f], contiguous.
+ * workspace: ezl_gemm_workspace_bytes(M, f, K). */
+int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy,
+                  int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same from a d that is there, n values of each, n % 8 == 0 (dgate may be gate or d, dup up). */
+int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, int64_t n, void* stream);
 
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----
  * table: cos/sin fp32 [npos, half_dim], theta = (p / scale_factor) * inv_freq[j].

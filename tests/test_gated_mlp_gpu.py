@@ -57,17 +57,20 @@ def expected(x, wg, wu, wd, dy, act):
     x, wg, wu, wd = (t.detach().double() for t in (x, wg, wu, wd))
     (g, g_err), (u, u_err) = product(x, None, wg.t()), product(x, None, wu.t())
     a, slope = act64(g, act)
-    # forward: gate and up may be rounded on their way to the gate
-    g1, u1 = g_err + g.abs() * H, u_err + u.abs() * H
-    a_err = 1.2 * g1 + a.abs() * 2.0 ** -15
     mid = a * u
-    mid_err = a_err * u.abs() + (a.abs() + a_err) * u1
-    mid_err = mid_err + (mid.abs() + mid_err) * H
-    out = {"y": product(mid, mid_err, wd.t())}
+
+    def middle(g1, u1):
+        """what act(g) and mid, rounded, are off by where g and u are off by g1 and u1"""
+        a_err = 1.2 * g1 + a.abs() * 2.0 ** -15
+        err = a_err * u.abs() + (a.abs() + a_err) * u1
+        return a_err, err + (mid.abs() + err) * H
+
+    out = {"y": product(mid, middle(g_err, u_err)[1], wd.t())}
+    g1, u1 = g_err + g.abs() * H, u_err + u.abs() * H  # (as the backward pass reads them)
+    a_err, mid_err = middle(g1, u1)
     if dy is not None:
         dy = dy.double()
         d, d_err = product(dy, None, wd)
-        d_err = d_err + d.abs() * H
         slope_err = 1.2 * g1 + slope.abs() * 2.0 ** -15
         if act == "relu":
             slope_err = slope_err * 0 + (g.abs() <= g1)
@@ -100,12 +103,34 @@ def check(F, T, h, f, act, h_out=None, seed=0, train=True, shape=None):
             near(g.reshape(want[name][0].shape), *want[name], name)
 
 
-SHAPES = [(1, 8, 8), (1, 64, 64), (2, 256, 688), (5, 1000, 24), (8, 512, 1368), (16, 264, 1000), (17, 72, 520), (33, 128, 16), (64, 64, 136), (100, 520, 264), (257, 768, 2048),
-          (389, 256, 688), (389, 1032, 2776), (300, 72, 1048), (1000, 776, 1032), (1024, 2048, 5504), (2500, 520, 4104), (513, 4096, 1024)]
+SMALL = [(1, 8, 8), (1, 64, 64), (2, 256, 688), (5, 1000, 24), (8, 512, 1368), (16, 264, 1000), (17, 72, 520), (33, 128, 16), (64, 64, 136), (100, 520, 264), (257, 768, 2048),
+         (389, 256, 688), (389, 1032, 2776), (300, 72, 1048), (1000, 776, 1032)]
+# the other tile shapes, whole and split, either way (asked for below); the last of them with a down projection to another width
+LARGE = [(513, 4096, 1024, 4096), (389, 4096, 512, 4096), (600, 4096, 1024, 4096), (1000, 1024, 2752, 1024), (4104, 256, 1024, 256), (389, 4096, 2560, 4096), (600, 4096, 2560, 4096),
+         (1531, 4096, 5504, 4096), (4000, 264, 4096, 264), (4096, 1024, 4104, 1032), (2500, 520, 4104, 520), (389, 256, 2560, 8192), (1300, 256, 2560, 4096), (1000, 256, 3136, 8192),
+         (4096, 64, 2048, 64), (1024, 256, 5504, 2048)]
+
+
+def test_the_sizes_reach_every_tile_shape():
+    from easyllm_amd import _lib
+    plan = lambda form, T, n, k: _lib.gemm_plan(form, [T], [n], k)[1:]  # noqa: E731
+    ways = [(*s, s[1]) for s in SMALL] + LARGE
+    fwd = {(p[0], p[1], p[2] > 1, p[0] == 64 and p[3]) for p in (plan("forward", T, (f + 15) // 16 * 32, h) for T, h, f, _ in ways)}
+    bwd = {(p[0], p[1], p[2] > 1, p[0] == 64 and p[3]) for p in (plan("input gradient", T, f, h_out) for T, _, f, h_out in ways)}
+    every = {(rows, cols, split, rows == 64 and 4) for rows, cols in ((256, 256), (192, 256), (256, 128), (192, 128), (128, 128), (64, 64)) for split in (False, True)} | {(64, 64, False, 8)}
+    assert every <= fwd, every - fwd
+    assert every <= bwd, every - bwd
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
-@pytest.mark.parametrize("T,h,f", SHAPES)
+@pytest.mark.parametrize("T,h,f,h_out", LARGE)
+def test_every_tile_shape(F, T, h, f, h_out, act):
+    print("gated", T, h, f, h_out, act, flush=True)
+    check(F, T, h, f, act, h_out=h_out)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T,h,f", SMALL)
 def test_forward_and_backward(F, T, h, f, act):
     print("gated", T, h, f, act, flush=True)
     check(F, T, h, f, act)
@@ -116,6 +141,34 @@ def test_forward_alone(F, T, h, f, h_out):
     print("gated", T, h, f, h_out, flush=True)
     for act in ("silu", "gelu"):
         check(F, T, h, f, act, h_out=h_out, train=False)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T,h,f", [(1, 8, 8), (100, 520, 264), (389, 256, 688), (2500, 520, 4104)])
+def test_the_gate_alone(F, T, h, f, act):
+    print("gated linear", T, h, f, act, flush=True)
+    x = rnd(T, h).requires_grad_()
+    wg, wu = (rnd(f, h, seed=1 + i, scale=1.5 * h ** -0.5).requires_grad_() for i in range(2))
+    dmid = rnd(T, f, seed=4)
+    mid = F.gated_linear(x, wg, wu, activation=act)
+    (g, g_err), (u, u_err) = product(x.double(), None, wg.double().t()), product(x.double(), None, wu.double().t())
+    (g, g_err, u, u_err) = (t.detach() for t in (g, g_err, u, u_err))
+    a, slope = act64(g, act)
+    a_err = 1.2 * g_err + a.abs() * 2.0 ** -15
+    near(mid, a * u, a_err * u.abs() + (a.abs() + a_err) * u_err, "mid")
+    got = torch.autograd.grad(mid, (x, wg, wu), dmid)
+    g1, u1, d = g_err + g.abs() * H, u_err + u.abs() * H, dmid.double()
+    a_err, slope_err = 1.2 * g1 + a.abs() * 2.0 ** -15, 1.2 * g1 + slope.abs() * 2.0 ** -15
+    if act == "relu":
+        slope_err = (g.abs() <= g1).double()
+    du, dg = d * a, d * u * slope
+    du_err = d.abs() * a_err
+    dg_err = d.abs() * (u1 * slope.abs() + (u.abs() + u1) * slope_err)
+    du_err, dg_err = du_err + (du.abs() + du_err) * H, dg_err + (dg.abs() + dg_err) * H
+    xd, wgd, wud = (t.detach().double() for t in (x, wg, wu))
+    one, two = product(dg, dg_err, wgd), product(du, du_err, wud)
+    for name, t, (ref, slack) in (("x", got[0], (one[0] + two[0], one[1] + two[1])), ("gate", got[1], product(dg.t(), dg_err.t(), xd)), ("up", got[2], product(du.t(), du_err.t(), xd))):
+        near(t, ref, slack, name)
 
 
 def test_shapes_around_the_rows(F):
