@@ -77,7 +77,7 @@ SIGNATURES = {
     "ezl_rotary": [_sidep, _sidep, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f32, _i32, _vp],
     "ezl_gated_fwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
     "ezl_gated_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
-    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "ezl_adamw8_list": [_i32, _adam8p, ctypes.POINTER(Adam8), _vp, _vp],
     "ezl_moments8_list": [_i32, _adam8p, _vpp, _vpp, _vp],
     "ezl_ids_in_range": [_vp, _i64, _i64, _vp, _vp],

@@ -17,7 +17,7 @@ __device__ __forceinline__ void gate_value_slope(float x, float& y, float& slope
     if constexpr (ACT == EZL_GATE_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
         y = x * s;
-        slope = s * (1.0f + x * (1.0f - s));
+        slope = fmaf(y, 1.0f - s, s);
     } else if constexpr (ACT == EZL_GATE_GELU) {
         float d;
         const float c = normal_cdf(x, d);

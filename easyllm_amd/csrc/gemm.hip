@@ -493,7 +493,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
     // newer than the A tile that is waited for: the B tile behind the next, and where an item begins the stores of the one before (a count
     // holds at most 63)
     typedef std::integral_constant<int, NB> ahead;
-    constexpr int STORES = kPairs<EPI> ? TM * 2 : TM * 8 * (int)sizeof(OutT) / 4;  // (the least there are: a gated product that keeps its parts has three times those)
+    constexpr int STORES = kPairs<EPI> ? TM * 2 : TM * 8 * (int)sizeof(OutT) / 4;  // (of a gated product: the least; its parts are more of them, waited for here at no cost that shows)
     typedef std::integral_constant<int, NB + STORES <= 63 ? NB + STORES : 63> ahead_and_stores;
     auto flip = [&]() {
         const int x = a0, y = b0;

@@ -516,27 +516,27 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
             for (int b = 0; b < NB / 2; ++b) {
                 const f32x4 ga = from_agprs<TM * TN>(acc[i][4 * b]), ua = from_agprs<TM * TN>(acc[i][4 * b + 1]);
                 const f32x4 gb = from_agprs<TM * TN>(acc[i][4 * b + 2]), ub = from_agprs<TM * TN>(acc[i][4 * b + 3]);
-                const auto out = [&](const f32x4& a, const f32x4& c, __amdgpu_buffer_rsrc_t to, int64_t ld) {
-                    float v[8];
+                float gate[8], up[8], y[8];
+                const auto eight = [](const f32x4& a, const f32x4& c, float (&v)[8]) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[r]), __float_as_uint(c[r]), false, false);
                         v[r] = __uint_as_float(sw[0]);
                         v[4 + r] = __uint_as_float(sw[1]);
                     }
+                };
+                eight(ga, gb, gate);
+                eight(ua, ub, up);
+                const auto out = [&](const float (&v)[8], __amdgpu_buffer_rsrc_t to, int64_t ld) {
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(v)), to, offset(i, b, ld), 0, 0);
                 };
                 if (keep) {
-                    out(ga, gb, gbuf, e.ld);
-                    out(ua, ub, ubuf, e.ld);
+                    out(gate, gbuf, e.ld);
+                    out(up, ubuf, e.ld);
                 }
-                f32x4 ya, yb;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    ya[r] = gate_value<ACT>(ga[r]) * ua[r];
-                    yb[r] = gate_value<ACT>(gb[r]) * ub[r];
-                }
-                out(ya, yb, cbuf, ldc);
+                for (int r = 0; r < 8; ++r) y[r] = gate_value<ACT>(gate[r]) * up[r];
+                out(y, cbuf, ldc);
                 if constexpr (TM * TN >= 48) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
@@ -579,20 +579,21 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
         off[jp] = (col < nrem ? (uint32_t)col * 2 : kOut) + (uint32_t)(row0 + (lane & 15)) * (uint32_t)(e.ld * 2);
     }
     const uint32_t row_step = (uint32_t)(32 * e.ld);
-    u32x4 old_g[2][TN / 2], old_u[2][TN / 2];
-    const auto fetch = [&](int i) {
-#pragma unroll
-        for (int jp = 0; jp < TN / 2; ++jp) {
-            old_g[i & 1][jp] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gbuf, off[jp] + i * row_step, 0, 0));
-            old_u[i & 1][jp] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ubuf, off[jp] + i * row_step, 0, 0));
-        }
+    constexpr int PIECES = TM * (TN / 2), DEPTH = PIECES < 3 ? PIECES : 3;  // of 16 bytes a lane, row by row; on the way at a time
+    u32x4 old_g[DEPTH], old_u[DEPTH];
+    const auto fetch = [&](int q) {
+        const uint32_t at = off[q % (TN / 2)] + q / (TN / 2) * row_step;
+        old_g[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gbuf, at, 0, 0));
+        old_u[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ubuf, at, 0, 0));
     };
-    fetch(0);
+#pragma unroll
+    for (int q = 0; q < DEPTH - 1; ++q) fetch(q);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        if (i + 1 < TM) fetch(i + 1);
 #pragma unroll
         for (int jp = 0; jp < TN / 2; ++jp) {
+            const int q = i * (TN / 2) + jp;
+            if (q + DEPTH - 1 < PIECES) fetch(q + DEPTH - 1);
             const f32x4 va = from_agprs<TM * TN>(acc[i][2 * jp]), vb = from_agprs<TM * TN>(acc[i][2 * jp + 1]);
             float d[8], dg[8], du[8], mid[8];
 #pragma unroll
@@ -601,7 +602,7 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
                 d[r] = __uint_as_float(sw[0]);
                 d[4 + r] = __uint_as_float(sw[1]);
             }
-            const bf16x8 gate = __builtin_bit_cast(bf16x8, old_g[i & 1][jp]), up = __builtin_bit_cast(bf16x8, old_u[i & 1][jp]);
+            const bf16x8 gate = __builtin_bit_cast(bf16x8, old_g[q % DEPTH]), up = __builtin_bit_cast(bf16x8, old_u[q % DEPTH]);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 float y, slope;

@@ -436,7 +436,7 @@ class GatedLinearFunction(torch.autograd.Function):
     @first_order
     def backward(ctx, dmid):
         x, gate_weight, up_weight, gate, up = ctx.saved_tensors
-        dgate, dup = K.gate_bwd(ctx.act, dmid.reshape(gate.shape).contiguous(), gate, up)
+        dgate, dup, _ = K.gate_bwd(ctx.act, dmid.reshape(gate.shape).contiguous(), gate, up)
         return (*_gated_products_bwd(x, gate_weight, up_weight, dgate, dup, ctx.needs_input_grad), None, None)
 
 

@@ -318,13 +318,14 @@ def gated_bwd(act, dy2d, down_weight, gate, up, want_mid=False):
     return dgate, dup, mid
 
 
-def gate_bwd(act, d, gate, up):
-    """-> (d * up * act'(gate), d * act(gate))"""
+def gate_bwd(act, d, gate, up, want_mid=False):
+    """-> (d * up * act'(gate), d * act(gate), act(gate) * up or None)"""
     _ready((d, gate, up), "d gate up")
     _need(gate.shape == up.shape == d.shape, "gate_bwd shape mismatch")
     dgate, dup = torch.empty_like(gate), torch.empty_like(up)
-    _lib.call("ezl_gate_bwd", GATES[act], _p(d), _p(gate), _p(up), _p(dgate), _p(dup), gate.numel(), _stream())
-    return dgate, dup
+    mid = torch.empty_like(gate) if want_mid else None
+    _lib.call("ezl_gate_bwd", GATES[act], _p(d), _p(gate), _p(up), _p(dgate), _p(dup), _p(mid), gate.numel(), _stream())
+    return dgate, dup, mid
 
 
 # ------------------------------------------------------------------------------------- RoPE

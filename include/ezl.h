@@ -128,7 +128,7 @@ int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* u
 int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy,
                   int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream);
 /* The same from a d that is there, n values of each, n % 8 == 0 (dgate may be gate or d, dup up). */
-int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, int64_t n, void* stream);
+int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t n, void* stream);
 
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----
  * table: cos/sin fp32 [npos, half_dim], theta = (p / scale_factor) * inv_freq[j].
