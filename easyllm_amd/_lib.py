@@ -37,6 +37,11 @@ class Epilogue(ctypes.Structure):
     _fields_ = [("bias", _vp), ("residual", _vp), ("pre", _vp), ("ldr", _i64), ("ldp", _i64), ("act", _i32)]
 
 
+class GatedMLP(ctypes.Structure):
+    """struct ezl_gated_mlp"""
+    _fields_ = [(n, _i64) for n in ("M", "h", "f", "n")] + [(n, _vp) for n in ("gate", "up", "down")] + [("ldw", _i64), ("ldd", _i64), ("act", _i32)]
+
+
 class RotarySide(ctypes.Structure):
     """struct ezl_rotary_side"""
     _fields_ = [("x", _vp), ("out", _vp), ("heads", _i64), ("seq_stride", _i64), ("batch_stride", _i64), ("head_stride", _i64)]
@@ -53,6 +58,7 @@ class Adam8(ctypes.Structure):
 
 
 _layerp = ctypes.POINTER(Layer)
+_mlpp = ctypes.POINTER(GatedMLP)
 _sidep = ctypes.POINTER(RotarySide)
 _adam8p = ctypes.POINTER(Adam8Tensor)
 _dropp = ctypes.POINTER(Dropout)
@@ -78,6 +84,8 @@ SIGNATURES = {
     "ezl_gated_fwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
     "ezl_gated_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
     "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gated_mlp_fwd": [_mlpp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gated_mlp_bwd": [_mlpp, _vp, _i64, _vp, _vp, _vp, _vp, _gradp, _gradp, _gradp, _vp, _i64, _vp],
     "ezl_adamw8_list": [_i32, _adam8p, ctypes.POINTER(Adam8), _vp, _vp],
     "ezl_moments8_list": [_i32, _adam8p, _vpp, _vpp, _vp],
     "ezl_ids_in_range": [_vp, _i64, _i64, _vp, _vp],
@@ -135,6 +143,7 @@ _SPECIAL = {
     "ezl_attn_plan": ([_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64], _i32),
     "ezl_gemm_workspace_bytes": ([_i64, _i64, _i64], _i64),
     "ezl_gated_workspace_bytes": ([_i64, _i64, _i64], _i64),
+    "ezl_gated_mlp_bytes": ([_mlpp, _i32], _i64),
     "ezl_gemm_group_workspace_bytes": ([_i32, _i64p, _i64p, _i64], _i64),
     "ezl_gemm_group_form_workspace_bytes": ([_i32, _i32, _i64p, _i64p, _i64], _i64),
     "ezl_gemm_searches": ([], _i64),
@@ -226,6 +235,11 @@ def gemm_workspace_bytes(M, N, K):
 @functools.lru_cache(maxsize=1024)
 def gated_workspace_bytes(M, f, K):
     return load().ezl_gated_workspace_bytes(M, f, K)
+
+
+@functools.lru_cache(maxsize=1024)
+def gated_mlp_bytes(M, h, f, n, backward):
+    return load().ezl_gated_mlp_bytes(GatedMLP(M, h, f, n), 1 if backward else 0)
 
 
 @functools.lru_cache(maxsize=1024)

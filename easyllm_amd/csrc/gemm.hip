@@ -31,6 +31,7 @@
 #include "gemm_tile.h"
 #include "gemm_list.h"
 #include "gemm_rows.h"
+#include "gated_rows.h"
 #include "../../include/ezl.h"
 
 #include <math.h>
@@ -1237,6 +1238,11 @@ extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, co
     EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
     if (const int rc = check_operands(x, gate_weight, M, f, K, ldx, ldw, f, 1, 1)) return rc;
     EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    if (stream_pairs_pay(M, K)) {
+        stream_rows_launch(x, gate_weight, up_weight, out, gate, up, (int)M, (int)f, (int)K, ldx, ldw, act, (hipStream_t)stream);
+        EZL_LAUNCH_CHECK(name);
+        return EZL_OK;
+    }
     launch_gate<GateForward>(x, gate_weight, out, (int)M, (int)f, (int)K, ldx, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
                              {(const bf16_t*)up_weight, (bf16_t*)gate, (bf16_t*)up, f, act});
     EZL_LAUNCH_CHECK(name);

@@ -448,8 +448,7 @@ class GatedMLPFunction(torch.autograd.Function):
     def forward(ctx, x, gate_weight, up_weight, down_weight, act, training):
         x2d = x.reshape(-1, x.shape[-1])
         keep = training and any(ctx.needs_input_grad[:4])
-        mid, gate, up = K.gated_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), keep)
-        y = K.linear_fwd(mid, down_weight)
+        y, gate, up = K.gated_mlp_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), down_weight, keep)
         ctx.act = act
         ctx.save_for_backward(x, gate_weight, up_weight, down_weight, gate, up)
         return y.view(*x.shape[:-1], y.shape[1])
@@ -459,16 +458,16 @@ class GatedMLPFunction(torch.autograd.Function):
     def backward(ctx, dy):
         x, gate_weight, up_weight, down_weight, gate, up = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dy2d = dy.reshape(-1, dy.shape[-1])
-        if not dy2d.is_contiguous():
-            dy2d = dy2d.contiguous()
-        dgate, dup, mid = K.gated_bwd(ctx.act, dy2d, down_weight, gate, up, need[3])
-        dw = None
-        if need[3]:
-            mg, acc = _main_grad_target(down_weight)
-            dw = K.linear_wgrad(dy2d, mid, out=mg, accumulate=acc)
-            dw = dw if mg is None else None
-        return (*_gated_products_bwd(x, gate_weight, up_weight, dgate, dup, need), dw, None, None)
+        targets, grads = [None] * 3, [None] * 3
+        for i in (2, 0, 1):  # (the order in which they are written)
+            if need[1 + i]:
+                weight = (gate_weight, up_weight, down_weight)[i]
+                mg, acc = _main_grad_target(weight)
+                if mg is None:
+                    grads[i] = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+                targets[i] = mg, grads[i], acc
+        dx = K.gated_mlp_bwd(ctx.act, dy.reshape(-1, dy.shape[-1]).contiguous(), x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight, gate, up, need[0], targets)
+        return (None if dx is None else dx.view(x.shape), *grads, None, None)
 
 
 def _check_gate(activation):

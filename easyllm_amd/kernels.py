@@ -168,13 +168,13 @@ def prepared_draw(threshold, draw):
     return c
 
 
-def _grad_target(target, n, what):
+def _grad_target(target, n, what, shape=None):
     """(f32 or None, bf16 or None, accumulate) -> C form; itself where it has that form; None: no gradient wanted"""
     if target is None or type(target) is _lib.LayerGrad:
         return target
     f32, bf16, accumulate = target
     if f32 is None:
-        _need(bf16.dtype is BF16 and bf16.shape == (n,) and bf16.is_contiguous(), "bad gradient of the " + what)
+        _need(bf16.dtype is BF16 and bf16.shape == (shape or (n,)) and bf16.is_contiguous(), "bad gradient of the " + what)
         _here(bf16, "the gradient of the " + what)
         return _lib.LayerGrad(None, bf16.data_ptr(), 0)
     _need(f32.dtype is torch.float32 and f32.is_contiguous() and f32.numel() == n, "bad main_grad of the " + what)
@@ -303,19 +303,45 @@ def gated_fwd(act, x2d, gate_weight, up_weight, keep=False):
     return out, gate, up
 
 
-def gated_bwd(act, dy2d, down_weight, gate, up, want_mid=False):
-    """with d = dy2d @ down_weight -> (d * up * act'(gate), d * act(gate), act(gate) * up or None)"""
-    lddy, ldw = _rows_ld(dy2d, "dy"), _rows_ld(down_weight, "down weight")
-    (T, n_out), f = dy2d.shape, down_weight.shape[1]
-    _ready((gate, up), "gate up")
-    _here(dy2d, "dy"); _here(down_weight, "down weight")
-    _need(down_weight.shape[0] == n_out and gate.shape == up.shape == (T, f), "gated_bwd: shape mismatch")
-    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
-    mid = torch.empty_like(gate) if want_mid else None
-    ws, nbytes = _gemm_workspace(T, f, n_out, dy2d.device)
-    _lib.call("ezl_gated_bwd", GATES[act], dy2d.data_ptr(), down_weight.data_ptr(), gate.data_ptr(), up.data_ptr(), dgate.data_ptr(), dup.data_ptr(), _p(mid), T, f, n_out, lddy, ldw,
-              _p(ws), nbytes, _stream())
-    return dgate, dup, mid
+def _gated_mlp(act, x2d, gate_weight, up_weight, down_weight):
+    """(the C form of a block, x's row stride)"""
+    ldx, ldw, ldd = _rows_ld(x2d, "x"), _rows_ld(gate_weight, "gate weight"), _rows_ld(down_weight, "down weight")
+    (T, h), (f, w_in), (n, d_in) = x2d.shape, gate_weight.shape, down_weight.shape
+    _need(up_weight.shape == gate_weight.shape and _rows_ld(up_weight, "up weight") == ldw, "gated_mlp: the first two weights must be alike")
+    if not (h == w_in and f == d_in and h > 0 and f > 0 and n > 0 and f % 8 == 0 and n % 8 == 0):
+        raise ValueError("gated_mlp: inner dimensions differ or are empty, or a width is no multiple of 8")
+    device = torch._C._cuda_getDevice()
+    for t, name in ((x2d, "x"), (gate_weight, "gate weight"), (up_weight, "up weight"), (down_weight, "down weight")):
+        if t.get_device() != device:
+            raise ValueError("%s is not on the current GPU" % name)
+    return _lib.GatedMLP(T, h, f, n, gate_weight.data_ptr(), up_weight.data_ptr(), down_weight.data_ptr(), ldw, ldd, GATES[act]), ldx
+
+
+def gated_mlp_fwd(act, x2d, gate_weight, up_weight, down_weight, keep=False):
+    """-> (y, and with `keep` x2d @ gate_weight^T and x2d @ up_weight^T, else None, None)"""
+    mlp, ldx = _gated_mlp(act, x2d, gate_weight, up_weight, down_weight)
+    new, device = torch.empty, x2d.device
+    y = new((mlp.M, mlp.n), dtype=BF16, device=device)
+    gate = up = None
+    if keep:
+        gate, up = new((mlp.M, mlp.f), dtype=BF16, device=device), new((mlp.M, mlp.f), dtype=BF16, device=device)
+    nbytes = _lib.gated_mlp_bytes(mlp.M, mlp.h, mlp.f, mlp.n, False)
+    temp = new(nbytes, dtype=torch.uint8, device=device)
+    _lib.call("ezl_gated_mlp_fwd", mlp, x2d.data_ptr(), ldx, y.data_ptr(), _p(gate), _p(up), temp.data_ptr(), nbytes, _stream())
+    return y, gate, up
+
+
+def gated_mlp_bwd(act, dy2d, x2d, gate_weight, up_weight, down_weight, gate, up, want_dx, grads):
+    """-> dx or None; the weights' gradients go to grads = (gate's, up's, down's), each (f32 or None, bf16 or None, accumulate), contiguous, or None, in the order down, gate, up."""
+    mlp, ldx = _gated_mlp(act, x2d, gate_weight, up_weight, down_weight)
+    _ready((dy2d, gate, up), "dy gate up")
+    _need(dy2d.shape == (mlp.M, mlp.n) and gate.shape == up.shape == (mlp.M, mlp.f), "gated_mlp_bwd: shape mismatch")
+    targets = [_grad_target(g, w.numel(), what, shape=w.shape) for g, w, what in zip(grads, (gate_weight, up_weight, down_weight), ("gate weight", "up weight", "down weight"))]
+    dx = torch.empty((mlp.M, mlp.h), dtype=BF16, device=x2d.device) if want_dx else None
+    nbytes = _lib.gated_mlp_bytes(mlp.M, mlp.h, mlp.f, mlp.n, True)
+    temp = torch.empty(nbytes, dtype=torch.uint8, device=x2d.device)
+    _lib.call("ezl_gated_mlp_bwd", mlp, x2d.data_ptr(), ldx, dy2d.data_ptr(), gate.data_ptr(), up.data_ptr(), _p(dx), *targets, temp.data_ptr(), nbytes, _stream())
+    return dx
 
 
 def gate_bwd(act, d, gate, up, want_mid=False):

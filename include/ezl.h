@@ -130,6 +130,21 @@ int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* 
 /* The same from a d that is there, n values of each, n % 8 == 0 (dgate may be gate or d, dup up). */
 int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t n, void* stream);
 
+/* The whole block, y = (act(x gate^T) * (x up^T)) down^T, forward or backward in one call: x [M, h] (rows ldx apart), gate and up [f, h] (rows ldw apart), down [n, f] (rows ldd apart),
+ * y and dy [M, n], contiguous.  gate_out and up_out [M, f], both or neither: what the backward call reads.  Of the gradients of the weights (contiguous; HOST pointers, NULL: not wanted) down's
+ * is written first, then gate's, then up's: accumulate flags hold for that order.  dx [M, h], contiguous, or NULL.  temp: ezl_gated_mlp_bytes(.., backward) bytes, 256-byte aligned
+ * best, 16 at least; free again when the call's work is done. */
+typedef struct {
+    int64_t M, h, f, n;
+    const void *gate, *up, *down;
+    int64_t ldw, ldd;
+    int act;
+} ezl_gated_mlp; /* HOST struct */
+int64_t ezl_gated_mlp_bytes(const ezl_gated_mlp* mlp, int backward);
+int ezl_gated_mlp_fwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, void* y, void* gate_out, void* up_out, void* temp, int64_t temp_bytes, void* stream);
+int ezl_gated_mlp_bwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, const void* dy, const void* gate_out, const void* up_out, void* dx, const ezl_layer_grad* dgate,
+                      const ezl_layer_grad* dup, const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream);
+
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----
  * table: cos/sin fp32 [npos, half_dim], theta = (p / scale_factor) * inv_freq[j].
  * apply: x/out bf16 [s*b rows (s-major), nheads, d] with row strides in elements (out may alias x);
