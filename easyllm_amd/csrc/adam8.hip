@@ -315,6 +315,7 @@ extern "C" int ezl_adamw8_list(int count, const ezl_adam8_tensor* tensors, const
         l.g[s] = (const float*)t.grad; l.param[s] = (bf16_t*)t.param_bf16; l.n[s] = t.n; l.number[s] = t.number; l.first[s] = l.chunks;
         l.chunks += (int)chunks;
     }
+    if (l.count == 0) return EZL_OK;  // (the last one ends a list that is not empty)
     flush();
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;
@@ -346,6 +347,7 @@ extern "C" int ezl_moments8_list(int count, const ezl_adam8_tensor* tensors, voi
         l.m_out[s] = (bf16_t*)exp_avg_bf16[i]; l.v_out[s] = (bf16_t*)exp_avg_sq_bf16[i]; l.n[s] = t.n; l.first[s] = l.chunks;
         l.chunks += (int)chunks;
     }
+    if (l.count == 0) return EZL_OK;  // (the last one ends a list that is not empty)
     flush();
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;

@@ -484,6 +484,9 @@ def gated_linear(x, gate_weight, up_weight, activation="silu"):
 def gated_mlp(x, gate_weight, up_weight, down_weight, activation="silu"):
     """gated_linear(x, gate_weight, up_weight, activation) down^T; down [h', f].  Of the tensors between x and the result the backward pass keeps two, x gate^T and x up^T."""
     _check_gate(activation)
+    if not (torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad or down_weight.requires_grad)):
+        y, _, _ = K.gated_mlp_fwd(activation, x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight)
+        return y.view(*x.shape[:-1], y.shape[1])
     return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation, torch.is_grad_enabled())
 
 
@@ -564,6 +567,8 @@ def rotary_embed(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0
     the sequence) have no limit that a table would set."""
     if inv_freq.requires_grad:
         raise ValueError("rotary_embed: frequencies are not learnt")
+    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):  # (a node costs the host 4 us, as much as a token's launch)
+        return K.rotary(_rotary_rows(q), _rotary_rows(k), inv_freq, position_ids, interleaved, float(scale))
     return RotaryEmbedFunction.apply(q, k, inv_freq, position_ids, bool(interleaved), float(scale))
 
 

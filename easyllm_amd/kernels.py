@@ -413,43 +413,46 @@ def rope_apply_pair(q, k, cos, sin, position_ids=None, backward=False):
     return qo, ko
 
 
-def _rotary_side(x, out):
-    s, b, heads, d = x.shape
-    st = x.stride()
-    return _lib.RotarySide(x.data_ptr(), out.data_ptr(), heads, st[0], st[1], st[2])
-
-
 def rotary_in_place_ok(x):
     """Whether the kernel reads x [s, b, heads, d] where it lies: rows of whole 16 bytes, each on its own strides."""
-    st = x.stride()
-    return st[3] == 1 and st[0] % 8 == 0 and st[1] % 8 == 0 and st[2] % 8 == 0 and x.data_ptr() % 16 == 0
+    seq, batch, head, one = x.stride()
+    return one == 1 and (seq | batch | head) % 8 == 0 and x.data_ptr() % 16 == 0
+
+
+def _rotary_side(x, name, device, out_of):
+    if not (x.dtype is BF16 and x.dim() == 4 and x.get_device() == device):
+        raise ValueError("%s must be a bf16 [s, b, heads, d] tensor on the current GPU" % name)
+    seq, batch, head, one = x.stride()
+    if one != 1 or (seq | batch | head) % 8:
+        raise ValueError("rotary: strides must be multiples of 8, the last 1")
+    out_of.append(torch.empty_like(x, memory_format=torch.contiguous_format))
+    return _lib.RotarySide(x.data_ptr(), out_of[-1].data_ptr(), x.shape[2], seq, batch, head)
 
 
 def rotary(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0, backward=False):
     """q [s, b, nq, d], k [s, b, nk, d] or None -> both turned (contiguous), k None where it is."""
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None:
-            continue
-        if not (t.dtype is BF16 and t.is_cuda and t.dim() == 4):
-            raise ValueError("%s must be a bf16 [s, b, heads, d] GPU tensor" % name)
-        _here(t, name)
-        _need(rotary_in_place_ok(t), "rotary: strides must be multiples of 8, the last 1")
+    device, outs = torch._C._cuda_getDevice(), []
+    q_side = _rotary_side(q, "q", device, outs)
     s, b, _, d = q.shape
-    _need(k is None or (k.shape[0] == s and k.shape[1] == b and k.shape[3] == d), "rotary: q / k shapes differ")
-    _need(inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.is_cuda,
-          "inv_freq must be a contiguous fp32 or fp64 [turned / 2] GPU tensor")
-    _here(inv_freq, "inv_freq")
-    _need(0 < 2 * inv_freq.numel() <= d and d % 8 == 0, "rotary: a frequency for each pair of the head's elements, at most half of them; the head's width a multiple of 8")
-    pos = (0, 0)
+    k_side = None
+    if k is not None:
+        k_side = _rotary_side(k, "k", device, outs)
+        if k.shape[0] != s or k.shape[1] != b or k.shape[3] != d:
+            raise ValueError("rotary: q / k shapes differ")
+    f64 = inv_freq.dtype is torch.float64
+    if not ((f64 or inv_freq.dtype is torch.float32) and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.get_device() == device):
+        raise ValueError("inv_freq must be a contiguous fp32 or fp64 [turned / 2] tensor on the current GPU")
+    turned = 2 * inv_freq.shape[0]
+    if not (0 < turned <= d and d % 8 == 0):
+        raise ValueError("rotary: a frequency for each pair of the head's elements, at most half of them; the head's width a multiple of 8")
+    pos_batch = pos_seq = 0
     if position_ids is not None:
-        _need(position_ids.is_cuda and position_ids.dtype is torch.int64 and tuple(position_ids.shape) == (b, s), "position_ids must be int64 [b, s]")
-        _here(position_ids, "position_ids")
-        pos = position_ids.stride()
-    q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=BF16, device=k.device)
-    _lib.call("ezl_rotary", _rotary_side(q, q_out), None if k is None else _rotary_side(k, k_out), inv_freq.data_ptr(), 1 if inv_freq.dtype is torch.float64 else 0,
-              _p(position_ids), pos[1], pos[0], s, b, d, 2 * inv_freq.numel(), 1 if interleaved else 0, float(scale), 1 if backward else 0, _stream())
-    return q_out, k_out
+        if not (position_ids.dtype is torch.int64 and position_ids.get_device() == device and position_ids.shape == (b, s)):
+            raise ValueError("position_ids must be int64 [b, s] on the current GPU")
+        pos_batch, pos_seq = position_ids.stride()
+    _lib.call("ezl_rotary", q_side, k_side, inv_freq.data_ptr(), 1 if f64 else 0, None if position_ids is None else position_ids.data_ptr(), pos_seq, pos_batch, s, b, d, turned,
+              1 if interleaved else 0, scale, 1 if backward else 0, _stream())
+    return outs[0], (None if k is None else outs[1])
 
 
 def ids_in_range_flag(ids, limit, host_flag=None):
@@ -1057,17 +1060,19 @@ def adamw_list(masters, exp_avgs, exp_avg_sqs, grads, params, lr, beta1, beta2, 
               1 if bias_correction else 0, _p(norm_coef), _stream())
 
 
-_ADAM8_MOMENTS = "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"
-
-
 def _adam8_moments(st, device):
     """(the addresses of a state's codes and scales, number of values)"""
-    m, v, ms, vs = ts = st["exp_avg"], st["exp_avg_sq"], st["exp_avg_scale"], st["exp_avg_sq_scale"]
+    m, v, ms, vs = st["exp_avg"], st["exp_avg_sq"], st["exp_avg_scale"], st["exp_avg_sq_scale"]
     n = m.numel()
     blocks = (n + 255) // 256
-    for t, length in zip(ts, (n, n, blocks, blocks)):
-        if not (t.dtype is torch.uint8 and t.get_device() == device and t.numel() == length and t.is_contiguous()):
-            raise ValueError("%s must be a contiguous uint8 tensor of %d values on the current GPU" % (_ADAM8_MOMENTS[[u is t for u in ts].index(True)], length))
+    u8 = torch.uint8
+    if not (m.dtype is u8 and v.dtype is u8 and ms.dtype is u8 and vs.dtype is u8 and v.numel() == n and ms.numel() == blocks and vs.numel() == blocks
+            and m.get_device() == v.get_device() == ms.get_device() == vs.get_device() == device
+            and m.is_contiguous() and v.is_contiguous() and ms.is_contiguous() and vs.is_contiguous()):
+        for name, length in (("exp_avg", n), ("exp_avg_sq", n), ("exp_avg_scale", blocks), ("exp_avg_sq_scale", blocks)):
+            t = st[name]
+            if not (t.dtype is u8 and t.get_device() == device and t.numel() == length and t.is_contiguous()):
+                raise ValueError("%s must be a contiguous uint8 tensor of %d values on the current GPU" % (name, length))
     return (m.data_ptr(), v.data_ptr(), ms.data_ptr(), vs.data_ptr()), n
 
 
@@ -1103,10 +1108,10 @@ def moments8_list(states):
     outs = []
     for i, st in enumerate(states):
         moments, n = _adam8_moments(st, device)
-        _need(st["master"].numel() == n, "moments8_list: size mismatch")
+        master = st["master"]
+        _need(master.numel() == n and master.is_contiguous(), "moments8_list: the master weights' shape is not the moments'")
         tensors[i] = (None, *moments, None, None, n, 0)
-        shape = st["master"].shape
-        outs.append((torch.empty(shape, dtype=BF16, device=st["exp_avg"].device), torch.empty(shape, dtype=BF16, device=st["exp_avg"].device)))
+        outs.append((torch.empty_like(master, dtype=BF16), torch.empty_like(master, dtype=BF16)))
     _lib.call("ezl_moments8_list", len(states), tensors, _pointers([m for m, _ in outs]), _pointers([v for _, v in outs]), _stream())
     return outs
 

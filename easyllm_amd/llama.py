@@ -120,6 +120,9 @@ class LlamaModelPipe(torch.nn.Module):
                 self.forward_funcs.append(spec)
             else:
                 self.forward_funcs.append(spec)
+        layers = [f for f in self.forward_funcs if isinstance(f, ParallelTransformerLayerPipe)]
+        if layers and all(f.self_attn.rotary_emb.general for f in layers):
+            self.forward_funcs[1].positions_in_tables = False
 
     # ---- dynamic checkpoint rule ------------------------------------------------------------
     def _is_checkpointable(self, funcs):

@@ -46,10 +46,13 @@ class FusedAdam:
     """apex.optimizers.FusedAdam's constructor surface (AdamW mode) over bf16 weights with fp32 master copies.
 
     Gradients are read from `param.main_grad` (fp32).  `step(clip_grad=c)` clips by the global L2 norm first when
-    c > 0 and returns the device tensor (norm, coefficient)."""
+    c > 0 and returns the device tensor (norm, coefficient).
+
+    state_bits 8 (of a group, or of all): moments in 8 bits (`adamw_8bit_step`) for parameters of min_8bit_size elements and more, norms and biases stay in 32.  Their random rounding
+    follows from `seed`, the step and the parameter's place in the list, so a run that goes on from a copy of `state` and of the groups' "step" makes the same bits."""
 
     def __init__(self, params, lr=1e-3, bias_correction=True, betas=(0.9, 0.999), eps=1e-8, adam_w_mode=True,
-                 weight_decay=0.0, amsgrad=False, set_grad_none=True):
+                 weight_decay=0.0, amsgrad=False, set_grad_none=True, state_bits=32, min_8bit_size=4096, seed=0):
         if amsgrad:
             raise RuntimeError("FusedAdam does not support the AMSGrad variant.")  # apex raises the same
         if not adam_w_mode:
@@ -57,19 +60,27 @@ class FusedAdam:
         params = list(params)
         if params and not isinstance(params[0], dict):
             params = [{"params": params}]
-        self.defaults = dict(lr=lr, bias_correction=bias_correction, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
+        self.defaults = dict(lr=lr, bias_correction=bias_correction, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits)
+        self.seed = int(seed)
         self.param_groups = []
         for g in params:
             group = dict(self.defaults)
             group.update(g)
             group["params"] = [p for p in group["params"] if p.requires_grad]
             group["step"] = 0
+            if group["state_bits"] not in (8, 32):
+                raise ValueError("state_bits must be 8 or 32, got %r" % (group["state_bits"],))
             self.param_groups.append(group)
         self.state = {}
+        number = -1
         for group in self.param_groups:
             for p in group["params"]:
+                number += 1
                 if getattr(p, "main_grad", None) is None:
                     raise ValueError("every optimised parameter needs an fp32 main_grad buffer (runner.attach_main_grads)")
+                if group["state_bits"] == 8 and p.numel() >= min_8bit_size:
+                    self.state[p] = new_8bit_state(p, number)
+                    continue
                 self.state[p] = {"master": p.detach().float().contiguous(), "exp_avg": torch.zeros_like(p, dtype=torch.float32),
                                  "exp_avg_sq": torch.zeros_like(p, dtype=torch.float32)}
         n = sum(len(g["params"]) for g in self.param_groups)
@@ -96,14 +107,24 @@ class FusedAdam:
                 continue
             group["step"] += 1
             b1, b2 = group["betas"]
-            states = [self.state[p] for p in group["params"]]
-            K.adamw_list([st["master"] for st in states], [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states],
-                         [p.main_grad for p in group["params"]], [p.data if p.dtype == torch.bfloat16 else None for p in group["params"]],
-                         group["lr"], b1, b2, group["eps"], group["weight_decay"], group["step"], group["bias_correction"], norm_coef)
-            for p, st in zip(group["params"], states):
+            pairs = [(p, self.state[p]) for p in group["params"]]
+            how = (group["lr"], b1, b2, group["eps"], group["weight_decay"], group["step"], group["bias_correction"], norm_coef)
+            wide, narrow = [(p, st) for p, st in pairs if "number" not in st], [(p, st) for p, st in pairs if "number" in st]
+            weight = lambda p: p.data if p.dtype == torch.bfloat16 else None  # noqa: E731
+            if wide:
+                K.adamw_list([st["master"] for _, st in wide], [st["exp_avg"] for _, st in wide], [st["exp_avg_sq"] for _, st in wide],
+                             [p.main_grad for p, _ in wide], [weight(p) for p, _ in wide], *how)
+            if narrow:
+                K.adamw8_list([st for _, st in narrow], [p.main_grad for p, _ in narrow], [weight(p) for p, _ in narrow], *how, self.seed)
+            for p, st in pairs:
                 if p.dtype != torch.bfloat16:
                     p.data.copy_(st["master"])
         return norm_coef
+
+    def moments(self, param):
+        """(exp_avg, exp_avg_sq) of a parameter as values of its shape: the fp32 tensors themselves, or what their 8 bits stand for, in bf16"""
+        state = self.state[param]
+        return moments_8bit([state])[0] if "number" in state else (state["exp_avg"], state["exp_avg_sq"])
 
     def refresh_fp32_params(self):
         """Re-reads the fp32 master copies from the model weights (called after a checkpoint was loaded into them)."""
@@ -141,12 +162,14 @@ def moments_8bit(states):
 
 
 def build_optimizer(cfg_optim, model, deepspeed=True):
-    """cfg_optim = {'type': 'FusedAdam', 'kwargs': {lr, weight_decay, betas, eps}} as in the reference's yaml `optimizer:`."""
+    """cfg_optim = {'type': 'FusedAdam', 'kwargs': {lr, weight_decay, betas, eps}} as in the reference's yaml `optimizer:`; 'AdamW8bit': moments of 8 bits."""
     if cfg_optim.get("cpu_optimizer", False):
         raise NotImplementedError("need to add cpu adam")  # same refusal as optimizer_helper.py:71-72
-    if cfg_optim["type"] not in ("FusedAdam", "AdamW"):
-        raise NotImplementedError("optimizer type %s is not built; FusedAdam / AdamW are" % cfg_optim["type"])
+    if cfg_optim["type"] not in ("FusedAdam", "AdamW", "AdamW8bit"):
+        raise NotImplementedError("optimizer type %s is not built; FusedAdam / AdamW / AdamW8bit are" % cfg_optim["type"])
     groups = filter_freeze_param_groups(list(get_params_for_weight_decay_optimization(model)))
     kwargs = dict(cfg_optim.get("kwargs", {}))
     kwargs.pop("params", None)
+    if cfg_optim["type"] == "AdamW8bit":
+        kwargs.setdefault("state_bits", 8)
     return FusedAdam(groups, **kwargs)

@@ -4,19 +4,85 @@
 `...self_attn.rotary_emb.inv_freq`).  The cos/sin cache is kept as fp32 half tables [S, d/2] -- the
 reference rounds its tables to bf16 when precision is bf16 (:33-35); keeping fp32 is closer to the
 exact rotation and is what the parity tests compare against.
+
+Not in the reference: `rotary_dim` (the part of a head that is turned), `interleaved` (pairs of neighbours instead of halves) and `scaling` (frequencies for
+contexts longer than those of pre-training).  Such positions have no tables: their angles are computed where they are used, in 64 bits, and position ids may
+lie anywhere.
 """
+import math
+
 import torch
 
 from . import functional as F_
 from . import kernels as K
 
 
+_SCALINGS = {"linear": ("factor",), "dynamic": ("factor", "original_length"), "yarn": ("factor", "original_length")}
+_SCALING_OPTIONS = {"linear": (), "dynamic": ("length",), "yarn": ("beta_fast", "beta_slow", "attention_factor")}
+
+
+def scaled_frequencies(inv_freq, base, scaling, length):
+    """(frequencies in fp64, what sines and cosines are multiplied by) of `inv_freq` [n] = base^(-j / n) under a scaling, a dict with a "type":
+
+    linear   all divided by "factor"
+    dynamic  a larger base for a text of `length` (or its own "length") tokens, where that is above "original_length": base ((factor length / original_length) - (factor - 1))^(n / (n - 1))
+    yarn     divided by "factor" where a wave turns less than "beta_slow" (1) times in "original_length", as they are where it turns more than "beta_fast" (32) times, in between by a
+             line over the index (Peng, Quesnelle, Fan, Shippole, "YaRN: efficient context window extension of large language models", 2023); "attention_factor"
+             (0.1 ln factor + 1)"""
+    inv_freq, n = inv_freq.double(), inv_freq.numel()
+    if scaling is None:
+        return inv_freq, 1.0
+    kind, factor = scaling["type"], float(scaling["factor"])
+    if kind == "linear":
+        return inv_freq / factor, 1.0
+    original = float(scaling["original_length"])
+    if kind == "dynamic":
+        length = scaling.get("length") or length
+        if length <= original or n == 1:
+            return inv_freq, 1.0
+        more = factor * length / original - (factor - 1)
+        j = torch.arange(n, dtype=torch.float64, device=inv_freq.device)
+        return inv_freq * more ** (-j / (n - 1)), 1.0
+
+    def index_of(turns):  # of the wave that turns so often in the original length
+        return n * math.log(original / (turns * 2 * math.pi)) / math.log(base)
+
+    low, high = max(math.floor(index_of(scaling.get("beta_fast", 32))), 0), min(math.ceil(index_of(scaling.get("beta_slow", 1))), 2 * n - 1)
+    j = torch.arange(n, dtype=torch.float64, device=inv_freq.device)
+    slow = ((j - low) / max(high - low, 1e-3)).clamp(0, 1)
+    attention_factor = scaling.get("attention_factor")
+    return inv_freq / factor * slow + inv_freq * (1 - slow), 0.1 * math.log(factor) + 1 if attention_factor is None else float(attention_factor)
+
+
+def _checked_scaling(scaling):
+    if scaling is None:
+        return None
+    kind = scaling.get("type")
+    if kind not in _SCALINGS:
+        raise NotImplementedError("scaling type %r: %s are built" % (kind, ", ".join(_SCALINGS)))
+    unknown = set(scaling) - {"type", *_SCALINGS[kind], *_SCALING_OPTIONS[kind]}
+    missing = set(_SCALINGS[kind]) - set(scaling)
+    if unknown or missing:
+        raise ValueError("scaling %r: %s" % (kind, "; ".join(["unknown %s" % n for n in sorted(unknown)] + ["%s is missing" % n for n in sorted(missing)])))
+    if not float(scaling["factor"]) >= 1 or ("original_length" in scaling and not scaling["original_length"] > 0):
+        raise ValueError("scaling: a factor of 1 or more, an original_length above 0")
+    return dict(scaling)
+
+
 class RotaryEmbedding(torch.nn.Module):
-    def __init__(self, dim, base=10000, precision=torch.half, scale_factor=1.0):
+    def __init__(self, dim, base=10000, precision=torch.half, scale_factor=1.0, rotary_dim=None, interleaved=False, scaling=None):
         super().__init__()
-        inv_freq = 1.0 / (base ** (torch.arange(0, dim, 2).float() / dim))
+        rotary_dim = dim if rotary_dim is None else rotary_dim
+        if not 0 < rotary_dim <= dim or rotary_dim % 2:
+            raise ValueError("rotary_dim must be even and at most the head's width, got %r of %r" % (rotary_dim, dim))
+        inv_freq = 1.0 / (base ** (torch.arange(0, rotary_dim, 2).float() / rotary_dim))
         self.register_buffer("inv_freq", inv_freq)
         self.dim = dim
+        self.base = base
+        self.interleaved = bool(interleaved)
+        self.scaling = _checked_scaling(scaling)
+        self.general = rotary_dim != dim or self.interleaved or self.scaling is not None  # (turned without tables, by rotate)
+        self._frequencies = None
         self.max_seq_len_cached = None
         self.cos_half = None
         self.sin_half = None
@@ -25,11 +91,38 @@ class RotaryEmbedding(torch.nn.Module):
 
     def tables(self, seq_len, device):
         """fp32 (cos, sin) half tables [>= seq_len, dim/2] on `device`, built by the HIP table kernel."""
+        if self.general:
+            raise NotImplementedError("a rotary_dim, interleaved pairs and scaled frequencies have no tables")
         if self.max_seq_len_cached is None or seq_len > self.max_seq_len_cached or self.cos_half.device != device:
             inv = self.inv_freq.to(device=device, dtype=torch.float32).contiguous()
             self.cos_half, self.sin_half = K.rope_table(inv, int(seq_len), self.scale_factor)
             self.max_seq_len_cached = int(seq_len)
         return self.cos_half, self.sin_half
+
+    def frequencies(self, seq_len, device):
+        """(fp64 [rotary_dim / 2] on `device`, the factor of sines and cosines) for a text of seq_len tokens"""
+        length = seq_len if self.scaling is not None and self.scaling["type"] == "dynamic" and not self.scaling.get("length") else None
+        if self._frequencies is None or self._frequencies[0] != (device, length):
+            inv_freq, factor = scaled_frequencies(self.inv_freq.to(device) / self.scale_factor, self.base, self.scaling, seq_len)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():  # (memory of the graph's, which nobody else may read later)
+                return inv_freq.contiguous(), factor
+            if device.type == "cuda":  # whatever stream reads them next, and whatever still reads the ones before
+                torch.cuda.synchronize(device)
+            self._frequencies = (device, length), inv_freq.contiguous(), factor
+        return self._frequencies[1:]
+
+    def _apply(self, fn, *args, **kwargs):
+        self._frequencies = None
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._frequencies = None
+
+    def rotate(self, q, k, position_ids=None):
+        """q [s, b, nq, d], k [s, b, nk, d] -> turned, whatever the options; position_ids int64 [b, s] or None (the place in the sequence)."""
+        inv_freq, factor = self.frequencies(q.shape[0], q.device)
+        return F_.rotary_embed(q, k, inv_freq, position_ids, interleaved=self.interleaved, scale=factor)
 
     def forward(self, x, seq_dim=1, seq_len=None):
         """Reference-shaped return value: (cos, sin) of shape [seq_len, 1, dim] in `precision`."""

@@ -12,6 +12,7 @@ to end (the attention kernels take token strides, so the reference's `s b ... ->
 :478/:491 do not exist); the residual add of :786 is fused into the RMSNorm that follows it; the
 SiLU and the product with `up` (:222) are one kernel.
 """
+import functools
 import math
 
 import torch
@@ -19,6 +20,7 @@ import torch
 from . import dist_env
 from . import functional as F_
 from .dropout import threshold_of
+from .kernels import GATES
 from .layers import (ColumnParallelLinear, MixedFusedLayerNorm, RMSNorm, RowParallelLinear, GLU_ACTIVATIONS, build_layer_norm,
                      get_initializer_from_cfg, get_torch_dtype)
 from .positional_embeddings import RotaryEmbedding, apply_rotary_pos_emb
@@ -115,15 +117,20 @@ class FlashAttention(torch.nn.Module):
 class ParallelMLP(torch.nn.Module):
     """down_proj(silu(gate_proj(x)) * up_proj(x)), or with glu_activation None down_proj(gelu(up_proj(x))), the products with their biases where
     mlp_bias is set and the activation in the first one's epilogue (exact; with the tanh where bias_gelu_fusion or use_openai_gelu ask for
-    it).  Returns (output, output_bias); with `residual`, which the plain form takes, the whole sum and None."""
+    it).  Returns (output, output_bias); with `residual`, which the plain form takes, the whole sum and None.  glu_fusion: the gated form with any of kernels.GATES for an
+    activation, as `functional.gated_mlp`, which keeps two tensors of the block's width for backward where the composed form keeps three."""
 
     def __init__(self, init_method, output_layer_init_method, hidden_size=1024, intermediate_size=4096,
                  use_cpu_initialization=False, params_dtype=torch.half, bias_gelu_fusion=False, glu_activation=None,
-                 use_openai_gelu=False, onnx_safe=False, sync_tp_duplicated_parameters=True, sequence_parallel=False, mlp_bias=False):
+                 use_openai_gelu=False, onnx_safe=False, sync_tp_duplicated_parameters=True, sequence_parallel=False, mlp_bias=False,
+                 glu_fusion=False):
         super().__init__()
         self.sequence_parallel = sequence_parallel
         self.glu = glu_activation is not None
-        if self.glu and glu_activation not in GLU_ACTIVATIONS:
+        self.fused_gate = glu_activation if glu_fusion else None
+        if glu_fusion and glu_activation not in GATES:
+            raise NotImplementedError("glu_fusion with glu_activation=%r: %s are built" % (glu_activation, ", ".join(GATES)))
+        if self.glu and not glu_fusion and glu_activation not in GLU_ACTIVATIONS:
             raise NotImplementedError("glu_activation=%r: the llama step uses 'silu' (default_cfg.py:163)" % (glu_activation,))
         if self.glu and mlp_bias:
             raise NotImplementedError("mlp_bias: the products of a gated MLP have no biases")
@@ -133,7 +140,7 @@ class ParallelMLP(torch.nn.Module):
         if self.glu:
             self.gate_proj = ColumnParallelLinear(hidden_size, intermediate_size, **common)
         self.up_proj = ColumnParallelLinear(hidden_size, intermediate_size, **common)
-        self.activation_func = GLU_ACTIVATIONS[glu_activation] if self.glu else None
+        self.activation_func = GLU_ACTIVATIONS[glu_activation] if self.glu and not glu_fusion else None
         self.activation = None if self.glu else "gelu_tanh" if bias_gelu_fusion or use_openai_gelu else "gelu"
         self.down_proj = RowParallelLinear(intermediate_size, hidden_size, input_is_parallel=True,
                                            init_method=output_layer_init_method, skip_bias_add=True, bias=mlp_bias,
@@ -145,6 +152,18 @@ class ParallelMLP(torch.nn.Module):
         """The activation as a pass of its own, PyTorch's: behind a hooked or replaced projection, whose result has to be seen without it."""
         x = x if bias is None else F_.bias_add(x, bias)
         return torch.nn.functional.gelu(x, approximate="tanh" if self.activation == "gelu_tanh" else "none")
+
+    def _fused(self, hidden_states):
+        if are_plain(((self.gate_proj, ColumnParallelLinear), (self.up_proj, ColumnParallelLinear))):
+            weights = self.gate_proj.weight, self.up_proj.weight
+            if is_plain(self.down_proj, RowParallelLinear):
+                return F_.gated_mlp(hidden_states, *weights, self.down_proj.weight, self.fused_gate), None
+            return self.down_proj(F_.gated_linear(hidden_states, *weights, self.fused_gate))
+        # a hooked or replaced projection's result has to be seen: the activation is a pass of its own, PyTorch's
+        gate, up = self.gate_proj(hidden_states)[0], self.up_proj(hidden_states)[0]
+        f = torch.nn.functional
+        act = {"silu": f.silu, "relu": f.relu, "gelu": f.gelu, "gelu_tanh": functools.partial(f.gelu, approximate="tanh")}[self.fused_gate]
+        return self.down_proj(act(gate) * up)
 
     def forward(self, hidden_states, residual=None):
         if not self.glu:
@@ -160,6 +179,8 @@ class ParallelMLP(torch.nn.Module):
             return F_.dropout_add(output, residual, bias), None
         if residual is not None:
             raise ValueError("a gated MLP leaves the residual sum to the layer")
+        if self.fused_gate is not None:
+            return self._fused(hidden_states)
         if are_plain(((self.gate_proj, ColumnParallelLinear), (self.up_proj, ColumnParallelLinear))):
             # gate_proj and up_proj share their input: one fan-out op (input gradient accumulated in the GEMM)
             h1, h2 = F_.fan_out_linear(hidden_states, self.gate_proj.weight, self.up_proj.weight)
@@ -266,8 +287,11 @@ class ParallelAttention(torch.nn.Module):
         q = query_layer.view(sq, bs, nq, d) if not self.qkv_pack else query_layer.unflatten(-1, (nq, d))
         k = key_layer.view(sq, bs, nk, d) if not self.qkv_pack else key_layer.unflatten(-1, (nk, d))
         v = value_layer.view(sq, bs, nk, d) if not self.qkv_pack else value_layer.unflatten(-1, (nk, d))
-        cos, sin = self.rotary_emb.tables(sq, q.device)
-        q, k = apply_rotary_pos_emb(q, k, cos, sin, position_ids)
+        if getattr(self.rotary_emb, "general", False):
+            q, k = self.rotary_emb.rotate(q, k, position_ids)
+        else:
+            cos, sin = self.rotary_emb.tables(sq, q.device)
+            q, k = apply_rotary_pos_emb(q, k, cos, sin, position_ids)
         if attention_mask is None or cu_seqlens is not None:  # :480-488: document boundaries replace the padding mask
             qk_mask = None
         elif attention_mask.dim() == 2:
@@ -292,7 +316,7 @@ class ParallelTransformerLayer(torch.nn.Module):
                  onnx_safe=None, sync_tp_duplicated_parameters=False, hidden_dropout=0, bias_dropout_fusion=False,
                  intermediate_size=4096, seq_length=1024, micro_batch_size=1, sequence_parallel=False, use_flash_attn=False,
                  initializer=None, output_initializer=None, use_matmul=False, qkv_pack=False, attention_qkv_bias=False,
-                 attention_o_bias=False, mlp_bias=False):
+                 attention_o_bias=False, mlp_bias=False, glu_fusion=False):
         super().__init__()
         assert layer_type in ("encoder", "decoder")
         assert position_embedding_type in _POSITION_TYPES and self_attn_mask_type in _MASK_TYPES
@@ -328,7 +352,7 @@ class ParallelTransformerLayer(torch.nn.Module):
             intermediate_size=intermediate_size, use_cpu_initialization=use_cpu_initialization, params_dtype=params_dtype,
             bias_gelu_fusion=bias_gelu_fusion, glu_activation=glu_activation, use_openai_gelu=use_openai_gelu,
             onnx_safe=onnx_safe, sync_tp_duplicated_parameters=sync_tp_duplicated_parameters,
-            sequence_parallel=sequence_parallel, mlp_bias=mlp_bias)
+            sequence_parallel=sequence_parallel, mlp_bias=mlp_bias, glu_fusion=glu_fusion)
         self.alibi = None
         # Layers of up to this many forward FLOPs make all their launches in one native call (see _native_inputs).
         self.native_call_flops = 1e12
@@ -347,6 +371,8 @@ class ParallelTransformerLayer(torch.nn.Module):
                 or self.apply_residual_connection_post_layernorm
                 or (attention_mask is not None and cu_seqlens is None) or not hidden_states.is_cuda
                 or hidden_states.dtype is not torch.bfloat16 or hidden_states.dim() != 3):
+            return None
+        if getattr(attn.rotary_emb, "general", False):  # (the call turns by tables)
             return None
         q, k, v, o, gate, up, down = attn.q_proj, attn.k_proj, attn.v_proj, attn.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj
         ln1, ln2, core, rotary = self.input_layernorm, self.post_attention_layernorm, attn.core_attention_flash, attn.rotary_emb

@@ -39,13 +39,15 @@ class Embedding(torch.nn.Module):
 
 
 class EmbeddingPipe(Embedding):
+    positions_in_tables = True  # whether the layers index rotary tables, one row per place in the sequence, with the position ids
+
     def forward(self, inputs, sequence_first=False, **kwargs):
         """sequence_first: the rows of the embeddings [b, s, h] lie in memory as [s, b, h], for `functional.transposed_rows` right behind."""
         input_ids, position_ids, attention_mask = inputs[0], inputs[1], inputs[2]
         embeddings = super().forward(input_ids, position_ids, True) if sequence_first else super().forward(input_ids, position_ids)
         if len(inputs) == 4:
-            # the layers index their rotary tables (one row per sequence position) with these ids
-            F_.check_position_ids(position_ids, input_ids.shape[1])
+            if self.positions_in_tables:
+                F_.check_position_ids(position_ids, input_ids.shape[1])
             return embeddings, attention_mask, inputs[3], position_ids
         # with a 3-tuple the mask and the position ids are dropped here, as in the reference (:169-172)
         return embeddings

@@ -180,3 +180,162 @@ def test_shapes_around_the_rows(F):
     assert y.shape == (0, 4, 64)
     grads = torch.autograd.grad(y.float().sum(), [x, *ws])
     assert grads[0].shape == x.shape and all(not bool(g.any()) and g.shape == w.shape for g, w in zip(grads[1:], ws))
+
+
+# up to 8 rows: a kernel of their own for the gate's products, and for the down projection up to rows x width = 48 K (otherwise, and where the tokens do not fit LDS, the tiles)
+@pytest.mark.parametrize("T,h,f,h_out", [(1, 8, 8, 8), (3, 24, 40, 16), (8, 4096, 264, 72), (7, 8712, 72, 8), (2, 20488, 136, 24), (1, 72, 8, 4104), (5, 520, 2056, 520), (1, 64, 11008, 4096),
+                                        (4, 1032, 11008, 264), (8, 256, 5512, 520), (6, 1024, 8200, 1032), (1, 64, 49160, 16), (8, 9224, 64, 64), (9, 4096, 264, 72)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_a_handful_of_tokens(F, T, h, f, h_out, act):
+    print("gated rows", T, h, f, h_out, act, flush=True)
+    check(F, T, h, f, act, h_out=h_out)
+    check(F, T, h, f, act, h_out=h_out, train=False, seed=50)
+
+
+def test_strides_and_views(F):
+    """x and the weights as parts of wider tensors (the two first with strides of their own, or not), an output gradient of any layout."""
+    T, h, f = 70, 64, 136
+    for rows in (T, 5):
+        x = rnd(rows, 3 * h, seed=1)[:, h:2 * h].detach().requires_grad_()
+        both = rnd(f, 2 * h, seed=2, scale=h ** -0.5)
+        wide = rnd(f, 4 * h, seed=3, scale=h ** -0.5)
+        down = rnd(h, f + 24, seed=4, scale=f ** -0.5)[:, 16:16 + f].detach().requires_grad_()
+        for wg, wu in ((both[:, :h], both[:, h:]), (both[:, :h], wide[:, h:2 * h])):
+            wg, wu = wg.detach().requires_grad_(), wu.detach().requires_grad_()
+            y = F.gated_mlp(x, wg, wu, down)
+            for dy in (rnd(rows, 2 * h, seed=5)[:, h:], rnd(h, rows, seed=6).t(), rnd(1, h, seed=7).expand(rows, h)):
+                want = expected(x, wg, wu, down, dy, "silu")
+                near(y, *want["y"], "y")
+                for name, g in zip(("x", "gate", "up", "down"), torch.autograd.grad(y, (x, wg, wu, down), dy, retain_graph=True)):
+                    near(g, *want[name], name)
+
+
+@pytest.mark.parametrize("leaf", range(4))
+def test_one_gradient_alone(F, leaf):
+    tensors = [rnd(40, 64), rnd(72, 64, seed=1, scale=0.125), rnd(72, 64, seed=2, scale=0.125), rnd(64, 72, seed=3, scale=0.11)]
+    dy = rnd(40, 64, seed=4)
+    tensors[leaf].requires_grad_()
+    (g,) = torch.autograd.grad(F.gated_mlp(*tensors), [tensors[leaf]], dy)
+    near(g, *expected(*tensors, dy, "silu")[("x", "gate", "up", "down")[leaf]], "gradient")
+    if leaf < 3:
+        (g,) = torch.autograd.grad(F.gated_linear(*tensors[:3]), [tensors[leaf]], rnd(40, 72, seed=5))
+        assert g.shape == tensors[leaf].shape
+
+
+def test_main_grads_accumulate_in_fp32(F):
+    """Overwritten where fresh, then added to; one weight in two places is added to twice."""
+    x, dy = rnd(300, 64), rnd(300, 64, seed=1)
+    ws = [torch.nn.Parameter(w) for w in (rnd(72, 64, seed=2, scale=0.125), rnd(72, 64, seed=3, scale=0.125), rnd(64, 72, seed=4, scale=0.11))]
+    want = expected(x, *ws, dy, "gelu")
+    for w in ws:
+        w.main_grad, w.main_grad_fresh = torch.full(w.shape, 7.0, device="cuda"), True
+    for times in (1, 2):
+        F.gated_mlp(x, *ws, activation="gelu").backward(dy)
+        for name, w in zip(("gate", "up", "down"), ws):
+            ref, slack = want[name]
+            off = (w.main_grad.double() - times * ref).abs() - times * slack - ref.abs() * 2.0 ** -20
+            assert w.grad is None and bool((off <= 0).all()), (name, times, off.max().item())
+    tied = torch.nn.Parameter(ws[0].detach().clone())
+    tied.main_grad, tied.main_grad_fresh = torch.full(tied.shape, 7.0, device="cuda"), True
+    F.gated_mlp(x, tied, tied, ws[2].detach()).backward(dy)
+    want = expected(x, tied, tied, ws[2], dy, "silu")
+    off = (tied.main_grad.double() - want["gate"][0] - want["up"][0]).abs() - want["gate"][1] - want["up"][1] - 2.0 ** -20 * want["gate"][0].abs()
+    assert bool((off <= 0).all())
+
+
+def test_an_evaluation_keeps_nothing(F):
+    x, ws = rnd(40, 64), [rnd(72, 64, seed=1).requires_grad_(), rnd(72, 64, seed=2).requires_grad_(), rnd(64, 72, seed=3).requires_grad_()]
+    with torch.no_grad():
+        assert F.gated_mlp(x, *ws).grad_fn is None and F.gated_linear(x, *ws[:2]).grad_fn is None
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        y = F.gated_mlp(x, *ws)
+    assert torch.cuda.memory_allocated() - before <= 512 * (1 + y.numel() * 2 // 512)
+    with torch.no_grad():
+        assert torch.equal(y, F.gated_mlp(x, *ws))
+    assert torch.equal(y, F.gated_mlp(x, *ws).detach())
+
+
+@pytest.mark.parametrize("T", [3, 500])
+def test_another_stream_and_captured_steps(F, T):
+    x, dy = rnd(T, 264), rnd(T, 264, seed=1)
+    ws = [rnd(520, 264, seed=2, scale=0.06), rnd(520, 264, seed=3, scale=0.06), rnd(264, 520, seed=4, scale=0.04)]
+    leaves = [t.requires_grad_() for t in (x, *ws)]
+
+    def step():
+        y = F.gated_mlp(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (5, 6, 7):
+        with torch.no_grad():
+            x.copy_(rnd(T, 264, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+def test_results_of_more_than_two_to_the_31_elements(F):
+    """Each way, the first and last rows of T x f > 2^31."""
+    from easyllm_amd import kernels as K
+    T, h, f = (1 << 18) + 24, 64, 8200
+    x, dy = rnd(T, h), rnd(T, h, seed=1)
+    wg, wu, wd = rnd(f, h, seed=2, scale=0.125), rnd(f, h, seed=3, scale=0.125), rnd(h, f, seed=4, scale=f ** -0.5)
+    mid, gate, up = K.gated_fwd("silu", x, wg, wu, True)
+    rows = [*range(3), *range(T - 300, T)]
+    g, u = x[rows].double() @ wg.double().t(), x[rows].double() @ wu.double().t()
+    g_err, u_err = (2 * (h + 4) * E * (x[rows].double().abs() @ w.double().abs().t()) for w in (wg, wu))
+    a, slope = act64(g, "silu")
+    near(gate[rows], g, g_err, "gate")
+    near(mid[rows], a * u, (1.2 * g_err + a.abs() * 2.0 ** -15) * (u.abs() + u_err) + a.abs() * u_err, "mid")
+    del mid
+    y, _, _ = K.gated_mlp_fwd("silu", x, wg, wu, wd)
+    near(y[rows], *expected(x[rows], wg, wu, wd, None, "silu")["y"], "y")
+    dx = K.gated_mlp_bwd("silu", dy, x, wg, wu, wd, gate, up, True, (None, None, None))
+    near(dx[rows], *expected(x[rows], wg, wu, wd, dy[rows], "silu")["x"], "dx")
+
+
+def test_values_that_are_not_finite(F):
+    """Infinities and NaN of a token stay in its row."""
+    for T in (4, 100):
+        x, ws = rnd(T, 64), [rnd(72, 64, seed=1), rnd(72, 64, seed=2), rnd(64, 72, seed=3)]
+        want = F.gated_mlp(x, *ws)
+        x[1, 5], x[2, 7] = float("inf"), float("nan")
+        got = F.gated_mlp(x, *ws)
+        keep = [i for i in range(T) if i not in (1, 2)]
+        assert torch.equal(got[keep], want[keep]) and bool(got[2].isnan().all()) and not bool(torch.isfinite(got[1]).any())
+
+
+def test_second_derivatives_are_refused(F):
+    x, ws = rnd(8, 64).requires_grad_(), [rnd(72, 64, seed=1), rnd(72, 64, seed=2), rnd(64, 72, seed=3)]
+    for y in (F.gated_mlp(x, *ws), F.gated_linear(x, *ws[:2])):
+        (dx,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+            dx.float().sum().backward()
+
+
+def test_refusals(F):
+    x, wg, wu, wd = rnd(8, 64), rnd(72, 64), rnd(72, 64), rnd(64, 72)
+    for args in ((x.float(), wg, wu, wd), (x, wg.float(), wu, wd), (x, wg, wu.half(), wd), (x, wg, wu, wd.float()), (x, wg, wu[:64], wd), (x[:, :56], wg, wu, wd), (x, wg, wu, wd[:, :64]),
+                 (x.cpu(), wg, wu, wd), (x, wg.cpu(), wu.cpu(), wd), (x, rnd(76, 64), rnd(76, 64), rnd(64, 76)), (rnd(8, 60), rnd(72, 60), rnd(72, 60), wd), (x, wg, wu, rnd(60, 72)),
+                 (x, wg[:0], wu[:0], wd[:, :0]), (rnd(8, 0), wg[:, :0], wu[:, :0], wd)):
+        for leaf in (False, True):
+            with pytest.raises((ValueError, RuntimeError)):
+                F.gated_mlp(args[0].detach().requires_grad_(leaf), *args[1:])
+    for activation in (None, "none", "tanh"):
+        with pytest.raises(ValueError, match="activation"):
+            F.gated_mlp(x, wg, wu, wd, activation)
+        with pytest.raises(ValueError, match="activation"):
+            F.gated_linear(x, wg, wu, activation)
+    with pytest.raises((ValueError, RuntimeError)):
+        F.gated_linear(x, wg, rnd(72, 56))
