@@ -280,7 +280,7 @@ extern "C" int ezl_adamw8_list(int count, const ezl_adam8_tensor* tensors, const
     EZL_REQUIRE(how->step >= 1 && how->step < (1LL << 32), EZL_EINVAL, "%s: step counts from 1, below 2^32", name);
     for (int i = 0; i < count; ++i) {
         const ezl_adam8_tensor& t = tensors[i];
-        EZL_REQUIRE(t.n >= 0 && t.n < (1LL << 40) && (t.n == 0 || (t.master && t.exp_avg && t.exp_avg_sq && t.exp_avg_scale && t.exp_avg_sq_scale && t.grad)), EZL_EINVAL,
+        EZL_REQUIRE(t.n >= 0 && t.n < (1LL << 35) && (t.n == 0 || (t.master && t.exp_avg && t.exp_avg_sq && t.exp_avg_scale && t.exp_avg_sq_scale && t.grad)), EZL_EINVAL,
                     "%s: null pointer or bad size", name);
         EZL_REQUIRE(ezl_aligned16(t.master) && ezl_aligned16(t.grad) && aligned(t.param_bf16, 8) && aligned(t.exp_avg, 16) && aligned(t.exp_avg_sq, 16) &&
                         aligned(t.exp_avg_scale, 16) && aligned(t.exp_avg_sq_scale, 16),
@@ -303,7 +303,7 @@ extern "C" int ezl_adamw8_list(int count, const ezl_adam8_tensor* tensors, const
         const ezl_adam8_tensor& t = tensors[i];
         if (t.n == 0) continue;
         const int64_t chunks = (t.n + kChunk8 - 1) / kChunk8, blocks = (t.n + kBlock8 - 1) / kBlock8;
-        bool again = l.count == kListMax8 || l.chunks + chunks >= (1LL << 30);
+        bool again = l.count == kListMax8 || l.chunks + chunks >= (1LL << 23);
         for (int j = 0; j < l.count && !again; ++j) {
             const int64_t other = (l.n[j] + kBlock8 - 1) / kBlock8;
             again = meet(t.master, t.n * 4, l.master[j], l.n[j] * 4) || meet(t.param_bf16, t.n * 2, l.param[j], l.n[j] * 2) || meet(t.exp_avg, t.n, l.m[j], l.n[j]) ||
@@ -326,7 +326,7 @@ extern "C" int ezl_moments8_list(int count, const ezl_adam8_tensor* tensors, voi
     EZL_REQUIRE(count >= 0 && (count == 0 || (tensors && exp_avg_bf16 && exp_avg_sq_bf16)), EZL_EINVAL, "%s: bad count or null argument", name);
     for (int i = 0; i < count; ++i) {
         const ezl_adam8_tensor& t = tensors[i];
-        EZL_REQUIRE(t.n >= 0 && t.n < (1LL << 40) && (t.n == 0 || (t.exp_avg && t.exp_avg_sq && t.exp_avg_scale && t.exp_avg_sq_scale && exp_avg_bf16[i] && exp_avg_sq_bf16[i])),
+        EZL_REQUIRE(t.n >= 0 && t.n < (1LL << 35) && (t.n == 0 || (t.exp_avg && t.exp_avg_sq && t.exp_avg_scale && t.exp_avg_sq_scale && exp_avg_bf16[i] && exp_avg_sq_bf16[i])),
                     EZL_EINVAL, "%s: null pointer or bad size", name);
         EZL_REQUIRE(aligned(t.exp_avg, 16) && aligned(t.exp_avg_sq, 16) && ezl_aligned16(exp_avg_bf16[i]) && ezl_aligned16(exp_avg_sq_bf16[i]), EZL_EINVAL,
                     "%s: pointers must be 16-byte aligned", name);
@@ -341,7 +341,7 @@ extern "C" int ezl_moments8_list(int count, const ezl_adam8_tensor* tensors, voi
         const ezl_adam8_tensor& t = tensors[i];
         if (t.n == 0) continue;
         const int64_t chunks = (t.n + kChunk8 - 1) / kChunk8;
-        if (l.count == kListMax8 || l.chunks + chunks >= (1LL << 30)) flush();
+        if (l.count == kListMax8 || l.chunks + chunks >= (1LL << 23)) flush();
         const int s = l.count++;
         l.m[s] = (const uint8_t*)t.exp_avg; l.v[s] = (const uint8_t*)t.exp_avg_sq; l.ms[s] = (const uint8_t*)t.exp_avg_scale; l.vs[s] = (const uint8_t*)t.exp_avg_sq_scale;
         l.m_out[s] = (bf16_t*)exp_avg_bf16[i]; l.v_out[s] = (bf16_t*)exp_avg_sq_bf16[i]; l.n[s] = t.n; l.first[s] = l.chunks;

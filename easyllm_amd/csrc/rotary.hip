@@ -79,9 +79,13 @@ __global__ __launch_bounds__(kRotaryBlock) void rotary_kernel(const RotaryArgs a
     if (token >= a.tokens) return;
     const int64_t si = a.b == 1 ? token : token / a.b, bi = a.b == 1 ? 0 : token - si * a.b;
     const bool turns = slot < a.turned_slots;
-    const int j0 = slot * (INTERLEAVED ? 4 : 8);                                   // its first pair
-    const int e0 = turns ? slot * 8 : a.turned + (slot - a.turned_slots) * 8;      // its first element
-    const int n = WHOLE ? 8 : turns ? min(8, (INTERLEAVED ? a.turned : half) - e0) : min(8, a.d - e0);
+    // Its first element, in the part of the head that its like share (of halves: the first of both).  The last slot of a part that is no multiple of 8 reaches back into the one before, whose
+    // thread writes the same there: every access is 16 bytes.
+    const int part = turns ? (INTERLEAVED ? a.turned : half) : a.d - a.turned;
+    int e = (turns ? slot : slot - a.turned_slots) * 8;
+    if (!WHOLE && part >= 8) e = min(e, part - 8);
+    const int n = WHOLE ? 8 : min(8, part - e), e0 = turns ? e : a.turned + e;
+    const int j0 = INTERLEAVED ? e / 2 : e;  // its first pair
     const bf16_t* x[HEADS];
     bf16_t* out[HEADS];
     bf16x8 v[HEADS], w[HEADS];

@@ -19,6 +19,13 @@ from . import kernels as K
 from .first_order import first_order
 
 
+def _differentiated(*tensors):
+    """Whether autograd has a say in a call on these: backward, or forward (where its own error is wanted)."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _main_grad_target(param):
     """(buffer or None, accumulate flag) for a parameter, consuming its 'fresh' mark."""
     mg = getattr(param, "main_grad", None)
@@ -484,7 +491,7 @@ def gated_linear(x, gate_weight, up_weight, activation="silu"):
 def gated_mlp(x, gate_weight, up_weight, down_weight, activation="silu"):
     """gated_linear(x, gate_weight, up_weight, activation) down^T; down [h', f].  Of the tensors between x and the result the backward pass keeps two, x gate^T and x up^T."""
     _check_gate(activation)
-    if not (torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad or down_weight.requires_grad)):
+    if not _differentiated(x, gate_weight, up_weight, down_weight):
         y, _, _ = K.gated_mlp_fwd(activation, x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight)
         return y.view(*x.shape[:-1], y.shape[1])
     return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation, torch.is_grad_enabled())
@@ -567,7 +574,7 @@ def rotary_embed(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0
     the sequence) have no limit that a table would set."""
     if inv_freq.requires_grad:
         raise ValueError("rotary_embed: frequencies are not learnt")
-    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):  # (a node costs the host 4 us, as much as a token's launch)
+    if not _differentiated(q, k):  # (a node costs the host 4 us, as much as a token's launch)
         return K.rotary(_rotary_rows(q), _rotary_rows(k), inv_freq, position_ids, interleaved, float(scale))
     return RotaryEmbedFunction.apply(q, k, inv_freq, position_ids, bool(interleaved), float(scale))
 

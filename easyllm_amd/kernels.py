@@ -1097,7 +1097,7 @@ def adamw8_list(states, grads, params, lr, beta1, beta2, eps, weight_decay, step
         if not 0 <= number < 2 ** 32:
             raise ValueError("a tensor's number has 32 bits")
         tensors[i] = (master.data_ptr(), *moments, grad.data_ptr(), None if param is None else param.data_ptr(), n, number)
-    how = _lib.Adam8(lr, beta1, beta2, eps, weight_decay, step, seed & 0xFFFFFFFFFFFFFFFF, 1 if bias_correction else 0)
+    how = _lib.Adam8(float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(step), seed & 0xFFFFFFFFFFFFFFFF, 1 if bias_correction else 0)
     _lib.call("ezl_adamw8_list", len(states), tensors, how, _p(norm_coef), _stream())
 
 

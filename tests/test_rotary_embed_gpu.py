@@ -173,3 +173,14 @@ def test_refusals(F):
             F.rotary_embed(*args)
     with pytest.raises(ValueError, match="not learnt"):
         F.rotary_embed(q, None, f.clone().requires_grad_())
+
+
+def test_forward_mode_derivatives_are_an_error(F):
+    from easyllm_amd import functional
+    q, f = rnd(4, 2, 3, 64), frequencies(64)
+    w = rnd(72, 64), rnd(72, 64, seed=1), rnd(64, 72, seed=2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: F.rotary_embed(dual, None, f), lambda: functional.gated_mlp(dual, *w), lambda: functional.gated_linear(dual, *w[:2])):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
