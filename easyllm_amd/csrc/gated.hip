@@ -1,4 +1,4 @@
-// The way back through the gate of an MLP as a pass of its own, where no product of the framework's stands in front of it.  HBM-bound: 10 bytes a value.
+// The way back through the gate of an MLP as a pass of its own, where no product of the framework's stands in front of it.  HBM-bound: 11 bytes a value.
 #include "common.h"
 #include "gate.h"
 
@@ -8,24 +8,22 @@ constexpr int kGateBlock = 256;
 
 // dgate = d * up * act'(gate), dup = d * act(gate)
 template <int ACT, bool STREAM>
-__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* dout, const bf16_t* gate, const bf16_t* up,
-                                                              bf16_t* dgate, bf16_t* dup, bf16_t* mid, int64_t n8) {
+__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const KeptParts kept, bf16_t* dgate, bf16_t* dup, int64_t n8) {
     for (int64_t i = (int64_t)blockIdx.x * kGateBlock + threadIdx.x; i < n8; i += (int64_t)gridDim.x * kGateBlock) {
-        float g[8], u[8], d[8], dg[8], du[8], m[8];
-        unpack8(ld_bf16x8_nt(gate + i * 8), g);
-        unpack8(ld_bf16x8_nt(up + i * 8), u);
-        unpack8(ld_bf16x8_nt(dout + i * 8), d);
+        const u32x4 kg = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kept.gate) + i), ku = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kept.up) + i);
+        const u32x2 kl = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kept.low) + i);
+        float g[8], u[8], d[8], dg[8], du[8];
+        kept_values<8>({kg[0], kg[1], kg[2], kg[3]}, {ku[0], ku[1], ku[2], ku[3]}, {kl[0], kl[1]}, g, u);
+        unpack8(ld_bf16x8_nt(d_in + i * 8), d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float y, slope;
             gate_value_slope<ACT>(g[k], y, slope);
             dg[k] = d[k] * u[k] * slope;
             du[k] = d[k] * y;
-            m[k] = y * u[k];
         }
         st_result<STREAM>(dgate + i * 8, pack8(dg));
         st_result<STREAM>(dup + i * 8, pack8(du));
-        if (mid) st_result<STREAM>(mid + i * 8, pack8(m));
     }
 }
 
@@ -36,17 +34,17 @@ unsigned gate_grid(int64_t n8) {
 
 }  // namespace
 
-extern "C" int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t n, void* stream) {
+extern "C" int ezl_gate_bwd(int act, const void* d, const ezl_kept_gate* kept, void* dgate, void* dup, int64_t n, void* stream) {
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "ezl_gate_bwd: act must be one of EZL_GATE_*");
     EZL_REQUIRE(n >= 0 && n % 8 == 0, EZL_EUNSUPPORTED, "ezl_gate_bwd: n must be a multiple of 8");
-    EZL_REQUIRE(ezl_aligned16(d) && ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) &&
-                    (n == 0 || (d && gate && up && dgate && dup)),
+    EZL_REQUIRE(n == 0 || (d && kept && kept->gate && kept->up && kept->low && dgate && dup && ezl_aligned16(d) && ezl_aligned16(kept->gate) && ezl_aligned16(kept->up) &&
+                           ezl_aligned16(kept->low) && ezl_aligned16(dgate) && ezl_aligned16(dup)),
                 EZL_EINVAL, "ezl_gate_bwd: null or misaligned pointer");
     if (n == 0) return EZL_OK;
     constexpr decltype(&gate_bwd_kernel<0, false>) kernels[][2] = {{gate_bwd_kernel<0, false>, gate_bwd_kernel<0, true>}, {gate_bwd_kernel<1, false>, gate_bwd_kernel<1, true>},
                                                                     {gate_bwd_kernel<2, false>, gate_bwd_kernel<2, true>}, {gate_bwd_kernel<3, false>, gate_bwd_kernel<3, true>}};
-    hipLaunchKernelGGL(kernels[act][ezl_streams(n * (mid ? 6 : 4))], dim3(gate_grid(n / 8)), dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, (const bf16_t*)gate,
-                       (const bf16_t*)up, (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, n / 8);
+    const KeptParts parts = {(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low};
+    hipLaunchKernelGGL(kernels[act][ezl_streams(n * 4)], dim3(gate_grid(n / 8)), dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, parts, (bf16_t*)dgate, (bf16_t*)dup, n / 8);
     EZL_LAUNCH_CHECK("ezl_gate_bwd");
     return EZL_OK;
 }

@@ -43,37 +43,37 @@ extern "C" int64_t ezl_gated_mlp_bytes(const ezl_gated_mlp* m, int backward) {
     return 3 * block_bytes(*m) + ws;
 }
 
-extern "C" int ezl_gated_mlp_fwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, void* y, void* gate, void* up, void* temp, int64_t temp_bytes, void* stream) {
+extern "C" int ezl_gated_mlp_fwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, void* y, const ezl_kept_gate* kept, void* temp, int64_t temp_bytes, void* stream) {
     const char* name = "ezl_gated_mlp_fwd";
     if (const int rc = check(name, m)) return rc;
     if (m->M == 0) return EZL_OK;
     EZL_REQUIRE(y && temp && ezl_aligned16(temp) && ezl_aligned16(y) && temp_bytes >= ezl_gated_mlp_bytes(m, 0), EZL_EINVAL, "%s: null, misaligned or too small a buffer", name);
     char* const ws = (char*)temp + block_bytes(*m);
     const int64_t ws_bytes = temp_bytes - block_bytes(*m);
-    if (const int rc = ezl_gated_fwd(m->act, x, m->gate, m->up, temp, gate, up, m->M, m->f, m->h, ldx, m->ldw, ws, ws_bytes, stream)) return rc;
+    if (const int rc = ezl_gated_fwd(m->act, x, m->gate, m->up, temp, kept, m->M, m->f, m->h, ldx, m->ldw, ws, ws_bytes, stream)) return rc;
     const ezl_epilogue none = {nullptr, nullptr, nullptr, 0, 0, EZL_ACT_NONE};
     if (gemm_rows_pays(m->M, m->n, m->f)) return ezl_gemm_bf16_epilogue(temp, m->down, y, m->M, m->n, m->f, m->f, m->ldd, m->n, &none, ws, ws_bytes, stream);
     if (stream_down_pays(m->M, m->f)) {
         EZL_REQUIRE(ezl_aligned16(m->down) && m->ldd % 8 == 0 && m->ldd >= m->f && m->ldd < (1LL << 22), EZL_EINVAL, "%s: bad down projection", name);
-        stream_rows_launch(temp, m->down, nullptr, y, nullptr, nullptr, (int)m->M, (int)m->n, (int)m->f, m->f, m->ldd, 0, (hipStream_t)stream);
+        stream_rows_launch(temp, m->down, nullptr, y, KeptParts{}, (int)m->M, (int)m->n, (int)m->f, m->f, m->ldd, 0, (hipStream_t)stream);
         EZL_LAUNCH_CHECK(name);
         return EZL_OK;
     }
     return ezl_gemm_bf16(temp, m->down, y, m->M, m->n, m->f, m->f, m->ldd, m->n, 1, 1, 0, 0, ws, ws_bytes, stream);
 }
 
-extern "C" int ezl_gated_mlp_bwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, const void* dy, const void* gate, const void* up, void* dx, const ezl_layer_grad* dgate,
-                                 const ezl_layer_grad* dup, const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream) {
+extern "C" int ezl_gated_mlp_bwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, const void* dy, const ezl_kept_gate* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
+                                 const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream) {
     const char* name = "ezl_gated_mlp_bwd";
     if (const int rc = check(name, m)) return rc;
-    EZL_REQUIRE(m->M == 0 || (x && dy && gate && up && temp && ezl_aligned16(temp) && temp_bytes >= ezl_gated_mlp_bytes(m, 1)), EZL_EINVAL, "%s: null, misaligned or too small a buffer", name);
+    EZL_REQUIRE(m->M == 0 || (x && dy && kept && temp && ezl_aligned16(temp) && temp_bytes >= ezl_gated_mlp_bytes(m, 1)), EZL_EINVAL, "%s: null, misaligned or too small a buffer", name);
     EZL_REQUIRE(m->M == 0 || !dx || ezl_aligned16(dx), EZL_EINVAL, "%s: misaligned dx", name);
     const int64_t block = block_bytes(*m);
     char* const t = (char*)temp;
     void *const dg = t, *const du = t + block, *const mid = t + 2 * block, *const ws = t + 3 * block;
     const int64_t ws_bytes = m->M ? temp_bytes - 3 * block : 0;
     if (m->M)
-        if (const int rc = ezl_gated_bwd(m->act, dy, m->down, gate, up, dg, du, wanted(ddown) ? mid : nullptr, m->M, m->f, m->n, m->n, m->ldd, ws, ws_bytes, stream)) return rc;
+        if (const int rc = ezl_gated_bwd(m->act, dy, m->down, kept, dg, du, wanted(ddown) ? mid : nullptr, m->M, m->f, m->n, m->n, m->ldd, ws, ws_bytes, stream)) return rc;
     if (wanted(ddown))
         if (const int rc = weight_gradient(dy, m->n, mid, m->f, m->f, ddown, m->M, ws, ws_bytes, stream)) return rc;
     const Products two(*m);

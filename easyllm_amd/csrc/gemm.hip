@@ -1227,41 +1227,42 @@ extern "C" int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int
 
 extern "C" int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K) { return M <= 0 || f <= 0 || K <= 0 ? 0 : plan_bytes(M, gate_columns(true, f), K); }
 
-extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* gate, void* up, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, const ezl_kept_gate* kept, int64_t M, int64_t f, int64_t K, int64_t ldx,
+                             int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* name = "ezl_gated_fwd";
     EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
-    EZL_REQUIRE(!gate == !up, EZL_EINVAL, "%s: gate and up are kept together or not at all", name);
+    const KeptParts parts = kept ? KeptParts{(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low} : KeptParts{};
+    EZL_REQUIRE(!kept || M == 0 || f == 0 || (parts.gate && parts.up && parts.low), EZL_EINVAL, "%s: what is kept needs all of its parts", name);
     if (M == 0 || f == 0) return EZL_OK;
     EZL_REQUIRE(out && up_weight, EZL_EINVAL, "%s: null pointer", name);
     EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
     if (const int rc = check_operands(x, gate_weight, M, f, K, ldx, ldw, f, 1, 1)) return rc;
-    EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(parts.gate) && ezl_aligned16(parts.up) && ezl_aligned16(parts.low) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
     if (stream_pairs_pay(M, K)) {
-        stream_rows_launch(x, gate_weight, up_weight, out, gate, up, (int)M, (int)f, (int)K, ldx, ldw, act, (hipStream_t)stream);
+        stream_rows_launch(x, gate_weight, up_weight, out, parts, (int)M, (int)f, (int)K, ldx, ldw, act, (hipStream_t)stream);
         EZL_LAUNCH_CHECK(name);
         return EZL_OK;
     }
     launch_gate<GateForward>(x, gate_weight, out, (int)M, (int)f, (int)K, ldx, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
-                             {(const bf16_t*)up_weight, (bf16_t*)gate, (bf16_t*)up, f, act});
+                             {(const bf16_t*)up_weight, parts, f, act});
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;
 }
 
-extern "C" int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy,
-                             int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const ezl_kept_gate* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K,
+                             int64_t lddy, int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* name = "ezl_gated_bwd";
     EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
     if (M == 0 || f == 0) return EZL_OK;
-    EZL_REQUIRE(gate && up && dgate && dup, EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(kept && kept->gate && kept->up && kept->low && dgate && dup, EZL_EINVAL, "%s: null pointer", name);
     EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
     if (const int rc = check_operands(dy, down_weight, M, f, K, lddy, ldw, f, 1, 0)) return rc;
-    EZL_REQUIRE(ezl_aligned16(gate) && ezl_aligned16(up) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) && ezl_aligned16(workspace), EZL_EINVAL,
+    EZL_REQUIRE(ezl_aligned16(kept->gate) && ezl_aligned16(kept->up) && ezl_aligned16(kept->low) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) && ezl_aligned16(workspace), EZL_EINVAL,
                 "%s: pointers must be 16-byte aligned", name);
     launch_gate<GateBackward>(dy, down_weight, dgate, (int)M, (int)f, (int)K, lddy, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
-                              {(const bf16_t*)gate, (const bf16_t*)up, (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, f, act});
+                              {{(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low}, (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, f, act});
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;
 }

@@ -452,23 +452,30 @@ __global__ __launch_bounds__(256) void gate_reduce_kernel(const float* __restric
             f32x4 y;
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = gate_value<act>(g[r]) * u[r];
-            if (epi.gate) {
-                store(epi.gate + (int64_t)row * epi.ld + col, g);
-                store(epi.up + (int64_t)row * epi.ld + col, u);
+            if (epi.kept.gate) {
+                const float gs[4] = {g[0], g[1], g[2], g[3]}, us[4] = {u[0], u[1], u[2], u[3]};
+                uint32_t kg[2], ku[2], kl[1];
+                keep<4>(gs, us, kg, ku, kl);
+                const int64_t to = (int64_t)row * epi.ld + col;
+                *reinterpret_cast<u32x2*>(epi.kept.gate + to) = u32x2{kg[0], kg[1]};
+                *reinterpret_cast<u32x2*>(epi.kept.up + to) = u32x2{ku[0], ku[1]};
+                *reinterpret_cast<uint32_t*>(epi.kept.low + to) = kl[0];
             }
             store(C + (int64_t)row * ldc + col, y);
         } else {
             const f32x4 d = sum(cl);
             const int64_t at = (int64_t)row * epi.ld + col;
-            const bf16x4 g = *reinterpret_cast<const bf16x4*>(epi.gate + at), u = *reinterpret_cast<const bf16x4*>(epi.up + at);
+            const u32x2 kg = *reinterpret_cast<const u32x2*>(epi.kept.gate + at), ku = *reinterpret_cast<const u32x2*>(epi.kept.up + at);
+            float g[4], u[4];
+            kept_values<4>({kg[0], kg[1]}, {ku[0], ku[1]}, {*reinterpret_cast<const uint32_t*>(epi.kept.low + at)}, g, u);
             f32x4 dg, du, mid;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float y, slope;
-                gate_value_slope<act>((float)g[r], y, slope);
-                dg[r] = d[r] * (float)u[r] * slope;
+                gate_value_slope<act>(g[r], y, slope);
+                dg[r] = d[r] * u[r] * slope;
                 du[r] = d[r] * y;
-                mid[r] = y * (float)u[r];
+                mid[r] = y * u[r];
             }
             store(epi.dgate + at, dg);
             store(epi.dup + at, du);

@@ -40,25 +40,28 @@ struct Epilogue {
 };
 
 // The first products of a gated MLP as one: C = act(A B^T) * (A B2^T), forward form, B and B2 alike.  A tile's columns are taken 16 of B, the same 16 of B2, and so on: the two
-// accumulators of a result lie in one lane, and a tile of 256 columns makes 128 of C.  gate and up (both or neither) receive the two products, rounded, for the backward pass; C is made of them
-// unrounded.
+// accumulators of a result lie in one lane, and a tile of 256 columns makes 128 of C.  `kept` (its pointers null: nothing) receives the two products for the backward pass; C is made of them as
+// they are.
 struct GateForward {
     const bf16_t* B2;
-    bf16_t *gate, *up;
-    int64_t ld;  // of gate and up
+    KeptParts kept;
+    int64_t ld;  // of what is kept
     int act;
-    __device__ __forceinline__ GateForward at(int64_t m, int64_t n) const { return {B2, gate ? gate + m * ld + n : nullptr, up ? up + m * ld + n : nullptr, ld, act}; }
+    __device__ __forceinline__ GateForward at(int64_t m, int64_t n) const {
+        const int64_t o = m * ld + n;
+        return {B2, kept.gate ? KeptParts{kept.gate + o, kept.up + o, kept.low + o} : kept, ld, act};
+    }
 };
 // The way back through it behind the input gradient d = A B of the down projection: dgate = d * up * act'(gate), dup = d * act(gate), and mid (may be null) =
 // act(gate) * up once more, which the down projection's weight gradient reads.  d itself is stored nowhere.  All [M, N], rows ld apart.
 struct GateBackward {
-    const bf16_t *gate, *up;
+    KeptParts kept;
     bf16_t *dgate, *dup, *mid;
     int64_t ld;
     int act;
     __device__ __forceinline__ GateBackward at(int64_t m, int64_t n) const {
         const int64_t o = m * ld + n;
-        return {gate + o, up + o, dgate + o, dup + o, mid ? mid + o : nullptr, ld, act};
+        return {{kept.gate + o, kept.up + o, kept.low + o}, dgate + o, dup + o, mid ? mid + o : nullptr, ld, act};
     }
 };
 template <class EPI>
@@ -498,8 +501,9 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
     const auto matrix = [&](bf16_t* p, int64_t ld) {
         return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(p), 0, (uint32_t)(((int64_t)(mrem - 1) * ld + nrem) * 2), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc), gbuf = matrix(e.gate, e.ld), ubuf = matrix(e.up, e.ld);
-    const bool keep = e.gate != nullptr;
+    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc), gbuf = matrix(e.kept.gate, e.ld), ubuf = matrix(e.kept.up, e.ld);
+    const __amdgpu_buffer_rsrc_t lbuf = __builtin_amdgcn_make_buffer_rsrc(e.kept.low, 0, (uint32_t)((mrem - 1) * e.ld + nrem), 0x00020000);
+    const bool keeps = e.kept.gate != nullptr;
     const int g = lane >> 4;
     uint32_t col_off[WIDE ? NB / 2 : NB];
 #pragma unroll
@@ -509,6 +513,7 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
     }
     const uint32_t row = (uint32_t)(row0 + (lane & 15));
     const auto offset = [&](int i, int b, int64_t ld) { return col_off[b] + row * (uint32_t)(ld * 2) + i * (uint32_t)(32 * ld); };
+    const auto byte_offset = [&](int i, int b) { return (col_off[b] == kOut ? kOut : col_off[b] / 2) + row * (uint32_t)e.ld + i * (uint32_t)(16 * e.ld); };
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         if constexpr (WIDE) {
@@ -530,9 +535,12 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
                 const auto out = [&](const float (&v)[8], __amdgpu_buffer_rsrc_t to, int64_t ld) {
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(v)), to, offset(i, b, ld), 0, 0);
                 };
-                if (keep) {
-                    out(gate, gbuf, e.ld);
-                    out(up, ubuf, e.ld);
+                if (keeps) {
+                    uint32_t kg[4], ku[4], kl[2];
+                    keep<8>(gate, up, kg, ku, kl);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{kg[0], kg[1], kg[2], kg[3]}, gbuf, offset(i, b, e.ld), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{ku[0], ku[1], ku[2], ku[3]}, ubuf, offset(i, b, e.ld), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{kl[0], kl[1]}, lbuf, byte_offset(i, b), 0, 0);
                 }
 #pragma unroll
                 for (int r = 0; r < 8; ++r) y[r] = gate_value<ACT>(gate[r]) * up[r];
@@ -540,24 +548,21 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
                 if constexpr (TM * TN >= 48) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const f32x4 ga = acc[i][2 * b], ua = acc[i][2 * b + 1];
-                const auto out = [&](const f32x4& a, __amdgpu_buffer_rsrc_t to, int64_t ld) {
-                    bf16x4 v;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (bf16_t)a[r];
-                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), to, offset(i, b, ld), 0, 0);
-                };
-                if (keep) {
-                    out(ga, gbuf, e.ld);
-                    out(ua, ubuf, e.ld);
+                const float gate[4] = {acc[i][2 * b][0], acc[i][2 * b][1], acc[i][2 * b][2], acc[i][2 * b][3]};
+                const float up[4] = {acc[i][2 * b + 1][0], acc[i][2 * b + 1][1], acc[i][2 * b + 1][2], acc[i][2 * b + 1][3]};
+                if (keeps) {
+                    uint32_t kg[2], ku[2], kl[1];
+                    keep<4>(gate, up, kg, ku, kl);
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{kg[0], kg[1]}, gbuf, offset(i, b, e.ld), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{ku[0], ku[1]}, ubuf, offset(i, b, e.ld), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(kl[0], lbuf, byte_offset(i, b), 0, 0);
                 }
-                f32x4 y;
+                bf16x4 y;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = gate_value<ACT>(ga[r]) * ua[r];
-                out(y, cbuf, ldc);
+                for (int r = 0; r < 4; ++r) y[r] = (bf16_t)(gate_value<ACT>(gate[r]) * up[r]);
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), cbuf, offset(i, b, ldc), 0, 0);
             }
         }
     }
@@ -569,7 +574,8 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
     const auto matrix = [&](const bf16_t* p) {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(p)), 0, (uint32_t)(((int64_t)(mrem - 1) * e.ld + nrem) * 2), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t gbuf = matrix(e.gate), ubuf = matrix(e.up), dgbuf = matrix(e.dgate), dubuf = matrix(e.dup), midbuf = matrix(e.mid);
+    const __amdgpu_buffer_rsrc_t lbuf = __builtin_amdgcn_make_buffer_rsrc(e.kept.low, 0, (uint32_t)((mrem - 1) * e.ld + nrem), 0x00020000);
+    const __amdgpu_buffer_rsrc_t gbuf = matrix(e.kept.gate), ubuf = matrix(e.kept.up), dgbuf = matrix(e.dgate), dubuf = matrix(e.dup), midbuf = matrix(e.mid);
     const bool want_mid = e.mid != nullptr;
     const int g = lane >> 4;
     uint32_t off[TN / 2];
@@ -581,10 +587,12 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
     const uint32_t row_step = (uint32_t)(32 * e.ld);
     constexpr int PIECES = TM * (TN / 2), DEPTH = PIECES < 3 ? PIECES : 3;  // of 16 bytes a lane, row by row; on the way at a time
     u32x4 old_g[DEPTH], old_u[DEPTH];
+    u32x2 old_l[DEPTH];
     const auto fetch = [&](int q) {
         const uint32_t at = off[q % (TN / 2)] + q / (TN / 2) * row_step;
         old_g[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gbuf, at, 0, 0));
         old_u[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ubuf, at, 0, 0));
+        old_l[q % DEPTH] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(lbuf, at >> 1, 0, 0));  // (an offset that is out of range stays so: 2^30)
     };
 #pragma unroll
     for (int q = 0; q < DEPTH - 1; ++q) fetch(q);
@@ -602,14 +610,16 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
                 d[r] = __uint_as_float(sw[0]);
                 d[4 + r] = __uint_as_float(sw[1]);
             }
-            const bf16x8 gate = __builtin_bit_cast(bf16x8, old_g[q % DEPTH]), up = __builtin_bit_cast(bf16x8, old_u[q % DEPTH]);
+            const u32x4 kg = old_g[q % DEPTH], ku = old_u[q % DEPTH];
+            float gate[8], up[8];
+            kept_values<8>({kg[0], kg[1], kg[2], kg[3]}, {ku[0], ku[1], ku[2], ku[3]}, {old_l[q % DEPTH][0], old_l[q % DEPTH][1]}, gate, up);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 float y, slope;
-                gate_value_slope<ACT>((float)gate[r], y, slope);
-                dg[r] = d[r] * (float)up[r] * slope;
+                gate_value_slope<ACT>(gate[r], y, slope);
+                dg[r] = d[r] * up[r] * slope;
                 du[r] = d[r] * y;
-                mid[r] = y * (float)up[r];
+                mid[r] = y * up[r];
             }
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(dg)), dgbuf, off[jp] + i * row_step, 0, 0);
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, pack8(du)), dubuf, off[jp] + i * row_step, 0, 0);

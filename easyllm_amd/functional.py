@@ -428,42 +428,42 @@ def _gated_products_bwd(x, gate_weight, up_weight, dgate, dup, need):
 
 
 class GatedLinearFunction(torch.autograd.Function):
-    """act(gate x) * up x, both products kept for backward in bf16 (half the bytes of fp32; the gradients that are made of them go through bf16 products anyway)."""
+    """act(gate x) * up x, both products kept for backward, in 12 bits of mantissa each."""
 
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, act, training):
         x2d = x.reshape(-1, x.shape[-1])
         keep = training and any(ctx.needs_input_grad[:3])
-        mid, gate, up = K.gated_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), keep)
+        mid, kept = K.gated_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), keep)
         ctx.act = act
-        ctx.save_for_backward(x, gate_weight, up_weight, gate, up)
+        ctx.save_for_backward(x, gate_weight, up_weight, kept)
         return mid.view(*x.shape[:-1], mid.shape[1])
 
     @staticmethod
     @first_order
     def backward(ctx, dmid):
-        x, gate_weight, up_weight, gate, up = ctx.saved_tensors
-        dgate, dup, _ = K.gate_bwd(ctx.act, dmid.reshape(gate.shape).contiguous(), gate, up)
+        x, gate_weight, up_weight, kept = ctx.saved_tensors
+        dgate, dup = K.gate_bwd(ctx.act, dmid.reshape(-1, dmid.shape[-1]).contiguous(), kept)
         return (*_gated_products_bwd(x, gate_weight, up_weight, dgate, dup, ctx.needs_input_grad), None, None)
 
 
 class GatedMLPFunction(torch.autograd.Function):
-    """down(act(gate x) * up x).  The two products' results are kept for backward (bf16), what they make together is not: the backward pass makes it again in the
+    """down(act(gate x) * up x).  The two products' results are kept for backward (12 bits of mantissa), what they make together is not: the backward pass makes it again in the
     launch that takes the output's gradient through the down projection and the gate, for the down projection's weight gradient."""
 
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, down_weight, act, training):
         x2d = x.reshape(-1, x.shape[-1])
         keep = training and any(ctx.needs_input_grad[:4])
-        y, gate, up = K.gated_mlp_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), down_weight, keep)
+        y, kept = K.gated_mlp_fwd(act, x2d, *_gate_weights(gate_weight, up_weight), down_weight, keep)
         ctx.act = act
-        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, gate, up)
+        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, kept)
         return y.view(*x.shape[:-1], y.shape[1])
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
-        x, gate_weight, up_weight, down_weight, gate, up = ctx.saved_tensors
+        x, gate_weight, up_weight, down_weight, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         targets, grads = [None] * 3, [None] * 3
         for i in (2, 0, 1):  # (the order in which they are written)
@@ -473,7 +473,7 @@ class GatedMLPFunction(torch.autograd.Function):
                 if mg is None:
                     grads[i] = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
                 targets[i] = mg, grads[i], acc
-        dx = K.gated_mlp_bwd(ctx.act, dy.reshape(-1, dy.shape[-1]).contiguous(), x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight, gate, up, need[0], targets)
+        dx = K.gated_mlp_bwd(ctx.act, dy.reshape(-1, dy.shape[-1]).contiguous(), x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight, kept, need[0], targets)
         return (None if dx is None else dx.view(x.shape), *grads, None, None)
 
 
@@ -489,10 +489,11 @@ def gated_linear(x, gate_weight, up_weight, activation="silu"):
 
 
 def gated_mlp(x, gate_weight, up_weight, down_weight, activation="silu"):
-    """gated_linear(x, gate_weight, up_weight, activation) down^T; down [h', f].  Of the tensors between x and the result the backward pass keeps two, x gate^T and x up^T."""
+    """gated_linear(x, gate_weight, up_weight, activation) down^T; down [h', f].  Of what lies between x and the result the backward pass keeps x gate^T and x up^T, five bytes
+    the pair of values."""
     _check_gate(activation)
     if not _differentiated(x, gate_weight, up_weight, down_weight):
-        y, _, _ = K.gated_mlp_fwd(activation, x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight)
+        y, _ = K.gated_mlp_fwd(activation, x.reshape(-1, x.shape[-1]), *_gate_weights(gate_weight, up_weight), down_weight)
         return y.view(*x.shape[:-1], y.shape[1])
     return GatedMLPFunction.apply(x, gate_weight, up_weight, down_weight, activation, torch.is_grad_enabled())
 

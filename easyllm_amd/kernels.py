@@ -285,22 +285,31 @@ def swiglu_bwd(dout, gate, up):
 GATES = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 
+def _new_kept(T, f, device):
+    """The three parts of an ezl_kept_gate in one tensor, one behind the other"""
+    return torch.empty(5 * T * f, dtype=torch.uint8, device=device)
+
+
+def _kept(kept, T, f):
+    at, n = kept.data_ptr(), T * f
+    _need(kept.numel() == 5 * n and kept.dtype is torch.uint8 and kept.is_contiguous(), "what a gated block kept does not fit")
+    return _lib.KeptGate(at, at + 2 * n, at + 4 * n)
+
+
 def gated_fwd(act, x2d, gate_weight, up_weight, keep=False):
-    """-> (act(x2d @ gate_weight^T) * (x2d @ up_weight^T), and with `keep` the two products, else None, None)"""
+    """-> (act(x2d @ gate_weight^T) * (x2d @ up_weight^T), with `keep` what the backward calls read of the two products, else None)"""
     ldx, ldw = _rows_ld(x2d, "x"), _rows_ld(gate_weight, "gate weight")
     (T, n_in), (f, w_in) = x2d.shape, gate_weight.shape
     _need(up_weight.shape == gate_weight.shape and _rows_ld(up_weight, "up weight") == ldw, "gated: the two weights must be alike")
     _need(n_in == w_in and n_in > 0 and f % 8 == 0, "gated: inner dimensions differ or are empty, or the width is no multiple of 8")
     _here(x2d, "x"); _here(gate_weight, "gate weight"); _here(up_weight, "up weight")
     out = torch.empty((T, f), dtype=BF16, device=x2d.device)
-    gate = up = None
-    if keep:
-        gate, up = torch.empty_like(out), torch.empty_like(out)
+    kept = _new_kept(T, f, x2d.device) if keep else None
     nbytes = _lib.gated_workspace_bytes(T, f, n_in)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x2d.device) if nbytes else None
-    _lib.call("ezl_gated_fwd", GATES[act], x2d.data_ptr(), gate_weight.data_ptr(), up_weight.data_ptr(), out.data_ptr(), _p(gate), _p(up), T, f, n_in, ldx, ldw, _p(ws), nbytes,
-              _stream())
-    return out, gate, up
+    _lib.call("ezl_gated_fwd", GATES[act], x2d.data_ptr(), gate_weight.data_ptr(), up_weight.data_ptr(), out.data_ptr(), _kept(kept, T, f) if keep else None, T, f, n_in, ldx, ldw, _p(ws),
+              nbytes, _stream())
+    return out, kept
 
 
 def _gated_mlp(act, x2d, gate_weight, up_weight, down_weight):
@@ -318,40 +327,37 @@ def _gated_mlp(act, x2d, gate_weight, up_weight, down_weight):
 
 
 def gated_mlp_fwd(act, x2d, gate_weight, up_weight, down_weight, keep=False):
-    """-> (y, and with `keep` x2d @ gate_weight^T and x2d @ up_weight^T, else None, None)"""
+    """-> (y, with `keep` what the backward call reads, else None)"""
     mlp, ldx = _gated_mlp(act, x2d, gate_weight, up_weight, down_weight)
-    new, device = torch.empty, x2d.device
-    y = new((mlp.M, mlp.n), dtype=BF16, device=device)
-    gate = up = None
-    if keep:
-        gate, up = new((mlp.M, mlp.f), dtype=BF16, device=device), new((mlp.M, mlp.f), dtype=BF16, device=device)
+    device = x2d.device
+    y = torch.empty((mlp.M, mlp.n), dtype=BF16, device=device)
+    kept = _new_kept(mlp.M, mlp.f, device) if keep else None
     nbytes = _lib.gated_mlp_bytes(mlp.M, mlp.h, mlp.f, mlp.n, False)
-    temp = new(nbytes, dtype=torch.uint8, device=device)
-    _lib.call("ezl_gated_mlp_fwd", mlp, x2d.data_ptr(), ldx, y.data_ptr(), _p(gate), _p(up), temp.data_ptr(), nbytes, _stream())
-    return y, gate, up
+    temp = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _lib.call("ezl_gated_mlp_fwd", mlp, x2d.data_ptr(), ldx, y.data_ptr(), _kept(kept, mlp.M, mlp.f) if keep else None, temp.data_ptr(), nbytes, _stream())
+    return y, kept
 
 
-def gated_mlp_bwd(act, dy2d, x2d, gate_weight, up_weight, down_weight, gate, up, want_dx, grads):
+def gated_mlp_bwd(act, dy2d, x2d, gate_weight, up_weight, down_weight, kept, want_dx, grads):
     """-> dx or None; the weights' gradients go to grads = (gate's, up's, down's), each (f32 or None, bf16 or None, accumulate), contiguous, or None, in the order down, gate, up."""
     mlp, ldx = _gated_mlp(act, x2d, gate_weight, up_weight, down_weight)
-    _ready((dy2d, gate, up), "dy gate up")
-    _need(dy2d.shape == (mlp.M, mlp.n) and gate.shape == up.shape == (mlp.M, mlp.f), "gated_mlp_bwd: shape mismatch")
+    _ready((dy2d,), "dy")
+    _need(dy2d.shape == (mlp.M, mlp.n), "gated_mlp_bwd: shape mismatch")
     targets = [_grad_target(g, w.numel(), what, shape=w.shape) for g, w, what in zip(grads, (gate_weight, up_weight, down_weight), ("gate weight", "up weight", "down weight"))]
     dx = torch.empty((mlp.M, mlp.h), dtype=BF16, device=x2d.device) if want_dx else None
     nbytes = _lib.gated_mlp_bytes(mlp.M, mlp.h, mlp.f, mlp.n, True)
     temp = torch.empty(nbytes, dtype=torch.uint8, device=x2d.device)
-    _lib.call("ezl_gated_mlp_bwd", mlp, x2d.data_ptr(), ldx, dy2d.data_ptr(), gate.data_ptr(), up.data_ptr(), _p(dx), *targets, temp.data_ptr(), nbytes, _stream())
+    _lib.call("ezl_gated_mlp_bwd", mlp, x2d.data_ptr(), ldx, dy2d.data_ptr(), _kept(kept, mlp.M, mlp.f), _p(dx), *targets, temp.data_ptr(), nbytes, _stream())
     return dx
 
 
-def gate_bwd(act, d, gate, up, want_mid=False):
-    """-> (d * up * act'(gate), d * act(gate), act(gate) * up or None)"""
-    _ready((d, gate, up), "d gate up")
-    _need(gate.shape == up.shape == d.shape, "gate_bwd shape mismatch")
-    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
-    mid = torch.empty_like(gate) if want_mid else None
-    _lib.call("ezl_gate_bwd", GATES[act], _p(d), _p(gate), _p(up), _p(dgate), _p(dup), _p(mid), gate.numel(), _stream())
-    return dgate, dup, mid
+def gate_bwd(act, d, kept):
+    """-> (d * up * act'(gate), d * act(gate)) of what gated_fwd kept"""
+    _ready((d,), "d")
+    T, f = d.shape
+    dgate, dup = torch.empty_like(d), torch.empty_like(d)
+    _lib.call("ezl_gate_bwd", GATES[act], d.data_ptr(), _kept(kept, T, f), dgate.data_ptr(), dup.data_ptr(), d.numel(), _stream())
+    return dgate, dup
 
 
 # ------------------------------------------------------------------------------------- RoPE

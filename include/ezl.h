@@ -116,22 +116,27 @@ int ezl_swiglu_bwd(const void* dout, const void* gate, const void* up, void* dga
 #define EZL_GATE_GELU 1
 #define EZL_GATE_GELU_TANH 2
 #define EZL_GATE_RELU 3
+/* What the backward pass reads of a gated block: its two products G and U [M, f], each rounded to 12 bits of mantissa; the upper halves of their fp32 bits (bf16 tensors), and in one
+ * byte for both the four bits behind those, G's in the lower half.  All contiguous, on 16 bytes. */
+typedef struct {
+    void *gate, *up, *low;
+} ezl_kept_gate; /* HOST struct */
 /* out[M, f] = act(x gate_weight^T) * (x up_weight^T) in one launch, fp32 from the reductions to the one rounding: x [M, K] (rows ldx elements apart), both weights [f, K] (rows
- * ldw apart).  gate and up (both or neither) receive the two products, rounded, for the backward pass.  out, gate, up contiguous; f % 8 == 0, below 2^21; K % 8 == 0, not 0.
+ * ldw apart).  kept (HOST pointer, or NULL) receives the two products.  out contiguous; f % 8 == 0, below 2^21; K % 8 == 0, not 0.
  * workspace as for ezl_gemm_bf16, ezl_gated_workspace_bytes(M, f, K) bytes. */
 int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K);
-int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* gate, void* up, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
+int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, const ezl_kept_gate* kept, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
                   void* workspace, int64_t workspace_bytes, void* stream);
-/* Its way back behind a down projection, from dy [M, K] (rows lddy apart) and down_weight [K, f] (rows ldw apart), in one launch: with d = dy down_weight, dgate = d * up * act'(gate),
- * dup = d * act(gate), and mid (may be NULL) = act(gate) * up again, which the down projection's weight gradient dy^T mid reads; d itself is not stored.  All [M, f], contiguous.
+/* Its way back behind a down projection, from dy [M, K] (rows lddy apart) and down_weight [K, f] (rows ldw apart), in one launch: with d = dy down_weight, dgate = d * U * act'(G),
+ * dup = d * act(G), and mid (may be NULL) = act(G) * U again, which the down projection's weight gradient dy^T mid reads; d itself is not stored.  All [M, f], contiguous.
  * workspace: ezl_gemm_workspace_bytes(M, f, K). */
-int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy,
-                  int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream);
-/* The same from a d that is there, n values of each, n % 8 == 0 (dgate may be gate or d, dup up). */
-int ezl_gate_bwd(int act, const void* d, const void* gate, const void* up, void* dgate, void* dup, void* mid, int64_t n, void* stream);
+int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const ezl_kept_gate* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy, int64_t ldw,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+/* The same from a bf16 d that is there, n values of each, n % 8 == 0 (dgate or dup may be d). */
+int ezl_gate_bwd(int act, const void* d, const ezl_kept_gate* kept, void* dgate, void* dup, int64_t n, void* stream);
 
 /* The whole block, y = (act(x gate^T) * (x up^T)) down^T, forward or backward in one call: x [M, h] (rows ldx apart), gate and up [f, h] (rows ldw apart), down [n, f] (rows ldd apart),
- * y and dy [M, n], contiguous.  gate_out and up_out [M, f], both or neither: what the backward call reads.  Of the gradients of the weights (contiguous; HOST pointers, NULL: not wanted) down's
+ * y and dy [M, n], contiguous.  kept (NULL forward: nothing) is what the backward call reads.  Of the gradients of the weights (contiguous; HOST pointers, NULL: not wanted) down's
  * is written first, then gate's, then up's: accumulate flags hold for that order.  dx [M, h], contiguous, or NULL.  temp: ezl_gated_mlp_bytes(.., backward) bytes, 256-byte aligned
  * best, 16 at least; free again when the call's work is done. */
 typedef struct {
@@ -141,9 +146,9 @@ typedef struct {
     int act;
 } ezl_gated_mlp; /* HOST struct */
 int64_t ezl_gated_mlp_bytes(const ezl_gated_mlp* mlp, int backward);
-int ezl_gated_mlp_fwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, void* y, void* gate_out, void* up_out, void* temp, int64_t temp_bytes, void* stream);
-int ezl_gated_mlp_bwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, const void* dy, const void* gate_out, const void* up_out, void* dx, const ezl_layer_grad* dgate,
-                      const ezl_layer_grad* dup, const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream);
+int ezl_gated_mlp_fwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, void* y, const ezl_kept_gate* kept, void* temp, int64_t temp_bytes, void* stream);
+int ezl_gated_mlp_bwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, const void* dy, const ezl_kept_gate* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
+                      const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream);
 
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----
  * table: cos/sin fp32 [npos, half_dim], theta = (p / scale_factor) * inv_freq[j].

@@ -2,14 +2,14 @@
 
 Tolerances, before any run.  E = 2^-24.  A sum of K products of bf16 values is off by at most 2 (K + 4) E times the sum of their magnitudes ("size").  An activation's slope is
 below 1.13 and its second derivative below 1.2 (ReLU's jumps: gates within their error of zero are left out by taking the larger of both slopes), its own arithmetic adds 2^-15 of its value.
-Roundings to bf16 are 2^-8 of a value: of gate and up where the backward pass reads them, of the products between the launches, of the results."""
+Roundings to bf16 are 2^-8 of a value: of the products between the launches, of the results.  gate and up, where the backward pass reads them, have 12 bits of mantissa: 2^-12."""
 import math
 
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
-E, H = 2.0 ** -24, 2.0 ** -8
+E, H, KEPT = 2.0 ** -24, 2.0 ** -8, 2.0 ** -12
 
 
 @pytest.fixture(scope="module")
@@ -52,6 +52,15 @@ def product(a, a_err, b, b_err=None):
     return a @ b, err + (a.abs() @ b.abs()) * (2 * (k + 4) * E)
 
 
+def kept_values(kept, T, f, rows=slice(None)):
+    """the two products of what K.gated_fwd kept, in fp64"""
+    n = T * f
+    gate, up = (kept[i * 2 * n:(i + 1) * 2 * n].view(torch.int16).view(T, f)[rows] for i in range(2))
+    low = kept[4 * n:].view(T, f)[rows].int()
+    bits = lambda upper, last: (upper.int() << 16 | last << 12).view(torch.float32).double()  # noqa: E731
+    return bits(gate, low & 15), bits(up, low >> 4)
+
+
 def expected(x, wg, wu, wd, dy, act):
     """name -> (reference, slack)"""
     x, wg, wu, wd = (t.detach().double() for t in (x, wg, wu, wd))
@@ -66,7 +75,7 @@ def expected(x, wg, wu, wd, dy, act):
         return a_err, err + (mid.abs() + err) * H
 
     out = {"y": product(mid, middle(g_err, u_err)[1], wd.t())}
-    g1, u1 = g_err + g.abs() * H, u_err + u.abs() * H  # (as the backward pass reads them)
+    g1, u1 = g_err + (g.abs() + g_err) * KEPT, u_err + (u.abs() + u_err) * KEPT  # (as the backward pass reads them)
     a_err, mid_err = middle(g1, u1)
     if dy is not None:
         dy = dy.double()
@@ -136,6 +145,24 @@ def test_forward_and_backward(F, T, h, f, act):
     check(F, T, h, f, act)
 
 
+@pytest.mark.parametrize("T,h,f", [(1, 8, 8), (5, 264, 1000), (8, 4096, 264), (17, 72, 520), (100, 520, 264), (257, 4096, 2048), (389, 4096, 512), (2500, 520, 4104), (4096, 1024, 4104)])
+def test_what_is_kept_has_12_bits(F, T, h, f):
+    """Either product within its own error and half a step of 12 bits, and not biased; infinities stay infinities."""
+    from easyllm_amd import kernels as K
+    x, wg, wu = rnd(T, h), rnd(f, h, seed=1, scale=h ** -0.5), rnd(f, h, seed=2, scale=h ** -0.5)
+    mid, kept = K.gated_fwd("silu", x, wg, wu, True)
+    alone, nothing = K.gated_fwd("silu", x, wg, wu)
+    assert nothing is None and torch.equal(mid, alone)
+    for got, w in zip(kept_values(kept, T, f), (wg, wu)):
+        ref, err = product(x.double(), None, w.double().t())
+        assert bool(((got - ref).abs() <= err + (ref.abs() + err) * KEPT).all())
+        # an error's mean over n values, each at most KEPT of its own and even about zero, lies within 6 KEPT |ref| / sqrt(n) of zero but for one in 10^8 (what the sums' own bias adds: err)
+        assert abs(float((got.abs() - ref.abs()).sum())) <= 6 * KEPT * float(ref.norm()) + float(err.sum())
+    x[0, 0] = float("inf")
+    gate, up = kept_values(K.gated_fwd("silu", x, wg, wu, True)[1], T, f)
+    assert bool((gate[0].abs() == float("inf")).all()) and bool((up[0] == wu[:, 0].double().sign() * float("inf")).all())
+
+
 @pytest.mark.parametrize("T,h,f,h_out", [(1, 4096, 11008, 4096), (4, 5120, 13696, 5120), (16, 4096, 4096, 1024), (40, 2048, 5504, 512), (1531, 1024, 2816, 1024)])
 def test_forward_alone(F, T, h, f, h_out):
     print("gated", T, h, f, h_out, flush=True)
@@ -157,7 +184,7 @@ def test_the_gate_alone(F, T, h, f, act):
     a_err = 1.2 * g_err + a.abs() * 2.0 ** -15
     near(mid, a * u, a_err * u.abs() + (a.abs() + a_err) * u_err, "mid")
     got = torch.autograd.grad(mid, (x, wg, wu), dmid)
-    g1, u1, d = g_err + g.abs() * H, u_err + u.abs() * H, dmid.double()
+    g1, u1, d = g_err + (g.abs() + g_err) * KEPT, u_err + (u.abs() + u_err) * KEPT, dmid.double()
     a_err, slope_err = 1.2 * g1 + a.abs() * 2.0 ** -15, 1.2 * g1 + slope.abs() * 2.0 ** -15
     if act == "relu":
         slope_err = (g.abs() <= g1).double()
@@ -291,17 +318,18 @@ def test_results_of_more_than_two_to_the_31_elements(F):
     T, h, f = (1 << 18) + 24, 64, 8200
     x, dy = rnd(T, h), rnd(T, h, seed=1)
     wg, wu, wd = rnd(f, h, seed=2, scale=0.125), rnd(f, h, seed=3, scale=0.125), rnd(h, f, seed=4, scale=f ** -0.5)
-    mid, gate, up = K.gated_fwd("silu", x, wg, wu, True)
+    mid, kept = K.gated_fwd("silu", x, wg, wu, True)
     rows = [*range(3), *range(T - 300, T)]
     g, u = x[rows].double() @ wg.double().t(), x[rows].double() @ wu.double().t()
     g_err, u_err = (2 * (h + 4) * E * (x[rows].double().abs() @ w.double().abs().t()) for w in (wg, wu))
     a, slope = act64(g, "silu")
-    near(gate[rows], g, g_err, "gate")
+    for got, ref, err in zip(kept_values(kept, T, f, rows), (g, u), (g_err, u_err)):
+        assert bool(((got - ref).abs() <= err + (ref.abs() + err) * KEPT).all())
     near(mid[rows], a * u, (1.2 * g_err + a.abs() * 2.0 ** -15) * (u.abs() + u_err) + a.abs() * u_err, "mid")
     del mid
-    y, _, _ = K.gated_mlp_fwd("silu", x, wg, wu, wd)
+    y, _ = K.gated_mlp_fwd("silu", x, wg, wu, wd)
     near(y[rows], *expected(x[rows], wg, wu, wd, None, "silu")["y"], "y")
-    dx = K.gated_mlp_bwd("silu", dy, x, wg, wu, wd, gate, up, True, (None, None, None))
+    dx = K.gated_mlp_bwd("silu", dy, x, wg, wu, wd, kept, True, (None, None, None))
     near(dx[rows], *expected(x[rows], wg, wu, wd, dy[rows], "silu")["x"], "dx")
 
 
