@@ -1408,7 +1408,7 @@ int64_t gemm_list_workspace_bytes(int pieces, const int* counts, const int64_t* 
 
 int gemm_list(int count, const void* const* A, const void* const* B, void* const* C, const int64_t* M, const int64_t* N, int64_t K,
               const int64_t* lda, const int64_t* ldb, const int64_t* ldc, int a_kc, int b_kc, int out_dtype, const int* accumulate,
-              void* workspace, int64_t workspace_bytes, void* stream) {
+              void* workspace, int64_t workspace_bytes, void* stream, bool large) {
     EZL_REQUIRE(count >= 1 && count <= kMaxProblems && A && B && C && M && N && lda && ldb && ldc && accumulate && K > 0, EZL_EINVAL,
                 "ezl_gemm_bf16_group: bad count, null argument array or empty reduction");
     EZL_REQUIRE((out_dtype == 0 && (a_kc || !b_kc)) || (out_dtype == 1 && !a_kc && !b_kc), EZL_EUNSUPPORTED,
@@ -1434,7 +1434,7 @@ int gemm_list(int count, const void* const* A, const void* const* B, void* const
         return EZL_OK;
     }
     GemmPlan plan;
-    bool list_256 = (a_kc ? b_kc && count > 1 : count > kGroupMax) && list_256_pays(!a_kc, count, M, N, K);
+    bool list_256 = (a_kc ? b_kc && count > 1 : count > kGroupMax || large) && list_256_pays(!a_kc, count, M, N, K);
     for (int i = 0; i < count; ++i) list_256 = list_256 && (out_dtype ? w4_stores_ok<float> : w4_stores_ok<bf16_t>)(C[i], N[i], ldc[i]);
     group_plan(!a_kc, count, M, N, K, INT64_MAX, plan, list_256);
     a.K = (int)K;

@@ -367,3 +367,38 @@ def test_refusals(F):
             F.gated_linear(x, wg, wu, activation)
     with pytest.raises((ValueError, RuntimeError)):
         F.gated_linear(x, wg, rnd(72, 56))
+
+
+@pytest.mark.parametrize("T,h,f", [(100, 72, 136), (1024, 256, 688), (1000, 768, 2048), (4000, 1536, 4096), (4100, 1544, 4104)])
+def test_weight_gradients_in_one_list(F, T, h, f):
+    """All three in fp32 and in bf16, on small tiles and 256 x 256 ones, and where one of them is of the other type (then they are no list)."""
+    x, dy = rnd(T, h), rnd(T, h, seed=1)
+    weights = [rnd(f, h, seed=2, scale=h ** -0.5), rnd(f, h, seed=3, scale=h ** -0.5), rnd(h, f, seed=4, scale=f ** -0.5)]
+    want = expected(x, *weights, dy, "silu")
+    for with_main in ((), (0, 1, 2), (2,), (0, 1), (1,)):
+        ws = [torch.nn.Parameter(w) for w in weights]
+        for i in with_main:
+            ws[i].main_grad = torch.full(ws[i].shape, 0.5, device="cuda")
+        F.gated_mlp(x, *ws).backward(dy)
+        for i, name in enumerate(("gate", "up", "down")):
+            ref, slack = want[name]
+            if i in with_main:
+                assert ws[i].grad is None and bool(((ws[i].main_grad.double() - 0.5 - ref).abs() <= slack + (ref.abs() + 0.5) * 2.0 ** -22).all()), (with_main, name)
+            else:
+                near(ws[i].grad, ref, slack, name)
+
+
+@pytest.mark.parametrize("T", [3, 100, 1024])
+def test_one_weight_in_all_three_places(F, T):
+    """Its gradients are written one behind the other, the first over what is there."""
+    n = 256
+    x, dy = rnd(T, n), rnd(T, n, seed=1)
+    w = torch.nn.Parameter(rnd(n, n, seed=2, scale=n ** -0.5))
+    want = expected(x, w, w, w, dy, "silu")
+    w.main_grad, w.main_grad_fresh = torch.full(w.shape, 7.0, device="cuda"), True
+    F.gated_mlp(x, w, w, w).backward(dy)
+    ref, slack = (sum(want[name][i] for name in ("down", "gate", "up")) for i in range(2))
+    size = sum(want[name][0].abs() for name in ("down", "gate", "up"))
+    assert bool(((w.main_grad.double() - ref).abs() <= slack + size * 2.0 ** -20).all())
+    (g,) = torch.autograd.grad(F.gated_mlp(x, u := w.detach().requires_grad_(), u, u), [u], dy)
+    assert bool(((g.double() - ref).abs() <= slack + 3 * H * (size + slack) + 2 * H * size).all())  # (three roundings of the parts, two of their sums)
