@@ -7,7 +7,7 @@
 // ---- gate and up as they are kept for the backward pass ----
 // In bf16 they would add as much again to the gradients' error as bf16 results have by themselves (relative error of dx and the weights' gradients 3.5e-3 instead of 2.4e-3, of
 // which the results' own rounding is 1.7e-3), in fp32 twice the bytes.  So each keeps 12 bits of mantissa: the upper half of its fp32 bits, rounded to 12 bits, in a bf16 tensor, and the
-// next four bits in half a byte of a third one, gate's in the lower half: five bytes the two, a quarter of the error's sixteenth part left.  A value is put together again by one byte
+// next four bits in half a byte of a third one, gate's in the lower half: five bytes the two, a sixteenth of the error left.  A value is put together again by one byte
 // permutation, as many instructions as widening a bf16; taking it apart costs three more a value.
 struct KeptParts {
     bf16_t *gate, *up;

@@ -564,7 +564,7 @@ class RotaryEmbedFunction(torch.autograd.Function):
 
 
 def _rotary_rows(x):
-    return x if x is None or x.dim() != 4 or K.rotary_in_place_ok(x) else x.contiguous()
+    return x if x is None or x.dim() != 4 or K.rotary_in_place_ok(x) else x.clone(memory_format=torch.contiguous_format)  # (`contiguous` would keep odd strides of single rows)
 
 
 def rotary_embed(q, k, inv_freq, position_ids=None, interleaved=False, scale=1.0):

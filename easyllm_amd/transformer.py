@@ -118,7 +118,7 @@ class ParallelMLP(torch.nn.Module):
     """down_proj(silu(gate_proj(x)) * up_proj(x)), or with glu_activation None down_proj(gelu(up_proj(x))), the products with their biases where
     mlp_bias is set and the activation in the first one's epilogue (exact; with the tanh where bias_gelu_fusion or use_openai_gelu ask for
     it).  Returns (output, output_bias); with `residual`, which the plain form takes, the whole sum and None.  glu_fusion: the gated form with any of kernels.GATES for an
-    activation, as `functional.gated_mlp`, which keeps two tensors of the block's width for backward where the composed form keeps three."""
+    activation, as `functional.gated_mlp`, which keeps five bytes a unit of the block's width for backward where the composed form keeps six."""
 
     def __init__(self, init_method, output_layer_init_method, hidden_size=1024, intermediate_size=4096,
                  use_cpu_initialization=False, params_dtype=torch.half, bias_gelu_fusion=False, glu_activation=None,

@@ -369,7 +369,7 @@ int ezl_adamw_list(int count, void* const* master, void* const* exp_avg, void* c
                    void* const* param_bf16, const int64_t* n, float lr, float beta1, float beta2, float eps, float weight_decay,
                    int64_t step, int bias_correction, const void* norm_coef, void* stream);
 
-/* ---- AdamW with moments of 8 bits (the reference's yaml type AdamW8bit, optimizer_helper.py) ----
+/* ---- AdamW with moments of 8 bits (beside the 32-bit step; llm/utils/model/optimizer_helper.py:70-98 is where the reference picks its optimizers) ----
  * Elements in blocks of 256.  A moment's block has a scale e: the exponent field of its largest |x|, as it is with 2^20 added to the fp32 bits
  * (255: not finite, the whole block reads as NaN).  A value's code is (bits of |x| 2^(K - e) + 16 r + 8) >> 20 with a random 16-bit r, so that it is right on
  * average: exp_avg K = 15, 7 bits and the sign above; exp_avg_sq K = 31, 8 bits, at least 1 where x > 0.  A code c stands for the fp32 number of the bits

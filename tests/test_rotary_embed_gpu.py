@@ -184,3 +184,19 @@ def test_forward_mode_derivatives_are_an_error(F):
         for call in (lambda: F.rotary_embed(dual, None, f), lambda: functional.gated_mlp(dual, *w), lambda: functional.gated_linear(dual, *w[:2])):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 call()
+
+
+def test_rows_that_lie_anywhere(F):
+    """Views whose rows do not begin on 16 bytes, and single rows whose strides are of the tensor they were cut from."""
+    inv_freq = frequencies(64)
+    whole = rnd(1, 1, 1, 129, seed=1)
+    for q in (whole[..., :128], whole[..., 1:], whole[0, :, :, 1:].unsqueeze(0), rnd(1 + 5 * 2 * 3 * 128, seed=2)[1:].view(5, 2, 3, 128), rnd(5, 2, 3, 136, seed=3)[..., 4:132],
+              rnd(128, 3, 2, 5, seed=4).permute(3, 2, 1, 0)):
+        q = q.detach().requires_grad_()
+        s, b = q.shape[:2]
+        positions = 77 * torch.arange(1, 1 + s * b, device="cuda").view(s, b).t()
+        y, _ = F.rotary_embed(q, None, inv_freq, positions)
+        check(y, q.detach(), inv_freq, positions, False, 1.0)
+        for dy in (rnd(*q.shape, seed=5), rnd(1, 1, 1, 129, seed=6)[..., 1:].expand(q.shape)):
+            (dq,) = torch.autograd.grad(y, q, dy, retain_graph=True)
+            check(dq, dy, inv_freq, positions, False, 1.0, back=True)
