@@ -1,4 +1,4 @@
-// Products of up to 8 rows whose weights are streamed once: act(X W^T) * (X W2^T) and X W^T, a handful of tokens through a gated MLP.
+// Products of up to 16 rows whose weights are streamed once: act(X W^T) * (X W2^T) and X W^T, a handful of tokens through a gated MLP.
 //
 // What bounds them is the weights' way from memory.  Every CU takes the same number of columns, to the column (as whole tiles of 16 some would take a fifth more), eight of W
 // and the same eight of W2 at a time, or sixteen of W alone: what a fragment has rows for past the CU's last column is read from that again, which costs

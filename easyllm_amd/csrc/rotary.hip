@@ -185,6 +185,8 @@ extern "C" int ezl_rotary(const ezl_rotary_side* q, const ezl_rotary_side* k, co
     a.sign = backward ? -1.f : 1.f;
     a.turned_slots = (int)(interleaved ? (turned + 7) / 8 : (turned / 2 + 7) / 8);
     a.slots = a.turned_slots + (int)((d - turned + 7) / 8);
+    EZL_REQUIRE(a.slots <= kRotaryBlock, EZL_EUNSUPPORTED, "ezl_rotary: a head's %lld elements, %lld of them turned, are more than %d pieces of 8", (long long)d, (long long)turned,
+                kRotaryBlock);
     const int most = kRotaryBlock / a.slots;  // heads a block has threads for
     // Heads of a thread: few items want threads, many want one set of angles and several loads each.  us with 1, 2, 4, 8, heads of 128, 32 + 8 of them: 1 token 3.0, 3.3, 3.9,
     // 4.9; 256 4.0, 3.8, 4.5, 5.5; 512 5.6, 4.5, 4.8, 6.0; 1024 8.4, 6.1, 6.3, 6.7; 2048 17.4, 10.8, 9.8, 10.2; 16384 of 32 + 32 136, 106, 91, 92; neighbours, which

@@ -161,7 +161,7 @@ int ezl_rope_apply(const void* x, void* out, const void* cos_table, const void* 
                    int backward, void* stream);
 /* Positions of either pairing, without a table: of every head's d elements the first `turned` (even) are pairs (j, j + turned / 2), or with
  * `interleaved` (2 j, 2 j + 1), that are turned by position * inv_freq[j] (turned / 2 fp32 values, or fp64; the product and its reduction are in fp64) and
- * multiplied by scale; the others are copied.  backward != 0 turns the other way (the gradient).  A side is x [s, b, heads, d] with its strides in elements
+ * multiplied by scale; the others are copied.  d: a multiple of 8 up to 2048, in at most 256 pieces of 8 (turned and copied parts each rounded up).  backward != 0 turns the other way (the gradient).  A side is x [s, b, heads, d] with its strides in elements
  * (multiples of 8, 0 allowed) and a contiguous out [s, b, heads, d]; k (HOST pointers both) may be NULL.  position_ids int64 with its strides, any value below 2^31 or so (an
  * angle is off by position * 2^-52), or NULL (position = s index). */
 typedef struct {

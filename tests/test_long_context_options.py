@@ -110,12 +110,14 @@ def test_the_library_refuses_before_it_launches():
     lib = _lib.load()
     side = _lib.RotarySide(16, 16, 2, 128, 128, 64)
 
-    def rotary(q=side, k=None, inv=16, s=4, b=1, d=64, turned=64, pos=None):
-        return lib.ezl_rotary(q, k, inv, 0, pos, 1, 1, s, b, d, turned, 0, 1.0, 0, None)
+    def rotary(q=side, k=None, inv=16, s=4, b=1, d=64, turned=64, pos=None, interleaved=0):
+        return lib.ezl_rotary(q, k, inv, 0, pos, 1, 1, s, b, d, turned, interleaved, 1.0, 0, None)
     for kw in (dict(q=None), dict(inv=None), dict(inv=18), dict(s=-1), dict(s=1 << 31), dict(d=60), dict(d=2056, turned=64), dict(turned=0), dict(turned=33), dict(turned=66), dict(pos=20),
                dict(q=_lib.RotarySide(None, 16, 2, 128, 128, 64)), dict(q=_lib.RotarySide(16, 24, 2, 128, 128, 64)), dict(q=_lib.RotarySide(16, 16, 2, 124, 128, 64)),
                dict(q=_lib.RotarySide(16, 16, -1, 128, 128, 64)), dict(q=_lib.RotarySide(16, 16, 2, 128, 128, -64)), dict(k=_lib.RotarySide(16, None, 2, 128, 128, 64))):
         assert rotary(**kw) in (-1, -2), kw
+    for turned, interleaved in ((2, 0), (6, 0), (2, 1), (1026, 1)):  # (257 pieces of 8 elements, one more than a workgroup has threads)
+        assert rotary(d=2048, turned=turned, interleaved=interleaved) == -2, (turned, interleaved)
     assert rotary(s=0) == 0 and rotary(q=_lib.RotarySide(None, None, 0, 0, 0, 0)) == 0
 
     def tensor(n=10, number=0, **kw):
