@@ -42,11 +42,6 @@ class GatedMLP(ctypes.Structure):
     _fields_ = [(n, _i64) for n in ("M", "h", "f", "n")] + [(n, _vp) for n in ("gate", "up", "down")] + [("ldw", _i64), ("ldd", _i64), ("act", _i32)]
 
 
-class KeptGate(ctypes.Structure):
-    """struct ezl_kept_gate"""
-    _fields_ = [("gate", _vp), ("up", _vp), ("low", _vp)]
-
-
 class RotarySide(ctypes.Structure):
     """struct ezl_rotary_side"""
     _fields_ = [("x", _vp), ("out", _vp), ("heads", _i64), ("seq_stride", _i64), ("batch_stride", _i64), ("head_stride", _i64)]
@@ -64,7 +59,6 @@ class Adam8(ctypes.Structure):
 
 _layerp = ctypes.POINTER(Layer)
 _mlpp = ctypes.POINTER(GatedMLP)
-_keptp = ctypes.POINTER(KeptGate)
 _sidep = ctypes.POINTER(RotarySide)
 _adam8p = ctypes.POINTER(Adam8Tensor)
 _dropp = ctypes.POINTER(Dropout)
@@ -87,11 +81,11 @@ SIGNATURES = {
     "ezl_rope_apply": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp],
     "ezl_rope_apply_pair": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "ezl_rotary": [_sidep, _sidep, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f32, _i32, _vp],
-    "ezl_gated_fwd": [_i32, _vp, _vp, _vp, _vp, _keptp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
-    "ezl_gated_bwd": [_i32, _vp, _vp, _keptp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
-    "ezl_gate_bwd": [_i32, _vp, _keptp, _vp, _vp, _i64, _vp],
-    "ezl_gated_mlp_fwd": [_mlpp, _vp, _i64, _vp, _keptp, _vp, _i64, _vp],
-    "ezl_gated_mlp_bwd": [_mlpp, _vp, _i64, _vp, _keptp, _vp, _gradp, _gradp, _gradp, _vp, _i64, _vp],
+    "ezl_gated_fwd": [_i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
+    "ezl_gated_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
+    "ezl_gate_bwd": [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
+    "ezl_gated_mlp_fwd": [_mlpp, _vp, _i64, _vp, _vp, _vp, _i64, _vp],
+    "ezl_gated_mlp_bwd": [_mlpp, _vp, _i64, _vp, _vp, _vp, _gradp, _gradp, _gradp, _vp, _i64, _vp],
     "ezl_adamw8_list": [_i32, _adam8p, ctypes.POINTER(Adam8), _vp, _vp],
     "ezl_moments8_list": [_i32, _adam8p, _vpp, _vpp, _vp],
     "ezl_ids_in_range": [_vp, _i64, _i64, _vp, _vp],
@@ -149,6 +143,7 @@ _SPECIAL = {
     "ezl_attn_plan": ([_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64], _i32),
     "ezl_gemm_workspace_bytes": ([_i64, _i64, _i64], _i64),
     "ezl_gated_workspace_bytes": ([_i64, _i64, _i64], _i64),
+    "ezl_gated_kept_bytes": ([_i64, _i64], _i64),
     "ezl_gated_mlp_bytes": ([_mlpp, _i32], _i64),
     "ezl_gemm_group_workspace_bytes": ([_i32, _i64p, _i64p, _i64], _i64),
     "ezl_gemm_group_form_workspace_bytes": ([_i32, _i32, _i64p, _i64p, _i64], _i64),

@@ -1,5 +1,4 @@
-// The way back through the gate of an MLP as a pass of its own, where no product of the framework's stands in front of it.  HBM-bound: 11 bytes a value,
-// 4096 x 11008 in 87 us (5.7 TB/s), 8192 x 2816 in 44 (5.8), 1024 x 688 in 3.3.
+// The way back through the gate of an MLP as a pass of its own, where no product of the framework's stands in front of it.  HBM-bound: 11 bytes a value.
 #include "common.h"
 #include "gate.h"
 
@@ -7,45 +6,46 @@ namespace {
 
 constexpr int kGateBlock = 256;
 
-// dgate = d * up * act'(gate), dup = d * act(gate)
-template <int ACT, bool STREAM>
-__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const KeptParts kept, bf16_t* dgate, bf16_t* dup, int64_t n8) {
-    for (int64_t i = (int64_t)blockIdx.x * kGateBlock + threadIdx.x; i < n8; i += (int64_t)gridDim.x * kGateBlock) {
-        const u32x4 kg = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kept.gate) + i), ku = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kept.up) + i);
-        const u32x2 kl = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kept.low) + i);
-        float g[8], u[8], d[8], dg[8], du[8];
-        kept_values<8>({kg[0], kg[1], kg[2], kg[3]}, {ku[0], ku[1], ku[2], ku[3]}, {kl[0], kl[1]}, g, u);
-        unpack8(ld_bf16x8_nt(d_in + i * 8), d);
+// dgate = d * up * act'(gate), dup = d * act(gate): a workgroup takes a row of four blocks of what was kept, a wave eight rows of two, so that d and the results are read and written in whole
+// lines as what was kept is.  4096 x 11008 in 87 us (5.7 TB/s), 8192 x 2816 48, 1531 x 11008 32; where rows end inside a line, 15094 x 15336, 647 (3.9 TB/s: both ends of a wave's pieces are
+// lines that others hold, too; past the caches 750, with a wave on one block 963).
+template <int ACT>
+__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const Kept kept, bf16_t* dgate, bf16_t* dup, int64_t M, int f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = (wave & 1) * 8 + (lane >> 3), col = (blockIdx.x * 2 + (wave >> 1)) * 2 * kKeptCols + (lane & 7) * 8;
+    if (col >= f) return;
+    for (int64_t rows = blockIdx.y; rows * kKeptRows + row < M; rows += gridDim.y) {
+        const KeptPlace from = kept_place(kept, rows * kKeptRows + row, col);
+        const u32x4 kg = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from.upper)), ku = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from.upper + kKeptUp));
+        const u32x2 kl = *reinterpret_cast<const u32x2*>(from.low);
+        const int64_t at = (rows * kKeptRows + row) * f + col;
+        float gate[8], up[8], d[8], dg[8], du[8];
+        unpack8(ld_bf16x8(d_in + at), d);
+        kept_values<8>({kg[0], kg[1], kg[2], kg[3]}, {ku[0], ku[1], ku[2], ku[3]}, {kl[0], kl[1]}, gate, up);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float y, slope;
-            gate_value_slope<ACT>(g[k], y, slope);
-            dg[k] = d[k] * u[k] * slope;
+            gate_value_slope<ACT>(gate[k], y, slope);
+            dg[k] = d[k] * up[k] * slope;
             du[k] = d[k] * y;
         }
-        st_result<STREAM>(dgate + i * 8, pack8(dg));
-        st_result<STREAM>(dup + i * 8, pack8(du));
+        st_bf16x8(dgate + at, pack8(dg));
+        st_bf16x8(dup + at, pack8(du));
     }
-}
-
-unsigned gate_grid(int64_t n8) {
-    const int64_t blocks = (n8 + kGateBlock - 1) / kGateBlock;
-    return (unsigned)(blocks < 8192 ? blocks : 8192);
 }
 
 }  // namespace
 
-extern "C" int ezl_gate_bwd(int act, const void* d, const ezl_kept_gate* kept, void* dgate, void* dup, int64_t n, void* stream) {
+extern "C" int ezl_gate_bwd(int act, const void* d, const void* kept, void* dgate, void* dup, int64_t M, int64_t f, void* stream) {
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "ezl_gate_bwd: act must be one of EZL_GATE_*");
-    EZL_REQUIRE(n >= 0 && n % 8 == 0, EZL_EUNSUPPORTED, "ezl_gate_bwd: n must be a multiple of 8");
-    EZL_REQUIRE(n == 0 || (d && kept && kept->gate && kept->up && kept->low && dgate && dup && ezl_aligned16(d) && ezl_aligned16(kept->gate) && ezl_aligned16(kept->up) &&
-                           ezl_aligned16(kept->low) && ezl_aligned16(dgate) && ezl_aligned16(dup)),
-                EZL_EINVAL, "ezl_gate_bwd: null or misaligned pointer");
-    if (n == 0) return EZL_OK;
-    constexpr decltype(&gate_bwd_kernel<0, false>) kernels[][2] = {{gate_bwd_kernel<0, false>, gate_bwd_kernel<0, true>}, {gate_bwd_kernel<1, false>, gate_bwd_kernel<1, true>},
-                                                                    {gate_bwd_kernel<2, false>, gate_bwd_kernel<2, true>}, {gate_bwd_kernel<3, false>, gate_bwd_kernel<3, true>}};
-    const KeptParts parts = {(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low};
-    hipLaunchKernelGGL(kernels[act][ezl_streams(n * 4)], dim3(gate_grid(n / 8)), dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, parts, (bf16_t*)dgate, (bf16_t*)dup, n / 8);
+    EZL_REQUIRE(M >= 0 && f >= 0 && f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "ezl_gate_bwd: the width must be a multiple of 8 below 2^21");
+    if (M == 0 || f == 0) return EZL_OK;
+    EZL_REQUIRE(d && kept && dgate && dup && ezl_aligned16(d) && ezl_aligned16(kept) && ezl_aligned16(dgate) && ezl_aligned16(dup), EZL_EINVAL, "ezl_gate_bwd: null or misaligned pointer");
+    constexpr decltype(&gate_bwd_kernel<0>) kernels[] = {gate_bwd_kernel<0>, gate_bwd_kernel<1>, gate_bwd_kernel<2>, gate_bwd_kernel<3>};
+    const Kept from = kept_of(kept, f);
+    const int64_t rows = (M + kKeptRows - 1) / kKeptRows;
+    const dim3 grid((unsigned)((from.blocks + 3) / 4), (unsigned)(rows < 65535 ? rows : 65535));
+    hipLaunchKernelGGL(kernels[act], grid, dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, from, (bf16_t*)dgate, (bf16_t*)dup, M, (int)f);
     EZL_LAUNCH_CHECK("ezl_gate_bwd");
     return EZL_OK;
 }

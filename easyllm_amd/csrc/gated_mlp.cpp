@@ -54,7 +54,7 @@ extern "C" int64_t ezl_gated_mlp_bytes(const ezl_gated_mlp* m, int backward) {
     return 3 * block_bytes(*m) + ws;
 }
 
-extern "C" int ezl_gated_mlp_fwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, void* y, const ezl_kept_gate* kept, void* temp, int64_t temp_bytes, void* stream) {
+extern "C" int ezl_gated_mlp_fwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, void* y, void* kept, void* temp, int64_t temp_bytes, void* stream) {
     const char* name = "ezl_gated_mlp_fwd";
     if (const int rc = check(name, m)) return rc;
     if (m->M == 0) return EZL_OK;
@@ -66,14 +66,14 @@ extern "C" int ezl_gated_mlp_fwd(const ezl_gated_mlp* m, const void* x, int64_t 
     if (gemm_rows_pays(m->M, m->n, m->f)) return ezl_gemm_bf16_epilogue(temp, m->down, y, m->M, m->n, m->f, m->f, m->ldd, m->n, &none, ws, ws_bytes, stream);
     if (stream_down_pays(m->M, m->f)) {
         EZL_REQUIRE(ezl_aligned16(m->down) && m->ldd % 8 == 0 && m->ldd >= m->f && m->ldd < (1LL << 22), EZL_EINVAL, "%s: bad down projection", name);
-        stream_rows_launch(temp, m->down, nullptr, y, KeptParts{}, (int)m->M, (int)m->n, (int)m->f, m->f, m->ldd, 0, (hipStream_t)stream);
+        stream_rows_launch(temp, m->down, nullptr, y, Kept{}, (int)m->M, (int)m->n, (int)m->f, m->f, m->ldd, 0, (hipStream_t)stream);
         EZL_LAUNCH_CHECK(name);
         return EZL_OK;
     }
     return ezl_gemm_bf16(temp, m->down, y, m->M, m->n, m->f, m->f, m->ldd, m->n, 1, 1, 0, 0, ws, ws_bytes, stream);
 }
 
-extern "C" int ezl_gated_mlp_bwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, const void* dy, const ezl_kept_gate* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
+extern "C" int ezl_gated_mlp_bwd(const ezl_gated_mlp* m, const void* x, int64_t ldx, const void* dy, const void* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
                                  const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream) {
     const char* name = "ezl_gated_mlp_bwd";
     if (const int rc = check(name, m)) return rc;

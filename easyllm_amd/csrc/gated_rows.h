@@ -14,5 +14,5 @@ inline bool stream_rows_fit(int64_t M, int64_t K) { return M <= kStreamMaxRows &
 inline bool stream_pairs_pay(int64_t M, int64_t K) { return M <= 8 && stream_rows_fit(M, K); }
 inline bool stream_down_pays(int64_t M, int64_t K) { return M * K <= 48 * 1024 && stream_rows_fit(M, K); }
 // C[M, cols] = act(X W^T) * (X W2^T), or with W2 null X W^T; all rows on 16 bytes, C contiguous
-__attribute__((visibility("hidden"))) void stream_rows_launch(const void* X, const void* W, const void* W2, void* C, const KeptParts& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act,
+__attribute__((visibility("hidden"))) void stream_rows_launch(const void* X, const void* W, const void* W2, void* C, const Kept& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act,
                                                               hipStream_t st);

@@ -15,7 +15,7 @@ constexpr int kWaves = 8;
 // SB: 64-wide blocks of K that a wave has in registers
 template <int SB, bool PAIRS>
 __global__ __launch_bounds__(kWaves * 64) void stream_rows_kernel(const bf16_t* __restrict__ X, const bf16_t* __restrict__ W, const bf16_t* __restrict__ W2, bf16_t* __restrict__ C,
-                                                                  const KeptParts kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, int segments) {
+                                                                  const Kept kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, int segments) {
     constexpr int COLS = PAIRS ? 8 : 16;  // of a tile
     __shared__ __attribute__((aligned(16))) bf16_t tokens[kStreamLdsBytes / 2];
     __shared__ f32x4 sums[2][kWaves][64];
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kWaves * 64) void stream_rows_kernel(const bf16_t* 
                 if constexpr (PAIRS) {
                     y = (act == EZL_GATE_SILU ? gate_value<EZL_GATE_SILU>(y) : act == EZL_GATE_GELU ? gate_value<EZL_GATE_GELU>(y)
                          : act == EZL_GATE_GELU_TANH ? gate_value<EZL_GATE_GELU_TANH>(y) : gate_value<EZL_GATE_RELU>(y)) * b[e];
-                    if (kept.gate) keep_one(a[e], b[e], kept, at + e);
+                    if (kept.p) keep_one(a[e], b[e], kept, r, n + e);
                 }
                 C[at + e] = (bf16_t)y;
             }
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(kWaves * 64) void stream_rows_kernel(const bf16_t* 
 }
 
 template <bool PAIRS>
-void launch_stream(const void* X, const void* W, const void* W2, void* C, const KeptParts& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, hipStream_t st) {
+void launch_stream(const void* X, const void* W, const void* W2, void* C, const Kept& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, hipStream_t st) {
     const int tiles = (cols + (PAIRS ? 7 : 15)) / (PAIRS ? 8 : 16), blocks = (K + 64 * kWaves - 1) / (64 * kWaves);
     const int segments = (blocks + 15) / 16, sb = (blocks + segments - 1) / segments;
     const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
@@ -147,6 +147,6 @@ void launch_stream(const void* X, const void* W, const void* W2, void* C, const 
 
 }  // namespace
 
-void stream_rows_launch(const void* X, const void* W, const void* W2, void* C, const KeptParts& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, hipStream_t st) {
+void stream_rows_launch(const void* X, const void* W, const void* W2, void* C, const Kept& kept, int M, int cols, int K, int64_t ldx, int64_t ldw, int act, hipStream_t st) {
     (W2 ? launch_stream<true> : launch_stream<false>)(X, W, W2, C, kept, M, cols, K, ldx, ldw, act, st);
 }

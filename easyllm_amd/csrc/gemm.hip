@@ -575,7 +575,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const bf16_t* __restric
             } else if constexpr (kGate<EPI>) {
                 EPI e = epi;
                 int l = lane;
-                asm volatile("" : "+s"(e.ld), "+v"(l));
+                if constexpr (kPairs<EPI>) asm volatile("" : "+s"(e.kept.blocks), "+v"(l));
+                else asm volatile("" : "+s"(e.ld), "+s"(e.kept.blocks), "+v"(l));
                 store_tile_gate<EPI, TM, 8>(acc, Ct, ld, mrem, N - it.n0, arow, kPairs<EPI> ? brow / 2 : brow, l, e.at(it.m0, it.n0));
             } else store_tile_flags<TM, 8, OutT, true, A_KC && B_KC>(acc, Ct, ld, mrem, N - it.n0, arow, brow, lane, accumulate);
         }
@@ -1114,7 +1115,9 @@ void launch_gate(const void* A, const void* B, void* C, int M, int N, int K, int
     const int tiles_m = (M + bm - 1) / bm, tiles_n = (N + cols - 1) / cols;
     const SplitPlan split = make_plan(kind, lines, (int64_t)tiles_m * tiles_n, nk, workspace, workspace_bytes);
     const int items = split.full + split.rest * split.nsplit;
-#define EZL_W4(KTAIL, TBM)                                                                                                                                         hipLaunchKernelGGL((gemm_w4_kernel<true, B_KC, bf16_t, false, KTAIL, false, TBM, EPI>), w4_grid(items), dim3(256), 0, st, (const bf16_t*)A, (const bf16_t*)B,                        (bf16_t*)C, M, N, K, lda, ldb, ldc, 0, tiles_m, tiles_n, items, split, KSegments(), NoList(), epi)
+#define EZL_W4(KTAIL, TBM)                                                                                                                                      \
+    hipLaunchKernelGGL((gemm_w4_kernel<true, B_KC, bf16_t, false, KTAIL, false, TBM, EPI>), w4_grid(items), dim3(256), 0, st, (const bf16_t*)A, (const bf16_t*)B, \
+                       (bf16_t*)C, M, N, K, lda, ldb, ldc, 0, tiles_m, tiles_n, items, split, KSegments(), NoList(), epi)
     if (kind == kTile192x256) EZL_W4(false, 192);
     else if (tail) EZL_W4(true, 256);
     else EZL_W4(false, 256);
@@ -1225,44 +1228,45 @@ extern "C" int ezl_gemm_bf16_epilogue(const void* A, const void* B, void* C, int
     return EZL_OK;
 }
 
+extern "C" int64_t ezl_gated_kept_bytes(int64_t M, int64_t f) {
+    return M <= 0 || f <= 0 ? 0 : (M + kKeptRows - 1) / kKeptRows * ((f + kKeptCols - 1) / kKeptCols) * kKeptBlock;
+}
 extern "C" int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K) { return M <= 0 || f <= 0 || K <= 0 ? 0 : plan_bytes(M, gate_columns(true, f), K); }
 
-extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, const ezl_kept_gate* kept, int64_t M, int64_t f, int64_t K, int64_t ldx,
-                             int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* kept, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
     const char* name = "ezl_gated_fwd";
     EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
-    const KeptParts parts = kept ? KeptParts{(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low} : KeptParts{};
-    EZL_REQUIRE(!kept || M == 0 || f == 0 || (parts.gate && parts.up && parts.low), EZL_EINVAL, "%s: what is kept needs all of its parts", name);
     if (M == 0 || f == 0) return EZL_OK;
     EZL_REQUIRE(out && up_weight, EZL_EINVAL, "%s: null pointer", name);
     EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
     if (const int rc = check_operands(x, gate_weight, M, f, K, ldx, ldw, f, 1, 1)) return rc;
-    EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(parts.gate) && ezl_aligned16(parts.up) && ezl_aligned16(parts.low) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
+    EZL_REQUIRE(ezl_aligned16(up_weight) && ezl_aligned16(out) && ezl_aligned16(kept) && ezl_aligned16(workspace), EZL_EINVAL, "%s: pointers must be 16-byte aligned", name);
     if (stream_pairs_pay(M, K)) {
-        stream_rows_launch(x, gate_weight, up_weight, out, parts, (int)M, (int)f, (int)K, ldx, ldw, act, (hipStream_t)stream);
+        stream_rows_launch(x, gate_weight, up_weight, out, kept_of(kept, f), (int)M, (int)f, (int)K, ldx, ldw, act, (hipStream_t)stream);
         EZL_LAUNCH_CHECK(name);
         return EZL_OK;
     }
     launch_gate<GateForward>(x, gate_weight, out, (int)M, (int)f, (int)K, ldx, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
-                             {(const bf16_t*)up_weight, parts, f, act});
+                             {(const bf16_t*)up_weight, kept_of(kept, f), act});
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;
 }
 
-extern "C" int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const ezl_kept_gate* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K,
+extern "C" int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K,
                              int64_t lddy, int64_t ldw, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* name = "ezl_gated_bwd";
     EZL_REQUIRE(M >= 0 && f >= 0 && K > 0, EZL_EINVAL, "%s: negative size or empty reduction", name);
     EZL_REQUIRE(act >= EZL_GATE_SILU && act <= EZL_GATE_RELU, EZL_EINVAL, "%s: act must be one of EZL_GATE_*", name);
     if (M == 0 || f == 0) return EZL_OK;
-    EZL_REQUIRE(kept && kept->gate && kept->up && kept->low && dgate && dup, EZL_EINVAL, "%s: null pointer", name);
+    EZL_REQUIRE(kept && dgate && dup, EZL_EINVAL, "%s: null pointer", name);
     EZL_REQUIRE(f % 8 == 0 && f < (1LL << 21), EZL_EUNSUPPORTED, "%s: the width must be a multiple of 8 below 2^21", name);
     if (const int rc = check_operands(dy, down_weight, M, f, K, lddy, ldw, f, 1, 0)) return rc;
-    EZL_REQUIRE(ezl_aligned16(kept->gate) && ezl_aligned16(kept->up) && ezl_aligned16(kept->low) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) && ezl_aligned16(workspace), EZL_EINVAL,
+    EZL_REQUIRE(ezl_aligned16(kept) && ezl_aligned16(dgate) && ezl_aligned16(dup) && ezl_aligned16(mid) && ezl_aligned16(workspace), EZL_EINVAL,
                 "%s: pointers must be 16-byte aligned", name);
     launch_gate<GateBackward>(dy, down_weight, dgate, (int)M, (int)f, (int)K, lddy, ldw, f, workspace, workspace_bytes, (hipStream_t)stream,
-                              {{(bf16_t*)kept->gate, (bf16_t*)kept->up, (uint8_t*)kept->low}, (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, f, act});
+                              {kept_of(kept, f), (bf16_t*)dgate, (bf16_t*)dup, (bf16_t*)mid, f, act});
     EZL_LAUNCH_CHECK(name);
     return EZL_OK;
 }

@@ -452,22 +452,25 @@ __global__ __launch_bounds__(256) void gate_reduce_kernel(const float* __restric
             f32x4 y;
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = gate_value<act>(g[r]) * u[r];
-            if (epi.kept.gate) {
+            if (epi.kept.p) {
                 const float gs[4] = {g[0], g[1], g[2], g[3]}, us[4] = {u[0], u[1], u[2], u[3]};
                 uint32_t kg[2], ku[2], kl[1];
                 keep<4>(gs, us, kg, ku, kl);
-                const int64_t to = (int64_t)row * epi.ld + col;
-                *reinterpret_cast<u32x2*>(epi.kept.gate + to) = u32x2{kg[0], kg[1]};
-                *reinterpret_cast<u32x2*>(epi.kept.up + to) = u32x2{ku[0], ku[1]};
-                *reinterpret_cast<uint32_t*>(epi.kept.low + to) = kl[0];
+                const KeptPlace to = kept_place(epi.kept, row, col);
+                const int half = col >> 2 & 1;  // (of the place's eight columns)
+                *reinterpret_cast<u32x2*>(to.upper + half * 8) = u32x2{kg[0], kg[1]};
+                *reinterpret_cast<u32x2*>(to.upper + kKeptUp + half * 8) = u32x2{ku[0], ku[1]};
+                *reinterpret_cast<uint32_t*>(to.low + half * 4) = kl[0];
             }
             store(C + (int64_t)row * ldc + col, y);
         } else {
             const f32x4 d = sum(cl);
             const int64_t at = (int64_t)row * epi.ld + col;
-            const u32x2 kg = *reinterpret_cast<const u32x2*>(epi.kept.gate + at), ku = *reinterpret_cast<const u32x2*>(epi.kept.up + at);
+            const KeptPlace from = kept_place(epi.kept, row, col);
+            const int half = col >> 2 & 1;
+            const u32x2 kg = *reinterpret_cast<const u32x2*>(from.upper + half * 8), ku = *reinterpret_cast<const u32x2*>(from.upper + kKeptUp + half * 8);
             float g[4], u[4];
-            kept_values<4>({kg[0], kg[1]}, {ku[0], ku[1]}, {*reinterpret_cast<const uint32_t*>(epi.kept.low + at)}, g, u);
+            kept_values<4>({kg[0], kg[1]}, {ku[0], ku[1]}, {*reinterpret_cast<const uint32_t*>(from.low + half * 4)}, g, u);
             f32x4 dg, du, mid;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {

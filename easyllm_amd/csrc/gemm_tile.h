@@ -40,31 +40,27 @@ struct Epilogue {
 };
 
 // The first products of a gated MLP as one: C = act(A B^T) * (A B2^T), forward form, B and B2 alike.  A tile's columns are taken 16 of B, the same 16 of B2, and so on: the two
-// accumulators of a result lie in one lane, and a tile of 256 columns makes 128 of C.  `kept` (its pointers null: nothing) receives the two products for the backward pass; C is made of them as
-// they are.  What it costs is the stores: tokens x h x f 4096 x 4096 x 11008 514 us, keeping the products 575; the two products alone 524 and a pass for the gate behind them 47 (8192 x 1024
-// x 2816: 82, 104 and 82 + 24; 1024 x 256 x 688: 5.5, 6.4 and 5.5 + 3.0).
+// accumulators of a result lie in one lane, and a tile of 256 columns makes 128 of C.  `kept` receives the two products for the backward pass; C is made of them as
+// they are.  What it costs is the stores: tokens x h x f 4096 x 4096 x 11008 529 us, keeping the products 563; the two products alone 540 and a pass for the gate behind them 47 (8192 x 1024
+// x 2816: 82, 95 and 84 + 24; 1024 x 256 x 688: 5.5, 6.4 and 5.5 + 3.0).
 struct GateForward {
     const bf16_t* B2;
-    KeptParts kept;
-    int64_t ld;  // of what is kept
+    Kept kept;
     int act;
-    __device__ __forceinline__ GateForward at(int64_t m, int64_t n) const {
-        const int64_t o = m * ld + n;
-        return {B2, kept.gate ? KeptParts{kept.gate + o, kept.up + o, kept.low + o} : kept, ld, act};
-    }
+    __device__ __forceinline__ GateForward at(int64_t m, int64_t n) const { return {B2, kept.at(m, n), act}; }
 };
 // The way back through it behind the input gradient d = A B of the down projection: dgate = d * up * act'(gate), dup = d * act(gate), and mid (may be null) =
 // act(gate) * up once more, which the down projection's weight gradient reads.  d itself is stored nowhere.  All [M, N], rows ld apart.
-// Tokens x h x f 4096 x 4096 x 11008 367 us, the product alone 272 and a pass that reads d 105 (87 without mid); 8192 x 1024 x 2816 102 against 45 + 57; 1531 x 4096 x 11008 152 against
-// 114 + 38: the fetches of a tile's five bytes a value and the stores of its six come when no product runs on that CU, so the launch gains d's four bytes and a launch, no more.
+// Tokens x h x f 4096 x 4096 x 11008 357 us, the product alone 276 and a pass that reads d 105 (87 without mid); 8192 x 1024 x 2816 95 against 46 + 57; 1531 x 4096 x 11008 149 against
+// 118 + 38: the fetches of a tile's five bytes a value and the stores of its six come when no product runs on that CU, so the launch gains d's four bytes and a launch, no more.
 struct GateBackward {
-    KeptParts kept;
+    Kept kept;
     bf16_t *dgate, *dup, *mid;
     int64_t ld;
     int act;
     __device__ __forceinline__ GateBackward at(int64_t m, int64_t n) const {
         const int64_t o = m * ld + n;
-        return {{kept.gate + o, kept.up + o, kept.low + o}, dgate + o, dup + o, mid ? mid + o : nullptr, ld, act};
+        return {kept.at(m, n), dgate + o, dup + o, mid ? mid + o : nullptr, ld, act};
     }
 };
 template <class EPI>
@@ -494,6 +490,22 @@ __device__ __forceinline__ void store_epilogue(float (&v)[N], bf16_t* C, int64_t
     store(C + m * ldc + n);
 }
 
+// Where a wave's pieces of 16 rows and 32 columns of what a gated MLP keeps lie, seen from the tile's first block: piece (i, b) of the wave's rows row0 + 16 i and columns col0 + 32 b, lane by
+// lane.  (A tile's 256 rows span less than 2.7 GB: its offsets fit 32 bits, and what lies past its last row is past the buffer's end.)
+struct KeptPieces {
+    __amdgpu_buffer_rsrc_t buf;
+    uint32_t upper, low, step;
+    int col0, nrem;
+    __device__ __forceinline__ KeptPieces(const Kept& k, int mrem, int nrem_, int row0, int col0_, int lane)
+        : upper((uint32_t)((row0 / kKeptRows * k.blocks + col0_ / kKeptCols) * kKeptBlock)), step((uint32_t)(k.blocks * kKeptBlock)), col0(col0_), nrem(nrem_) {
+        const int rows = (min(mrem, 256) + kKeptRows - 1) / kKeptRows, cols = (min(nrem, 256) + kKeptCols - 1) / kKeptCols;
+        buf = __builtin_amdgcn_make_buffer_rsrc(k.p, 0, ((uint32_t)(rows - 1) * (uint32_t)k.blocks + (uint32_t)cols) * (uint32_t)kKeptBlock, 0x00020000);
+        low = upper + kKeptLow + lane * 8;
+        upper += lane * 16;
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t from, int i, int b) const { return col0 + b * kKeptCols < nrem ? from + i * step + b * kKeptBlock : 0xf0000000u; }
+};
+
 // The same for the two forms of a gated MLP.  Forward: acc[i][2 b], acc[i][2 b + 1] are the gate's and the up projection's columns col0 + 16 b .. (of C).  Lanes l and l ^ 16 trade halves
 // of two neighbouring blocks as above; where a wave has one block only, its stores are 8 bytes.
 template <int ACT, int TM, int TN>
@@ -504,9 +516,9 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
     const auto matrix = [&](bf16_t* p, int64_t ld) {
         return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(p), 0, (uint32_t)(((int64_t)(mrem - 1) * ld + nrem) * 2), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc), gbuf = matrix(e.kept.gate, e.ld), ubuf = matrix(e.kept.up, e.ld);
-    const __amdgpu_buffer_rsrc_t lbuf = __builtin_amdgcn_make_buffer_rsrc(e.kept.low, 0, (uint32_t)((mrem - 1) * e.ld + nrem), 0x00020000);
-    const bool keeps = e.kept.gate != nullptr;
+    const __amdgpu_buffer_rsrc_t cbuf = matrix(C, ldc);
+    const bool keeps = e.kept.p != nullptr;
+    KeptPieces kept(e.kept, mrem, nrem, row0, col0, lane);
     const int g = lane >> 4;
     uint32_t col_off[WIDE ? NB / 2 : NB];
 #pragma unroll
@@ -516,7 +528,6 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
     }
     const uint32_t row = (uint32_t)(row0 + (lane & 15));
     const auto offset = [&](int i, int b, int64_t ld) { return col_off[b] + row * (uint32_t)(ld * 2) + i * (uint32_t)(32 * ld); };
-    const auto byte_offset = [&](int i, int b) { return (col_off[b] == kOut ? kOut : col_off[b] / 2) + row * (uint32_t)e.ld + i * (uint32_t)(16 * e.ld); };
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         if constexpr (WIDE) {
@@ -541,9 +552,10 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
                 if (keeps) {
                     uint32_t kg[4], ku[4], kl[2];
                     keep<8>(gate, up, kg, ku, kl);
-                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{kg[0], kg[1], kg[2], kg[3]}, gbuf, offset(i, b, e.ld), 0, 0);
-                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{ku[0], ku[1], ku[2], ku[3]}, ubuf, offset(i, b, e.ld), 0, 0);
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{kl[0], kl[1]}, lbuf, byte_offset(i, b), 0, 0);
+                    const uint32_t upper = kept.at(kept.upper, i, b);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{kg[0], kg[1], kg[2], kg[3]}, kept.buf, upper, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{ku[0], ku[1], ku[2], ku[3]}, kept.buf, upper + kKeptUp, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{kl[0], kl[1]}, kept.buf, kept.at(kept.low, i, b), 0, 0);
                 }
 #pragma unroll
                 for (int r = 0; r < 8; ++r) y[r] = gate_value<ACT>(gate[r]) * up[r];
@@ -558,9 +570,14 @@ __device__ __forceinline__ void store_gate_forward(const f32x4 (&acc)[TM][TN], b
                 if (keeps) {
                     uint32_t kg[2], ku[2], kl[1];
                     keep<4>(gate, up, kg, ku, kl);
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{kg[0], kg[1]}, gbuf, offset(i, b, e.ld), 0, 0);
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{ku[0], ku[1]}, ubuf, offset(i, b, e.ld), 0, 0);
-                    __builtin_amdgcn_raw_buffer_store_b32(kl[0], lbuf, byte_offset(i, b), 0, 0);
+                    // four columns of a block's eight
+                    const int col = col0 + b * 16 + 4 * g;
+                    if (col < nrem && (int)row + i * 16 < mrem) {
+                        const KeptPlace to = kept_place(e.kept, row + i * 16, col);
+                        *reinterpret_cast<u32x2*>(to.upper + (g & 1) * 8) = u32x2{kg[0], kg[1]};
+                        *reinterpret_cast<u32x2*>(to.upper + kKeptUp + (g & 1) * 8) = u32x2{ku[0], ku[1]};
+                        *reinterpret_cast<uint32_t*>(to.low + (g & 1) * 4) = kl[0];
+                    }
                 }
                 bf16x4 y;
 #pragma unroll
@@ -577,8 +594,8 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
     const auto matrix = [&](const bf16_t* p) {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(p)), 0, (uint32_t)(((int64_t)(mrem - 1) * e.ld + nrem) * 2), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t lbuf = __builtin_amdgcn_make_buffer_rsrc(e.kept.low, 0, (uint32_t)((mrem - 1) * e.ld + nrem), 0x00020000);
-    const __amdgpu_buffer_rsrc_t gbuf = matrix(e.kept.gate), ubuf = matrix(e.kept.up), dgbuf = matrix(e.dgate), dubuf = matrix(e.dup), midbuf = matrix(e.mid);
+    KeptPieces kept(e.kept, mrem, nrem, row0, col0, lane);
+    const __amdgpu_buffer_rsrc_t dgbuf = matrix(e.dgate), dubuf = matrix(e.dup), midbuf = matrix(e.mid);
     const bool want_mid = e.mid != nullptr;
     const int g = lane >> 4;
     uint32_t off[TN / 2];
@@ -592,10 +609,10 @@ __device__ __forceinline__ void store_gate_backward(const f32x4 (&acc)[TM][TN], 
     u32x4 old_g[DEPTH], old_u[DEPTH];
     u32x2 old_l[DEPTH];
     const auto fetch = [&](int q) {
-        const uint32_t at = off[q % (TN / 2)] + q / (TN / 2) * row_step;
-        old_g[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gbuf, at, 0, 0));
-        old_u[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ubuf, at, 0, 0));
-        old_l[q % DEPTH] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(lbuf, at >> 1, 0, 0));  // (an offset that is out of range stays so: 2^30)
+        const uint32_t upper = kept.at(kept.upper, q / (TN / 2), q % (TN / 2));
+        old_g[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kept.buf, upper, 0, 0));
+        old_u[q % DEPTH] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kept.buf, upper + kKeptUp, 0, 0));
+        old_l[q % DEPTH] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(kept.buf, kept.at(kept.low, q / (TN / 2), q % (TN / 2)), 0, 0));
     };
 #pragma unroll
     for (int q = 0; q < DEPTH - 1; ++q) fetch(q);

@@ -285,15 +285,17 @@ def swiglu_bwd(dout, gate, up):
 GATES = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 
+def _kept_bytes(T, f):
+    return (T + 15) // 16 * ((f + 31) // 32) * 2560  # (ezl_gated_kept_bytes, without a call)
+
+
 def _new_kept(T, f, device):
-    """The three parts of an ezl_kept_gate in one tensor, one behind the other"""
-    return torch.empty(5 * T * f, dtype=torch.uint8, device=device)
+    return torch.empty(_kept_bytes(T, f), dtype=torch.uint8, device=device)
 
 
 def _kept(kept, T, f):
-    at, n = kept.data_ptr(), T * f
-    _need(kept.numel() == 5 * n and kept.dtype is torch.uint8 and kept.is_contiguous(), "what a gated block kept does not fit")
-    return _lib.KeptGate(at, at + 2 * n, at + 4 * n)
+    _need(kept.numel() == _kept_bytes(T, f) and kept.dtype is torch.uint8 and kept.is_contiguous(), "what a gated block kept does not fit")
+    return kept.data_ptr()
 
 
 def gated_fwd(act, x2d, gate_weight, up_weight, keep=False):
@@ -356,7 +358,7 @@ def gate_bwd(act, d, kept):
     _ready((d,), "d")
     T, f = d.shape
     dgate, dup = torch.empty_like(d), torch.empty_like(d)
-    _lib.call("ezl_gate_bwd", GATES[act], d.data_ptr(), _kept(kept, T, f), dgate.data_ptr(), dup.data_ptr(), d.numel(), _stream())
+    _lib.call("ezl_gate_bwd", GATES[act], d.data_ptr(), _kept(kept, T, f), dgate.data_ptr(), dup.data_ptr(), T, f, _stream())
     return dgate, dup
 
 

@@ -116,24 +116,23 @@ int ezl_swiglu_bwd(const void* dout, const void* gate, const void* up, void* dga
 #define EZL_GATE_GELU 1
 #define EZL_GATE_GELU_TANH 2
 #define EZL_GATE_RELU 3
-/* What the backward pass reads of a gated block: its two products G and U [M, f], each rounded to 12 bits of mantissa; the upper halves of their fp32 bits (bf16 tensors), and in one
- * byte for both the four bits behind those, G's in the lower half.  All contiguous, on 16 bytes. */
-typedef struct {
-    void *gate, *up, *low;
-} ezl_kept_gate; /* HOST struct */
+/* What the backward pass reads of a gated block, `kept` below: its two products G and U [M, f], each rounded to 12 bits of mantissa, ezl_gated_kept_bytes(M, f) bytes in blocks of 16 rows and
+ * 32 columns (ceil(f / 32) of them side by side, 2560 bytes each): 64 x 8 bf16, the upper halves of G's fp32 bits, the same of U's, and 64 x 8 bytes, the four bits behind those, G's in the
+ * lower half.  Of the 64 places of a block, row r's columns 8 c .. 8 c + 7 have the place 16 (c / 2 + 2 (c % 2)) + r. */
+int64_t ezl_gated_kept_bytes(int64_t M, int64_t f);
 /* out[M, f] = act(x gate_weight^T) * (x up_weight^T) in one launch, fp32 from the reductions to the one rounding: x [M, K] (rows ldx elements apart), both weights [f, K] (rows
- * ldw apart).  kept (HOST pointer, or NULL) receives the two products.  out contiguous; f % 8 == 0, below 2^21; K % 8 == 0, not 0.
+ * ldw apart).  kept (or NULL) receives the two products.  out contiguous; f % 8 == 0, below 2^21; K % 8 == 0, not 0.
  * workspace as for ezl_gemm_bf16, ezl_gated_workspace_bytes(M, f, K) bytes. */
 int64_t ezl_gated_workspace_bytes(int64_t M, int64_t f, int64_t K);
-int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, const ezl_kept_gate* kept, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
+int ezl_gated_fwd(int act, const void* x, const void* gate_weight, const void* up_weight, void* out, void* kept, int64_t M, int64_t f, int64_t K, int64_t ldx, int64_t ldw,
                   void* workspace, int64_t workspace_bytes, void* stream);
 /* Its way back behind a down projection, from dy [M, K] (rows lddy apart) and down_weight [K, f] (rows ldw apart), in one launch: with d = dy down_weight, dgate = d * U * act'(G),
  * dup = d * act(G), and mid (may be NULL) = act(G) * U again, which the down projection's weight gradient dy^T mid reads; d itself is not stored.  All [M, f], contiguous.
  * workspace: ezl_gemm_workspace_bytes(M, f, K). */
-int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const ezl_kept_gate* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy, int64_t ldw,
+int ezl_gated_bwd(int act, const void* dy, const void* down_weight, const void* kept, void* dgate, void* dup, void* mid, int64_t M, int64_t f, int64_t K, int64_t lddy, int64_t ldw,
                   void* workspace, int64_t workspace_bytes, void* stream);
-/* The same from a bf16 d that is there, n values of each, n % 8 == 0 (dgate or dup may be d). */
-int ezl_gate_bwd(int act, const void* d, const ezl_kept_gate* kept, void* dgate, void* dup, int64_t n, void* stream);
+/* The same from a bf16 d [M, f] that is there (dgate or dup may be d). */
+int ezl_gate_bwd(int act, const void* d, const void* kept, void* dgate, void* dup, int64_t M, int64_t f, void* stream);
 
 /* The whole block, y = (act(x gate^T) * (x up^T)) down^T, forward or backward in one call: x [M, h] (rows ldx apart), gate and up [f, h] (rows ldw apart), down [n, f] (rows ldd apart),
  * y and dy [M, n], contiguous.  kept (NULL forward: nothing) is what the backward call reads.  Of the gradients of the weights (contiguous; HOST pointers, NULL: not wanted) down's
@@ -146,8 +145,8 @@ typedef struct {
     int act;
 } ezl_gated_mlp; /* HOST struct */
 int64_t ezl_gated_mlp_bytes(const ezl_gated_mlp* mlp, int backward);
-int ezl_gated_mlp_fwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, void* y, const ezl_kept_gate* kept, void* temp, int64_t temp_bytes, void* stream);
-int ezl_gated_mlp_bwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, const void* dy, const ezl_kept_gate* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
+int ezl_gated_mlp_fwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, void* y, void* kept, void* temp, int64_t temp_bytes, void* stream);
+int ezl_gated_mlp_bwd(const ezl_gated_mlp* mlp, const void* x, int64_t ldx, const void* dy, const void* kept, void* dx, const ezl_layer_grad* dgate, const ezl_layer_grad* dup,
                       const ezl_layer_grad* ddown, void* temp, int64_t temp_bytes, void* stream);
 
 /* ---- rotary embedding: llama/positional_embeddings.py:17-36 (table), :94-96,105-122 (apply) ----

@@ -54,9 +54,13 @@ def product(a, a_err, b, b_err=None):
 
 def kept_values(kept, T, f, rows=slice(None)):
     """the two products of what K.gated_fwd kept, in fp64"""
-    n = T * f
-    gate, up = (kept[i * 2 * n:(i + 1) * 2 * n].view(torch.int16).view(T, f)[rows] for i in range(2))
-    low = kept[4 * n:].view(T, f)[rows].int()
+    rows = torch.arange(T, device="cuda")[rows]
+    blocks = kept.view((T + 15) // 16, (f + 31) // 32, 2560)[rows // 16]
+    place = torch.tensor([16 * (c // 2 + 2 * (c % 2)) for c in range(4)], device="cuda") + (rows % 16)[:, None]  # [row, eight columns of a block's 32]
+    here = torch.arange(len(rows), device="cuda")[:, None]
+    of = lambda part: part.unflatten(-1, (64, 8)).transpose(1, 2)[here, place].transpose(1, 2).reshape(len(rows), -1)[:, :f]  # noqa: E731
+    gate, up = (of(blocks[..., 1024 * i:1024 * (i + 1)].contiguous().view(torch.int16)) for i in range(2))
+    low = of(blocks[..., 2048:]).int()
     bits = lambda upper, last: (upper.int() << 16 | last << 12).view(torch.float32).double()  # noqa: E731
     return bits(gate, low & 15), bits(up, low >> 4)
 

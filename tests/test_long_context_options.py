@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from easyllm_amd import _lib, optimizer
+from easyllm_amd import _lib, kernels as K, optimizer
 from easyllm_amd.positional_embeddings import RotaryEmbedding, scaled_frequencies
 
 
@@ -136,33 +136,32 @@ def test_the_library_refuses_before_it_launches():
     assert lib.ezl_adamw8_list(0, None, how(), None, None) == 0 and lib.ezl_adamw8_list(1, tensor(n=0), how(), None, None) == 0
     assert lib.ezl_moments8_list(1, tensor(), null, null, None) == -1 and lib.ezl_moments8_list(0, None, None, None, None) == 0
 
-    whole = _lib.KeptGate(16, 16, 16)
-    partial = [_lib.KeptGate(None, 16, 16), _lib.KeptGate(16, None, 16), _lib.KeptGate(16, 16, None), _lib.KeptGate(24, 16, 16), _lib.KeptGate(16, 24, 16), _lib.KeptGate(16, 16, 24)]
-
     def gated(act=0, x=16, wg=16, wu=16, out=16, kept=None, M=4, f=16, K=16, ldx=16, ldw=16, ws=None):
         return lib.ezl_gated_fwd(act, x, wg, wu, out, kept, M, f, K, ldx, ldw, ws, 0, None)
-    for kw in (dict(act=-1), dict(act=4), dict(x=None), dict(wg=None), dict(wu=None), dict(out=None), *[dict(kept=k) for k in partial], dict(M=-1), dict(f=12), dict(K=0), dict(K=12, ldx=16), dict(ldx=8),
+    for kw in (dict(act=-1), dict(act=4), dict(x=None), dict(wg=None), dict(wu=None), dict(out=None), dict(kept=24), dict(M=-1), dict(f=12), dict(K=0), dict(K=12, ldx=16), dict(ldx=8),
                dict(ldw=12), dict(x=24), dict(wu=24), dict(out=24), dict(f=1 << 21, ldw=16), dict(ws=24)):
         assert gated(**kw) in (-1, -2), kw
     assert gated(M=0) == 0 and gated(f=0) == 0
 
-    def gated_bwd(act=0, dy=16, wd=16, kept=whole, dg=16, du=16, mid=None, M=4, f=16, K=16, lddy=16, ldw=16):
+    def gated_bwd(act=0, dy=16, wd=16, kept=16, dg=16, du=16, mid=None, M=4, f=16, K=16, lddy=16, ldw=16):
         return lib.ezl_gated_bwd(act, dy, wd, kept, dg, du, mid, M, f, K, lddy, ldw, None, 0, None)
-    for kw in (dict(act=9), dict(dy=None), dict(wd=None), dict(kept=None), *[dict(kept=k) for k in partial], dict(dg=None), dict(du=None), dict(mid=24), dict(M=-1), dict(f=12), dict(K=0), dict(lddy=8), dict(ldw=8)):
+    for kw in (dict(act=9), dict(dy=None), dict(wd=None), dict(kept=None), dict(kept=24), dict(dg=None), dict(du=None), dict(mid=24), dict(M=-1), dict(f=12), dict(K=0), dict(lddy=8), dict(ldw=8)):
         assert gated_bwd(**kw) in (-1, -2), kw
-    for kw in (dict(act=4), dict(n=12), dict(n=-8), dict(d=None), dict(d=24), dict(kept=None), dict(dg=8), dict(du=None), *[dict(kept=k) for k in partial]):
-        c = dict(dict(act=0, d=16, kept=whole, dg=16, du=16, n=16), **kw)
-        assert lib.ezl_gate_bwd(c["act"], c["d"], c["kept"], c["dg"], c["du"], c["n"], None) in (-1, -2), kw
-    assert lib.ezl_gate_bwd(0, None, None, None, None, 0, None) == 0
+    for kw in (dict(act=4), dict(f=12), dict(f=-8), dict(M=-1), dict(f=1 << 21), dict(d=None), dict(d=24), dict(kept=None), dict(kept=24), dict(dg=8), dict(du=None)):
+        c = dict(dict(act=0, d=16, kept=16, dg=16, du=16, M=3, f=16), **kw)
+        assert lib.ezl_gate_bwd(*c.values(), None) in (-1, -2), kw
+    assert lib.ezl_gate_bwd(0, None, None, None, None, 0, 16, None) == 0 and lib.ezl_gate_bwd(0, None, None, None, None, 5, 0, None) == 0
+    for M, f in ((1, 8), (16, 32), (17, 40), (100, 688), (0, 64), (1 << 20, 13696)):
+        assert lib.ezl_gated_kept_bytes(M, f) == K._kept_bytes(M, f) >= 5 * M * f
     mlp = lambda **kw: _lib.GatedMLP(**dict(dict(M=4, h=16, f=16, n=16, gate=16, up=16, down=16, ldw=16, ldd=16, act=0), **kw))  # noqa: E731
     nbytes = lib.ezl_gated_mlp_bytes(mlp(), 0)
     assert nbytes > 0 and lib.ezl_gated_mlp_bytes(mlp(), 1) > nbytes and lib.ezl_gated_mlp_bytes(mlp(h=0), 0) == -1 and lib.ezl_gated_mlp_bytes(None, 0) == -1
     for m, kw in ((mlp(h=12), {}), (mlp(f=12), {}), (mlp(n=12), {}), (mlp(M=-1), {}), (mlp(gate=None), {}), (mlp(down=None), {}), (mlp(act=7), {}), (None, {}), (mlp(), dict(x=None)), (mlp(), dict(y=None)),
-                  (mlp(), dict(temp=None)), (mlp(), dict(temp=24)), (mlp(), dict(nbytes=nbytes - 1)), *[(mlp(), dict(kept=k)) for k in partial]):
+                  (mlp(), dict(temp=None)), (mlp(), dict(temp=24)), (mlp(), dict(nbytes=nbytes - 1)), (mlp(), dict(kept=24))):
         c = dict(dict(x=16, y=16, kept=None, temp=16, nbytes=1 << 40), **kw)
         assert lib.ezl_gated_mlp_fwd(m, c["x"], 16, c["y"], c["kept"], c["temp"], c["nbytes"], None) in (-1, -2), (m, kw)
-    for kw in (dict(x=None), dict(dy=None), dict(kept=None), *[dict(kept=k) for k in partial], dict(temp=None), dict(nbytes=8), dict(dx=24)):
-        c = dict(dict(x=16, dy=16, kept=whole, dx=16, temp=16, nbytes=1 << 40), **kw)
+    for kw in (dict(x=None), dict(dy=None), dict(kept=None), dict(kept=24), dict(temp=None), dict(nbytes=8), dict(dx=24)):
+        c = dict(dict(x=16, dy=16, kept=16, dx=16, temp=16, nbytes=1 << 40), **kw)
         assert lib.ezl_gated_mlp_bwd(mlp(), c["x"], 16, c["dy"], c["kept"], c["dx"], None, None, None, c["temp"], c["nbytes"], None) in (-1, -2), kw
 
 
