@@ -20,8 +20,9 @@ from .first_order import first_order
 
 
 def _differentiated(*tensors):
-    """Whether autograd has a say in a call on these: backward, or forward (where its own error is wanted)."""
-    if torch.autograd.forward_ad._current_level >= 0:
+    """Whether autograd has a say in a call on these: backward, or forward (where its own error is wanted).  Also where the call is traced: a trace records functions, of a bare
+    launch only the allocation of its results."""
+    if torch.autograd.forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None:
         return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
