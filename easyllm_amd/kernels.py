@@ -295,6 +295,7 @@ def _new_kept(T, f, device):
 
 def _kept(kept, T, f):
     _need(kept.numel() == _kept_bytes(T, f) and kept.dtype is torch.uint8 and kept.is_contiguous(), "what a gated block kept does not fit")
+    _here(kept, "what a gated block kept")
     return kept.data_ptr()
 
 
