@@ -69,6 +69,10 @@ def _checked_scaling(scaling):
     return dict(scaling)
 
 
+def _capturing(device):
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class RotaryEmbedding(torch.nn.Module):
     def __init__(self, dim, base=10000, precision=torch.half, scale_factor=1.0, rotary_dim=None, interleaved=False, scaling=None):
         super().__init__()
@@ -100,11 +104,15 @@ class RotaryEmbedding(torch.nn.Module):
         return self.cos_half, self.sin_half
 
     def frequencies(self, seq_len, device):
-        """(fp64 [rotary_dim / 2] on `device`, the factor of sines and cosines) for a text of seq_len tokens"""
+        """(fp64 [rotary_dim / 2] on `device`, the factor of sines and cosines) for a text of seq_len tokens.
+
+        They are kept for the next call.  A captured graph computes its own on every replay, from what inv_freq holds then: it has no reference to a tensor that was there before it, whose
+        memory another length's call or a loaded checkpoint would free under its replays."""
+        capturing = _capturing(device)
         length = seq_len if self.scaling is not None and self.scaling["type"] == "dynamic" and not self.scaling.get("length") else None
-        if self._frequencies is None or self._frequencies[0] != (device, length):
+        if capturing or self._frequencies is None or self._frequencies[0] != (device, length):
             inv_freq, factor = scaled_frequencies(self.inv_freq.to(device) / self.scale_factor, self.base, self.scaling, seq_len)
-            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():  # (memory of the graph's, which nobody else may read later)
+            if capturing:  # (memory of the graph's, which nobody else may read later)
                 return inv_freq.contiguous(), factor
             if device.type == "cuda":  # whatever stream reads them next, and whatever still reads the ones before
                 torch.cuda.synchronize(device)

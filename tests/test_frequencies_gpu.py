@@ -1,0 +1,73 @@
+"""Frequencies of rotary positions under captured graphs."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+SCALINGS = {"dynamic": {"type": "dynamic", "factor": 2.0, "original_length": 16}, "linear": {"type": "linear", "factor": 3.0}, "yarn": {"type": "yarn", "factor": 4.0, "original_length": 32}, "none": None}
+
+
+def rnd(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").bfloat16()
+
+
+def small_tensors():
+    """What a freed block of frequencies would be used for next."""
+    return [torch.full((n,), 7.0, dtype=torch.float64, device="cuda") for n in (8, 16, 24, 32, 64) for _ in range(200)]
+
+
+@pytest.mark.parametrize("name", SCALINGS)
+def test_a_captured_call_outlives_whatever_the_module_does(name):
+    from easyllm_amd.positional_embeddings import RotaryEmbedding
+    rope = RotaryEmbedding(64, rotary_dim=48, interleaved=True, scaling=SCALINGS[name]).cuda()
+    q, k, dq, dk = rnd(40, 2, 4, 64, seed=1).requires_grad_(), rnd(40, 2, 2, 64, seed=2).requires_grad_(), rnd(40, 2, 4, 64, seed=3), rnd(40, 2, 2, 64, seed=4)
+
+    def step():
+        outs = rope.rotate(q, k)
+        return [*(y.detach() for y in outs), *torch.autograd.grad(outs, (q, k), (dq, dk))]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    other = {"inv_freq": rope.inv_freq.clone() * 0.75}
+    for between in (lambda: rope.rotate(rnd(300, 2, 4, 64), None), lambda: rope.load_state_dict(dict(rope.state_dict())), lambda: rope.load_state_dict(other), rope.cuda):
+        between()
+        torch.cuda.synchronize()
+        keep = small_tensors()
+        with torch.no_grad():
+            q.copy_(rnd(40, 2, 4, 64, seed=5))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step())), between
+        del keep
+
+
+@pytest.mark.parametrize("name", SCALINGS)
+def test_a_captured_training_step_does_too(name):
+    from easyllm_amd import runner
+    torch.manual_seed(5)
+    cfg = dict(num_layers=2, hidden_size=128, num_attention_heads=2, intermediate_size=136, vocab_size=72, seq_length=64, bf16=True, fp32_logits=False, checkpoint_activations=False,
+               position_embedding_kwargs=dict(interleaved=True, scaling=SCALINGS[name]))
+    model = runner.build_model({"type": "llama_custom", "kwargs": cfg}).cuda()
+    runner.attach_main_grads(model)
+
+    def batch(seed, s=64):
+        ids = torch.randint(0, 72, (2, s), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+        return (ids, torch.arange(s, device="cuda").expand(2, s).contiguous(), None), (ids.roll(-1, 1), torch.ones(2, s, device="cuda"))
+
+    step = runner.GraphedStep(model, *batch(1))
+    for seed in (2, 3, 4):
+        with torch.no_grad():
+            model(batch(seed, 200)[0])
+        model.load_state_dict({n: v.clone() for n, v in model.state_dict().items()})
+        torch.cuda.synchronize()
+        keep = small_tensors()
+        loss = step(*batch(seed))
+        torch.cuda.synchronize()
+        step.flush()
+        captured = loss.item(), {n: p.main_grad.clone() for n, p in model.named_parameters()}
+        runner.zero_main_grads(model)
+        eager = runner.forward_step(model, *batch(seed))
+        assert eager.item() == captured[0] and all(torch.equal(p.main_grad, captured[1][n]) for n, p in model.named_parameters())
+        del eager, keep
