@@ -111,7 +111,7 @@ class RotaryEmbedding(torch.nn.Module):
         capturing = _capturing(device)
         length = seq_len if self.scaling is not None and self.scaling["type"] == "dynamic" and not self.scaling.get("length") else None
         if capturing or self._frequencies is None or self._frequencies[0] != (device, length):
-            inv_freq, factor = scaled_frequencies(self.inv_freq.to(device) / self.scale_factor, self.base, self.scaling, seq_len)
+            inv_freq, factor = scaled_frequencies(self.inv_freq.to(device).double() / self.scale_factor, self.base, self.scaling, seq_len)
             if capturing:  # (memory of the graph's, which nobody else may read later)
                 return inv_freq.contiguous(), factor
             if device.type == "cuda":  # whatever stream reads them next, and whatever still reads the ones before
