@@ -29,29 +29,42 @@ def scaled_frequencies(inv_freq, base, scaling, length):
     yarn     divided by "factor" where a wave turns less than "beta_slow" (1) times in "original_length", as they are where it turns more than "beta_fast" (32) times, in between by a
              line over the index (Peng, Quesnelle, Fan, Shippole, "YaRN: efficient context window extension of large language models", 2023); "attention_factor"
              (0.1 ln factor + 1)"""
-    inv_freq, n = inv_freq.double(), inv_freq.numel()
+    n, device = inv_freq.numel(), inv_freq.device
+    stretch, factor = _stretch(n, base, scaling, device)
+    if _goes_by_length(scaling):
+        stretch = _dynamic_stretch(stretch, scaling, length)
+    return inv_freq.double() * stretch, factor
+
+
+def _goes_by_length(scaling):
+    return scaling is not None and scaling["type"] == "dynamic" and not scaling.get("length")
+
+
+def _dynamic_stretch(exponents, scaling, length):
+    factor, original = float(scaling["factor"]), float(scaling["original_length"])
+    return 1.0 if length <= original else (factor * length / original - (factor - 1)) ** exponents
+
+
+def _stretch(n, base, scaling, device):
+    """(what n frequencies are multiplied by, in fp64, or a dynamic scaling's exponents where the length is not known yet; what sines and cosines are multiplied by)"""
+    j = torch.arange(n, dtype=torch.float64, device=device)
     if scaling is None:
-        return inv_freq, 1.0
+        return torch.ones_like(j), 1.0
     kind, factor = scaling["type"], float(scaling["factor"])
     if kind == "linear":
-        return inv_freq / factor, 1.0
-    original = float(scaling["original_length"])
+        return torch.full_like(j, 1 / factor), 1.0
     if kind == "dynamic":
-        length = scaling.get("length") or length
-        if length <= original or n == 1:
-            return inv_freq, 1.0
-        more = factor * length / original - (factor - 1)
-        j = torch.arange(n, dtype=torch.float64, device=inv_freq.device)
-        return inv_freq * more ** (-j / (n - 1)), 1.0
+        exponents = j / -max(n - 1, 1)  # (one frequency stays as it is)
+        return exponents if _goes_by_length(scaling) else torch.ones_like(j) * _dynamic_stretch(exponents, scaling, scaling["length"]), 1.0
+    original = float(scaling["original_length"])
 
     def index_of(turns):  # of the wave that turns so often in the original length
         return n * math.log(original / (turns * 2 * math.pi)) / math.log(base)
 
     low, high = max(math.floor(index_of(scaling.get("beta_fast", 32))), 0), min(math.ceil(index_of(scaling.get("beta_slow", 1))), 2 * n - 1)
-    j = torch.arange(n, dtype=torch.float64, device=inv_freq.device)
     slow = ((j - low) / max(high - low, 1e-3)).clamp(0, 1)
     attention_factor = scaling.get("attention_factor")
-    return inv_freq / factor * slow + inv_freq * (1 - slow), 0.1 * math.log(factor) + 1 if attention_factor is None else float(attention_factor)
+    return slow / factor + (1 - slow), 0.1 * math.log(factor) + 1 if attention_factor is None else float(attention_factor)
 
 
 def _checked_scaling(scaling):
@@ -69,10 +82,6 @@ def _checked_scaling(scaling):
     return dict(scaling)
 
 
-def _capturing(device):
-    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
-
-
 class RotaryEmbedding(torch.nn.Module):
     def __init__(self, dim, base=10000, precision=torch.half, scale_factor=1.0, rotary_dim=None, interleaved=False, scaling=None):
         super().__init__()
@@ -86,7 +95,9 @@ class RotaryEmbedding(torch.nn.Module):
         self.interleaved = bool(interleaved)
         self.scaling = _checked_scaling(scaling)
         self.general = rotary_dim != dim or self.interleaved or self.scaling is not None  # (turned without tables, by rotate)
-        self._frequencies = None
+        self._before = []
+        self._host_stretch, self._factor = _stretch(rotary_dim // 2, base, self.scaling, "cpu")
+        self._settle()
         self.max_seq_len_cached = None
         self.cos_half = None
         self.sin_half = None
@@ -106,30 +117,35 @@ class RotaryEmbedding(torch.nn.Module):
     def frequencies(self, seq_len, device):
         """(fp64 [rotary_dim / 2] on `device`, the factor of sines and cosines) for a text of seq_len tokens.
 
-        They are kept for the next call.  A captured graph computes its own on every replay, from what inv_freq holds then: it has no reference to a tensor that was there before it, whose
-        memory another length's call or a loaded checkpoint would free under its replays."""
-        capturing = _capturing(device)
-        length = seq_len if self.scaling is not None and self.scaling["type"] == "dynamic" and not self.scaling.get("length") else None
-        if capturing or self._frequencies is None or self._frequencies[0] != (device, length):
-            inv_freq, factor = scaled_frequencies(self.inv_freq.to(device).double() / self.scale_factor, self.base, self.scaling, seq_len)
-            if capturing:  # (memory of the graph's, which nobody else may read later)
-                return inv_freq.contiguous(), factor
-            if device.type == "cuda":  # whatever stream reads them next, and whatever still reads the ones before
-                torch.cuda.synchronize(device)
-            self._frequencies = (device, length), inv_freq.contiguous(), factor
-        return self._frequencies[1:]
+        A product of inv_freq and of what its options make of it, computed for every call, on its stream or in its graph: another call, another length, a loaded checkpoint or a moved module
+        find nothing of it to replace."""
+        stretch = self._stretch if self._stretch.device == device else self._host_stretch.to(device)
+        if _goes_by_length(self.scaling):
+            stretch = _dynamic_stretch(stretch, self.scaling, seq_len)
+        inv_freq = self.inv_freq.to(device)
+        inv_freq = inv_freq * stretch if torch.is_tensor(stretch) else inv_freq.double()
+        return (inv_freq if self.scale_factor == 1 else inv_freq / self.scale_factor), self._factor
+
+    def _settle(self):
+        """The factors of the frequencies go where those are, in 64 bits whatever the module is cast to."""
+        device = self.inv_freq.device
+        self._stretch = self._host_stretch if device.type in ("cpu", "meta") else self._host_stretch.to(device)
 
     def _apply(self, fn, *args, **kwargs):
-        self._frequencies = None
-        return super()._apply(fn, *args, **kwargs)
-
-    def _load_from_state_dict(self, *args, **kwargs):
-        super()._load_from_state_dict(*args, **kwargs)
-        self._frequencies = None
+        inv_freq, stretch = self.inv_freq, self._stretch
+        super()._apply(fn, *args, **kwargs)
+        if stretch.device != self.inv_freq.device:
+            self._settle()
+        # (what a captured graph may go on reading: a cast to the type that the weights have leaves them, and with them the graph, as they were)
+        self._before += [old for old, new in ((inv_freq, self.inv_freq), (stretch, self._stretch)) if old is not new and old.is_cuda]
+        return self
 
     def rotate(self, q, k, position_ids=None):
         """q [s, b, nq, d], k [s, b, nk, d] -> turned, whatever the options; position_ids int64 [b, s] or None (the place in the sequence)."""
-        inv_freq, factor = self.frequencies(q.shape[0], q.device)
+        if self.scaling is None and self.scale_factor == 1 and self.inv_freq.dtype is torch.float32 and self.inv_freq.device == q.device:
+            inv_freq, factor = self.inv_freq, 1.0  # (widened where it is read)
+        else:
+            inv_freq, factor = self.frequencies(q.shape[0], q.device)
         return F_.rotary_embed(q, k, inv_freq, position_ids, interleaved=self.interleaved, scale=factor)
 
     def forward(self, x, seq_dim=1, seq_len=None):

@@ -1,8 +1,12 @@
 """What a module of rotary positions keeps of its frequencies, and for whom (CPU)."""
+import copy
+import pickle
+import sys
+import threading
+
 import pytest
 import torch
 
-from easyllm_amd import positional_embeddings as P
 from easyllm_amd.positional_embeddings import RotaryEmbedding
 
 CPU = torch.device("cpu")
@@ -10,17 +14,62 @@ SCALINGS = [None, {"type": "linear", "factor": 3.0}, {"type": "dynamic", "factor
 
 
 @pytest.mark.parametrize("scaling", SCALINGS)
-def test_a_captured_call_has_frequencies_of_its_own(monkeypatch, scaling):
-    """A graph holds no reference to a tensor that was there before it: whatever replaces that one, the replays would read freed memory."""
+def test_nothing_of_a_call_is_kept_for_the_next(scaling):
+    """A captured graph holds no reference to a tensor that was there before it, and another stream or thread does not wait for one: a call's frequencies are its own."""
     rope = RotaryEmbedding(64, rotary_dim=32, scaling=scaling)
-    eager = rope.frequencies(40, CPU)
-    assert rope.frequencies(40, CPU)[0] is eager[0]
-    monkeypatch.setattr(P, "_capturing", lambda device: True)
+    held = lambda: {t.data_ptr() for t in vars(rope).values() if torch.is_tensor(t)} | {rope.inv_freq.data_ptr()}  # noqa: E731
+    before = held()
     first, second = rope.frequencies(40, CPU), rope.frequencies(40, CPU)
-    assert len({t.data_ptr() for t in (rope.inv_freq, eager[0], first[0], second[0])}) == 4
-    assert torch.equal(first[0], eager[0]) and torch.equal(second[0], eager[0]) and first[1] == second[1] == eager[1]
-    monkeypatch.undo()
-    assert rope.frequencies(40, CPU)[0] is eager[0]  # (nor does anybody else read the graph's)
+    assert torch.equal(first[0], second[0]) and first[0].data_ptr() != second[0].data_ptr() and held() == before and not {first[0].data_ptr(), second[0].data_ptr()} & before
+    want = rope.frequencies(7, CPU)[0].clone()
+    rope.load_state_dict({"inv_freq": rope.inv_freq * 2})
+    assert torch.equal(rope.frequencies(7, CPU)[0], 2 * want) and held() == before
+
+
+@pytest.mark.parametrize("scaling", SCALINGS)
+def test_an_evaluation_leaves_nothing_that_training_cannot_use(scaling):
+    """Tensors made under inference_mode cannot be saved for a backward pass."""
+    rope = RotaryEmbedding(64, rotary_dim=32, scaling=scaling)
+    with torch.inference_mode():
+        rope.frequencies(40, CPU)
+    assert not rope.frequencies(40, CPU)[0].is_inference()
+
+
+def test_threads_of_different_lengths_get_their_own():
+    rope = RotaryEmbedding(64, scaling={"type": "dynamic", "factor": 2.0, "original_length": 16})
+    lengths = range(20, 420, 100)
+    want = {n: rope.frequencies(n, CPU)[0].clone() for n in lengths}
+    wrong = []
+
+    def ask(n):
+        for _ in range(300):
+            if not torch.equal(rope.frequencies(n, CPU)[0], want[n]):
+                wrong.append(n)
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=ask, args=(n,)) for n in lengths]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        sys.setswitchinterval(interval)
+    assert not wrong
+
+
+@pytest.mark.parametrize("scaling", SCALINGS)
+def test_a_module_that_is_cast_or_copied(scaling):
+    """The factors stay in 64 bits whatever inv_freq is held in; a module on no device at all goes on to a real one."""
+    rope = RotaryEmbedding(64, rotary_dim=32, scaling=scaling)
+    want = rope.frequencies(40, CPU)[0]
+    low = copy.deepcopy(rope).bfloat16()
+    off = (low.frequencies(40, CPU)[0] - want).abs() / want
+    assert low.frequencies(40, CPU)[0].dtype is torch.float64 and bool((off <= 2.0 ** -8).all())
+    assert torch.equal(pickle.loads(pickle.dumps(rope)).frequencies(40, CPU)[0], want)
+    with torch.device("meta"):
+        empty = RotaryEmbedding(64, rotary_dim=32, scaling=scaling)
+    empty = empty.to_empty(device="cpu")
+    empty.load_state_dict(rope.state_dict())
+    assert torch.equal(empty.frequencies(40, CPU)[0], want)
 
 
 @pytest.mark.parametrize("scaling", SCALINGS)

@@ -71,3 +71,52 @@ def test_a_captured_training_step_does_too(name):
         eager = runner.forward_step(model, *batch(seed))
         assert eager.item() == captured[0] and all(torch.equal(p.main_grad, captured[1][n]) for n, p in model.named_parameters())
         del eager, keep
+
+
+def test_lengths_that_change_stop_nothing(monkeypatch):
+    """Ten lengths in turn, forward and backward: no call waits for the device."""
+    from easyllm_amd.positional_embeddings import RotaryEmbedding
+    rope = RotaryEmbedding(64, scaling=SCALINGS["dynamic"]).cuda()
+    inputs = [(rnd(s, 2, 4, 64, seed=s).requires_grad_(), rnd(s, 2, 2, 64, seed=s + 1)) for s in range(8, 58, 5)]
+
+    def waits(*_):
+        raise AssertionError("a call waited for the device")
+    monkeypatch.setattr(torch.cuda, "synchronize", waits)
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for q, k in inputs:
+            y, z = rope.rotate(q, k)
+            torch.autograd.grad(y, q, torch.ones_like(y))
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+
+
+def test_an_evaluation_under_inference_mode_and_a_training_step_behind_it():
+    from easyllm_amd.positional_embeddings import RotaryEmbedding
+    for scaling in SCALINGS.values():
+        rope = RotaryEmbedding(64, rotary_dim=32, scaling=scaling).cuda()
+        q = rnd(40, 2, 4, 64)
+        with torch.inference_mode():
+            seen = rope.rotate(q, None)[0]
+        leaf = q.clone().requires_grad_()
+        y = rope.rotate(leaf, None)[0]
+        assert torch.equal(seen, y) and torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == q.shape
+
+
+def test_a_cast_that_leaves_the_weights_leaves_a_captured_call():
+    """bf16 weights stay where they are under .bfloat16(), and a graph of them may be replayed; inv_freq does not."""
+    from easyllm_amd.positional_embeddings import RotaryEmbedding
+    rope = RotaryEmbedding(64, scaling=SCALINGS["yarn"]).cuda()
+    q = rnd(40, 2, 4, 64)
+    want = rope.rotate(q, None)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = rope.rotate(q, None)[0]
+    rope.bfloat16()
+    torch.cuda.synchronize()
+    keep = small_tensors()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+    del keep
