@@ -25,7 +25,7 @@ def scaled_frequencies(inv_freq, base, scaling, length):
     """(frequencies in fp64, what sines and cosines are multiplied by) of `inv_freq` [n] = base^(-j / n) under a scaling, a dict with a "type":
 
     linear   all divided by "factor"
-    dynamic  a larger base for a text of `length` (or its own "length") tokens, where that is above "original_length": base ((factor length / original_length) - (factor - 1))^(n / (n - 1))
+    dynamic  a larger base for texts of `length` (or its own "length") tokens, where that is above "original_length": base ((factor length / original_length) - (factor - 1))^(n / (n - 1))
     yarn     divided by "factor" where a wave turns less than "beta_slow" (1) times in "original_length", as they are where it turns more than "beta_fast" (32) times, in between by a
              line over the index (Peng, Quesnelle, Fan, Shippole, "YaRN: efficient context window extension of large language models", 2023); "attention_factor"
              (0.1 ln factor + 1)"""
@@ -140,8 +140,12 @@ class RotaryEmbedding(torch.nn.Module):
         self._before += [old for old, new in ((inv_freq, self.inv_freq), (stretch, self._stretch)) if old is not new and old.is_cuda]
         return self
 
-    def rotate(self, q, k, position_ids=None):
-        """q [s, b, nq, d], k [s, b, nk, d] -> turned, whatever the options; position_ids int64 [b, s] or None (the place in the sequence)."""
+    def rotate(self, q, k, position_ids=None, cu_seqlens=None):
+        """q [s, b, nq, d], k [s, b, nk, d] -> turned, whatever the options; position_ids int64 [b, s] or None (the place in the sequence).  cu_seqlens: None, or what says that rows hold
+        several documents."""
+        if _goes_by_length(self.scaling) and (position_ids is not None or cu_seqlens is not None):
+            # One set of frequencies holds for a call.  A row's length is that of none of its documents, which would turn by what else lies in the row, and the largest position is the device's.
+            raise ValueError('a dynamic scaling goes by the length of texts that fill their rows: with documents packed in a row, or position ids, it needs a "length"')
         if self.scaling is None and self.scale_factor == 1 and self.inv_freq.dtype is torch.float32 and self.inv_freq.device == q.device:
             inv_freq, factor = self.inv_freq, 1.0  # (widened where it is read)
         else:

@@ -288,7 +288,7 @@ class ParallelAttention(torch.nn.Module):
         k = key_layer.view(sq, bs, nk, d) if not self.qkv_pack else key_layer.unflatten(-1, (nk, d))
         v = value_layer.view(sq, bs, nk, d) if not self.qkv_pack else value_layer.unflatten(-1, (nk, d))
         if getattr(self.rotary_emb, "general", False):
-            q, k = self.rotary_emb.rotate(q, k, position_ids)
+            q, k = self.rotary_emb.rotate(q, k, position_ids, cu_seqlens)
         else:
             cos, sin = self.rotary_emb.tables(sq, q.device)
             q, k = apply_rotary_pos_emb(q, k, cos, sin, position_ids)

@@ -7,6 +7,7 @@ import threading
 import pytest
 import torch
 
+from easyllm_amd import positional_embeddings as P
 from easyllm_amd.positional_embeddings import RotaryEmbedding
 
 CPU = torch.device("cpu")
@@ -78,3 +79,43 @@ def test_a_scale_factor_divides_in_64_bits(scaling):
     rope, whole = (RotaryEmbedding(64, scale_factor=f, scaling=scaling) for f in (3.0, 1.0))
     got, want = rope.frequencies(40, CPU)[0], whole.frequencies(40, CPU)[0] / 3.0
     assert got.dtype is torch.float64 and bool(((got - want).abs() <= want * 2.0 ** -50).all())
+
+
+DYNAMIC = {"type": "dynamic", "factor": 2.0, "original_length": 16}
+
+
+def test_a_row_of_several_texts_has_no_length_of_its_own():
+    """A document of 12 tokens is not stretched when it is alone; in a row of 40 it was turned as one of 40, and one at position 1000 of a longer text as if it began there."""
+    q = torch.zeros(40, 1, 2, 64, dtype=torch.bfloat16)
+    ids = torch.cat((torch.arange(12), torch.arange(28)))[None]
+    rope = RotaryEmbedding(64, scaling=DYNAMIC)
+    assert torch.equal(rope.frequencies(12, CPU)[0], rope.inv_freq.double()) and not torch.equal(rope.frequencies(40, CPU)[0], rope.inv_freq.double())
+    for kw in (dict(position_ids=ids), dict(cu_seqlens=torch.tensor([0, 12, 40])), dict(position_ids=ids, cu_seqlens=torch.tensor([0, 12, 40]))):
+        with pytest.raises(ValueError, match='needs a "length"'):
+            rope.rotate(q, q, **kw)
+
+
+def test_texts_that_have_a_length_are_turned(monkeypatch):
+    """Whole rows go by their length; packed ones by the scaling's own, whatever they hold."""
+    seen = []
+    monkeypatch.setattr(P.F_, "rotary_embed", lambda q, k, inv_freq, ids, **kw: seen.append(inv_freq) or (q, k))
+    q, ids, cu = torch.zeros(40, 1, 2, 64), torch.arange(40)[None], torch.tensor([0, 12, 40])
+    RotaryEmbedding(64, scaling=DYNAMIC).rotate(q, q)
+    fixed = RotaryEmbedding(64, scaling=dict(DYNAMIC, length=100))
+    fixed.rotate(q, q, ids, cu)
+    fixed.rotate(q[:12], q[:12], ids[:, :12])
+    j = torch.arange(32, dtype=torch.float64)
+    for got, length in zip(seen, (40, 100, 100)):
+        want = fixed.inv_freq.double() * (2 * length / 16 - 1) ** (-j / 31)
+        assert bool(((got - want).abs() <= want * 2.0 ** -48).all())
+    for scaling in (None, {"type": "linear", "factor": 3.0}, {"type": "yarn", "factor": 4.0, "original_length": 32}):
+        RotaryEmbedding(64, rotary_dim=32, scaling=scaling).rotate(q, q, ids, cu)
+
+
+def test_an_attention_tells_its_positions_of_documents(monkeypatch):
+    from easyllm_amd import runner, transformer
+    cfg = dict(num_layers=1, hidden_size=64, num_attention_heads=1, intermediate_size=72, vocab_size=64, seq_length=16, bf16=True, position_embedding_kwargs={"scaling": DYNAMIC})
+    attn = runner.build_model({"type": "llama_custom", "kwargs": cfg}).get_submodule("3").self_attn
+    monkeypatch.setattr(transformer.F_, "fan_out_linear", lambda x, *weights: tuple(x @ w.t() for w in weights))
+    with pytest.raises(ValueError, match='needs a "length"'):
+        attn(torch.zeros(40, 1, 64, dtype=torch.bfloat16), None, torch.tensor([0, 12, 40]))

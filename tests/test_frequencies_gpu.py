@@ -120,3 +120,29 @@ def test_a_cast_that_leaves_the_weights_leaves_a_captured_call():
         torch.cuda.synchronize()
         assert torch.equal(captured, want)
     del keep
+
+
+def test_a_document_is_turned_alone_as_it_is_packed():
+    """With a length in the scaling, whatever lies in the row beside it."""
+    from easyllm_amd.positional_embeddings import RotaryEmbedding
+    rope = RotaryEmbedding(64, scaling=dict(SCALINGS["dynamic"], length=90)).cuda()
+    lengths = (12, 40, 7, 31)
+    q, k = rnd(sum(lengths), 1, 4, 64, seed=1), rnd(sum(lengths), 1, 2, 64, seed=2)
+    ids, cu = torch.cat([torch.arange(n) for n in lengths])[None].cuda(), torch.tensor([0, 12, 52, 59, 90]).cuda()
+    packed = rope.rotate(q, k, ids, cu)
+    for first, n in zip((0, 12, 52, 59), lengths):
+        alone = rope.rotate(q[first:first + n], k[first:first + n])
+        assert all(torch.equal(a, b[first:first + n]) for a, b in zip(alone, packed))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_stack_with_a_dynamic_scaling_of_a_length(monkeypatch, packed):
+    """Loss and gradients against 64 bits, of frequencies by the rule: inv_freq (2 length / 48 - 1)^(-j / (n - 1)), here of 512 tokens and 24 frequencies.  (A power and a product in 64 bits: a few
+    times 2^-53.)"""
+    import test_long_context_training_gpu as T
+    name = "a larger base for 512 tokens"
+    monkeypatch.setitem(T.STACKS, name, (dict(rotary_dim=48, scaling={"type": "dynamic", "factor": 2.0, "original_length": 48, "length": 512}), "silu"))
+    rope = T.build(name).get_submodule("3").self_attn.rotary_emb
+    want = rope.inv_freq.double() * (2 * 512 / 48 - 1) ** -(torch.arange(24, dtype=torch.float64, device="cuda") / 23)
+    assert bool(((rope.frequencies(T.S, torch.device("cuda", 0))[0] - want).abs() <= want * 2.0 ** -48).all())
+    T.test_loss_and_gradients(name, packed)
