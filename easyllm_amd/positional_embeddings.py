@@ -82,6 +82,10 @@ def _checked_scaling(scaling):
     return dict(scaling)
 
 
+def _capturing(device):
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class RotaryEmbedding(torch.nn.Module):
     def __init__(self, dim, base=10000, precision=torch.half, scale_factor=1.0, rotary_dim=None, interleaved=False, scaling=None):
         super().__init__()
@@ -101,6 +105,7 @@ class RotaryEmbedding(torch.nn.Module):
         self.max_seq_len_cached = None
         self.cos_half = None
         self.sin_half = None
+        self._captured = []
         self.precision = precision
         self.scale_factor = scale_factor
 
@@ -108,10 +113,17 @@ class RotaryEmbedding(torch.nn.Module):
         """fp32 (cos, sin) half tables [>= seq_len, dim/2] on `device`, built by the HIP table kernel."""
         if self.general:
             raise NotImplementedError("a rotary_dim, interleaved pairs and scaled frequencies have no tables")
+        capturing = _capturing(device)
         if self.max_seq_len_cached is None or seq_len > self.max_seq_len_cached or self.cos_half.device != device:
-            inv = self.inv_freq.to(device=device, dtype=torch.float32).contiguous()
-            self.cos_half, self.sin_half = K.rope_table(inv, int(seq_len), self.scale_factor)
+            with torch.inference_mode(False):  # (what an evaluation makes is saved for a backward pass later)
+                inv = self.inv_freq.to(device=device, dtype=torch.float32).contiguous()
+                tables = K.rope_table(inv, int(seq_len), self.scale_factor)
+            if capturing:  # (memory of the graph's, which holds nothing before its first replay)
+                return tables
+            self.cos_half, self.sin_half = tables
             self.max_seq_len_cached = int(seq_len)
+        elif capturing and not any(cos is self.cos_half for cos, _ in self._captured):
+            self._captured.append((self.cos_half, self.sin_half))  # (the graph holds no reference to what it reads)
         return self.cos_half, self.sin_half
 
     def frequencies(self, seq_len, device):
