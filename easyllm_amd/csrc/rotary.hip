@@ -139,16 +139,14 @@ __global__ __launch_bounds__(kRotaryBlock) void rotary_kernel(const RotaryArgs a
     }
 }
 
-template <bool INTERLEAVED, bool WHOLE, int HEADS>
-void launch_stream(const RotaryArgs& a, dim3 grid, dim3 block, bool stream_out, hipStream_t st) {
-    if (stream_out) hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, HEADS, WHOLE>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, HEADS, false>), grid, block, 0, st, a);
-}
+// (stream_out: only results of many pieces are more than the caches hold)
 template <bool INTERLEAVED, bool WHOLE>
 void launch_heads(const RotaryArgs& a, int per_thread, dim3 grid, dim3 block, bool stream_out, hipStream_t st) {
-    if (per_thread == 1) launch_stream<INTERLEAVED, WHOLE, 1>(a, grid, block, stream_out, st);
-    else if (per_thread == 2) launch_stream<INTERLEAVED, WHOLE, 2>(a, grid, block, stream_out, st);
-    else launch_stream<INTERLEAVED, WHOLE, INTERLEAVED ? 8 : 4>(a, grid, block, stream_out, st);
+    constexpr int MANY = INTERLEAVED ? 8 : 4;
+    if (per_thread == 1) hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, 1, false>), grid, block, 0, st, a);
+    else if (per_thread == 2) hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, 2, false>), grid, block, 0, st, a);
+    else if (stream_out) hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, MANY, WHOLE>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<INTERLEAVED, WHOLE, MANY, false>), grid, block, 0, st, a);
 }
 
 }  // namespace
