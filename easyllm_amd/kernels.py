@@ -1120,8 +1120,9 @@ def moments8_list(states):
         master = st["master"]
         _need(master.numel() == n and master.is_contiguous(), "moments8_list: the master weights' shape is not the moments'")
         tensors[i] = (None, *moments, None, None, n, 0)
-        # (where the codes are: the master weights may lie on the host)
-        outs.append(tuple(torch.empty(master.shape, dtype=BF16, device=st["exp_avg"].device) for _ in range(2)))
+        if master.device != st["exp_avg"].device:  # (the results lie where the codes do: the master weights may be on the host)
+            master = st["exp_avg"].view(master.shape)
+        outs.append((torch.empty_like(master, dtype=BF16), torch.empty_like(master, dtype=BF16)))
     _lib.call("ezl_moments8_list", len(states), tensors, _pointers([m for m, _ in outs]), _pointers([v for _, v in outs]), _stream())
     return outs
 
