@@ -71,18 +71,13 @@ __device__ __forceinline__ uint32_t code_of(float x, uint32_t r, int e) {
     return c | (BITS == 7 ? __float_as_uint(x) >> 31 << 7 : 0u);
 }
 
-// The root and the quotient by the bare instructions, 1 ulp each (2^-23): the change of a weight is rounded away behind its eighth digit anyway.  (With the correctly rounded forms, 25
-// instructions a value more, 202 million parameters took 776 us where these take 757: the instructions would bind as much as the memory.)
-__device__ __forceinline__ float root(float x) {
-    const bool small = x < 0x1p-96f;  // (where the instruction loses bits)
-    const float r = __builtin_amdgcn_sqrtf(small ? x * 0x1p64f : x);
-    return small ? r * 0x1p-32f : r;
-}
+// The root and the quotient correctly rounded, as all else: the weights are their definition's bit by bit.  (25 instructions a value more than the bare ones, which are off by 1 ulp each; 202
+// million parameters take 665 us either way but for 3: the memory binds.)
 __device__ __forceinline__ void adam8_one(float& p, float& m, float& v, float g, float beta1, float beta2, const Adam8Args& a) {
 #pragma clang fp contract(off)
     m = m * beta1 + g * a.one_beta1;
     v = v * beta2 + g * g * a.one_beta2;
-    const float update = (m * a.inv_bc1) * __builtin_amdgcn_rcpf(root(v * a.inv_bc2) + a.eps);
+    const float update = (m * a.inv_bc1) / (sqrtf(v * a.inv_bc2) + a.eps);
     p = p - (update + p * a.weight_decay) * a.lr;
 }
 
@@ -214,8 +209,8 @@ __device__ void last_blocks(const WavePlace& at, const Adam8Args& a, float coef,
 
 // A wave takes four blocks of 256, a lane four values of each: a block's largest value is a wave's.  Chunks go out from the last to the first: a norm of the gradients that went through them
 // in the other direction has left the last ones in the last-level cache.
-// Bound by HBM: 18 bytes a parameter.  A workgroup per chunk; 202 million parameters in seven tensors 659 us, 5.5 TB/s (a large copy 5.3), with 2048 workgroups that walk over the chunks
-// 762, with 8192 730: a new workgroup's loads are out while the old ones compute.
+// Bound by HBM: 18 bytes a parameter.  A workgroup per chunk; 202 million parameters in nine tensors 665 us, 5.5 TB/s (a large copy 5.3; with 2048 workgroups that walk over the chunks
+// a sixth longer, with 8192 a tenth): a new workgroup's loads are out while the old ones compute.
 __global__ __launch_bounds__(kThreads8) void adam8_kernel(const MomentsList l, const Adam8Args a, const float* __restrict__ norm_coef) {
     const float coef = norm_coef ? norm_coef[1] : 1.0f;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
