@@ -7,8 +7,8 @@ namespace {
 constexpr int kGateBlock = 256;
 
 // dgate = d * up * act'(gate), dup = d * act(gate): a workgroup takes a row of four blocks of what was kept, a wave eight rows of two, so that d and the results are read and written in whole
-// lines as what was kept is.  4096 x 11008 in 87 us (5.7 TB/s), 8192 x 2816 48, 1531 x 11008 32; where rows end inside a line, 15094 x 15336, 647 (3.9 TB/s: both ends of a wave's pieces are
-// lines that others hold, too; past the caches 750, with a wave on one block 963).
+// lines as what was kept is.  4096 x 11008 in 88 us (5.6 TB/s), 8192 x 2816 46.5, 1531 x 11008 34.6 (of values kept in rows, as d lies, 90, 45.4 and 33.2); where rows end inside a line, 15094 x 15336, 647
+// (3.9 TB/s: both ends of a wave's pieces are lines that others hold, too; of rows 545; past the caches 750, with a wave on one block 963).  The blocks are what the products' epilogues want.
 template <int ACT>
 __global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const Kept kept, bf16_t* dgate, bf16_t* dup, int64_t M, int f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
