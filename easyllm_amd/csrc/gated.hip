@@ -7,14 +7,16 @@ namespace {
 constexpr int kGateBlock = 256;
 
 // dgate = d * up * act'(gate), dup = d * act(gate): a workgroup takes a row of four blocks of what was kept, a wave eight rows of two, so that d and the results are read and written in whole
-// lines as what was kept is.  4096 x 11008 in 88 us (5.6 TB/s), 8192 x 2816 46.5, 1531 x 11008 34.6 (of values kept in rows, as d lies, 90, 45.4 and 33.2); where rows end inside a line, 15094 x 15336, 647
-// (3.9 TB/s: both ends of a wave's pieces are lines that others hold, too; of rows 545; past the caches 750, with a wave on one block 963).  The blocks are what the products' epilogues want.
+// lines as what was kept is.  Workgroups i, i + 8, i + 16, .. - an XCD's - are neighbours in a stripe of 16 rows: where rows end inside a line, both of its halves come together in one L2.
+// 4096 x 11008 in 88 us (5.6 TB/s), 8192 x 2816 46.8, 1531 x 11008 34.8; 15094 x 15336, whose rows end inside lines, 490 (5.2 TB/s; with an XCD's workgroups apart 647, past the caches 750, with a wave on
+// one block 963).
 template <int ACT>
-__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const Kept kept, bf16_t* dgate, bf16_t* dup, int64_t M, int f) {
+__global__ __launch_bounds__(kGateBlock) void gate_bwd_kernel(const bf16_t* d_in, const Kept kept, bf16_t* dgate, bf16_t* dup, int64_t M, int f, int across) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = (wave & 1) * 8 + (lane >> 3), col = (blockIdx.x * 2 + (wave >> 1)) * 2 * kKeptCols + (lane & 7) * 8;
+    const int row = (wave & 1) * 8 + (lane >> 3), col = ((int)(blockIdx.x / 8) % across * 2 + (wave >> 1)) * 2 * kKeptCols + (lane & 7) * 8;
     if (col >= f) return;
-    for (int64_t rows = blockIdx.y; rows * kKeptRows + row < M; rows += gridDim.y) {
+    const int stripes = gridDim.x / across;
+    for (int64_t rows = (int)(blockIdx.x / 8) / across * 8 + blockIdx.x % 8; rows * kKeptRows + row < M; rows += stripes) {
         const KeptPlace from = kept_place(kept, rows * kKeptRows + row, col);
         const u32x4 kg = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from.upper)), ku = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from.upper + kKeptUp));
         const u32x2 kl = *reinterpret_cast<const u32x2*>(from.low);
@@ -44,8 +46,10 @@ extern "C" int ezl_gate_bwd(int act, const void* d, const void* kept, void* dgat
     constexpr decltype(&gate_bwd_kernel<0>) kernels[] = {gate_bwd_kernel<0>, gate_bwd_kernel<1>, gate_bwd_kernel<2>, gate_bwd_kernel<3>};
     const Kept from = kept_of(kept, f);
     const int64_t rows = (M + kKeptRows - 1) / kKeptRows;
-    const dim3 grid((unsigned)((from.blocks + 3) / 4), (unsigned)(rows < 65535 ? rows : 65535));
-    hipLaunchKernelGGL(kernels[act], grid, dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, from, (bf16_t*)dgate, (bf16_t*)dup, M, (int)f);
+    const int across = (from.blocks + 3) / 4;  // workgroups of a stripe of 16 rows
+    const int64_t most = (1 << 24) / across / 8 * 8, stripes = (rows + 7) / 8 * 8;
+    hipLaunchKernelGGL(kernels[act], dim3((unsigned)((stripes < most ? stripes : most) * across)), dim3(kGateBlock), 0, (hipStream_t)stream, (const bf16_t*)d, from, (bf16_t*)dgate, (bf16_t*)dup, M,
+                       (int)f, across);
     EZL_LAUNCH_CHECK("ezl_gate_bwd");
     return EZL_OK;
 }
